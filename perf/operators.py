@@ -273,22 +273,25 @@ def _graph(case: dict[str, Any]) -> Any:
         with O.graph(name="mx4_projection") as gb:
             O.mx4_matmul(*O.mx4_quantize(x), wc, ws, out_dtype=case["out"], name="Y")
         return gb.graph
-    sizes = O.tensor((case["e"],), "int32", name="sizes")
+    # a graph's inputs are in the order in which the tensors were made
     if kind == "mx4_grp":
         x = O.tensor((case["t"], k), "bfloat16", name="X")
         wc = O.tensor((case["e"], case["n"], nb * 16), "uint8", name="W_codes")
         ws = O.tensor((case["e"], case["n"], nb), "uint8", name="W_scales")
+        sizes = O.tensor((case["e"],), "int32", name="sizes")
         with O.graph(name="mx4_experts") as gb:
             O.grouped_mx4_matmul(*O.mx4_quantize(x), wc, ws, sizes, out_dtype=case["out"], name="Y")
         return gb.graph
     x = O.tensor((case["t"], k), case["dtype"], name="X")
     if kind == "grad_w":
         dy = O.tensor((case["t"], case["n"]), case["dtype"], name="dY")
+        sizes = O.tensor((case["e"],), "int32", name="sizes")
         with O.graph(name="experts_grad_w") as gb:
             O.grouped_matmul_grad_w(x, dy, sizes, out_dtype=case["out"], name="dW")
         return gb.graph
     layout = {"layout": [0, 2, 1]} if case["trans_w"] else {}
     w = O.tensor((case["e"], k, case["n"]), case["dtype"], name="W", **layout)
+    sizes = O.tensor((case["e"],), "int32", name="sizes")
     with O.graph(name="experts") as gb:
         O.grouped_matmul(x, w, sizes, out_dtype=case["out"], name="Y")
     return gb.graph

@@ -252,14 +252,99 @@ int xtc_hip_unpad(const void *x, void *y, int elem_bytes, int ndim,
 int xtc_hip_cast_f32_to_bf16(const float *x, uint16_t *y, uint64_t n, void *stream);
 int xtc_hip_cast_bf16_to_f32(const uint16_t *x, float *y, uint64_t n, void *stream);
 
+/* Products by group: rows of x sorted by group (the tokens of a layer of
+ * experts, sorted by expert), one matrix for each group.  No counterpart in
+ * the reference, whose matmul (operators.py:159-221) has one matrix.
+ *
+ *   y[r, :] = x[r, :] op(w[e])   for the rows r of group e
+ *
+ * sizes[e] (int32, device memory) is the number of rows of group e; the groups
+ * follow one another from row 0.  Rows past the last group give zeros, sizes
+ * below zero count as zero, and rows past T are dropped, so no content of
+ * sizes reads or writes outside the operands.  Groups may be empty.  The
+ * sizes are read by the kernels: the host neither waits for them nor copies
+ * them.  y must not overlap an operand.
+ * trans_w: w[e] is stored [N][ldw >= K] (a checkpoint's [out][in]; with the
+ * stored forward weights, the gradient of x, dy op(w)^T). */
+typedef struct {
+  int dtype;             /* XTC_HIP_F32 or XTC_HIP_BF16: x and w */
+  int out_dtype;         /* XTC_HIP_F32, or XTC_HIP_BF16 for bf16 operands: sums
+                            are fp32 and rounded once */
+  int E;                 /* groups, >= 1 */
+  int T, N, K;           /* rows of x in all (0: nothing to do), columns of y, columns of x */
+  int ldx, ldw, ldy;     /* row strides in elements, 0 = dense */
+  int trans_w;           /* 1: w[e] stored [N][K], 0: [K][N] */
+  int64_t stride_w;      /* elements between the matrices of two groups, 0 = dense */
+  void *stream;          /* hipStream_t, NULL = library stream */
+} xtc_hip_grouped_matmul_desc;
+
+int xtc_hip_grouped_matmul(const xtc_hip_grouped_matmul_desc *desc, const void *x,
+                           const void *w, const int32_t *sizes, void *y);
+
+/* The gradient of w: dw[e] = x_e^T dy_e over the rows of group e, zeros where
+ * it has none.  x [T][ldx >= K] and dy [T][ldy >= N] of type dtype, dw [K][ldw >=
+ * N] matrices of type out_dtype, stride_w apart; trans_w must be 0 (the transposed
+ * gradient is this one with x and dy exchanged).  The order of the sums depends
+ * on the sizes alone. */
+int xtc_hip_grouped_matmul_grad_w(const xtc_hip_grouped_matmul_desc *desc, const void *x,
+                                  const void *dy, const int32_t *sizes, void *dw);
+
+/* Microscaled 4-bit floats (the OCP MX format of E2M1 elements with E8M0
+ * scales): every 32 consecutive elements of a row share a scale.  No
+ * counterpart in the reference.
+ *   scales  [rows][ceil(K / 32)] bytes s, the scale is 2^(s - 127):
+ *           s = max(0, 125 + floor(log2 max|x|)); 255 (all of the block stands
+ *           for NaN) where the block holds an infinity or a NaN
+ *   codes   [rows][16 ceil(K / 32)] bytes, two elements a byte, the even one in
+ *           the low half: a sign bit above the index of 0, .5, 1, 1.5, 2, 3, 4,
+ *           6 nearest to |x| / scale, ties to the even index, 6 beyond 6.
+ * The last block of a row is filled up with zeros.  Codes are 16-byte aligned. */
+typedef struct {
+  int dtype;             /* XTC_HIP_F32 or XTC_HIP_BF16: x and the values */
+  int64_t rows;          /* 0: nothing to do */
+  int K;                 /* elements of a row */
+  int ld;                /* row stride in elements of x (dequantize: of the values), 0 = dense */
+  void *stream;          /* hipStream_t, NULL = library stream */
+} xtc_hip_mx4_desc;
+
+/* Codes, scales and the (dense) values that they stand for; each may be NULL. */
+int xtc_hip_mx4_quantize(const xtc_hip_mx4_desc *desc, const void *x, uint8_t *codes,
+                         uint8_t *scales, void *values);
+
+/* Codes for given scales (0 in blocks whose scale is 255, and for NaN). */
+int xtc_hip_mx4_encode(const xtc_hip_mx4_desc *desc, const void *x, const uint8_t *scales,
+                       uint8_t *codes);
+
+int xtc_hip_mx4_dequantize(const xtc_hip_mx4_desc *desc, const uint8_t *codes,
+                           const uint8_t *scales, void *values);
+
+/* c[m, n] = sum_k a[m, k] b[n, k] of microscaled operands, both with k along
+ * their rows; fp32 sums.  With E > 0 the rows of a are sorted by group (sizes
+ * as in xtc_hip_grouped_matmul) and b holds one matrix for each group; with E
+ * = 0 sizes is NULL and b is one matrix. */
+typedef struct {
+  int out_dtype;         /* XTC_HIP_F32 or XTC_HIP_BF16 */
+  int E;                 /* groups, 0: one product */
+  int M, N, blocks;      /* rows of a (0: nothing to do), rows of b, blocks of 32 of k */
+  int ldc;               /* row stride of c in elements, 0 = dense */
+  void *stream;          /* hipStream_t, NULL = library stream */
+} xtc_hip_mx4_matmul_desc;
+
+int xtc_hip_mx4_matmul(const xtc_hip_mx4_matmul_desc *desc, const uint8_t *a_codes,
+                       const uint8_t *a_scales, const uint8_t *b_codes,
+                       const uint8_t *b_scales, const int32_t *sizes, void *c);
+
 /* sizeof(xtc_hip_matmul_desc) and sizeof(xtc_hip_conv2d_desc) as this library
- * was compiled: a binding that declares the descriptors itself (ctypes, cgo)
+ * was compiled (and of the other descriptors, below): a binding that declares the descriptors itself (ctypes, cgo)
  * checks its own struct sizes against these before the first call, so a
  * field it lacks fails loudly instead of being read past the end of its
  * struct.  No counterpart in the reference, whose mgpu* calls
  * (GPUDevice.py:131-207) take no structs. */
 int xtc_hip_matmul_desc_size(void);
 int xtc_hip_conv2d_desc_size(void);
+int xtc_hip_grouped_matmul_desc_size(void);
+int xtc_hip_mx4_desc_size(void);
+int xtc_hip_mx4_matmul_desc_size(void);
 
 /* Compiled kernel instances.  A schedule maps onto one of these; the HIP
  * Scheduler rejects schedules that map to none. */

@@ -53,7 +53,7 @@ from ...itf.comp import Compiler
 from ...runtimes.hip import capi
 from ...utils.bf16 import itemsize
 from .lowering import Launch, Plan
-from .mapping import GemmConfig, SplitConfig, map_node
+from .mapping import GemmConfig, SplitConfig, check_unscheduled, map_node
 from .scheduler import HipSchedule, ScheduleError
 
 if TYPE_CHECKING:
@@ -297,6 +297,30 @@ def _emit_launch(plan: Plan, ln: Launch, cfg: GemmConfig | SplitConfig | None, i
             f"  if ((rc = xtc_hip_memcpy_d2d({dst}, {_ptr(plan, ln.inputs[0])}, {nbytes}ull))) "
             f"{{ record(rc, {where}); return; }}"
         )
+    elif ln.kind in ("grouped_matmul", "grouped_matmul_grad_w"):
+        args = ", ".join(_ptr(plan, u) for u in ln.inputs)
+        lines.append(
+            f"  {{ static const xtc_hip_grouped_matmul_desc d = {{{_DTYPE_ENUM[a['dtype']]}, {_DTYPE_ENUM[a['out']]}, "
+            f"{a['E']}, {a['T']}, {a['N']}, {a['K']}, 0, 0, 0, {1 if a['trans_w'] else 0}, 0, 0}};"
+        )
+        lines.append(f"    if ((rc = xtc_hip_{ln.kind}(&d, {args}, {dst}))) {{ record(rc, {where}); return; }} }}")
+    elif ln.kind in ("mx4_quantize", "mx4_encode", "mx4_dequantize"):
+        args = ", ".join(_ptr(plan, u) for u in ln.inputs) + ", "
+        if ln.kind == "mx4_quantize":
+            args += ", ".join(_ptr(plan, u) if u else "0" for u in (a["codes"], ln.output, a["values"]))
+        else:
+            args += dst
+        lines.append(
+            f"  {{ static const xtc_hip_mx4_desc d = {{{_DTYPE_ENUM[a['dtype']]}, {a['rows']}ll, {a['K']}, 0, 0}};"
+        )
+        lines.append(f"    if ((rc = xtc_hip_{ln.kind}(&d, {args}))) {{ record(rc, {where}); return; }} }}")
+    elif ln.kind == "mx4_matmul":
+        args = ", ".join([*(_ptr(plan, u) for u in ln.inputs), *(() if a["E"] else ("0",)), dst])
+        lines.append(
+            f"  {{ static const xtc_hip_mx4_matmul_desc d = {{{_DTYPE_ENUM[a['out']]}, {a['E']}, {a['M']}, {a['N']}, "
+            f"{a['blocks']}, 0, 0}};"
+        )
+        lines.append(f"    if ((rc = xtc_hip_mx4_matmul(&d, {args}))) {{ record(rc, {where}); return; }} }}")
     else:
         raise ScheduleError(f"no code generator for launch kind {ln.kind}")
     return lines
@@ -457,6 +481,8 @@ class HipCompiler(Compiler):
         for ln in self._backend.plan.launches:
             if ln.kind in ("matmul", "conv2d"):
                 configs[ln.node] = map_node(ln.attrs, ln.kind == "conv2d", schedule.node(ln.node), policy)
+            elif ln.kind.startswith(("grouped_", "mx4_")):
+                check_unscheduled(ln.kind, schedule.node(ln.node))
         return configs
 
     def check_fusions(self, schedule: HipSchedule) -> None:

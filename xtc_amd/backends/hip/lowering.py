@@ -9,8 +9,9 @@ HBM):
     implicit-GEMM loader (out-of-window taps read `constant_value`);
   * bias_add on a matmul/conv2d result -> GEMM epilogue;
   * relu on a matmul/conv2d(/bias_add) result -> GEMM epilogue.
-A fusion happens only when the intermediate is used once and is not a graph
-output.  A matmul operand with layout [1, 0] (stored transposed) becomes the
+Such a fusion happens only when the intermediate is used once and is not a graph
+output.  mx4_scales, the mx4_codes of the same tensor for these scales and a
+mx4_dequantize of the pair are one launch that writes all of them.  A matmul operand with layout [1, 0] (stored transposed) becomes the
 launch's trans_a / trans_b flag; other operators require natural layouts.  reshape is a view; unpad
 is a crop kernel (16-byte row copies when the innermost dim is kept).  The reference lowers each node to its own
 linalg op (src/xtc/backends/mlir/MlirOps.py:166-887) and fuses only through
@@ -61,7 +62,10 @@ class Launch:
     """One kernel launch.  `node` is the scheduled node the launch serves
     (the matmul/conv2d for fused GEMMs); `absorbed` lists fused nodes."""
 
-    kind: str  # "matmul" | "conv2d" | "relu" | "pad" | "unpad" | "copy" | "cast"
+    # "matmul" | "conv2d" | "relu" | "pad" | "unpad" | "copy" | "cast" |
+    # "grouped_matmul" | "grouped_matmul_grad_w" |
+    # "mx4_quantize" | "mx4_encode" | "mx4_dequantize" | "mx4_matmul"
+    kind: str
     node: str
     inputs: list[str]
     output: str
@@ -200,10 +204,12 @@ def lower_graph(graph: Any) -> Plan:
                 flags.append(False)
             elif n.operation.name == "matmul" and idx < 2 and len(shp) == 2 and list(lay) == [1, 0]:
                 flags.append(True)
+            elif n.operation.name == "grouped_matmul" and idx == 1 and list(lay) == [0, 2, 1]:
+                flags.append(True)
             else:
                 raise UnsupportedGraph(
                     f"{n.operation.name} {n.name}: tensor layout {list(lay)} of input {idx} is not supported "
-                    "(only [1, 0] on a 2-D matmul operand)"
+                    "(only [1, 0] on a 2-D matmul operand and [0, 2, 1] on the matrices of grouped_matmul)"
                 )
         return tuple(flags)
 
@@ -331,6 +337,53 @@ def lower_graph(graph: Any) -> Plan:
             attrs = {"shape": ishape, "pads": per, "elem": 2 if dt == BF16 else 8 if dt == F64 else 4}
             launches.append(Launch("unpad", n.name, [n.inputs[0]], n.uid, attrs))
             scheduled[n.name] = n
+        elif name in ("grouped_matmul", "grouped_matmul_grad_w"):
+            xs, ws = _shape(out_type(n.inputs[0])), _shape(out_type(n.inputs[1]))
+            attrs = {"dtype": _dtype(out_type(n.inputs[0])), "out": _dtype(t_out), "trans_w": trans[1],
+                     "E": _shape(out_type(n.inputs[2]))[0], "T": xs[0], "K": xs[1], "N": ws[-1]}
+            launches.append(Launch(name, n.name, list(n.inputs), n.uid, attrs))
+            scheduled[n.name] = n
+        elif name == "mx4_scales":
+            # the codes for these scales and the values of the pair come from the
+            # same pass over x
+            xs = _shape(out_type(n.inputs[0]))
+            attrs = {"dtype": _dtype(out_type(n.inputs[0])), "rows": prod(xs[:-1]), "K": xs[-1], "codes": None,
+                     "values": None}
+            fused = []
+            own = [u for u in users.get(n.uid, [])
+                   if u.operation.name == "mx4_codes" and list(u.inputs) == [n.inputs[0], n.uid]]
+            if own:
+                attrs["codes"] = own[0].uid
+                fused.append(own[0])
+                pair = [u for u in users.get(own[0].uid, [])
+                        if u.operation.name == "mx4_dequantize" and list(u.inputs) == [own[0].uid, n.uid]
+                        and _shape(u.outputs_types[0]) == xs and _dtype(u.outputs_types[0]) == attrs["dtype"]]
+                if pair:
+                    attrs["values"] = pair[0].uid
+                    fused.append(pair[0])
+            for u in fused:
+                transposed_inputs(u)
+                absorbed.add(u.uid)
+                if u.uid not in buffers:
+                    buffers[u.uid] = Buffer(u.uid, _shape(u.outputs_types[0]), _dtype(u.outputs_types[0]), "temp")
+            launches.append(Launch("mx4_quantize", n.name, [n.inputs[0]], n.uid, attrs, [u.name for u in fused]))
+            scheduled[n.name] = n
+        elif name == "mx4_codes":
+            xs = _shape(out_type(n.inputs[0]))
+            attrs = {"dtype": _dtype(out_type(n.inputs[0])), "rows": prod(xs[:-1]), "K": xs[-1]}
+            launches.append(Launch("mx4_encode", n.name, list(n.inputs), n.uid, attrs))
+            scheduled[n.name] = n
+        elif name == "mx4_dequantize":
+            shape = _shape(t_out)
+            attrs = {"dtype": _dtype(t_out), "rows": prod(shape[:-1]), "K": shape[-1]}
+            launches.append(Launch("mx4_dequantize", n.name, list(n.inputs), n.uid, attrs))
+            scheduled[n.name] = n
+        elif name in ("mx4_matmul", "grouped_mx4_matmul"):
+            bs = _shape(out_type(n.inputs[3]))
+            attrs = {"out": _dtype(t_out), "E": bs[0] if name == "grouped_mx4_matmul" else 0,
+                     "M": _shape(t_out)[0], "N": bs[-2], "blocks": bs[-1]}
+            launches.append(Launch("mx4_matmul", n.name, list(n.inputs), n.uid, attrs))
+            scheduled[n.name] = n
         elif name == "reshape":
             if n.uid in outputs:
                 launches.append(Launch("copy", n.name, [n.inputs[0]], n.uid, {}))
@@ -340,7 +393,9 @@ def lower_graph(graph: Any) -> Plan:
         else:
             raise UnsupportedGraph(
                 f"operator {name} ({n.name}) is not supported by the HIP backend "
-                "(supported: matmul, conv2d, relu, pad, pad2d, unpad, bias_add after matmul/conv2d, reshape)"
+                "(supported: matmul, conv2d, relu, pad, pad2d, unpad, bias_add after matmul/conv2d, reshape, "
+                "grouped_matmul, grouped_matmul_grad_w, mx4_scales, mx4_codes, mx4_dequantize, mx4_matmul, "
+                "grouped_mx4_matmul)"
             )
 
     # workspace layout: temps packed at 256-byte alignment

@@ -373,6 +373,21 @@ def map_gemm(
     return GemmConfig(dtype, conv, *tile, split_k=split_k, group_m=group_m, exact=False, source="nearest")
 
 
+def check_unscheduled(kind: str, sched: HipNodeSchedule | None) -> None:
+    """Operators whose kernels choose their own tiles (from the sizes, which
+    may be known on the device only) take no transformations."""
+    if sched is None:
+        return
+    asked = [what for what, given in (
+        ("strip_mine/tile", any(sched.tiles.values())), ("split", sched.segments or sched.splits),
+        ("interchange", sched.base_order() != sched.dims), ("vectorize", sched.vectorization),
+        ("parallelize", sched.parallelization), ("unroll", sched.unrolling),
+        ("pack/buffer", sched.packed_buffers or sched.buffers)) if given]
+    if asked:
+        raise ScheduleError(f"{sched.node_name}: {', '.join(asked)} of {kind} has no HIP mapping: its kernels choose "
+                            "their own tiles")
+
+
 def map_node(
     launch_attrs: dict[str, Any],
     conv: bool,

@@ -1,0 +1,22 @@
+// SPDX-License-Identifier: BSD-3-Clause
+// What the library's translation units share of the runtime: the error
+// message of the calling thread, the current device and its streams.
+// Defined in runtime.hip.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace xtc_hip {
+namespace core {
+
+// Sets the thread's message (printf form) and returns 1.
+int fail(const char* fmt, ...);
+// Whether xtc_hip_init has run.
+bool ready();
+// `stream`, or the library stream where it is null.
+hipStream_t pick_stream(void* stream);
+
+inline bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
+
+}  // namespace core
+}  // namespace xtc_hip

@@ -1,0 +1,99 @@
+// SPDX-License-Identifier: BSD-3-Clause
+// Entry points of the products by group (rows sorted by expert).
+#include "xtc_hip.h"
+#include "core.hpp"
+#include "grouped_any.hpp"
+
+using namespace xtc_hip;
+using core::fail;
+
+namespace {
+
+// Largest extent: tiles and slabs past it stay within 32 bits.
+constexpr int kMost = 0x7fffffff - 1023;
+
+int check(const xtc_hip_grouped_matmul_desc* d, const char* what) {
+  if (!core::ready()) return fail("xtc_hip_init not called");
+  if (!d) return fail("%s: null descriptor", what);
+  if (d->dtype != XTC_HIP_F32 && d->dtype != XTC_HIP_BF16) return fail("%s: unsupported dtype %d", what, d->dtype);
+  if (d->out_dtype != XTC_HIP_F32 && !(d->out_dtype == XTC_HIP_BF16 && d->dtype == XTC_HIP_BF16))
+    return fail("%s: unsupported result dtype %d for operands of dtype %d", what, d->out_dtype, d->dtype);
+  if (d->E < 1 || d->T < 0 || d->N < 1 || d->K < 1)
+    return fail("%s: invalid sizes E=%d T=%d N=%d K=%d", what, d->E, d->T, d->N, d->K);
+  if (d->E > kMost || d->T > kMost || d->N > kMost || d->K > kMost)
+    return fail("%s: sizes E=%d T=%d N=%d K=%d are too many, past %d", what, d->E, d->T, d->N, d->K, kMost);
+  return 0;
+}
+
+int stride(int given, int dense, const char* what, const char* name, int* out) {
+  *out = given ? given : dense;
+  if (*out < dense) return fail("%s: row stride %d of %s is below its %d columns", what, given, name, dense);
+  return 0;
+}
+
+template <bool GRAD>
+int launch_any(const xtc_hip_grouped_matmul_desc& d, const GroupedArgs& a, int64_t groups, hipStream_t s) {
+  if (groups < 1 || groups >= (int64_t)1 << 31) return fail("grouped_matmul: %lld workgroups are too many", (long long)groups);
+  const dim3 grid((unsigned)groups), block(gany::NT);
+  const bool wt = !GRAD && d.trans_w, out16 = d.out_dtype == XTC_HIP_BF16;
+#define XTC_ANY(T, U)                                                                                  \
+  do {                                                                                                 \
+    if (wt) hipLaunchKernelGGL((grouped_any<T, U, !GRAD, GRAD>), grid, block, 0, s, a);                \
+    else hipLaunchKernelGGL((grouped_any<T, U, false, GRAD>), grid, block, 0, s, a);                   \
+  } while (0)
+  if (d.dtype == XTC_HIP_F32) XTC_ANY(float, float);
+  else if (out16) XTC_ANY(__bf16, __bf16);
+  else XTC_ANY(__bf16, float);
+#undef XTC_ANY
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? 0 : fail("grouped_matmul: launch failed: %s", hipGetErrorString(e));
+}
+
+}  // namespace
+
+extern "C" {
+
+int xtc_hip_grouped_matmul_desc_size(void) { return (int)sizeof(xtc_hip_grouped_matmul_desc); }
+
+int xtc_hip_grouped_matmul(const xtc_hip_grouped_matmul_desc* desc, const void* x, const void* w, const int32_t* sizes,
+                           void* y) {
+  const char* const what = "grouped_matmul";
+  if (check(desc, what)) return 1;
+  const xtc_hip_grouped_matmul_desc& d = *desc;
+  if (d.T == 0) return 0;
+  if (!x || !w || !sizes || !y) return fail("%s: null operand", what);
+  GroupedArgs a{};
+  a.x = x, a.w = w, a.sizes = sizes, a.y = y;
+  a.E = d.E, a.T = d.T, a.N = d.N, a.K = d.K;
+  if (stride(d.ldx, d.K, what, "x", &a.ldx) || stride(d.ldw, d.trans_w ? d.K : d.N, what, "w", &a.ldw) ||
+      stride(d.ldy, d.N, what, "y", &a.ldy))
+    return 1;
+  const int64_t matrix = (int64_t)(d.trans_w ? d.N : d.K) * a.ldw;
+  a.stride_w = d.stride_w ? d.stride_w : matrix;
+  if (a.stride_w < 0) return fail("%s: negative stride between matrices", what);
+  a.tiles_n = (d.N + gany::BN - 1) / gany::BN;
+  return launch_any<false>(d, a, most_tiles(d.T, d.E, gany::BM) * a.tiles_n, core::pick_stream(d.stream));
+}
+
+int xtc_hip_grouped_matmul_grad_w(const xtc_hip_grouped_matmul_desc* desc, const void* x, const void* dy,
+                                  const int32_t* sizes, void* dw) {
+  const char* const what = "grouped_matmul_grad_w";
+  if (check(desc, what)) return 1;
+  const xtc_hip_grouped_matmul_desc& d = *desc;
+  if (d.trans_w) return fail("%s: a transposed gradient is the gradient with x and dy exchanged", what);
+  if (!sizes || !dw || (d.T > 0 && (!x || !dy))) return fail("%s: null operand", what);
+  GroupedArgs a{};
+  a.x = x, a.w = dy, a.sizes = sizes, a.y = dw;
+  a.E = d.E, a.T = d.T, a.N = d.N, a.K = d.K;
+  if (stride(d.ldx, d.K, what, "x", &a.ldx) || stride(d.ldy, d.N, what, "dy", &a.ldw) ||
+      stride(d.ldw, d.N, what, "dw", &a.ldy))
+    return 1;
+  const int64_t matrix = (int64_t)d.K * a.ldy;
+  a.stride_y = d.stride_w ? d.stride_w : matrix;
+  if (a.stride_y < matrix) return fail("%s: a stride of %lld lets the gradients of two groups overlap", what, (long long)d.stride_w);
+  a.tiles_n = (d.N + gany::BN - 1) / gany::BN;
+  a.tiles_k = (d.K + gany::BM - 1) / gany::BM;
+  return launch_any<true>(d, a, (int64_t)d.E * a.tiles_k * a.tiles_n, core::pick_stream(d.stream));
+}
+
+}  // extern "C"

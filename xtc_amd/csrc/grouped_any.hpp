@@ -1,0 +1,195 @@
+// SPDX-License-Identifier: BSD-3-Clause
+// Products by group for operands of any size, stride and alignment:
+//   y[r, :] = x[r, :] w[e]            for the rows r of group e      (GRAD = false)
+//   dw[e]   = sum_r x[r, :]^T dy[r, :] over the rows r of group e    (GRAD = true)
+// Both are sums C[i, j] = sum_k A[i, k] B[k, j]: i the rows and k the depth of w,
+// or i the depth of w and k the rows.
+//
+// One workgroup of 2 x 2 waves computes a 64 x 64 tile of C, k in slabs of 32
+// through two LDS buffers, the next slab in registers meanwhile.  An operand is
+// loaded 8 elements a lane along its contiguous axis (unaligned vectors, which
+// global memory takes at element alignment; element by element where the
+// operand ends inside) and kept in LDS with k contiguous, so that a lane's
+// fragment is one (bf16) or two (fp32) 16-byte reads.  bf16 runs on
+// v_mfma_f32_16x16x32_bf16, fp32 on v_mfma_f32_16x16x4_f32 (exact products, the
+// lane's 8 k of a slab in any order as long as A and B agree).  Sums are fp32;
+// a bf16 result is rounded once, at the store.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "groups.hpp"
+
+namespace xtc_hip {
+
+struct GroupedArgs {
+  const void* x;     // [T][ldx]
+  const void* w;     // [E] matrices, stride_w elements apart; GRAD: dy [T][ldw]
+  const int* sizes;  // [E]
+  void* y;           // [T][ldy]; GRAD: [E] matrices [K][ldy], stride_y apart
+  int64_t stride_w, stride_y;
+  int E, T, N, K;
+  int ldx, ldw, ldy;
+  int tiles_n, tiles_k;
+};
+
+namespace gany {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+
+constexpr int BM = 64, BN = 64, BK = 32, NT = 256;
+
+template <typename T> struct Row { static constexpr int STRIDE = BK + 16 / (int)sizeof(T); };  // elements; 16-byte rows
+
+// the 8 elements at p, of which the first n exist
+template <typename T>
+__device__ __forceinline__ void load8(T (&v)[8], const T* p, int n) {
+  if (n >= 8) {
+    __builtin_memcpy(v, p, 8 * sizeof(T));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : (T)0.f;
+  }
+}
+
+// a lane's share of a slab: KC: 8 k of one row, else 8 rows at one k
+template <typename T, bool KC>
+__device__ __forceinline__ void load(T (&v)[8], const T* p, int64_t ld, int rows, int depth) {
+  const int tid = threadIdx.x;
+  if constexpr (KC) {
+    const int r = tid >> 2, k = (tid & 3) * 8;
+    load8(v, p + (int64_t)r * ld + k, r < rows ? depth - k : 0);
+  } else {
+    const int k = tid >> 3, r = (tid & 7) * 8;
+    load8(v, p + (int64_t)k * ld + r, k < depth ? rows - r : 0);
+  }
+}
+
+template <typename T, bool KC>
+__device__ __forceinline__ void store(T* lds, const T (&v)[8]) {
+  constexpr int S = Row<T>::STRIDE;
+  const int tid = threadIdx.x;
+  if constexpr (KC) {
+    __builtin_memcpy(__builtin_assume_aligned(lds + (tid >> 2) * S + (tid & 3) * 8, 16), v, 8 * sizeof(T));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) lds[((tid & 7) * 8 + i) * S + (tid >> 3)] = v[i];
+  }
+}
+
+__device__ __forceinline__ void mma(f32x4& c, const __bf16* b, const __bf16* a, int g) {
+  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(const bf16x8*)(b + 8 * g), *(const bf16x8*)(a + 8 * g), c, 0, 0, 0);
+}
+__device__ __forceinline__ void mma(f32x4& c, const float* b, const float* a, int g) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const f32x4 bv = *(const f32x4*)(b + 16 * h + 4 * g), av = *(const f32x4*)(a + 16 * h + 4 * g);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) c = __builtin_amdgcn_mfma_f32_16x16x4f32(bv[q], av[q], c, 0, 0, 0);
+  }
+}
+
+__device__ __forceinline__ void put(float* p, f32x4 v, int n) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (i < n) p[i] = v[i];
+}
+__device__ __forceinline__ void put(__bf16* p, f32x4 v, int n) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (i < n) p[i] = (__bf16)v[i];
+}
+
+}  // namespace gany
+
+// T: operands, U: result; WT: w stored transposed ([N][K]; GRAD: unused)
+template <typename T, typename U, bool WT, bool GRAD>
+__global__ void __launch_bounds__(256) grouped_any(GroupedArgs p) {
+  using namespace gany;
+  constexpr int S = Row<T>::STRIDE;
+  constexpr bool A_KC = !GRAD, B_KC = WT && !GRAD;
+  __shared__ __attribute__((aligned(16))) T lds[2][2][64 * S];
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int l16 = lane & 15, g = lane >> 4, wm = wave >> 1, wn = wave & 1;
+  const T* const x = (const T*)p.x;
+  const T* const w = (const T*)p.w;
+
+  const T *a, *b;
+  U* c;
+  int rows, cols, depth;  // of the tile and its sums
+  int64_t a_step, b_step;  // a slab further along k
+  int n0;
+  if constexpr (GRAD) {
+    const int e = blockIdx.x / (p.tiles_k * p.tiles_n), t = blockIdx.x % (p.tiles_k * p.tiles_n);
+    const int k0 = t / p.tiles_n * BM;
+    n0 = t % p.tiles_n * BN;
+    const RowGroup gr = find_group(p.sizes, p.E, p.T, e);
+    a = x + (int64_t)gr.begin * p.ldx + k0;
+    b = w + (int64_t)gr.begin * p.ldw + n0;
+    c = (U*)p.y + e * p.stride_y + (int64_t)k0 * p.ldy + n0;
+    rows = p.K - k0;
+    depth = gr.end - gr.begin;
+    a_step = (int64_t)BK * p.ldx;
+    b_step = (int64_t)BK * p.ldw;
+  } else {
+    const int mt = blockIdx.x / p.tiles_n;
+    n0 = blockIdx.x % p.tiles_n * BN;
+    const RowGroup gr = find_tile<BM>(p.sizes, p.E, p.T, mt);
+    if (gr.e < 0) return;
+    a = x + (int64_t)gr.begin * p.ldx;
+    b = w + (gr.e < p.E ? gr.e : 0) * p.stride_w + (int64_t)n0 * (WT ? p.ldw : 1);
+    c = (U*)p.y + (int64_t)gr.begin * p.ldy + n0;
+    rows = gr.end - gr.begin;
+    depth = gr.e < p.E ? p.K : 0;  // rows of no group: zeros
+    a_step = BK;
+    b_step = WT ? (int64_t)BK : (int64_t)BK * p.ldw;
+  }
+  rows = min(rows, BM);
+  cols = min(p.N - n0, BN);
+
+  f32x4 acc[2][2] = {};
+  const int steps = (depth + BK - 1) / BK;
+  T av[8], bv[8];
+  if (steps > 0) {
+    load<T, A_KC>(av, a, p.ldx, rows, depth);
+    load<T, B_KC>(bv, b, p.ldw, cols, depth);
+    store<T, A_KC>(lds[0][0], av);
+    store<T, B_KC>(lds[0][1], bv);
+  }
+  for (int s = 0; s < steps; ++s) {
+    __syncthreads();
+    if (s + 1 < steps) {
+      a += a_step;
+      b += b_step;
+      depth -= BK;
+      load<T, A_KC>(av, a, p.ldx, rows, depth);
+      load<T, B_KC>(bv, b, p.ldw, cols, depth);
+    }
+    const T* la = lds[s & 1][0] + (wm * 32 + l16) * S;
+    const T* lb = lds[s & 1][1] + (wn * 32 + l16) * S;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) mma(acc[i][j], lb + j * 16 * S, la + i * 16 * S, g);
+    if (s + 1 < steps) {
+      store<T, A_KC>(lds[(s + 1) & 1][0], av);
+      store<T, B_KC>(lds[(s + 1) & 1][1], bv);
+    }
+  }
+  // a lane holds C[i][j .. j+3]: B is the first MFMA operand
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int m = wm * 32 + i * 16 + l16;
+    if (m >= rows) continue;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int n = wn * 32 + j * 16 + 4 * g;
+      put(c + (int64_t)m * p.ldy + n, acc[i][j], cols - n);
+    }
+  }
+}
+
+}  // namespace xtc_hip

@@ -1,0 +1,123 @@
+// SPDX-License-Identifier: BSD-3-Clause
+// Entry points of the microscaled 4-bit operators.
+#include "xtc_hip.h"
+#include "core.hpp"
+#include "mx4_any.hpp"
+
+using namespace xtc_hip;
+using core::aligned16;
+using core::fail;
+
+namespace {
+
+// Largest extent: tiles and blocks past it stay within 32 bits.
+constexpr int kMost = 0x7fffffff - 1023;
+
+int done(const char* what) {
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? 0 : fail("%s: launch failed: %s", what, hipGetErrorString(e));
+}
+
+int check(const xtc_hip_mx4_desc* d, const char* what) {
+  if (!core::ready()) return fail("xtc_hip_init not called");
+  if (!d) return fail("%s: null descriptor", what);
+  if (d->dtype != XTC_HIP_F32 && d->dtype != XTC_HIP_BF16) return fail("%s: unsupported dtype %d", what, d->dtype);
+  if (d->rows < 0 || d->K < 1 || d->K > kMost)
+    return fail("%s: invalid sizes rows=%lld K=%d", what, (long long)d->rows, d->K);
+  if (d->ld && d->ld < d->K) return fail("%s: row stride %d is below the %d elements of a row", what, d->ld, d->K);
+  return 0;
+}
+
+Mx4QuantArgs args_of(const xtc_hip_mx4_desc& d) {
+  Mx4QuantArgs a{};
+  a.rows = d.rows, a.K = d.K, a.blocks = (d.K + 31) / 32;
+  a.ldx = d.ld ? d.ld : d.K, a.ldv = d.K;
+  return a;
+}
+
+dim3 grid_of(const Mx4QuantArgs& a) {
+  return dim3((unsigned)((4 * (int64_t)a.blocks + 255) / 256), (unsigned)(a.rows < 65535 ? a.rows : 65535));
+}
+
+int quantize(const xtc_hip_mx4_desc& d, const Mx4QuantArgs& a, const char* what) {
+  if (!aligned16(a.codes)) return fail("%s: codes must be 16-byte aligned", what);
+  if (d.dtype == XTC_HIP_F32)
+    hipLaunchKernelGGL(mx4_quantize<float>, grid_of(a), dim3(256), 0, core::pick_stream(d.stream), a);
+  else
+    hipLaunchKernelGGL(mx4_quantize<__bf16>, grid_of(a), dim3(256), 0, core::pick_stream(d.stream), a);
+  return done(what);
+}
+
+}  // namespace
+
+extern "C" {
+
+int xtc_hip_mx4_desc_size(void) { return (int)sizeof(xtc_hip_mx4_desc); }
+int xtc_hip_mx4_matmul_desc_size(void) { return (int)sizeof(xtc_hip_mx4_matmul_desc); }
+
+int xtc_hip_mx4_quantize(const xtc_hip_mx4_desc* desc, const void* x, uint8_t* codes, uint8_t* scales, void* values) {
+  const char* const what = "mx4_quantize";
+  if (check(desc, what)) return 1;
+  if (desc->rows == 0) return 0;
+  if (!x || (!codes && !scales && !values)) return fail("%s: null operand", what);
+  Mx4QuantArgs a = args_of(*desc);
+  a.x = x, a.codes = codes, a.scales = scales, a.values = values;
+  return quantize(*desc, a, what);
+}
+
+int xtc_hip_mx4_encode(const xtc_hip_mx4_desc* desc, const void* x, const uint8_t* scales, uint8_t* codes) {
+  const char* const what = "mx4_encode";
+  if (check(desc, what)) return 1;
+  if (desc->rows == 0) return 0;
+  if (!x || !scales || !codes) return fail("%s: null operand", what);
+  Mx4QuantArgs a = args_of(*desc);
+  a.x = x, a.scales_in = scales, a.codes = codes;
+  return quantize(*desc, a, what);
+}
+
+int xtc_hip_mx4_dequantize(const xtc_hip_mx4_desc* desc, const uint8_t* codes, const uint8_t* scales, void* values) {
+  const char* const what = "mx4_dequantize";
+  if (check(desc, what)) return 1;
+  if (desc->rows == 0) return 0;
+  if (!codes || !scales || !values) return fail("%s: null operand", what);
+  if (!aligned16(codes)) return fail("%s: codes must be 16-byte aligned", what);
+  Mx4QuantArgs a = args_of(*desc);
+  a.codes_in = codes, a.scales_in = scales, a.values = values;
+  a.ldv = a.ldx;
+  if (desc->dtype == XTC_HIP_F32)
+    hipLaunchKernelGGL(mx4_dequantize<float>, grid_of(a), dim3(256), 0, core::pick_stream(desc->stream), a);
+  else
+    hipLaunchKernelGGL(mx4_dequantize<__bf16>, grid_of(a), dim3(256), 0, core::pick_stream(desc->stream), a);
+  return done(what);
+}
+
+int xtc_hip_mx4_matmul(const xtc_hip_mx4_matmul_desc* desc, const uint8_t* a_codes, const uint8_t* a_scales,
+                       const uint8_t* b_codes, const uint8_t* b_scales, const int32_t* sizes, void* c) {
+  const char* const what = "mx4_matmul";
+  if (!core::ready()) return fail("xtc_hip_init not called");
+  if (!desc) return fail("%s: null descriptor", what);
+  const xtc_hip_mx4_matmul_desc& d = *desc;
+  if (d.out_dtype != XTC_HIP_F32 && d.out_dtype != XTC_HIP_BF16) return fail("%s: unsupported result dtype %d", what, d.out_dtype);
+  if (d.E < 0 || d.M < 0 || d.N < 1 || d.blocks < 1)
+    return fail("%s: invalid sizes E=%d M=%d N=%d blocks=%d", what, d.E, d.M, d.N, d.blocks);
+  if (d.E > kMost || d.M > kMost || d.N > kMost || d.blocks > kMost / 32)
+    return fail("%s: sizes E=%d M=%d N=%d blocks=%d are too many", what, d.E, d.M, d.N, d.blocks);
+  if ((d.E > 0) != (sizes != nullptr)) return fail("%s: E=%d groups %s sizes", what, d.E, sizes ? "with" : "without");
+  if (d.ldc && d.ldc < d.N) return fail("%s: row stride %d of c is below its %d columns", what, d.ldc, d.N);
+  if (d.M == 0) return 0;
+  if (!a_codes || !a_scales || !b_codes || !b_scales || !c) return fail("%s: null operand", what);
+  if (!aligned16(a_codes) || !aligned16(b_codes)) return fail("%s: codes must be 16-byte aligned", what);
+  Mx4Args a{};
+  a.a_codes = a_codes, a.a_scales = a_scales, a.b_codes = b_codes, a.b_scales = b_scales, a.sizes = sizes, a.c = c;
+  a.E = d.E > 0 ? d.E : 1, a.M = d.M, a.N = d.N, a.blocks = d.blocks, a.ldc = d.ldc ? d.ldc : d.N;
+  a.tiles_n = (d.N + mx4::BN - 1) / mx4::BN;
+  const int64_t rows = sizes ? most_tiles(d.M, d.E, mx4::BM) : ((int64_t)d.M + mx4::BM - 1) / mx4::BM;
+  if (rows * a.tiles_n < 1 || rows * a.tiles_n >= (int64_t)1 << 31)
+    return fail("%s: %lld workgroups are too many", what, (long long)(rows * a.tiles_n));
+  const dim3 grid((unsigned)(rows * a.tiles_n));
+  if (d.out_dtype == XTC_HIP_F32) hipLaunchKernelGGL(mx4_any<float>, grid, dim3(256), 0, core::pick_stream(d.stream), a);
+  else hipLaunchKernelGGL(mx4_any<__bf16>, grid, dim3(256), 0, core::pick_stream(d.stream), a);
+  return done(what);
+}
+
+}  // extern "C"

@@ -27,6 +27,7 @@
 #include "gemm_f32_lds.hpp"
 #include "gemm_f64.hpp"
 #include "conv_direct.hpp"
+#include "core.hpp"
 #include "mfma_peak.hpp"
 #include "planes_table.hpp"
 #include "registry.hpp"
@@ -2282,6 +2283,24 @@ GemmArgs conv_args(const xtc_hip_conv2d_desc& d, int OH, int OW, const void* inp
 }
 
 }  // namespace
+
+// what the other translation units use (core.hpp)
+namespace xtc_hip {
+namespace core {
+
+int fail(const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof(buf), fmt, ap);
+  va_end(ap);
+  return ::fail("%s", buf);
+}
+bool ready() { return current_state() != nullptr; }
+hipStream_t pick_stream(void* stream) { return ::pick_stream(stream); }
+
+}  // namespace core
+}  // namespace xtc_hip
 
 extern "C" {
 

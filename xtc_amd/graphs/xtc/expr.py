@@ -13,6 +13,15 @@ from typing import Any
 
 from ...itf.data import Tensor, TensorType
 from .data import XTCTensor, XTCTensorType
+from .expert_operators import (
+    XTCOperGroupedMatmul,
+    XTCOperGroupedMatmulGradW,
+    XTCOperGroupedMx4Matmul,
+    XTCOperMx4Codes,
+    XTCOperMx4Dequantize,
+    XTCOperMx4Matmul,
+    XTCOperMx4Scales,
+)
 from .operators import (
     XTCOperator,
     XTCOperBiasAdd,
@@ -198,4 +207,11 @@ OP_EXPRS = {
     "reshape": _op_expr(XTCOperReshape, 1),
     "transpose": _op_expr(XTCOperTranspose, 1),
     "bias_add": _op_expr(XTCOperBiasAdd, 2),
+    "grouped_matmul": _op_expr(XTCOperGroupedMatmul, 3),
+    "grouped_matmul_grad_w": _op_expr(XTCOperGroupedMatmulGradW, 3),
+    "mx4_scales": _op_expr(XTCOperMx4Scales, 1),
+    "mx4_codes": _op_expr(XTCOperMx4Codes, 2),
+    "mx4_dequantize": _op_expr(XTCOperMx4Dequantize, 2),
+    "mx4_matmul": _op_expr(XTCOperMx4Matmul, 4),
+    "grouped_mx4_matmul": _op_expr(XTCOperGroupedMx4Matmul, 5),
 }

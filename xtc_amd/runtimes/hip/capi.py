@@ -23,6 +23,9 @@ __all__ = [
     "Tile",
     "MatmulDesc",
     "Conv2dDesc",
+    "GroupedMatmulDesc",
+    "Mx4Desc",
+    "Mx4MatmulDesc",
     "GemmInstance",
     "lib",
     "check",
@@ -103,6 +106,45 @@ class Conv2dDesc(ctypes.Structure):
         ("stream", ctypes.c_void_p),
         ("relu_threshold_f64", ctypes.c_double),
         ("pad_value_f64", ctypes.c_double),
+    ]
+
+
+class GroupedMatmulDesc(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int),
+        ("out_dtype", ctypes.c_int),
+        ("E", ctypes.c_int),
+        ("T", ctypes.c_int),
+        ("N", ctypes.c_int),
+        ("K", ctypes.c_int),
+        ("ldx", ctypes.c_int),
+        ("ldw", ctypes.c_int),
+        ("ldy", ctypes.c_int),
+        ("trans_w", ctypes.c_int),
+        ("stride_w", ctypes.c_int64),
+        ("stream", ctypes.c_void_p),
+    ]
+
+
+class Mx4Desc(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int),
+        ("rows", ctypes.c_int64),
+        ("K", ctypes.c_int),
+        ("ld", ctypes.c_int),
+        ("stream", ctypes.c_void_p),
+    ]
+
+
+class Mx4MatmulDesc(ctypes.Structure):
+    _fields_ = [
+        ("out_dtype", ctypes.c_int),
+        ("E", ctypes.c_int),
+        ("M", ctypes.c_int),
+        ("N", ctypes.c_int),
+        ("blocks", ctypes.c_int),
+        ("ldc", ctypes.c_int),
+        ("stream", ctypes.c_void_p),
     ]
 
 
@@ -190,8 +232,17 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     ),
     "xtc_hip_cast_f32_to_bf16": (_i, [_vp, _vp, _u64, _vp]),
     "xtc_hip_cast_bf16_to_f32": (_i, [_vp, _vp, _u64, _vp]),
+    "xtc_hip_grouped_matmul": (_i, [ctypes.POINTER(GroupedMatmulDesc), _vp, _vp, _vp, _vp]),
+    "xtc_hip_grouped_matmul_grad_w": (_i, [ctypes.POINTER(GroupedMatmulDesc), _vp, _vp, _vp, _vp]),
+    "xtc_hip_mx4_quantize": (_i, [ctypes.POINTER(Mx4Desc), _vp, _vp, _vp, _vp]),
+    "xtc_hip_mx4_encode": (_i, [ctypes.POINTER(Mx4Desc), _vp, _vp, _vp]),
+    "xtc_hip_mx4_dequantize": (_i, [ctypes.POINTER(Mx4Desc), _vp, _vp, _vp]),
+    "xtc_hip_mx4_matmul": (_i, [ctypes.POINTER(Mx4MatmulDesc), _vp, _vp, _vp, _vp, _vp, _vp]),
     "xtc_hip_matmul_desc_size": (_i, []),
     "xtc_hip_conv2d_desc_size": (_i, []),
+    "xtc_hip_grouped_matmul_desc_size": (_i, []),
+    "xtc_hip_mx4_desc_size": (_i, []),
+    "xtc_hip_mx4_matmul_desc_size": (_i, []),
     "xtc_hip_gemm_instance_count": (_i, []),
     "xtc_hip_gemm_instance_get": (_i, [_i, ctypes.POINTER(GemmInstance)]),
     "xtc_hip_default_tile": (
@@ -255,7 +306,10 @@ def lib() -> ctypes.CDLL:
                 fn.restype = res
                 fn.argtypes = args
             for struct, size_fn in ((MatmulDesc, handle.xtc_hip_matmul_desc_size),
-                                    (Conv2dDesc, handle.xtc_hip_conv2d_desc_size)):
+                                    (Conv2dDesc, handle.xtc_hip_conv2d_desc_size),
+                                    (GroupedMatmulDesc, handle.xtc_hip_grouped_matmul_desc_size),
+                                    (Mx4Desc, handle.xtc_hip_mx4_desc_size),
+                                    (Mx4MatmulDesc, handle.xtc_hip_mx4_matmul_desc_size)):
                 if ctypes.sizeof(struct) != size_fn():
                     raise HipError(f"{struct.__name__} is {ctypes.sizeof(struct)} bytes here but "
                                    f"{size_fn()} in {LIB_PATH.name}: the binding and include/xtc_hip.h differ")

@@ -8,8 +8,9 @@ tensor, hands its bare pointer to payloads, and copies back on demand.
 device (an extension: the reference has no bf16).
 
 `layout` follows the reference's tensor layouts (ndarray.py:70-102): the
-array keeps its logical shape, and with layout [1, 0] (2-D only) the device
-holds the transpose, row-major.  copy_from / numpy take and return the
+array keeps its logical shape, and with layout [1, 0] (2-D) the device holds the
+transpose, row-major, with [0, 2, 1] (3-D, an extension) the transpose of every
+matrix.  copy_from / numpy take and return the
 logical array.
 """
 
@@ -36,8 +37,8 @@ class DeviceArray:
         self.shape = tuple(int(d) for d in shape)
         self.dtype = str(dtype)
         self.layout = None if layout is None or list(layout) == list(range(len(self.shape))) else list(layout)
-        if self.layout is not None and (len(self.shape) != 2 or self.layout != [1, 0]):
-            raise ValueError(f"layout {layout} is not supported (only [1, 0] on 2-D arrays)")
+        if self.layout is not None and (len(self.shape), self.layout) not in ((2, [1, 0]), (3, [0, 2, 1])):
+            raise ValueError(f"layout {layout} is not supported (only [1, 0] on 2-D arrays and [0, 2, 1] on 3-D ones)")
         self.size = int(np.prod(self.shape, dtype=np.int64)) if self.shape else 1
         self.nbytes = self.size * itemsize(self.dtype)
         self.handle: int | None = self.device.memory_allocate(self.nbytes)
@@ -65,14 +66,14 @@ class DeviceArray:
         return ctypes.c_void_p(self.data)
 
     def is_transposed(self) -> bool:
-        return self.layout == [1, 0]
+        return self.layout is not None
 
     def copy_from(self, array: np.ndarray) -> None:
         a = np.asarray(array)
         if a.shape != self.shape and a.size != self.size:
             raise ValueError(f"shape {a.shape} does not match device array {self.shape}")
         if self.is_transposed():
-            a = np.ascontiguousarray(a.reshape(self.shape).T)
+            a = np.ascontiguousarray(a.reshape(self.shape).swapaxes(-1, -2))
         if is_bf16(self.dtype):
             host = f32_to_bf16_bits(a.astype(np.float32)).reshape(-1)
         else:
@@ -81,7 +82,7 @@ class DeviceArray:
 
     def numpy(self, out: np.ndarray | None = None) -> np.ndarray:
         """Host copy (float32 values for bf16 arrays)."""
-        stored = self.shape[::-1] if self.is_transposed() else self.shape
+        stored = (*self.shape[:-2], self.shape[-1], self.shape[-2]) if self.is_transposed() else self.shape
         if is_bf16(self.dtype):
             raw = np.empty(self.size, np.uint16)
             self.device.memory_copy_from(self.data, raw.ctypes.data_as(ctypes.c_void_p), self.nbytes)
@@ -90,7 +91,7 @@ class DeviceArray:
             host = np.empty(stored, host_dtype(self.dtype))
             self.device.memory_copy_from(self.data, host.ctypes.data_as(ctypes.c_void_p), self.nbytes)
         if self.is_transposed():
-            host = np.ascontiguousarray(host.T)
+            host = np.ascontiguousarray(host.swapaxes(-1, -2))
         if out is not None:
             out[...] = host
             return out

@@ -213,3 +213,12 @@ def test_graph_file_round_trip(tmp_path):
         O.graph.load(tmp_path / "g.yaml")
     a = np.random.default_rng(4).normal(size=(4, 64)).astype(np.float32)
     np.testing.assert_array_equal(forward(again.graph, a)[0], forward(gb.graph, a)[0])
+
+
+def test_equal_graphs_make_equal_payloads():
+    """Unnamed nodes do not tell two builds of one graph apart."""
+    def source():
+        backend = Backend(build(lambda x: O.mx4_matmul(*O.mx4_quantize(x), *O.mx4_quantize(x)), ((4, 64), F)))
+        return backend.get_compiler().compile(backend.get_scheduler().schedule()).source
+
+    assert source() == source()

@@ -247,3 +247,27 @@ def test_no_rows():
     assert not got.any()
     for p in (sizes, dw):
         dev.memory_free(p)
+
+
+# grids large enough for the 128 x 128 and the 256 x 256 tiles, cut in every
+# direction: rows and columns inside a tile, K inside a slab, one slab and fewer
+# slabs than stages, groups of one row and of none
+@pytest.mark.parametrize("out", ["float32", "bfloat16"])
+@pytest.mark.parametrize("T,N", [(1500, 2056), (4100, 3336)])
+@pytest.mark.parametrize("K", [8, 32, 72, 136, 200])
+def test_large_tiles(out, T, N, K):
+    sizes = [T // 3, 1, 0, T // 5, 257, T // 4]
+    x, w = ints(21, (T, K), 3), ints(22, (6, K, N), 3)
+    print(f"[experts tiles] {out} {T}x{K}x{N}", flush=True)
+    want = rounded(plain_grouped(x, w, sizes), out)
+    for trans in (False, True):
+        np.testing.assert_array_equal(grouped(x, w, sizes, "bfloat16", out, trans), want)
+
+
+@pytest.mark.parametrize("out", ["float32", "bfloat16"])
+@pytest.mark.parametrize("K,N,sizes", [(904, 776, [70, 0, 33, 1, 8, 129]), (1544, 1800, [32, 300, 0, 5, 97])])
+def test_large_gradient_tiles(out, K, N, sizes):
+    T = sum(sizes) + 6
+    x, dy = ints(23, (T, K), 3), ints(24, (T, N), 3)
+    print(f"[experts gradient tiles] {out} {T}x{K}x{N}", flush=True)
+    np.testing.assert_array_equal(grad_w(x, dy, sizes, "bfloat16", out), rounded(plain_grad_w(x, dy, sizes), out))

@@ -221,3 +221,19 @@ def test_same_results_every_time_on_any_stream():
         for s in (None, stream, stream):
             np.testing.assert_array_equal(mx4_matmul(*a, *b, stream=s), first)
     capi.check(L.xtc_hip_stream_destroy(stream))
+
+
+# grids large enough for the 128 x 128 and the 256 x 256 tiles, cut in rows and
+# columns, with fewer slabs than stages and more
+@pytest.mark.parametrize("out", ["float32", "bfloat16"])
+@pytest.mark.parametrize("M,N", [(1500, 2056), (4100, 3336)])
+@pytest.mark.parametrize("nb", [4, 8, 20, 36])
+def test_large_tiles(out, M, N, nb):
+    print(f"[mx4 tiles] {out} {M}x{N} blocks {nb}", flush=True)
+    a, b = operand(15, (M,), nb), operand(16, (N,), nb)
+    want, spread = plain(*a, *b, None)
+    check_product(mx4_matmul(*a, *b, out_dtype=out), want, spread, 32 * nb, out)
+    sizes = [M // 3, 1, 0, M // 5, 257, M // 4]
+    b = operand(17, (6, N), nb)
+    want, spread = plain(*a, *b, sizes)
+    check_product(mx4_matmul(*a, *b, sizes=sizes, out_dtype=out), want, spread, 32 * nb, out)

@@ -218,8 +218,11 @@ def _emit_split_matmul(plan: Plan, ln: Launch, cfg: SplitConfig) -> list[str]:
 def _emit_launch(plan: Plan, ln: Launch, cfg: GemmConfig | SplitConfig | None, idx: int) -> list[str]:
     a = ln.attrs
     dst = _ptr(plan, ln.output)
-    where = f'"{ln.kind} {ln.node}"'
-    lines: list[str] = [f"  /* {ln.kind} {ln.node}{' + ' + ', '.join(ln.absorbed) if ln.absorbed else ''} */"]
+    names = [ln.node, *ln.absorbed]
+    if ln.kind.startswith(("grouped_", "mx4_")):
+        names = [_label(plan, n) for n in names]
+    where = f'"{ln.kind} {names[0]}"'
+    lines: list[str] = [f"  /* {ln.kind} {names[0]}{' + ' + ', '.join(names[1:]) if ln.absorbed else ''} */"]
     if isinstance(cfg, SplitConfig):
         assert ln.kind == "matmul"
         return lines + _emit_split_matmul(plan, ln, cfg)
@@ -324,6 +327,13 @@ def _emit_launch(plan: Plan, ln: Launch, cfg: GemmConfig | SplitConfig | None, i
     else:
         raise ScheduleError(f"no code generator for launch kind {ln.kind}")
     return lines
+
+
+def _label(plan: Plan, node: str) -> str:
+    """The node's name; an unnamed one's uid counts from the graph's first
+    input, as in a graph file, so that equal graphs make equal sources."""
+    uids = [int(u[1:]) for u in (node, *plan.args[:1]) if u[:1] == "%" and u[1:].isdigit()]
+    return f"%{uids[0] - uids[1]}" if len(uids) == 2 and node[:1] == "%" else node
 
 
 def _cc() -> str:

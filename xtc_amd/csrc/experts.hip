@@ -3,6 +3,7 @@
 #include "xtc_hip.h"
 #include "core.hpp"
 #include "grouped_any.hpp"
+#include "grouped_dma.hpp"
 
 using namespace xtc_hip;
 using core::fail;
@@ -29,6 +30,47 @@ int stride(int given, int dense, const char* what, const char* name, int* out) {
   *out = given ? given : dense;
   if (*out < dense) return fail("%s: row stride %d of %s is below its %d columns", what, given, name, dense);
   return 0;
+}
+
+// ---- bf16 in whole vectors
+
+typedef void (*DmaLaunch)(const DmaArgs&, unsigned, hipStream_t);
+template <bool GRAD, bool B_ROW, int WGM, int WGN, int TM, int TN, int STAGES, bool PP>
+void dma_launch(const DmaArgs& a, unsigned groups, hipStream_t s) {
+  hipLaunchKernelGGL((grouped_dma<false, GRAD, B_ROW, WGM, WGN, TM, TN, STAGES, PP>), dim3(groups), dim3(WGM * WGN * 64), 0, s, a);
+}
+struct DmaTile {
+  int bm, bn;
+  DmaLaunch natural, transposed, grad;
+};
+#define XTC_DMA(...) &dma_launch<false, false, __VA_ARGS__>, &dma_launch<false, true, __VA_ARGS__>, &dma_launch<true, false, __VA_ARGS__>
+const DmaTile kDmaTiles[] = {
+    {256, 256, XTC_DMA(2, 4, 8, 4, 4, true)},
+    {128, 128, XTC_DMA(2, 2, 4, 4, 4, false)},
+    {64, 64, XTC_DMA(2, 2, 2, 2, 4, false)},
+};
+#undef XTC_DMA
+
+// Strides of whole vectors whose offsets within a tile stay within 2^31 bytes.
+bool vectors(const void* p, int ld) { return core::aligned16(p) && ld % 8 == 0 && ld < (1 << 22); }
+
+const DmaTile* dma_tile(int64_t rows, int64_t groups, int N, bool grad, int K) {
+  for (const DmaTile& t : kDmaTiles) {
+    const int64_t tn = (N + t.bn - 1) / t.bn;
+    const int64_t tm = grad ? groups * ((K + t.bm - 1) / t.bm) : rows / t.bm + 1;
+    if (tm * tn >= 192) return &t;
+  }
+  return &kDmaTiles[2];
+}
+
+int launch_dma(const DmaTile& t, DmaLaunch run, DmaArgs& a, int64_t matrices, hipStream_t s) {
+  a.tiles_n = (a.N + t.bn - 1) / t.bn;
+  a.band = a.tiles_m < 8 ? a.tiles_m : 8;
+  const int64_t groups = dma_groups(a, matrices);
+  if (groups < 1 || groups >= (int64_t)1 << 31) return fail("grouped_matmul: %lld workgroups are too many", (long long)groups);
+  run(a, (unsigned)groups, s);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? 0 : fail("grouped_matmul: launch failed: %s", hipGetErrorString(e));
 }
 
 template <bool GRAD>
@@ -71,6 +113,17 @@ int xtc_hip_grouped_matmul(const xtc_hip_grouped_matmul_desc* desc, const void* 
   const int64_t matrix = (int64_t)(d.trans_w ? d.N : d.K) * a.ldw;
   a.stride_w = d.stride_w ? d.stride_w : matrix;
   if (a.stride_w < 0) return fail("%s: negative stride between matrices", what);
+  if (d.dtype == XTC_HIP_BF16 && d.K % 8 == 0 && (d.trans_w || d.N % 8 == 0) && vectors(x, a.ldx) && vectors(w, a.ldw) &&
+      a.stride_w % 8 == 0) {
+    const DmaTile& t = *dma_tile(d.T, d.E, d.N, false, d.K);
+    DmaArgs v{};
+    v.a = (const uint8_t*)x, v.b = (const uint8_t*)w, v.sizes = sizes, v.c = y;
+    v.stride_b = 2 * a.stride_w;
+    v.E = d.E, v.M = d.T, v.N = d.N, v.K = d.K / 8;
+    v.lda = 2 * a.ldx, v.ldb = 2 * a.ldw, v.ldc = a.ldy, v.out16 = d.out_dtype == XTC_HIP_BF16;
+    v.tiles_m = (int)most_tiles(d.T, d.E, t.bm);
+    return launch_dma(t, d.trans_w ? t.transposed : t.natural, v, 1, core::pick_stream(d.stream));
+  }
   a.tiles_n = (d.N + gany::BN - 1) / gany::BN;
   return launch_any<false>(d, a, most_tiles(d.T, d.E, gany::BM) * a.tiles_n, core::pick_stream(d.stream));
 }
@@ -91,6 +144,16 @@ int xtc_hip_grouped_matmul_grad_w(const xtc_hip_grouped_matmul_desc* desc, const
   const int64_t matrix = (int64_t)d.K * a.ldy;
   a.stride_y = d.stride_w ? d.stride_w : matrix;
   if (a.stride_y < matrix) return fail("%s: a stride of %lld lets the gradients of two groups overlap", what, (long long)d.stride_w);
+  if (d.dtype == XTC_HIP_BF16 && d.K % 8 == 0 && d.N % 8 == 0 && vectors(x, a.ldx) && vectors(dy, a.ldw)) {
+    const DmaTile& t = *dma_tile(d.T, d.E, d.N, true, d.K);
+    DmaArgs v{};
+    v.a = (const uint8_t*)x, v.b = (const uint8_t*)dy, v.sizes = sizes, v.c = dw;
+    v.stride_c = a.stride_y;
+    v.E = d.E, v.M = d.T, v.N = d.N, v.K = d.K;
+    v.lda = 2 * a.ldx, v.ldb = 2 * a.ldw, v.ldc = a.ldy, v.out16 = d.out_dtype == XTC_HIP_BF16;
+    v.tiles_m = (d.K + t.bm - 1) / t.bm;
+    return launch_dma(t, t.grad, v, d.E, core::pick_stream(d.stream));
+  }
   a.tiles_n = (d.N + gany::BN - 1) / gany::BN;
   a.tiles_k = (d.K + gany::BM - 1) / gany::BM;
   return launch_any<true>(d, a, (int64_t)d.E * a.tiles_k * a.tiles_n, core::pick_stream(d.stream));

@@ -1,0 +1,400 @@
+// SPDX-License-Identifier: BSD-3-Clause
+// Products by group of bf16 or microscaled 4-bit operands in whole 16-byte
+// vectors, staged through LDS by DMA:
+//   C[i, j] = sum_k A[i, k] B[k, j]
+// for the rows i of a group and its matrix B, or (GRAD) over the rows k of a
+// group: see grouped_any.hpp and mx4_any.hpp, which take what this kernel does
+// not.
+//
+// Tile and slab.  A workgroup of WGM x WGN waves computes (16 WGM TM) x
+// (16 WGN TN) outputs, k in slabs of 64 bytes a row: 32 bf16 or 128 4-bit
+// elements, one v_mfma_f32_16x16x32_bf16 or v_mfma_scale_f32_16x16x128_f8f6f4
+// deep.  Both take 16 bytes of a row a lane and 16 cycles, so one kernel feeds
+// both.  B is the first MFMA operand: a lane ends with four neighbouring
+// columns of one row.
+//
+// Operands come in two forms.
+//   ROW  k contiguous: staged [rows][64 B], its 16-byte chunk c of row r at
+//        c ^ ((r >> 1) & 3), read by ds_read_b128.
+//   COL  k strided (bf16): staged [32 k][16-bit columns], its 32-byte chunk c of
+//        row k at c ^ swz(k), read transposed by ds_read_b64_tr_b16.
+// 4-bit operands bring 4 scale bytes a row and slab, staged [rows][4].
+//
+// Edges cost nothing in the loop: every DMA goes through a buffer descriptor
+// that ends where the tile's rows end, and what lies past it arrives in LDS as
+// zeros.  Only a slab cut by K within ROW rows needs a lane to give up its chunk
+// (an offset past the descriptor's end).  Rows and columns past the tile's edge
+// hold zeros or neighbours and are not stored.
+//
+// Schedules.  PP ("ping-pong", 2 x 4 waves, one workgroup a CU): two groups of
+// four waves, one of each on every SIMD, run half a step apart, so that one
+// computes while the other reads LDS; the barriers and waits are those of
+// gemm_bf16_pingpong.hpp.  Otherwise the plain loop: wait for the slab, barrier,
+// start the DMA of the slab STAGES - 1 ahead, read, compute; several workgroups
+// share a CU and fill each other's gaps.
+//
+// Raster.  Tiles run in bands of (at most 8) tile rows, down the band first;
+// 4 columns of a band go to one XCD (workgroups reach the XCDs in turn), whose
+// 32 CUs then share 8 panels of A and 4 of B in its L2.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "gemm_bf16_pingpong.hpp"
+#include "groups.hpp"
+
+namespace xtc_hip {
+
+struct DmaArgs {
+  const uint8_t* a;   // ROW: [M] rows; GRAD: x, [M] rows of K columns
+  const uint8_t* b;   // matrices of E groups, stride_b bytes apart; GRAD: dy
+  const uint8_t* sa;  // scales of 4-bit operands, `slabs` dwords a row
+  const uint8_t* sb;
+  const int* sizes;   // null: one group of all rows
+  void* c;
+  int64_t stride_b, stride_sb;  // bytes
+  int64_t stride_c;             // elements (GRAD)
+  int E, M, N;        // groups, rows in all, columns of C
+  int K;              // GRAD: rows of C; otherwise 16-byte chunks of a row of A
+  int lda, ldb;       // bytes
+  int ldc;            // elements
+  int tiles_m, tiles_n;  // tiles_m: of all groups (at most), GRAD: of one C
+  int band;           // tile rows of a band
+  int out16;          // C is bf16
+};
+
+namespace gdma {
+
+using big::bf16x8;
+using big::f32x4;
+using big::i16x4;
+using big::lds_i16x4;
+using big::lds_u32x4;
+using big::u32x4;
+using big::waitcnt_vm;
+using pingpong::phase_barrier;
+using pingpong::waitcnt_lgkm0;
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+
+constexpr unsigned PAST = 0x80000000u;  // an offset past every descriptor's end
+
+// Buffer descriptor of `bytes` (clamped to 0 .. 2^31 - 1) from p.
+__device__ __forceinline__ u32x4 descriptor(const uint8_t* p, int64_t bytes) {
+  const uint64_t at = (uint64_t)p;
+  const int64_t n = bytes < 0 ? 0 : bytes > 0x7fffffff ? 0x7fffffff : bytes;
+  return u32x4{(unsigned)at, (unsigned)(at >> 32) & 0xffffu, (unsigned)n, 0x00020000u};
+}
+
+// 16 (or 4) bytes a lane from descriptor r at `off` to lds + 16 (4) lane; zeros
+// where off passes the descriptor's end.  Issued from asm, as in lds_dma.hpp; the
+// wait states cover M0 and a descriptor written right before.
+__device__ __forceinline__ unsigned lds_address(const void* p) {
+  typedef __attribute__((address_space(3))) void lds_void_t;
+  return __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(lds_void_t*)p);
+}
+__device__ __forceinline__ void dma16(u32x4 r, unsigned off, void* lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(r), "s"(lds_address(lds))
+               : "memory", "m0");
+}
+__device__ __forceinline__ void dma4(u32x4 r, unsigned off, void* lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(off), "s"(r), "s"(lds_address(lds))
+               : "memory", "m0");
+}
+
+__device__ __forceinline__ int swz_row(int r) { return (r >> 1) & 3; }
+template <int COLS>
+__device__ __forceinline__ int swz_col(int k) {
+  return COLS >= 128 ? ((k & 3) | ((k >> 1) & 4)) : (k & 3);
+}
+
+// Where lane `lane` finds its 16 bytes of KB `kb` of an operand's stage: bytes
+// from the operand's tile corner.
+template <bool ROW, int LEN>
+__device__ __forceinline__ unsigned source(int kb, int lane, int ld) {
+  if constexpr (ROW) {
+    const int r = kb * 16 + (lane >> 2);
+    return (unsigned)r * (unsigned)ld + (unsigned)(((lane & 3) ^ swz_row(r)) * 16);
+  } else {
+    constexpr int SLOTS = LEN / 8, PER = 64 / SLOTS;  // 16-byte slots of a k row, k rows of a KB
+    const int k = kb * PER + lane / SLOTS, slot = lane % SLOTS;
+    return (unsigned)k * (unsigned)ld + (unsigned)(((slot >> 1) ^ swz_col<LEN>(k)) * 32 + (slot & 1) * 16);
+  }
+}
+
+// Fragment `f` (16 rows or columns from f0) of an operand's stage.
+template <bool ROW, int LEN>
+__device__ __forceinline__ u32x4 fragment(const unsigned char* st, int f0, int f, int l16, int g) {
+  if constexpr (ROW) {
+    const int r = (f0 + f) * 16 + l16;
+    return *(const lds_u32x4*)(st + r * 64 + 16 * (g ^ swz_row(l16)));
+  } else {
+    const int k = 8 * g + (l16 >> 2);
+    const unsigned char* p = st + k * (2 * LEN) + 32 * ((f0 + f) ^ swz_col<LEN>(k)) + 8 * (l16 & 3);
+    const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)p);
+    const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(p + 8 * LEN));
+    return __builtin_bit_cast(u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+}
+
+template <bool MX>
+__device__ __forceinline__ f32x4 mfma(u32x4 b, int sb, u32x4 a, int sa, f32x4 c) {
+  if constexpr (MX) {
+    const i32x8 bv = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
+    const i32x8 av = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(bv, av, c, 4, 4, 0, sb, 0, sa);
+  } else {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b), __builtin_bit_cast(bf16x8, a), c, 0, 0, 0);
+  }
+}
+
+// columns n .. n+3 (those below `cols`) of a row
+__device__ __forceinline__ void store4(void* c, int out16, int64_t at, f32x4 v, int n, int cols, bool whole) {
+  if (out16) {
+    __bf16* p = (__bf16*)c + at + n;
+    const bf16x4 h = __builtin_convertvector(v, bf16x4);
+    if (whole && n + 4 <= cols) *(bf16x4*)p = h;
+    else
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (n + i < cols) p[i] = h[i];
+  } else {
+    float* p = (float*)c + at + n;
+    if (whole && n + 4 <= cols) *(f32x4*)p = v;
+    else
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (n + i < cols) p[i] = v[i];
+  }
+}
+
+}  // namespace gdma
+
+template <bool MX, bool GRAD, bool B_ROW, int WGM, int WGN, int TM, int TN, int STAGES, bool PP>
+__global__ void __launch_bounds__(WGM* WGN * 64) grouped_dma(DmaArgs p) {
+  using namespace gdma;
+  constexpr bool A_ROW = !GRAD;
+  constexpr int WAVES = WGM * WGN, BM = WGM * TM * 16, BN = WGN * TN * 16;
+  constexpr int A_KB = BM / 16, B_KB = BN / 16, PER = (A_KB + B_KB) / WAVES;  // DMA kilobytes
+  constexpr int SA_N = MX ? (BM + 63) / 64 : 0, SB_N = MX ? (BN + 63) / 64 : 0, S_PER = (SA_N + SB_N + WAVES - 1) / WAVES;
+  constexpr int DMA = PER + S_PER;  // DMA instructions a wave and slab
+  constexpr int A_AT = 0, B_AT = BM * 64, SA_AT = B_AT + BN * 64, SB_AT = SA_AT + SA_N * 256, STAGE = SB_AT + SB_N * 256;
+  constexpr int D = STAGES - 1;
+  static_assert(PER * WAVES == A_KB + B_KB, "a slab splits evenly over the waves");
+  static_assert(!MX || (B_ROW && !GRAD), "4-bit operands have k along their rows");
+  static_assert(!PP || (WGM == 2 && WGN == 4), "two groups of four waves");
+  static_assert(STAGES * STAGE <= 160 * 1024 && D * DMA < 64, "LDS and wait counts");
+
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[STAGES * STAGE];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / WGN, wn = wave % WGN;
+  const int l16 = lane & 15, g = lane >> 4;
+
+  // ---- the workgroup's tile
+  const int slot = blockIdx.x >> 3, run = 4 * p.band;  // run: tiles that follow one another on an XCD
+  const int t = (slot / run * 8 + (blockIdx.x & 7)) * run + slot % run;
+  const int per_matrix = (p.tiles_m + p.band - 1) / p.band * p.band * p.tiles_n;
+  const int e_grad = GRAD ? t / per_matrix : 0;
+  const int tt = GRAD ? t - e_grad * per_matrix : t;
+  const int in_band = tt % (p.band * p.tiles_n);
+  const int mt = tt / (p.band * p.tiles_n) * p.band + in_band % p.band, n0 = in_band / p.band * BN;
+  if (mt >= p.tiles_m || (GRAD && e_grad >= p.E)) return;
+
+  const uint8_t *a, *b;        // tile corners
+  const uint8_t *as = nullptr, *bs = nullptr;
+  int64_t a_left, b_left;      // bytes from there to the operand's end
+  int64_t as_left = 0, bs_left = 0;
+  int64_t a_step, b_step;      // bytes from a slab to the next
+  int64_t c_at;                // element of C at the tile's corner
+  int rows, nk, chunks = 0;    // rows of C, slabs, 16-byte chunks of a ROW row
+  const int cols = p.N - n0;
+  if constexpr (GRAD) {
+    const RowGroup gr = find_group(p.sizes, p.E, p.M, e_grad);
+    const int m0 = mt * BM, depth = gr.end - gr.begin;
+    rows = p.K - m0;
+    nk = (depth + 31) / 32;
+    a = p.a + (int64_t)gr.begin * p.lda + 2 * m0;
+    b = p.b + (int64_t)gr.begin * p.ldb + 2 * n0;
+    a_left = (int64_t)(depth - 1) * p.lda + 2 * rows;
+    b_left = (int64_t)(depth - 1) * p.ldb + 2 * cols;
+    a_step = (int64_t)32 * p.lda;
+    b_step = (int64_t)32 * p.ldb;
+    c_at = (int64_t)e_grad * p.stride_c + (int64_t)m0 * p.ldc + n0;
+  } else {
+    RowGroup gr{0, mt * BM, p.M};
+    if (p.sizes) gr = find_tile<BM>(p.sizes, p.E, p.M, mt);
+    if (gr.e < 0) return;
+    const int e = gr.e < p.E ? gr.e : 0;
+    rows = min(gr.end - gr.begin, BM);
+    chunks = gr.e < p.E ? p.K : 0;  // rows of no group: zeros
+    nk = (chunks + 3) / 4;
+    a = p.a + (int64_t)gr.begin * p.lda;
+    a_left = (int64_t)(rows - 1) * p.lda + 16 * (int64_t)chunks;
+    a_step = 64;
+    const uint8_t* m = p.b + e * p.stride_b;
+    if constexpr (B_ROW) {
+      b = m + (int64_t)n0 * p.ldb;
+      b_left = (int64_t)(min(cols, BN) - 1) * p.ldb + 16 * (int64_t)chunks;
+      b_step = 64;
+    } else {
+      b = m + 2 * n0;
+      b_left = (int64_t)(8 * chunks - 1) * p.ldb + 2 * cols;
+      b_step = (int64_t)32 * p.ldb;
+    }
+    if constexpr (MX) {
+      as = p.sa + (int64_t)gr.begin * 4 * nk;
+      as_left = (int64_t)rows * 4 * nk;
+      bs = p.sb + e * p.stride_sb + (int64_t)n0 * 4 * nk;
+      bs_left = (int64_t)min(cols, BN) * 4 * nk;
+    }
+    c_at = (int64_t)gr.begin * p.ldc + n0;
+  }
+
+  // ---- this wave's share of a slab's DMA
+  unsigned off[PER];
+  int chunk[PER];  // ROW: chunk of the slab that the lane loads
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int kb = wave * PER + i;
+    if (kb < A_KB) {
+      off[i] = source<A_ROW, BM>(kb, lane, p.lda);
+      chunk[i] = A_ROW ? (lane & 3) ^ swz_row(kb * 16 + (lane >> 2)) : 0;
+    } else {
+      off[i] = source<B_ROW, BN>(kb - A_KB, lane, p.ldb);
+      chunk[i] = B_ROW ? (lane & 3) ^ swz_row((kb - A_KB) * 16 + (lane >> 2)) : 0;
+    }
+  }
+  // K stagger: tiles that share a panel start their walk at different slabs
+  const int kofs = nk > 0 ? ((mt + 2 * (n0 / BN)) & 15) % nk : 0;
+
+  auto issue = [&](int kt, unsigned char* st) {
+    int kr = kt + kofs;
+    kr = kr >= nk ? kr - nk : kr;
+    const u32x4 ra = descriptor(a + kr * a_step, a_left - kr * a_step);
+    const u32x4 rb = descriptor(b + kr * b_step, b_left - kr * b_step);
+    const int left = GRAD ? 4 : chunks - 4 * kr;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int kb = wave * PER + i;
+      const bool is_a = kb < A_KB;
+      unsigned o = off[i];
+      if (A_ROW && left < 4 && chunk[i] >= left) o = PAST;
+      dma16(is_a ? ra : rb, o, st + kb * 1024);
+    }
+    if constexpr (MX) {
+#pragma unroll
+      for (int i = 0; i < S_PER; ++i) {
+        const int kb = min(wave * S_PER + i, SA_N + SB_N - 1);  // a wave without a share repeats the last
+        const bool is_a = kb < SA_N;
+        const u32x4 r = is_a ? descriptor(as + 4 * kr, as_left - 4 * kr) : descriptor(bs + 4 * kr, bs_left - 4 * kr);
+        dma4(r, (unsigned)((is_a ? kb : kb - SA_N) * 64 + lane) * 4u * (unsigned)nk, st + SA_AT + kb * 256);
+      }
+    }
+  };
+
+  f32x4 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  u32x4 fa[TM], fb[TN];
+  int ha[TM], hb[TN];
+  auto read = [&](const unsigned char* st) {
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      fa[i] = fragment<A_ROW, BM>(st + A_AT, wm * TM, i, l16, g);
+      ha[i] = MX ? st[SA_AT + ((wm * TM + i) * 16 + l16) * 4 + g] : 0;
+    }
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      fb[j] = fragment<B_ROW, BN>(st + B_AT, wn * TN, j, l16, g);
+      hb[j] = MX ? st[SB_AT + ((wn * TN + j) * 16 + l16) * 4 + g] : 0;
+    }
+  };
+  auto mma = [&]() {
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) acc[i][j] = mfma<MX>(fb[j], hb[j], fa[i], ha[i], acc[i][j]);
+  };
+
+  if (nk > 0) {
+#pragma unroll
+    for (int s = 0; s < D; ++s)
+      if (s < nk) issue(s, lds + s * STAGE);
+    if constexpr (PP) {
+      // this wave's DMA of slab t+1 has landed (slabs through min(t+D, nk-1) issued)
+      auto wait_next = [&](int kt) {
+        if (kt + D < nk)
+          __builtin_amdgcn_s_waitcnt(waitcnt_vm((D - 1) * DMA));
+        else
+          __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+      };
+      const int group = wm;
+      if (nk >= D)
+        __builtin_amdgcn_s_waitcnt(waitcnt_vm((D - 1) * DMA));
+      else
+        __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+      phase_barrier();
+      if (group == 1) phase_barrier();
+      auto step = [&](int kt, const int s) {
+        // ---- memory phase
+        if (kt + D < nk) issue(kt + D, lds + (s + D) % STAGES * STAGE);
+        read(lds + s * STAGE);
+        __builtin_amdgcn_s_waitcnt(waitcnt_lgkm0());
+        if (group == 1) wait_next(kt);
+        phase_barrier();
+        // ---- compute phase
+        mma();
+        if (group == 0) wait_next(kt);
+        if (group == 0 || kt + 1 < nk) phase_barrier();
+      };
+      for (int kt = 0; kt < nk; kt += STAGES) {
+#pragma unroll
+        for (int s = 0; s < STAGES; ++s)
+          if (kt + s < nk) step(kt + s, s);
+      }
+    } else {
+      for (int kt = 0; kt < nk; kt += STAGES) {
+#pragma unroll
+        for (int s = 0; s < STAGES; ++s) {
+          if (kt + s >= nk) break;
+          // slab kt+s has landed; the ones after it may be in flight
+          if (kt + s + D - 1 < nk)
+            __builtin_amdgcn_s_waitcnt(waitcnt_vm((D - 1) * DMA));
+          else
+            __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+          // everyone has read slab kt+s-1, whose stage the DMA now fills
+          phase_barrier();
+          if (kt + s + D < nk) issue(kt + s + D, lds + (s + D) % STAGES * STAGE);
+          read(lds + s * STAGE);
+          mma();
+        }
+      }
+    }
+  }
+
+  // ---- a lane holds C[m][n .. n+3] of each 16 x 16
+  const bool whole = (p.ldc & 3) == 0 && ((uintptr_t)p.c & (p.out16 ? 7 : 15)) == 0 && (!GRAD || (p.stride_c & 3) == 0);
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+    const int m = (wm * TM + i) * 16 + l16;
+    if (m >= rows) continue;
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+      store4(p.c, p.out16, c_at + (int64_t)m * p.ldc, acc[i][j], (wn * TN + j) * 16 + 4 * g, cols, whole);
+  }
+}
+
+// Workgroups of `a` (its tiles and band set): bands and runs filled up.
+inline int64_t dma_groups(const DmaArgs& a, int64_t matrices) {
+  const int64_t per_matrix = ((int64_t)a.tiles_m + a.band - 1) / a.band * a.band * a.tiles_n;
+  const int64_t whole = (int64_t)8 * 4 * a.band;
+  return (matrices * per_matrix + whole - 1) / whole * whole;
+}
+
+}  // namespace xtc_hip

@@ -2,6 +2,7 @@
 // Entry points of the microscaled 4-bit operators.
 #include "xtc_hip.h"
 #include "core.hpp"
+#include "grouped_dma.hpp"
 #include "mx4_any.hpp"
 
 using namespace xtc_hip;
@@ -46,6 +47,28 @@ int quantize(const xtc_hip_mx4_desc& d, const Mx4QuantArgs& a, const char* what)
   else
     hipLaunchKernelGGL(mx4_quantize<__bf16>, grid_of(a), dim3(256), 0, core::pick_stream(d.stream), a);
   return done(what);
+}
+
+// ---- products of whole slabs (4 blocks)
+
+struct DmaTile {
+  int bm, bn;
+  void (*launch)(const DmaArgs&, unsigned, hipStream_t);
+};
+template <int WGM, int WGN, int TM, int TN, int STAGES, bool PP>
+void dma_launch(const DmaArgs& a, unsigned groups, hipStream_t s) {
+  hipLaunchKernelGGL((grouped_dma<true, false, true, WGM, WGN, TM, TN, STAGES, PP>), dim3(groups), dim3(WGM * WGN * 64), 0, s, a);
+}
+const DmaTile kDmaTiles[] = {
+    {256, 256, &dma_launch<2, 4, 8, 4, 4, true>},
+    {128, 128, &dma_launch<2, 2, 4, 4, 4, false>},
+    {64, 64, &dma_launch<2, 2, 2, 2, 4, false>},
+};
+
+const DmaTile& dma_tile(int64_t rows, int N) {
+  for (const DmaTile& t : kDmaTiles)
+    if ((rows / t.bm + 1) * ((N + t.bn - 1) / t.bn) >= 192) return t;
+  return kDmaTiles[2];
 }
 
 }  // namespace
@@ -110,6 +133,22 @@ int xtc_hip_mx4_matmul(const xtc_hip_mx4_matmul_desc* desc, const uint8_t* a_cod
   Mx4Args a{};
   a.a_codes = a_codes, a.a_scales = a_scales, a.b_codes = b_codes, a.b_scales = b_scales, a.sizes = sizes, a.c = c;
   a.E = d.E > 0 ? d.E : 1, a.M = d.M, a.N = d.N, a.blocks = d.blocks, a.ldc = d.ldc ? d.ldc : d.N;
+  if (d.blocks % 4 == 0 && d.blocks < (1 << 19) && ((uintptr_t)a_scales & 3) == 0 && ((uintptr_t)b_scales & 3) == 0) {
+    const DmaTile& t = dma_tile(d.M, d.N);
+    DmaArgs v{};
+    v.a = a_codes, v.b = b_codes, v.sa = a_scales, v.sb = b_scales, v.sizes = sizes, v.c = c;
+    v.E = a.E, v.M = d.M, v.N = d.N, v.K = d.blocks;
+    v.lda = v.ldb = 16 * d.blocks, v.ldc = a.ldc;
+    v.stride_b = (int64_t)d.N * v.ldb, v.stride_sb = (int64_t)d.N * d.blocks;
+    v.tiles_m = (int)(sizes ? most_tiles(d.M, d.E, t.bm) : ((int64_t)d.M + t.bm - 1) / t.bm);
+    v.tiles_n = (d.N + t.bn - 1) / t.bn;
+    v.band = v.tiles_m < 8 ? v.tiles_m : 8;
+    v.out16 = d.out_dtype == XTC_HIP_BF16;
+    const int64_t groups = dma_groups(v, 1);
+    if (groups >= (int64_t)1 << 31) return fail("%s: %lld workgroups are too many", what, (long long)groups);
+    t.launch(v, (unsigned)groups, core::pick_stream(d.stream));
+    return done(what);
+  }
   a.tiles_n = (d.N + mx4::BN - 1) / mx4::BN;
   const int64_t rows = sizes ? most_tiles(d.M, d.E, mx4::BM) : ((int64_t)d.M + mx4::BM - 1) / mx4::BM;
   if (rows * a.tiles_n < 1 || rows * a.tiles_n >= (int64_t)1 << 31)

@@ -18,7 +18,9 @@
 //        c ^ ((r >> 1) & 3), read by ds_read_b128.
 //   COL  k strided (bf16): staged [32 k][16-bit columns], its 32-byte chunk c of
 //        row k at c ^ swz(k), read transposed by ds_read_b64_tr_b16.
-// 4-bit operands bring 4 scale bytes a row and slab, staged [rows][4].
+// 4-bit operands bring 4 scale bytes a row and slab.  They are staged for four
+// slabs at a time, [rows][16], a quarter of the rows with each slab, one group
+// ahead: 4 bytes of each row a slab would touch as many cache lines as the codes.
 //
 // Edges cost nothing in the loop: every DMA goes through a buffer descriptor
 // that ends where the tile's rows end, and what lies past it arrives in LDS as
@@ -177,16 +179,20 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_dma(DmaArgs p) {
   constexpr bool A_ROW = !GRAD;
   constexpr int WAVES = WGM * WGN, BM = WGM * TM * 16, BN = WGN * TN * 16;
   constexpr int A_KB = BM / 16, B_KB = BN / 16, PER = (A_KB + B_KB) / WAVES;  // DMA kilobytes
-  constexpr int SA_N = MX ? (BM + 63) / 64 : 0, SB_N = MX ? (BN + 63) / 64 : 0, S_PER = (SA_N + SB_N + WAVES - 1) / WAVES;
+  constexpr int S_ALL = MX ? (BM + BN) / 16 : 0;  // scale DMA of four slabs: 16 rows each
+  constexpr int S_PER = (S_ALL + 4 * WAVES - 1) / (4 * WAVES);  // a wave's with each slab
   constexpr int DMA = PER + S_PER;  // DMA instructions a wave and slab
-  constexpr int A_AT = 0, B_AT = BM * 64, SA_AT = B_AT + BN * 64, SB_AT = SA_AT + SA_N * 256, STAGE = SB_AT + SB_N * 256;
+  constexpr int A_AT = 0, B_AT = BM * 64, STAGE = B_AT + BN * 64;
+  constexpr int S_STAGE = S_ALL * 256, S_STAGES = 3;
   constexpr int D = STAGES - 1;
   static_assert(PER * WAVES == A_KB + B_KB, "a slab splits evenly over the waves");
   static_assert(!MX || (B_ROW && !GRAD), "4-bit operands have k along their rows");
   static_assert(!PP || (WGM == 2 && WGN == 4), "two groups of four waves");
-  static_assert(STAGES * STAGE <= 160 * 1024 && D * DMA < 64, "LDS and wait counts");
+  static_assert(STAGES * STAGE + S_STAGES * S_STAGE <= 160 * 1024 && D * DMA < 64, "LDS and wait counts");
+  static_assert(!MX || D <= 4, "scales are read before their stage is filled again");
 
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[STAGES * STAGE];
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[STAGES * STAGE + S_STAGES * S_STAGE];
+  unsigned char* const lds_s = lds + STAGES * STAGE;
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -268,7 +274,20 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_dma(DmaArgs p) {
     }
   }
   // K stagger: tiles that share a panel start their walk at different slabs
-  const int kofs = nk > 0 ? ((mt + 2 * (n0 / BN)) & 15) % nk : 0;
+  const int kofs = !MX && nk > 0 ? ((mt + 2 * (n0 / BN)) & 15) % nk : 0;
+
+  // Scales of slabs 4 q .. 4 q + 3: part `part` of 4 of this wave's DMA; past
+  // the last slab they are zeros that nobody reads
+  auto issue_scales = [&](int q, int part) {
+    const u32x4 ra = descriptor(as + 16 * q, as_left - 16 * q), rb = descriptor(bs + 16 * q, bs_left - 16 * q);
+#pragma unroll
+    for (int i = 0; i < S_PER; ++i) {
+      const int kb = min((part * WAVES + wave) * S_PER + i, S_ALL - 1);  // without a share: the last one again
+      const bool is_a = kb < BM / 16;
+      const unsigned row = (unsigned)((is_a ? kb : kb - BM / 16) * 16 + (lane >> 2));
+      dma4(is_a ? ra : rb, row * 4u * (unsigned)nk + (unsigned)(lane & 3) * 4u, lds_s + q % S_STAGES * S_STAGE + kb * 256);
+    }
+  };
 
   auto issue = [&](int kt, unsigned char* st) {
     int kr = kt + kofs;
@@ -284,15 +303,7 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_dma(DmaArgs p) {
       if (A_ROW && left < 4 && chunk[i] >= left) o = PAST;
       dma16(is_a ? ra : rb, o, st + kb * 1024);
     }
-    if constexpr (MX) {
-#pragma unroll
-      for (int i = 0; i < S_PER; ++i) {
-        const int kb = min(wave * S_PER + i, SA_N + SB_N - 1);  // a wave without a share repeats the last
-        const bool is_a = kb < SA_N;
-        const u32x4 r = is_a ? descriptor(as + 4 * kr, as_left - 4 * kr) : descriptor(bs + 4 * kr, bs_left - 4 * kr);
-        dma4(r, (unsigned)((is_a ? kb : kb - SA_N) * 64 + lane) * 4u * (unsigned)nk, st + SA_AT + kb * 256);
-      }
-    }
+    if constexpr (MX) issue_scales(kt / 4 + 1, kt % 4);
   };
 
   f32x4 acc[TM][TN];
@@ -303,16 +314,17 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_dma(DmaArgs p) {
 
   u32x4 fa[TM], fb[TN];
   int ha[TM], hb[TN];
-  auto read = [&](const unsigned char* st) {
+  auto read = [&](int kt, const unsigned char* st) {
+    const unsigned char* ss = lds_s + kt / 4 % S_STAGES * S_STAGE + kt % 4 * 4 + g;
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
       fa[i] = fragment<A_ROW, BM>(st + A_AT, wm * TM, i, l16, g);
-      ha[i] = MX ? st[SA_AT + ((wm * TM + i) * 16 + l16) * 4 + g] : 0;
+      ha[i] = MX ? ss[((wm * TM + i) * 16 + l16) * 16] : 0;
     }
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
       fb[j] = fragment<B_ROW, BN>(st + B_AT, wn * TN, j, l16, g);
-      hb[j] = MX ? st[SB_AT + ((wn * TN + j) * 16 + l16) * 4 + g] : 0;
+      hb[j] = MX ? ss[(BM + (wn * TN + j) * 16 + l16) * 16] : 0;
     }
   };
   auto mma = [&]() {
@@ -323,6 +335,9 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_dma(DmaArgs p) {
   };
 
   if (nk > 0) {
+    if constexpr (MX)
+#pragma unroll
+      for (int part = 0; part < 4; ++part) issue_scales(0, part);
 #pragma unroll
     for (int s = 0; s < D; ++s)
       if (s < nk) issue(s, lds + s * STAGE);
@@ -344,7 +359,7 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_dma(DmaArgs p) {
       auto step = [&](int kt, const int s) {
         // ---- memory phase
         if (kt + D < nk) issue(kt + D, lds + (s + D) % STAGES * STAGE);
-        read(lds + s * STAGE);
+        read(kt, lds + s * STAGE);
         __builtin_amdgcn_s_waitcnt(waitcnt_lgkm0());
         if (group == 1) wait_next(kt);
         phase_barrier();
@@ -371,7 +386,7 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_dma(DmaArgs p) {
           // everyone has read slab kt+s-1, whose stage the DMA now fills
           phase_barrier();
           if (kt + s + D < nk) issue(kt + s + D, lds + (s + D) % STAGES * STAGE);
-          read(lds + s * STAGE);
+          read(kt + s, lds + s * STAGE);
           mma();
         }
       }

@@ -36,12 +36,25 @@ Mx4QuantArgs args_of(const xtc_hip_mx4_desc& d) {
   return a;
 }
 
+constexpr int kQuarters = 4;  // of a block a lane, dense rows
+
 dim3 grid_of(const Mx4QuantArgs& a) {
   return dim3((unsigned)((4 * (int64_t)a.blocks + 255) / 256), (unsigned)(a.rows < 65535 ? a.rows : 65535));
 }
 
 int quantize(const xtc_hip_mx4_desc& d, const Mx4QuantArgs& a, const char* what) {
   if (!aligned16(a.codes)) return fail("%s: codes must be 16-byte aligned", what);
+  if (a.K % 32 == 0 && a.ldx == a.K && !a.scales_in && aligned16(a.x) && aligned16(a.values)) {
+    const int64_t quarters = a.rows * (a.K / 8), groups = (quarters + 256 * kQuarters - 1) / (256 * kQuarters);
+    if (groups < (int64_t)1 << 31) {
+      const dim3 grid((unsigned)groups);
+      if (d.dtype == XTC_HIP_F32)
+        hipLaunchKernelGGL((mx4_quantize_dense<float, kQuarters>), grid, dim3(256), 0, core::pick_stream(d.stream), a, quarters);
+      else
+        hipLaunchKernelGGL((mx4_quantize_dense<__bf16, kQuarters>), grid, dim3(256), 0, core::pick_stream(d.stream), a, quarters);
+      return done(what);
+    }
+  }
   if (d.dtype == XTC_HIP_F32)
     hipLaunchKernelGGL(mx4_quantize<float>, grid_of(a), dim3(256), 0, core::pick_stream(d.stream), a);
   else

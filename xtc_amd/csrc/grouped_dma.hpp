@@ -7,11 +7,12 @@
 // not.
 //
 // Tile and slab.  A workgroup of WGM x WGN waves computes (16 WGM TM) x
-// (16 WGN TN) outputs, k in slabs of 64 bytes a row: 32 bf16 or 128 4-bit
-// elements, one v_mfma_f32_16x16x32_bf16 or v_mfma_scale_f32_16x16x128_f8f6f4
-// deep.  Both take 16 bytes of a row a lane and 16 cycles, so one kernel feeds
-// both.  B is the first MFMA operand: a lane ends with four neighbouring
-// columns of one row.
+// (16 WGN TN) outputs, k in slabs of 64 bytes a row: 32 bf16, one
+// v_mfma_f32_16x16x32_bf16 deep, or 128 4-bit elements, two
+// v_mfma_scale_f32_32x32x64_f8f6f4 deep (registers only: 6.5 PFLOP/s, the
+// 16x16x128 form 5.6: the scales take issue slots).  A lane feeds either with 16
+// bytes of a row.  B is the first MFMA operand: a lane ends with four
+// neighbouring columns of one row.
 //
 // Operands come in two forms.
 //   ROW  k contiguous: staged [rows][64 B], its 16-byte chunk c of row r at
@@ -19,8 +20,10 @@
 //   COL  k strided (bf16): staged [32 k][16-bit columns], its 32-byte chunk c of
 //        row k at c ^ swz(k), read transposed by ds_read_b64_tr_b16.
 // 4-bit operands bring 4 scale bytes a row and slab.  They are staged for four
-// slabs at a time, [rows][16], a quarter of the rows with each slab, one group
-// ahead: 4 bytes of each row a slab would touch as many cache lines as the codes.
+// slabs at a time, [rows][16], with every fourth slab and one group ahead (4 bytes
+// of each row a slab would touch as many cache lines as the codes), and a lane
+// reads its row's 16 at once and keeps the 8 of its k (byte reads for every slab
+// cost 8192^3 80 us).
 //
 // Edges cost nothing in the loop: every DMA goes through a buffer descriptor
 // that ends where the tile's rows end, and what lies past it arrives in LDS as
@@ -41,6 +44,8 @@
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+
+#include <type_traits>
 
 #include "gemm_bf16_pingpong.hpp"
 #include "groups.hpp"
@@ -78,6 +83,7 @@ using pingpong::phase_barrier;
 using pingpong::waitcnt_lgkm0;
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 
 constexpr unsigned PAST = 0x80000000u;  // an offset past every descriptor's end
@@ -89,8 +95,8 @@ __device__ __forceinline__ u32x4 descriptor(const uint8_t* p, int64_t bytes) {
   return u32x4{(unsigned)at, (unsigned)(at >> 32) & 0xffffu, (unsigned)n, 0x00020000u};
 }
 
-// 16 (or 4) bytes a lane from descriptor r at `off` to lds + 16 (4) lane; zeros
-// where off passes the descriptor's end.  Issued from asm, as in lds_dma.hpp; the
+// 16 bytes a lane from descriptor r at `off` (4-byte aligned) to lds + 16 lane;
+// dwords past the descriptor's end arrive as zeros.  Issued from asm, as in lds_dma.hpp; the
 // wait states cover M0 and a descriptor written right before.
 __device__ __forceinline__ unsigned lds_address(const void* p) {
   typedef __attribute__((address_space(3))) void lds_void_t;
@@ -100,11 +106,6 @@ __device__ __forceinline__ void dma16(u32x4 r, unsigned off, void* lds) {
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(r), "s"(lds_address(lds))
                : "memory", "m0");
 }
-__device__ __forceinline__ void dma4(u32x4 r, unsigned off, void* lds) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(off), "s"(r), "s"(lds_address(lds))
-               : "memory", "m0");
-}
-
 __device__ __forceinline__ int swz_row(int r) { return (r >> 1) & 3; }
 template <int COLS>
 __device__ __forceinline__ int swz_col(int k) {
@@ -140,15 +141,15 @@ __device__ __forceinline__ u32x4 fragment(const unsigned char* st, int f0, int f
   }
 }
 
-template <bool MX>
-__device__ __forceinline__ f32x4 mfma(u32x4 b, int sb, u32x4 a, int sa, f32x4 c) {
-  if constexpr (MX) {
-    const i32x8 bv = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
-    const i32x8 av = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0};
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(bv, av, c, 4, 4, 0, sb, 0, sa);
-  } else {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b), __builtin_bit_cast(bf16x8, a), c, 0, 0, 0);
-  }
+__device__ __forceinline__ f32x4 mfma(u32x4 b, u32x4 a, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b), __builtin_bit_cast(bf16x8, a), c, 0, 0, 0);
+}
+// 4-bit; the scales are byte `BYTE` of sa and sb
+template <int BYTE>
+__device__ __forceinline__ f32x16 mfma(u32x4 b, unsigned sb, u32x4 a, unsigned sa, f32x16 c) {
+  const i32x8 bv = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
+  const i32x8 av = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(bv, av, c, 4, 4, BYTE, (int)sb, BYTE, (int)sa);
 }
 
 // columns n .. n+3 (those below `cols`) of a row
@@ -171,6 +172,15 @@ __device__ __forceinline__ void store4(void* c, int out16, int64_t at, f32x4 v, 
   }
 }
 
+// f(0) .. f(N - 1), the argument a compile-time constant
+template <int N, int I = 0, typename F>
+__device__ __forceinline__ void each_stage(F&& f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>());
+    each_stage<N, I + 1>(f);
+  }
+}
+
 }  // namespace gdma
 
 template <bool MX, bool GRAD, bool B_ROW, int WGM, int WGN, int TM, int TN, int STAGES, bool PP>
@@ -179,17 +189,16 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_dma(DmaArgs p) {
   constexpr bool A_ROW = !GRAD;
   constexpr int WAVES = WGM * WGN, BM = WGM * TM * 16, BN = WGN * TN * 16;
   constexpr int A_KB = BM / 16, B_KB = BN / 16, PER = (A_KB + B_KB) / WAVES;  // DMA kilobytes
-  constexpr int S_ALL = MX ? (BM + BN) / 16 : 0;  // scale DMA of four slabs: 16 rows each
-  constexpr int S_PER = (S_ALL + 4 * WAVES - 1) / (4 * WAVES);  // a wave's with each slab
-  constexpr int DMA = PER + S_PER;  // DMA instructions a wave and slab
+  constexpr int S_ALL = MX ? (BM + BN) / 64 : 0;        // scale DMA of four slabs: 64 rows each
+  constexpr int S_PER = (S_ALL + WAVES - 1) / WAVES;    // a wave's with every fourth slab
   constexpr int A_AT = 0, B_AT = BM * 64, STAGE = B_AT + BN * 64;
-  constexpr int S_STAGE = S_ALL * 256, S_STAGES = 3;
+  constexpr int S_STAGE = S_ALL * 1024, S_STAGES = 2;
   constexpr int D = STAGES - 1;
   static_assert(PER * WAVES == A_KB + B_KB, "a slab splits evenly over the waves");
   static_assert(!MX || (B_ROW && !GRAD), "4-bit operands have k along their rows");
   static_assert(!PP || (WGM == 2 && WGN == 4), "two groups of four waves");
-  static_assert(STAGES * STAGE + S_STAGES * S_STAGE <= 160 * 1024 && D * DMA < 64, "LDS and wait counts");
-  static_assert(!MX || D <= 4, "scales are read before their stage is filled again");
+  static_assert(STAGES * STAGE + S_STAGES * S_STAGE <= 160 * 1024 && D * PER + S_PER < 64, "LDS and wait counts");
+  static_assert(!MX || STAGES == 4, "a slab's place in its group of four is its stage");
 
   __shared__ __attribute__((aligned(1024))) unsigned char lds[STAGES * STAGE + S_STAGES * S_STAGE];
   unsigned char* const lds_s = lds + STAGES * STAGE;
@@ -276,16 +285,16 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_dma(DmaArgs p) {
   // K stagger: tiles that share a panel start their walk at different slabs
   const int kofs = !MX && nk > 0 ? ((mt + 2 * (n0 / BN)) & 15) % nk : 0;
 
-  // Scales of slabs 4 q .. 4 q + 3: part `part` of 4 of this wave's DMA; past
-  // the last slab they are zeros that nobody reads
-  auto issue_scales = [&](int q, int part) {
+  // Scales of slabs 4 q .. 4 q + 3; past the last slab they are the next row's
+  // or zeros, and nobody reads them
+  auto issue_scales = [&](int q) {
     const u32x4 ra = descriptor(as + 16 * q, as_left - 16 * q), rb = descriptor(bs + 16 * q, bs_left - 16 * q);
 #pragma unroll
     for (int i = 0; i < S_PER; ++i) {
-      const int kb = min((part * WAVES + wave) * S_PER + i, S_ALL - 1);  // without a share: the last one again
-      const bool is_a = kb < BM / 16;
-      const unsigned row = (unsigned)((is_a ? kb : kb - BM / 16) * 16 + (lane >> 2));
-      dma4(is_a ? ra : rb, row * 4u * (unsigned)nk + (unsigned)(lane & 3) * 4u, lds_s + q % S_STAGES * S_STAGE + kb * 256);
+      const int kb = min(wave * S_PER + i, S_ALL - 1);  // without a share: the last one again
+      const bool is_a = kb < BM / 64;
+      const unsigned row = (unsigned)((is_a ? kb : kb - BM / 64) * 64 + lane);
+      dma16(is_a ? ra : rb, row * 4u * (unsigned)nk, lds_s + q % S_STAGES * S_STAGE + kb * 1024);
     }
   };
 
@@ -303,105 +312,150 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_dma(DmaArgs p) {
       if (A_ROW && left < 4 && chunk[i] >= left) o = PAST;
       dma16(is_a ? ra : rb, o, st + kb * 1024);
     }
-    if constexpr (MX) issue_scales(kt / 4 + 1, kt % 4);
+    if (MX && kt % 4 == 0) issue_scales(kt / 4 + 1);
   };
 
-  f32x4 acc[TM][TN];
-#pragma unroll
-  for (int i = 0; i < TM; ++i)
-#pragma unroll
-    for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // DMA instructions of this wave's slabs kt+first .. kt+last, kt % 4 == s
+  auto dma_count = [](int s, int first, int last) constexpr {
+    int n = 0;
+    for (int i = first; i <= last; ++i) n += PER + (MX && (s + i) % 4 == 0 ? S_PER : 0);
+    return n;
+  };
 
-  u32x4 fa[TM], fb[TN];
-  int ha[TM], hb[TN];
-  auto read = [&](int kt, const unsigned char* st) {
-    const unsigned char* ss = lds_s + kt / 4 % S_STAGES * S_STAGE + kt % 4 * 4 + g;
+  // 16 x 16 tiles of bf16, or 32 x 32 tiles of 4-bit products
+  constexpr int IM = MX ? TM / 2 : TM, JN = MX ? TN / 2 : TN, STEPS = MX ? 2 : 1;
+  typedef std::conditional_t<MX, f32x16, f32x4> Acc;
+  Acc acc[IM][JN];
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      fa[i] = fragment<A_ROW, BM>(st + A_AT, wm * TM, i, l16, g);
-      ha[i] = MX ? ss[((wm * TM + i) * 16 + l16) * 16] : 0;
-    }
+  for (int i = 0; i < IM; ++i)
 #pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      fb[j] = fragment<B_ROW, BN>(st + B_AT, wn * TN, j, l16, g);
-      hb[j] = MX ? ss[(BM + (wn * TN + j) * 16 + l16) * 16] : 0;
+    for (int j = 0; j < JN; ++j) acc[i][j] = Acc{};
+
+  u32x4 fa[STEPS][IM], fb[STEPS][JN];
+  unsigned ha[IM][2], hb[JN][2];  // scales of this lane's row and half of k: slabs 0, 1 and 2, 3 of a group
+  const int l32 = lane & 31, half = lane >> 5;
+  auto read = [&](int kt, const int s, const unsigned char* st) {
+    if constexpr (MX) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int i = 0; i < IM; ++i)
+          fa[h][i] = *(const lds_u32x4*)(st + A_AT + ((wm * IM + i) * 32 + l32) * 64 + 16 * ((2 * h + half) ^ swz_row(l32)));
+#pragma unroll
+        for (int j = 0; j < JN; ++j)
+          fb[h][j] = *(const lds_u32x4*)(st + B_AT + ((wn * JN + j) * 32 + l32) * 64 + 16 * ((2 * h + half) ^ swz_row(l32)));
+      }
+      if (s == 0) {
+        const unsigned char* ss = lds_s + kt / 4 % S_STAGES * S_STAGE + l32 * 16;
+        const unsigned pick = half ? 0x07050301u : 0x06040200u;
+        auto keep = [&](unsigned (&h)[2], int row) {
+          const u32x4 v = *(const lds_u32x4*)(ss + row * 16);
+          h[0] = __builtin_amdgcn_perm(v[1], v[0], pick);
+          h[1] = __builtin_amdgcn_perm(v[3], v[2], pick);
+        };
+#pragma unroll
+        for (int i = 0; i < IM; ++i) keep(ha[i], (wm * IM + i) * 32);
+#pragma unroll
+        for (int j = 0; j < JN; ++j) keep(hb[j], BM + (wn * JN + j) * 32);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < IM; ++i) fa[0][i] = fragment<A_ROW, BM>(st + A_AT, wm * TM, i, l16, g);
+#pragma unroll
+      for (int j = 0; j < JN; ++j) fb[0][j] = fragment<B_ROW, BN>(st + B_AT, wn * TN, j, l16, g);
     }
   };
-  auto mma = [&]() {
+  auto mma = [&](const int s) {
 #pragma unroll
-    for (int i = 0; i < TM; ++i)
+    for (int h = 0; h < STEPS; ++h)
 #pragma unroll
-      for (int j = 0; j < TN; ++j) acc[i][j] = mfma<MX>(fb[j], hb[j], fa[i], ha[i], acc[i][j]);
+      for (int i = 0; i < IM; ++i)
+#pragma unroll
+        for (int j = 0; j < JN; ++j) {
+          if constexpr (MX) {
+            const unsigned sb = hb[j][s / 2], sa = ha[i][s / 2];
+            const int byte = s % 2 * 2 + h;
+            acc[i][j] = byte == 0 ? mfma<0>(fb[h][j], sb, fa[h][i], sa, acc[i][j])
+                        : byte == 1 ? mfma<1>(fb[h][j], sb, fa[h][i], sa, acc[i][j])
+                        : byte == 2 ? mfma<2>(fb[h][j], sb, fa[h][i], sa, acc[i][j])
+                                    : mfma<3>(fb[h][j], sb, fa[h][i], sa, acc[i][j]);
+          } else {
+            acc[i][j] = mfma(fb[h][j], fa[h][i], acc[i][j]);
+          }
+        }
   };
 
   if (nk > 0) {
-    if constexpr (MX)
-#pragma unroll
-      for (int part = 0; part < 4; ++part) issue_scales(0, part);
+    if constexpr (MX) issue_scales(0);
 #pragma unroll
     for (int s = 0; s < D; ++s)
       if (s < nk) issue(s, lds + s * STAGE);
     if constexpr (PP) {
-      // this wave's DMA of slab t+1 has landed (slabs through min(t+D, nk-1) issued)
-      auto wait_next = [&](int kt) {
-        if (kt + D < nk)
-          __builtin_amdgcn_s_waitcnt(waitcnt_vm((D - 1) * DMA));
-        else
-          __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
-      };
       const int group = wm;
       if (nk >= D)
-        __builtin_amdgcn_s_waitcnt(waitcnt_vm((D - 1) * DMA));
+        __builtin_amdgcn_s_waitcnt(waitcnt_vm(dma_count(0, 1, D - 1)));
       else
         __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
       phase_barrier();
       if (group == 1) phase_barrier();
-      auto step = [&](int kt, const int s) {
-        // ---- memory phase
-        if (kt + D < nk) issue(kt + D, lds + (s + D) % STAGES * STAGE);
-        read(kt, lds + s * STAGE);
-        __builtin_amdgcn_s_waitcnt(waitcnt_lgkm0());
-        if (group == 1) wait_next(kt);
-        phase_barrier();
-        // ---- compute phase
-        mma();
-        if (group == 0) wait_next(kt);
-        if (group == 0 || kt + 1 < nk) phase_barrier();
-      };
-      for (int kt = 0; kt < nk; kt += STAGES) {
-#pragma unroll
-        for (int s = 0; s < STAGES; ++s)
-          if (kt + s < nk) step(kt + s, s);
-      }
-    } else {
-      for (int kt = 0; kt < nk; kt += STAGES) {
-#pragma unroll
-        for (int s = 0; s < STAGES; ++s) {
-          if (kt + s >= nk) break;
-          // slab kt+s has landed; the ones after it may be in flight
-          if (kt + s + D - 1 < nk)
-            __builtin_amdgcn_s_waitcnt(waitcnt_vm((D - 1) * DMA));
+      auto step = [&](int kt, auto stage) {
+        constexpr int s = decltype(stage)::value;
+        // this wave's DMA of slab kt+1 has landed (slabs through min(kt+D, nk-1) issued)
+        auto wait_next = [&]() {
+          if (kt + D < nk)
+            __builtin_amdgcn_s_waitcnt(waitcnt_vm(dma_count(s, 2, D)));
           else
             __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
-          // everyone has read slab kt+s-1, whose stage the DMA now fills
-          phase_barrier();
-          if (kt + s + D < nk) issue(kt + s + D, lds + (s + D) % STAGES * STAGE);
-          read(kt + s, lds + s * STAGE);
-          mma();
-        }
-      }
+        };
+        // ---- memory phase
+        if (kt + D < nk) issue(kt + D, lds + (s + D) % STAGES * STAGE);
+        read(kt, s, lds + s * STAGE);
+        __builtin_amdgcn_s_waitcnt(waitcnt_lgkm0());
+        if (group == 1) wait_next();
+        phase_barrier();
+        // ---- compute phase
+        mma(s);
+        if (group == 0) wait_next();
+        if (group == 0 || kt + 1 < nk) phase_barrier();
+      };
+      for (int kt = 0; kt < nk; kt += STAGES) each_stage<STAGES>([&](auto s) { if (kt + s < nk) step(kt + s, s); });
+    } else {
+      auto step = [&](int kt, auto stage) {
+        constexpr int s = decltype(stage)::value;
+        // slab kt has landed; the ones after it may be in flight
+        if (kt + D - 1 < nk)
+          __builtin_amdgcn_s_waitcnt(waitcnt_vm(dma_count(s, 1, D - 1)));
+        else
+          __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+        // everyone has read slab kt-1, whose stage the DMA now fills
+        phase_barrier();
+        if (kt + D < nk) issue(kt + D, lds + (s + D) % STAGES * STAGE);
+        read(kt, s, lds + s * STAGE);
+        mma(s);
+      };
+      for (int kt = 0; kt < nk; kt += STAGES) each_stage<STAGES>([&](auto s) { if (kt + s < nk) step(kt + s, s); });
     }
   }
 
-  // ---- a lane holds C[m][n .. n+3] of each 16 x 16
+  // ---- a lane holds C[m][n .. n+3] of each 16 x 16, or n, n+8, n+16 and n+24 of
+  // each 32 x 32
   const bool whole = (p.ldc & 3) == 0 && ((uintptr_t)p.c & (p.out16 ? 7 : 15)) == 0 && (!GRAD || (p.stride_c & 3) == 0);
 #pragma unroll
-  for (int i = 0; i < TM; ++i) {
-    const int m = (wm * TM + i) * 16 + l16;
+  for (int i = 0; i < IM; ++i) {
+    const int m = MX ? (wm * IM + i) * 32 + l32 : (wm * IM + i) * 16 + l16;
     if (m >= rows) continue;
+    const int64_t at = c_at + (int64_t)m * p.ldc;
 #pragma unroll
-    for (int j = 0; j < TN; ++j)
-      store4(p.c, p.out16, c_at + (int64_t)m * p.ldc, acc[i][j], (wn * TN + j) * 16 + 4 * g, cols, whole);
+    for (int j = 0; j < JN; ++j) {
+      if constexpr (MX) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          store4(p.c, p.out16, at, f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]},
+                 (wn * JN + j) * 32 + 8 * q + 4 * half, cols, whole);
+      } else {
+        store4(p.c, p.out16, at, acc[i][j], (wn * JN + j) * 16 + 4 * g, cols, whole);
+      }
+    }
   }
 }
 

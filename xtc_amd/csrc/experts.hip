@@ -52,7 +52,7 @@ const DmaTile kDmaTiles[] = {
 #undef XTC_DMA
 
 // Strides of whole vectors whose offsets within a tile stay within 2^31 bytes.
-bool vectors(const void* p, int ld) { return core::aligned16(p) && ld % 8 == 0 && ld < (1 << 22); }
+bool vectors(const void* p, int ld) { return core::aligned16(p) && ld % 8 == 0 && ld < (1 << 22) - 8; }
 
 const DmaTile* dma_tile(int64_t rows, int64_t groups, int N, bool grad, int K) {
   for (const DmaTile& t : kDmaTiles) {

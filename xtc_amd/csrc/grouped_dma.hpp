@@ -86,26 +86,54 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 
-constexpr unsigned PAST = 0x80000000u;  // an offset past every descriptor's end
+constexpr unsigned PAST = 0x80000000u;  // an offset past every descriptor's end (they are shorter)
 
-// Buffer descriptor of `bytes` (clamped to 0 .. 2^31 - 1) from p.
-__device__ __forceinline__ u32x4 descriptor(const uint8_t* p, int64_t bytes) {
-  const uint64_t at = (uint64_t)p;
-  const int64_t n = bytes < 0 ? 0 : bytes > 0x7fffffff ? 0x7fffffff : bytes;
-  return u32x4{(unsigned)at, (unsigned)(at >> 32) & 0xffffu, (unsigned)n, 0x00020000u};
+// Issued from asm, as in lds_dma.hpp: 16 bytes a lane from `off` (4-byte aligned)
+// into buffer `r` go to LDS at `lds` + `ADD` + 16 lane; dwords past the
+// descriptor's end arrive as zeros.  The wait states cover M0 and, in the FIRST
+// one of a run, a descriptor written right before.
+template <bool FIRST, int ADD>
+__device__ __forceinline__ void dma16(u32x4 r, unsigned off, unsigned lds) {
+  if constexpr (FIRST)
+    asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(r), "s"(lds),
+                 "n"(ADD)
+                 : "memory", "m0", "scc");
+  else
+    asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(r), "s"(lds),
+                 "n"(ADD)
+                 : "memory", "m0", "scc");
 }
-
-// 16 bytes a lane from descriptor r at `off` (4-byte aligned) to lds + 16 lane;
-// dwords past the descriptor's end arrive as zeros.  Issued from asm, as in lds_dma.hpp; the
-// wait states cover M0 and a descriptor written right before.
+__device__ __forceinline__ u32x4 descriptor(uint64_t at, unsigned bytes) {
+  return u32x4{(unsigned)at, (unsigned)(at >> 32) & 0xffffu, bytes, 0x00020000u};
+}
 __device__ __forceinline__ unsigned lds_address(const void* p) {
   typedef __attribute__((address_space(3))) void lds_void_t;
-  return __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(lds_void_t*)p);
+  return (unsigned)(uintptr_t)(lds_void_t*)p;
 }
-__device__ __forceinline__ void dma16(u32x4 r, unsigned off, void* lds) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(r), "s"(lds_address(lds))
-               : "memory", "m0");
-}
+
+// The bytes of an operand that its next slab may touch, a slab after the other
+// from slab `first`, then from the start.  All of it is wave-uniform.
+template <bool ROW>
+struct Walk {
+  uint64_t start, at;  // tile's corner in slab 0, in the next slab
+  uint64_t step;       // bytes from a slab to the next
+  int slab, slabs;
+  int ld;              // COL: bytes of a k row
+  unsigned width;      // ROW: bytes from the corner to the end; COL: of the last k row
+  int depth;           // COL: k rows in all
+
+  __device__ __forceinline__ u32x4 next() {
+    unsigned bytes;
+    if constexpr (ROW) bytes = width - 64u * (unsigned)slab;
+    else bytes = (unsigned)((min(depth - 32 * slab, 32) - 1) * ld) + width;
+    const u32x4 r = descriptor(at, bytes);
+    ++slab;
+    at += step;
+    if (slab == slabs) slab = 0, at = start;
+    return r;
+  }
+};
+
 __device__ __forceinline__ int swz_row(int r) { return (r >> 1) & 3; }
 template <int COLS>
 __device__ __forceinline__ int swz_col(int k) {
@@ -194,7 +222,7 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_dma(DmaArgs p) {
   constexpr int A_AT = 0, B_AT = BM * 64, STAGE = B_AT + BN * 64;
   constexpr int S_STAGE = S_ALL * 1024, S_STAGES = 2;
   constexpr int D = STAGES - 1;
-  static_assert(PER * WAVES == A_KB + B_KB, "a slab splits evenly over the waves");
+  static_assert(PER * WAVES == A_KB + B_KB && A_KB % PER == 0, "a slab splits evenly over the waves, one operand each");
   static_assert(!MX || (B_ROW && !GRAD), "4-bit operands have k along their rows");
   static_assert(!PP || (WGM == 2 && WGN == 4), "two groups of four waves");
   static_assert(STAGES * STAGE + S_STAGES * S_STAGE <= 160 * 1024 && D * PER + S_PER < 64, "LDS and wait counts");
@@ -218,25 +246,20 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_dma(DmaArgs p) {
   const int mt = tt / (p.band * p.tiles_n) * p.band + in_band % p.band, n0 = in_band / p.band * BN;
   if (mt >= p.tiles_m || (GRAD && e_grad >= p.E)) return;
 
-  const uint8_t *a, *b;        // tile corners
-  const uint8_t *as = nullptr, *bs = nullptr;
-  int64_t a_left, b_left;      // bytes from there to the operand's end
-  int64_t as_left = 0, bs_left = 0;
-  int64_t a_step, b_step;      // bytes from a slab to the next
-  int64_t c_at;                // element of C at the tile's corner
-  int rows, nk, chunks = 0;    // rows of C, slabs, 16-byte chunks of a ROW row
+  const uint8_t *a, *b;                        // tile corners
+  const uint8_t *as = nullptr, *bs = nullptr;  // and those of the scales
+  int64_t c_at;              // element of C at the tile's corner
+  int rows, nk, chunks = 0;  // rows of C, slabs, 16-byte chunks of a ROW row
+  int depth = 0;             // k rows of a COL operand
   const int cols = p.N - n0;
   if constexpr (GRAD) {
     const RowGroup gr = find_group(p.sizes, p.E, p.M, e_grad);
-    const int m0 = mt * BM, depth = gr.end - gr.begin;
+    const int m0 = mt * BM;
     rows = p.K - m0;
+    depth = gr.end - gr.begin;
     nk = (depth + 31) / 32;
     a = p.a + (int64_t)gr.begin * p.lda + 2 * m0;
     b = p.b + (int64_t)gr.begin * p.ldb + 2 * n0;
-    a_left = (int64_t)(depth - 1) * p.lda + 2 * rows;
-    b_left = (int64_t)(depth - 1) * p.ldb + 2 * cols;
-    a_step = (int64_t)32 * p.lda;
-    b_step = (int64_t)32 * p.ldb;
     c_at = (int64_t)e_grad * p.stride_c + (int64_t)m0 * p.ldc + n0;
   } else {
     RowGroup gr{0, mt * BM, p.M};
@@ -245,72 +268,75 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_dma(DmaArgs p) {
     const int e = gr.e < p.E ? gr.e : 0;
     rows = min(gr.end - gr.begin, BM);
     chunks = gr.e < p.E ? p.K : 0;  // rows of no group: zeros
+    depth = 8 * chunks;
     nk = (chunks + 3) / 4;
     a = p.a + (int64_t)gr.begin * p.lda;
-    a_left = (int64_t)(rows - 1) * p.lda + 16 * (int64_t)chunks;
-    a_step = 64;
-    const uint8_t* m = p.b + e * p.stride_b;
-    if constexpr (B_ROW) {
-      b = m + (int64_t)n0 * p.ldb;
-      b_left = (int64_t)(min(cols, BN) - 1) * p.ldb + 16 * (int64_t)chunks;
-      b_step = 64;
-    } else {
-      b = m + 2 * n0;
-      b_left = (int64_t)(8 * chunks - 1) * p.ldb + 2 * cols;
-      b_step = (int64_t)32 * p.ldb;
-    }
+    b = p.b + e * p.stride_b + (B_ROW ? (int64_t)n0 * p.ldb : 2 * (int64_t)n0);
     if constexpr (MX) {
       as = p.sa + (int64_t)gr.begin * 4 * nk;
-      as_left = (int64_t)rows * 4 * nk;
       bs = p.sb + e * p.stride_sb + (int64_t)n0 * 4 * nk;
-      bs_left = (int64_t)min(cols, BN) * 4 * nk;
     }
     c_at = (int64_t)gr.begin * p.ldc + n0;
   }
 
-  // ---- this wave's share of a slab's DMA
+  // ---- this wave's share of a slab's DMA: PER kilobytes of one operand
+  const bool is_a = wave * PER < A_KB;
+  const int kb0 = is_a ? wave * PER : wave * PER - A_KB;  // in the operand's stage
+  const int ld = is_a ? p.lda : p.ldb;
+  const int lines = is_a ? min(rows, BM) : min(cols, BN);  // rows (ROW) or columns (COL) of the operand in the tile
   unsigned off[PER];
   int chunk[PER];  // ROW: chunk of the slab that the lane loads
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const int kb = wave * PER + i;
-    if (kb < A_KB) {
-      off[i] = source<A_ROW, BM>(kb, lane, p.lda);
-      chunk[i] = A_ROW ? (lane & 3) ^ swz_row(kb * 16 + (lane >> 2)) : 0;
-    } else {
-      off[i] = source<B_ROW, BN>(kb - A_KB, lane, p.ldb);
-      chunk[i] = B_ROW ? (lane & 3) ^ swz_row((kb - A_KB) * 16 + (lane >> 2)) : 0;
-    }
+    off[i] = is_a ? source<A_ROW, BM>(kb0 + i, lane, ld) : source<B_ROW, BN>(kb0 + i, lane, ld);
+    chunk[i] = (lane & 3) ^ swz_row((kb0 + i) * 16 + (lane >> 2));
   }
   // K stagger: tiles that share a panel start their walk at different slabs
   const int kofs = !MX && nk > 0 ? ((mt + 2 * (n0 / BN)) & 15) % nk : 0;
+  const bool row = is_a ? A_ROW : B_ROW;
+  Walk<true> by_row;
+  Walk<false> by_col;
+  if (row) {
+    by_row.start = (uint64_t)(is_a ? a : b);
+    by_row.step = 64;
+    by_row.width = (unsigned)(lines - 1) * (unsigned)ld + 16u * (unsigned)chunks;
+    by_row.slab = kofs, by_row.slabs = nk;
+    by_row.at = by_row.start + (uint64_t)kofs * 64;
+  } else {
+    by_col.start = (uint64_t)(is_a ? a : b);
+    by_col.step = (uint64_t)32 * (uint64_t)ld;
+    by_col.ld = ld, by_col.width = 2u * (unsigned)lines, by_col.depth = depth;
+    by_col.slab = kofs, by_col.slabs = nk;
+    by_col.at = by_col.start + (uint64_t)kofs * by_col.step;
+  }
+  const unsigned lds0 = __builtin_amdgcn_readfirstlane(lds_address(lds)), share = (unsigned)((is_a ? 0 : B_AT) + kb0 * 1024);
 
   // Scales of slabs 4 q .. 4 q + 3; past the last slab they are the next row's
   // or zeros, and nobody reads them
+  const int s_kb = min(wave * S_PER, S_ALL - S_PER);  // a wave without a share repeats the last one
+  const bool s_is_a = s_kb < BM / 64;
+  const uint64_t s_at = (uint64_t)(s_is_a ? as : bs);
+  const unsigned s_bytes = (unsigned)(s_is_a ? min(rows, BM) : min(cols, BN)) * 4u * (unsigned)nk;
+  const unsigned s_off = (unsigned)((s_is_a ? s_kb : s_kb - BM / 64) * 64 + lane) * 4u * (unsigned)nk;
   auto issue_scales = [&](int q) {
-    const u32x4 ra = descriptor(as + 16 * q, as_left - 16 * q), rb = descriptor(bs + 16 * q, bs_left - 16 * q);
-#pragma unroll
-    for (int i = 0; i < S_PER; ++i) {
-      const int kb = min(wave * S_PER + i, S_ALL - 1);  // without a share: the last one again
-      const bool is_a = kb < BM / 64;
-      const unsigned row = (unsigned)((is_a ? kb : kb - BM / 64) * 64 + lane);
-      dma16(is_a ? ra : rb, row * 4u * (unsigned)nk, lds_s + q % S_STAGES * S_STAGE + kb * 1024);
-    }
+    static_assert(S_PER <= 1, "one DMA of scales a wave");
+    dma16<true, 0>(descriptor(s_at + 16 * (uint64_t)q, (unsigned)max((int)s_bytes - 16 * q, 0)), s_off,
+                   lds0 + STAGES * STAGE + q % S_STAGES * S_STAGE + s_kb * 1024);
   };
 
-  auto issue = [&](int kt, unsigned char* st) {
-    int kr = kt + kofs;
-    kr = kr >= nk ? kr - nk : kr;
-    const u32x4 ra = descriptor(a + kr * a_step, a_left - kr * a_step);
-    const u32x4 rb = descriptor(b + kr * b_step, b_left - kr * b_step);
-    const int left = GRAD ? 4 : chunks - 4 * kr;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int kb = wave * PER + i;
-      const bool is_a = kb < A_KB;
-      unsigned o = off[i];
-      if (A_ROW && left < 4 && chunk[i] >= left) o = PAST;
-      dma16(is_a ? ra : rb, o, st + kb * 1024);
+  auto issue = [&](int kt, const int stage) {
+    const unsigned at = lds0 + share + stage * STAGE;
+    if (row) {
+      const int left = chunks - 4 * by_row.slab;
+      const u32x4 r = by_row.next();
+      if (!MX && left < 4) {
+        each_stage<PER>([&](auto i) { dma16<i == 0, i * 1024>(r, chunk[i] < left ? off[i] : PAST, at); });
+      } else {
+        each_stage<PER>([&](auto i) { dma16<i == 0, i * 1024>(r, off[i], at); });
+      }
+    } else {
+      const u32x4 r = by_col.next();
+      each_stage<PER>([&](auto i) { dma16<i == 0, i * 1024>(r, off[i], at); });
     }
     if (MX && kt % 4 == 0) issue_scales(kt / 4 + 1);
   };
@@ -389,7 +415,7 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_dma(DmaArgs p) {
     if constexpr (MX) issue_scales(0);
 #pragma unroll
     for (int s = 0; s < D; ++s)
-      if (s < nk) issue(s, lds + s * STAGE);
+      if (s < nk) issue(s, s);
     if constexpr (PP) {
       const int group = wm;
       if (nk >= D)
@@ -408,7 +434,7 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_dma(DmaArgs p) {
             __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
         };
         // ---- memory phase
-        if (kt + D < nk) issue(kt + D, lds + (s + D) % STAGES * STAGE);
+        if (kt + D < nk) issue(kt + D, (s + D) % STAGES);
         read(kt, s, lds + s * STAGE);
         __builtin_amdgcn_s_waitcnt(waitcnt_lgkm0());
         if (group == 1) wait_next();
@@ -429,7 +455,7 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_dma(DmaArgs p) {
           __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
         // everyone has read slab kt-1, whose stage the DMA now fills
         phase_barrier();
-        if (kt + D < nk) issue(kt + D, lds + (s + D) % STAGES * STAGE);
+        if (kt + D < nk) issue(kt + D, (s + D) % STAGES);
         read(kt, s, lds + s * STAGE);
         mma(s);
       };

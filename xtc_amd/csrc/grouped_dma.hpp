@@ -16,7 +16,7 @@
 //
 // Operands come in two forms.
 //   ROW  k contiguous: staged [rows][64 B], its 16-byte chunk c of row r at
-//        c ^ ((r >> 1) & 3), read by ds_read_b128.
+//        c ^ ((r >> 1) & 3), 4-bit c ^ ((r >> 2) & 3), read by ds_read_b128.
 //   COL  k strided (bf16): staged [32 k][16-bit columns], its 32-byte chunk c of
 //        row k at c ^ swz(k), read transposed by ds_read_b64_tr_b16.
 // 4-bit operands bring 4 scale bytes a row and slab.  They are staged for four
@@ -112,12 +112,14 @@ __device__ __forceinline__ unsigned lds_address(const void* p) {
 }
 
 // The bytes of an operand that its next slab may touch, a slab after the other
-// from slab `first`, then from the start.  All of it is wave-uniform.
+// from slab `slab`, then from the start; none once all `left` slabs are done, so
+// that the loops start a DMA with every step and wait for constant counts.  All
+// of it is wave-uniform.
 template <bool ROW>
 struct Walk {
   uint64_t start, at;  // tile's corner in slab 0, in the next slab
   uint64_t step;       // bytes from a slab to the next
-  int slab, slabs;
+  int slab, slabs, left;
   int ld;              // COL: bytes of a k row
   unsigned width;      // ROW: bytes from the corner to the end; COL: of the last k row
   int depth;           // COL: k rows in all
@@ -126,7 +128,8 @@ struct Walk {
     unsigned bytes;
     if constexpr (ROW) bytes = width - 64u * (unsigned)slab;
     else bytes = (unsigned)((min(depth - 32 * slab, 32) - 1) * ld) + width;
-    const u32x4 r = descriptor(at, bytes);
+    const u32x4 r = descriptor(at, left > 0 ? bytes : 0u);
+    --left;
     ++slab;
     at += step;
     if (slab == slabs) slab = 0, at = start;
@@ -134,7 +137,12 @@ struct Walk {
   }
 };
 
-__device__ __forceinline__ int swz_row(int r) { return (r >> 1) & 3; }
+// A ds_read_b128 serves lanes 0-3, 12-15, 20-27 (and 4-11, 16-19, 28-31) at once: the
+// chunk that 16-row (32-row) fragments find without bank conflicts
+template <bool MX>
+__device__ __forceinline__ int swz_row(int r) {
+  return MX ? (r >> 2) & 3 : (r >> 1) & 3;
+}
 template <int COLS>
 __device__ __forceinline__ int swz_col(int k) {
   return COLS >= 128 ? ((k & 3) | ((k >> 1) & 4)) : (k & 3);
@@ -142,11 +150,11 @@ __device__ __forceinline__ int swz_col(int k) {
 
 // Where lane `lane` finds its 16 bytes of KB `kb` of an operand's stage: bytes
 // from the operand's tile corner.
-template <bool ROW, int LEN>
+template <bool MX, bool ROW, int LEN>
 __device__ __forceinline__ unsigned source(int kb, int lane, int ld) {
   if constexpr (ROW) {
     const int r = kb * 16 + (lane >> 2);
-    return (unsigned)r * (unsigned)ld + (unsigned)(((lane & 3) ^ swz_row(r)) * 16);
+    return (unsigned)r * (unsigned)ld + (unsigned)(((lane & 3) ^ swz_row<MX>(r)) * 16);
   } else {
     constexpr int SLOTS = LEN / 8, PER = 64 / SLOTS;  // 16-byte slots of a k row, k rows of a KB
     const int k = kb * PER + lane / SLOTS, slot = lane % SLOTS;
@@ -159,7 +167,7 @@ template <bool ROW, int LEN>
 __device__ __forceinline__ u32x4 fragment(const unsigned char* st, int f0, int f, int l16, int g) {
   if constexpr (ROW) {
     const int r = (f0 + f) * 16 + l16;
-    return *(const lds_u32x4*)(st + r * 64 + 16 * (g ^ swz_row(l16)));
+    return *(const lds_u32x4*)(st + r * 64 + 16 * (g ^ swz_row<false>(l16)));
   } else {
     const int k = 8 * g + (l16 >> 2);
     const unsigned char* p = st + k * (2 * LEN) + 32 * ((f0 + f) ^ swz_col<LEN>(k)) + 8 * (l16 & 3);
@@ -288,10 +296,11 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_dma(DmaArgs p) {
   int chunk[PER];  // ROW: chunk of the slab that the lane loads
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    off[i] = is_a ? source<A_ROW, BM>(kb0 + i, lane, ld) : source<B_ROW, BN>(kb0 + i, lane, ld);
-    chunk[i] = (lane & 3) ^ swz_row((kb0 + i) * 16 + (lane >> 2));
+    off[i] = is_a ? source<MX, A_ROW, BM>(kb0 + i, lane, ld) : source<MX, B_ROW, BN>(kb0 + i, lane, ld);
+    chunk[i] = (lane & 3) ^ swz_row<MX>((kb0 + i) * 16 + (lane >> 2));
   }
   // K stagger: tiles that share a panel start their walk at different slabs
+  // (bf16 8192^3 850 -> 830 us; 4-bit ones gain nothing from whole groups of four)
   const int kofs = !MX && nk > 0 ? ((mt + 2 * (n0 / BN)) & 15) % nk : 0;
   const bool row = is_a ? A_ROW : B_ROW;
   Walk<true> by_row;
@@ -300,13 +309,13 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_dma(DmaArgs p) {
     by_row.start = (uint64_t)(is_a ? a : b);
     by_row.step = 64;
     by_row.width = (unsigned)(lines - 1) * (unsigned)ld + 16u * (unsigned)chunks;
-    by_row.slab = kofs, by_row.slabs = nk;
+    by_row.slab = kofs, by_row.slabs = by_row.left = nk;
     by_row.at = by_row.start + (uint64_t)kofs * 64;
   } else {
     by_col.start = (uint64_t)(is_a ? a : b);
     by_col.step = (uint64_t)32 * (uint64_t)ld;
     by_col.ld = ld, by_col.width = 2u * (unsigned)lines, by_col.depth = depth;
-    by_col.slab = kofs, by_col.slabs = nk;
+    by_col.slab = kofs, by_col.slabs = by_col.left = nk;
     by_col.at = by_col.start + (uint64_t)kofs * by_col.step;
   }
   const unsigned lds0 = __builtin_amdgcn_readfirstlane(lds_address(lds)), share = (unsigned)((is_a ? 0 : B_AT) + kb0 * 1024);
@@ -366,10 +375,10 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_dma(DmaArgs p) {
       for (int h = 0; h < 2; ++h) {
 #pragma unroll
         for (int i = 0; i < IM; ++i)
-          fa[h][i] = *(const lds_u32x4*)(st + A_AT + ((wm * IM + i) * 32 + l32) * 64 + 16 * ((2 * h + half) ^ swz_row(l32)));
+          fa[h][i] = *(const lds_u32x4*)(st + A_AT + ((wm * IM + i) * 32 + l32) * 64 + 16 * ((2 * h + half) ^ swz_row<MX>(l32)));
 #pragma unroll
         for (int j = 0; j < JN; ++j)
-          fb[h][j] = *(const lds_u32x4*)(st + B_AT + ((wn * JN + j) * 32 + l32) * 64 + 16 * ((2 * h + half) ^ swz_row(l32)));
+          fb[h][j] = *(const lds_u32x4*)(st + B_AT + ((wn * JN + j) * 32 + l32) * 64 + 16 * ((2 * h + half) ^ swz_row<MX>(l32)));
       }
       if (s == 0) {
         const unsigned char* ss = lds_s + kt / 4 % S_STAGES * S_STAGE + l32 * 16;
@@ -413,54 +422,46 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_dma(DmaArgs p) {
 
   if (nk > 0) {
     if constexpr (MX) issue_scales(0);
-#pragma unroll
-    for (int s = 0; s < D; ++s)
-      if (s < nk) issue(s, s);
+    each_stage<D>([&](auto s) { issue(s, s); });
     if constexpr (PP) {
       const int group = wm;
-      if (nk >= D)
-        __builtin_amdgcn_s_waitcnt(waitcnt_vm(dma_count(0, 1, D - 1)));
-      else
-        __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+      __builtin_amdgcn_s_waitcnt(waitcnt_vm(dma_count(0, 1, D - 1)));
       phase_barrier();
       if (group == 1) phase_barrier();
       auto step = [&](int kt, auto stage) {
         constexpr int s = decltype(stage)::value;
-        // this wave's DMA of slab kt+1 has landed (slabs through min(kt+D, nk-1) issued)
-        auto wait_next = [&]() {
-          if (kt + D < nk)
-            __builtin_amdgcn_s_waitcnt(waitcnt_vm(dma_count(s, 2, D)));
-          else
-            __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
-        };
         // ---- memory phase
-        if (kt + D < nk) issue(kt + D, (s + D) % STAGES);
+        issue(kt + D, (s + D) % STAGES);
         read(kt, s, lds + s * STAGE);
         __builtin_amdgcn_s_waitcnt(waitcnt_lgkm0());
-        if (group == 1) wait_next();
+        // this wave's DMA of slab kt+1 has landed: group 0 waits after computing
+        if (group == 1) __builtin_amdgcn_s_waitcnt(waitcnt_vm(dma_count(s, 2, D)));
         phase_barrier();
-        // ---- compute phase
+        // ---- compute phase, ahead of the SIMD's other wave
+        __builtin_amdgcn_s_setprio(1);
         mma(s);
-        if (group == 0) wait_next();
-        if (group == 0 || kt + 1 < nk) phase_barrier();
+        __builtin_amdgcn_s_setprio(0);
+        __builtin_amdgcn_sched_barrier(0);
+        if (group == 0) __builtin_amdgcn_s_waitcnt(waitcnt_vm(dma_count(s, 2, D)));
+        phase_barrier();
       };
       for (int kt = 0; kt < nk; kt += STAGES) each_stage<STAGES>([&](auto s) { if (kt + s < nk) step(kt + s, s); });
+      if (group == 0) phase_barrier();
     } else {
       auto step = [&](int kt, auto stage) {
         constexpr int s = decltype(stage)::value;
         // slab kt has landed; the ones after it may be in flight
-        if (kt + D - 1 < nk)
-          __builtin_amdgcn_s_waitcnt(waitcnt_vm(dma_count(s, 1, D - 1)));
-        else
-          __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+        __builtin_amdgcn_s_waitcnt(waitcnt_vm(dma_count(s, 1, D - 1)));
         // everyone has read slab kt-1, whose stage the DMA now fills
         phase_barrier();
-        if (kt + D < nk) issue(kt + D, (s + D) % STAGES);
+        issue(kt + D, (s + D) % STAGES);
         read(kt, s, lds + s * STAGE);
         mma(s);
       };
       for (int kt = 0; kt < nk; kt += STAGES) each_stage<STAGES>([&](auto s) { if (kt + s < nk) step(kt + s, s); });
     }
+    // no DMA may write LDS after the workgroup has left it
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
   }
 
   // ---- a lane holds C[m][n .. n+3] of each 16 x 16, or n, n+8, n+16 and n+24 of

@@ -12,6 +12,8 @@ namespace {
 
 // Largest extent: tiles and slabs past it stay within 32 bits.
 constexpr int kMost = 0x7fffffff - 1023;
+// 64 x 64 tiles of any operands that make them worth their barriers.
+constexpr int64_t kSmallTiles = 512;
 
 int check(const xtc_hip_grouped_matmul_desc* d, const char* what) {
   if (!core::ready()) return fail("xtc_hip_init not called");
@@ -73,20 +75,35 @@ int launch_dma(const DmaTile& t, DmaLaunch run, DmaArgs& a, int64_t matrices, hi
   return e == hipSuccess ? 0 : fail("grouped_matmul: launch failed: %s", hipGetErrorString(e));
 }
 
+// ---- any operands: 64 x 64 tiles, or 32 x 32 tiles of split depth where those
+// would leave the CUs idle
 template <bool GRAD>
-int launch_any(const xtc_hip_grouped_matmul_desc& d, const GroupedArgs& a, int64_t groups, hipStream_t s) {
+int launch_any(const xtc_hip_grouped_matmul_desc& d, GroupedArgs& a, hipStream_t s) {
+  auto tiles = [&](int bm, int bn) {
+    a.tiles_n = (a.N + bn - 1) / bn;
+    a.tiles_k = (a.K + bm - 1) / bm;
+    return a.tiles_n * (GRAD ? (int64_t)a.E * a.tiles_k : most_tiles(a.T, a.E, bm));
+  };
+  const bool small = tiles(gany::BM, gany::BN) < kSmallTiles;
+  const int64_t groups = small ? tiles(gany::SM, gany::SN) : tiles(gany::BM, gany::BN);
   if (groups < 1 || groups >= (int64_t)1 << 31) return fail("grouped_matmul: %lld workgroups are too many", (long long)groups);
-  const dim3 grid((unsigned)groups), block(gany::NT);
+  const dim3 grid((unsigned)groups), block(small ? 64 * gany::SWAVES : gany::NT);
   const bool wt = !GRAD && d.trans_w, out16 = d.out_dtype == XTC_HIP_BF16;
-#define XTC_ANY(T, U)                                                                                  \
-  do {                                                                                                 \
-    if (wt) hipLaunchKernelGGL((grouped_any<T, U, !GRAD, GRAD>), grid, block, 0, s, a);                \
-    else hipLaunchKernelGGL((grouped_any<T, U, false, GRAD>), grid, block, 0, s, a);                   \
+#define XTC_ANY_OF(KERNEL, T, U)                                                      \
+  do {                                                                                \
+    if (wt) hipLaunchKernelGGL((KERNEL<T, U, !GRAD, GRAD>), grid, block, 0, s, a);    \
+    else hipLaunchKernelGGL((KERNEL<T, U, false, GRAD>), grid, block, 0, s, a);       \
+  } while (0)
+#define XTC_ANY(T, U)                                  \
+  do {                                                 \
+    if (small) XTC_ANY_OF(grouped_small, T, U);        \
+    else XTC_ANY_OF(grouped_any, T, U);                \
   } while (0)
   if (d.dtype == XTC_HIP_F32) XTC_ANY(float, float);
   else if (out16) XTC_ANY(__bf16, __bf16);
   else XTC_ANY(__bf16, float);
 #undef XTC_ANY
+#undef XTC_ANY_OF
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? 0 : fail("grouped_matmul: launch failed: %s", hipGetErrorString(e));
 }
@@ -124,8 +141,7 @@ int xtc_hip_grouped_matmul(const xtc_hip_grouped_matmul_desc* desc, const void* 
     v.tiles_m = (int)most_tiles(d.T, d.E, t.bm);
     return launch_dma(t, d.trans_w ? t.transposed : t.natural, v, 1, core::pick_stream(d.stream));
   }
-  a.tiles_n = (d.N + gany::BN - 1) / gany::BN;
-  return launch_any<false>(d, a, most_tiles(d.T, d.E, gany::BM) * a.tiles_n, core::pick_stream(d.stream));
+  return launch_any<false>(d, a, core::pick_stream(d.stream));
 }
 
 int xtc_hip_grouped_matmul_grad_w(const xtc_hip_grouped_matmul_desc* desc, const void* x, const void* dy,
@@ -154,9 +170,7 @@ int xtc_hip_grouped_matmul_grad_w(const xtc_hip_grouped_matmul_desc* desc, const
     v.tiles_m = (d.K + t.bm - 1) / t.bm;
     return launch_dma(t, t.grad, v, d.E, core::pick_stream(d.stream));
   }
-  a.tiles_n = (d.N + gany::BN - 1) / gany::BN;
-  a.tiles_k = (d.K + gany::BM - 1) / gany::BM;
-  return launch_any<true>(d, a, (int64_t)d.E * a.tiles_k * a.tiles_n, core::pick_stream(d.stream));
+  return launch_any<true>(d, a, core::pick_stream(d.stream));
 }
 
 }  // extern "C"

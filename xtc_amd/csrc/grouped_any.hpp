@@ -14,6 +14,12 @@
 // v_mfma_f32_16x16x32_bf16, fp32 on v_mfma_f32_16x16x4_f32 (exact products, the
 // lane's 8 k of a slab in any order as long as A and B agree).  Sums are fp32;
 // a bf16 result is rounded once, at the store.
+//
+// grouped_small takes the calls whose 64 x 64 tiles do not fill the card: a
+// workgroup computes a 32 x 32 tile with 8 waves that share out the depth in turn,
+// load their fragments straight into registers, two steps ahead, and add their sums
+// up in LDS, in order.  No barrier but that one: the loads of a whole call are in
+// flight together (777 fp32 rows over 5 experts of 509 x 301: 22 us in slabs).
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -102,7 +108,132 @@ __device__ __forceinline__ void put(__bf16* p, f32x4 v, int n) {
     if (i < n) p[i] = (__bf16)v[i];
 }
 
+// grouped_small: what a lane feeds to the 16 x 16 x STEP products of one step
+constexpr int SM = 32, SN = 32, SWAVES = 8;
+template <typename T> struct Small;
+template <> struct Small<float> {
+  static constexpr int STEP = 16, PER = 4;  // k of a step, of a lane in it
+  static __device__ __forceinline__ void mma(f32x4& c, const float (&b)[4], const float (&a)[4]) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) c = __builtin_amdgcn_mfma_f32_16x16x4f32(b[q], a[q], c, 0, 0, 0);
+  }
+};
+template <> struct Small<__bf16> {
+  static constexpr int STEP = 32, PER = 8;
+  static __device__ __forceinline__ void mma(f32x4& c, const __bf16 (&b)[8], const __bf16 (&a)[8]) {
+    bf16x8 bv, av;
+    __builtin_memcpy(&bv, b, 16);
+    __builtin_memcpy(&av, a, 16);
+    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bv, av, c, 0, 0, 0);
+  }
+};
+
+// PER elements along k from q, of which the first n exist, zeros for the others;
+// `ld` from one to the next unless KC
+template <typename T, bool KC, int PER>
+__device__ __forceinline__ void small_load(T (&v)[PER], const T* q, int64_t ld, int n) {
+  if (n >= PER) {
+    if constexpr (KC) {
+      __builtin_memcpy(v, q, sizeof(v));
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) v[i] = q[i * ld];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) v[i] = i < n ? q[KC ? i : i * ld] : (T)0.f;
+  }
+}
+
 }  // namespace gany
+
+template <typename T, typename U, bool WT, bool GRAD>
+__global__ void __launch_bounds__(64 * gany::SWAVES) grouped_small(GroupedArgs p) {
+  using namespace gany;
+  typedef Small<T> S;
+  constexpr bool A_KC = !GRAD, B_KC = WT && !GRAD;
+  __shared__ float sums[SWAVES][SM][SN + 4];
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int l16 = lane & 15, g = lane >> 4;
+  const T *a = (const T*)p.x, *b = (const T*)p.w;
+  U* c = (U*)p.y;
+  int rows, depth, n0;
+  if constexpr (GRAD) {
+    const int e = blockIdx.x / (p.tiles_k * p.tiles_n), t = blockIdx.x % (p.tiles_k * p.tiles_n);
+    const int k0 = t / p.tiles_n * SM;
+    n0 = t % p.tiles_n * SN;
+    const RowGroup gr = find_group(p.sizes, p.E, p.T, e);
+    a += (int64_t)gr.begin * p.ldx + k0;
+    b += (int64_t)gr.begin * p.ldw + n0;
+    c += e * p.stride_y + (int64_t)k0 * p.ldy + n0;
+    rows = min(p.K - k0, SM);
+    depth = gr.end - gr.begin;
+  } else {
+    n0 = blockIdx.x % p.tiles_n * SN;
+    const RowGroup gr = find_tile<SM>(p.sizes, p.E, p.T, blockIdx.x / p.tiles_n);
+    if (gr.e < 0) return;
+    a += (int64_t)gr.begin * p.ldx;
+    b += (gr.e < p.E ? gr.e : 0) * p.stride_w + (int64_t)n0 * (WT ? p.ldw : 1);
+    c += (int64_t)gr.begin * p.ldy + n0;
+    rows = min(gr.end - gr.begin, SM);
+    depth = gr.e < p.E ? p.K : 0;  // rows of no group: zeros
+  }
+  const int cols = min(p.N - n0, SN);
+  // the lane's elements of the wave's first step; rows and columns past the
+  // tile's edge repeat the last one and are not stored
+  constexpr int STRIDE = SWAVES * S::STEP, RING = 3;
+  const int k0 = wave * S::STEP, kl = k0 + g * S::PER;
+  const int64_t a_next = A_KC ? STRIDE : STRIDE * (int64_t)p.ldx, b_next = B_KC ? STRIDE : STRIDE * (int64_t)p.ldw;
+  const T *pa[2], *pb[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = min(l16 + 16 * i, rows - 1), n = min(l16 + 16 * i, cols - 1);
+    pa[i] = a + (A_KC ? (int64_t)r * p.ldx + kl : (int64_t)kl * p.ldx + r);
+    pb[i] = b + (B_KC ? (int64_t)n * p.ldw + kl : (int64_t)kl * p.ldw + n);
+  }
+  f32x4 acc[2][2] = {};
+  T av[RING][2][S::PER], bv[RING][2][S::PER];
+  int left = depth - kl;  // k from the lane's next element on
+  auto load = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      small_load<T, A_KC>(av[buf][i], pa[i], p.ldx, left);
+      small_load<T, B_KC>(bv[buf][i], pb[i], p.ldw, left);
+      pa[i] += a_next;
+      pb[i] += b_next;
+    }
+    left -= STRIDE;
+  };
+  const int steps = (depth - k0 + STRIDE - 1) / STRIDE;  // of this wave
+#pragma unroll
+  for (int s = 0; s < RING - 1; ++s)
+    if (s < steps) load(s);
+  for (int s = 0; s < steps; s += RING) {
+#pragma unroll
+    for (int q = 0; q < RING; ++q) {
+      if (s + q >= steps) break;
+      if (s + q + RING - 1 < steps) load((q + RING - 1) % RING);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) S::mma(acc[i][j], bv[q][j], av[q][i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) *(f32x4*)&sums[wave][i * 16 + l16][j * 16 + 4 * g] = acc[i][j];
+  __syncthreads();
+  for (int t = threadIdx.x; t < SM * SN; t += 64 * SWAVES) {
+    const int m = t / SN, n = t % SN;
+    if (m >= rows || n >= cols) continue;
+    float v = sums[0][m][n];
+#pragma unroll
+    for (int w = 1; w < SWAVES; ++w) v += sums[w][m][n];
+    c[(int64_t)m * p.ldy + n] = (U)v;
+  }
+}
 
 // T: operands, U: result; WT: w stored transposed ([N][K]; GRAD: unused)
 template <typename T, typename U, bool WT, bool GRAD>

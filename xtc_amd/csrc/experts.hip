@@ -12,8 +12,8 @@ namespace {
 
 // Largest extent: tiles and slabs past it stay within 32 bits.
 constexpr int kMost = 0x7fffffff - 1023;
-// 64 x 64 tiles of any operands that make them worth their barriers.
-constexpr int64_t kSmallTiles = 512;
+// Workgroups that fill the card, two a CU.
+constexpr int64_t kFill = 512;
 
 int check(const xtc_hip_grouped_matmul_desc* d, const char* what) {
   if (!core::ready()) return fail("xtc_hip_init not called");
@@ -42,31 +42,37 @@ void dma_launch(const DmaArgs& a, unsigned groups, hipStream_t s) {
   hipLaunchKernelGGL((grouped_dma<false, GRAD, B_ROW, WGM, WGN, TM, TN, STAGES, PP>), dim3(groups), dim3(WGM * WGN * 64), 0, s, a);
 }
 struct DmaTile {
-  int bm, bn;
+  DmaCost cost;
   DmaLaunch natural, transposed, grad;
 };
 #define XTC_DMA(...) &dma_launch<false, false, __VA_ARGS__>, &dma_launch<false, true, __VA_ARGS__>, &dma_launch<true, false, __VA_ARGS__>
+// Costs as measured: 8 rows over 8 experts, 1024 and 4096 deep (light), 8192^3 and
+// 4096 rows over 32 experts of 4096 x 2048 (full).
 const DmaTile kDmaTiles[] = {
-    {256, 256, XTC_DMA(2, 4, 8, 4, 4, true)},
-    {128, 128, XTC_DMA(2, 2, 4, 4, 4, false)},
-    {64, 64, XTC_DMA(2, 2, 2, 2, 4, false)},
+    {{256, 256, 1, 0.57, 0.80}, XTC_DMA(2, 4, 8, 4, 4, true)},
+    {{128, 128, 2, 0.29, 0.60}, XTC_DMA(2, 2, 4, 4, 4, false)},
+    {{64, 64, 4, 0.13, 0.73}, XTC_DMA(2, 2, 2, 2, 4, false)},
 };
 #undef XTC_DMA
 
 // Strides of whole vectors whose offsets within a tile stay within 2^31 bytes.
 bool vectors(const void* p, int ld) { return core::aligned16(p) && ld % 8 == 0 && ld < (1 << 22) - 8; }
 
-const DmaTile* dma_tile(int64_t rows, int64_t groups, int N, bool grad, int K) {
+// The cheapest tile for `slabs` of k a tile; grad: E matrices of K x N.
+const DmaTile& dma_tile(bool grad, int64_t T, int64_t E, int K, int N) {
+  const DmaTile* best = nullptr;
+  double least = 0;
   for (const DmaTile& t : kDmaTiles) {
-    const int64_t tn = (N + t.bn - 1) / t.bn;
-    const int64_t tm = grad ? groups * ((K + t.bm - 1) / t.bm) : rows / t.bm + 1;
-    if (tm * tn >= 192) return &t;
+    const double tn = (N + t.cost.bn - 1) / t.cost.bn, tk = (K + t.cost.bm - 1) / t.cost.bm;
+    const double cost = grad ? dma_cost(t.cost, E * tk * tn, T / (32.0 * E) + 1)
+                             : dma_cost(t.cost, likely_tiles(T, E, t.cost.bm) * tn, K / 32.0);
+    if (!best || cost < least) best = &t, least = cost;
   }
-  return &kDmaTiles[2];
+  return *best;
 }
 
 int launch_dma(const DmaTile& t, DmaLaunch run, DmaArgs& a, int64_t matrices, hipStream_t s) {
-  a.tiles_n = (a.N + t.bn - 1) / t.bn;
+  a.tiles_n = (a.N + t.cost.bn - 1) / t.cost.bn;
   a.band = a.tiles_m < 8 ? a.tiles_m : 8;
   const int64_t groups = dma_groups(a, matrices);
   if (groups < 1 || groups >= (int64_t)1 << 31) return fail("grouped_matmul: %lld workgroups are too many", (long long)groups);
@@ -75,37 +81,64 @@ int launch_dma(const DmaTile& t, DmaLaunch run, DmaArgs& a, int64_t matrices, hi
   return e == hipSuccess ? 0 : fail("grouped_matmul: launch failed: %s", hipGetErrorString(e));
 }
 
-// ---- any operands: 64 x 64 tiles, or 32 x 32 tiles of split depth where those
-// would leave the CUs idle
-template <bool GRAD>
-int launch_any(const xtc_hip_grouped_matmul_desc& d, GroupedArgs& a, hipStream_t s) {
-  auto tiles = [&](int bm, int bn) {
-    a.tiles_n = (a.N + bn - 1) / bn;
-    a.tiles_k = (a.K + bm - 1) / bm;
-    return a.tiles_n * (GRAD ? (int64_t)a.E * a.tiles_k : most_tiles(a.T, a.E, bm));
-  };
-  const bool small = tiles(gany::BM, gany::BN) < kSmallTiles;
-  const int64_t groups = small ? tiles(gany::SM, gany::SN) : tiles(gany::BM, gany::BN);
+// ---- any operands
+
+typedef void (*AnyLaunch)(const GroupedArgs&, unsigned, hipStream_t);
+template <typename T, typename U, bool WT, bool GRAD>
+void any_launch(const GroupedArgs& a, unsigned groups, hipStream_t s) {
+  hipLaunchKernelGGL((grouped_any<T, U, WT, GRAD>), dim3(groups), dim3(gany::NT), 0, s, a);
+}
+template <typename T, typename U, bool WT, bool GRAD, int TM, int TN>
+void small_launch(const GroupedArgs& a, unsigned groups, hipStream_t s) {
+  hipLaunchKernelGGL((grouped_small<T, U, WT, GRAD, TM, TN>), dim3(groups), dim3(64 * gany::SWAVES), 0, s, a);
+}
+struct AnyTile {
+  int bm, bn;
+  AnyLaunch run[3][3];  // natural, transposed, gradient of w; fp32, bf16 to fp32, bf16
+};
+#define XTC_TYPES(F, ...) {&F<float, float, __VA_ARGS__>, &F<__bf16, float, __VA_ARGS__>, &F<__bf16, __bf16, __VA_ARGS__>}
+#define XTC_SMALL(TM, TN) \
+  {16 * TM, 16 * TN, {XTC_TYPES(small_launch, false, false, TM, TN), XTC_TYPES(small_launch, true, false, TM, TN), {}}}
+const AnyTile kSlabs = {gany::BM, gany::BN, {XTC_TYPES(any_launch, false, false), XTC_TYPES(any_launch, true, false),
+                                            XTC_TYPES(any_launch, false, true)}};
+const AnyTile kSmall16 = XTC_SMALL(1, 1), kSmall32 = XTC_SMALL(1, 2), kSmall64 = XTC_SMALL(1, 4);
+const AnyTile kSmallGrad = {32, 32, {{}, {}, XTC_TYPES(small_launch, false, true, 2, 2)}};
+#undef XTC_SMALL
+#undef XTC_TYPES
+
+int launch_any(const xtc_hip_grouped_matmul_desc& d, const AnyTile& t, bool grad, GroupedArgs& a, hipStream_t s) {
+  a.tiles_n = (a.N + t.bn - 1) / t.bn;
+  a.tiles_k = (a.K + t.bm - 1) / t.bm;
+  const int64_t groups = a.tiles_n * (grad ? (int64_t)a.E * a.tiles_k : most_tiles(a.T, a.E, t.bm));
   if (groups < 1 || groups >= (int64_t)1 << 31) return fail("grouped_matmul: %lld workgroups are too many", (long long)groups);
-  const dim3 grid((unsigned)groups), block(small ? 64 * gany::SWAVES : gany::NT);
-  const bool wt = !GRAD && d.trans_w, out16 = d.out_dtype == XTC_HIP_BF16;
-#define XTC_ANY_OF(KERNEL, T, U)                                                      \
-  do {                                                                                \
-    if (wt) hipLaunchKernelGGL((KERNEL<T, U, !GRAD, GRAD>), grid, block, 0, s, a);    \
-    else hipLaunchKernelGGL((KERNEL<T, U, false, GRAD>), grid, block, 0, s, a);       \
-  } while (0)
-#define XTC_ANY(T, U)                                  \
-  do {                                                 \
-    if (small) XTC_ANY_OF(grouped_small, T, U);        \
-    else XTC_ANY_OF(grouped_any, T, U);                \
-  } while (0)
-  if (d.dtype == XTC_HIP_F32) XTC_ANY(float, float);
-  else if (out16) XTC_ANY(__bf16, __bf16);
-  else XTC_ANY(__bf16, float);
-#undef XTC_ANY
-#undef XTC_ANY_OF
+  t.run[grad ? 2 : d.trans_w ? 1 : 0][d.dtype == XTC_HIP_F32 ? 0 : 1 + d.out_dtype](a, (unsigned)groups, s);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? 0 : fail("grouped_matmul: launch failed: %s", hipGetErrorString(e));
+}
+
+// Tiles that a call has at most.
+int64_t tiles_of(const AnyTile& t, bool grad, const GroupedArgs& a) {
+  const int64_t n = (a.N + t.bn - 1) / t.bn;
+  return n * (grad ? (int64_t)a.E * ((a.K + t.bm - 1) / t.bm) : most_tiles(a.T, a.E, t.bm));
+}
+
+// Few rows a group: the matrices are streamed once, by waves that share out their
+// depth.  Matrices in rows of n are read 64 columns wide (8 rows over 8 experts of
+// 4096 x 2048: 19 us, 25 at 32 columns, DMA tiles 27), matrices in rows of k 16
+// columns a tile (16 us, 22; DMA 21).  From 8 and 4 rows a group on DMA tiles are
+// as fast (8: 31 and 35 us against 35 and 33).
+const AnyTile* stream_tile(bool trans_w, const GroupedArgs& a) {
+  const int rows = trans_w ? 4 : 8;
+  return a.T > rows * (int64_t)a.E ? nullptr : trans_w ? &kSmall16 : &kSmall64;
+}
+
+// Any operands: tiles of shared depth where those of slabs would not fill the
+// card, the wider ones where they do.  777 fp32 rows over 5 experts of 509 x 301:
+// 10 us (32 columns), 22 in slabs; 4096 bf16 rows over 8 of 1001 x 999: 103, 68.
+const AnyTile& any_tile(bool grad, const GroupedArgs& a) {
+  if (tiles_of(kSlabs, grad, a) >= kFill) return kSlabs;
+  if (grad) return kSmallGrad;
+  return tiles_of(kSmall64, false, a) >= kFill ? kSmall64 : kSmall32;
 }
 
 }  // namespace
@@ -130,18 +163,20 @@ int xtc_hip_grouped_matmul(const xtc_hip_grouped_matmul_desc* desc, const void* 
   const int64_t matrix = (int64_t)(d.trans_w ? d.N : d.K) * a.ldw;
   a.stride_w = d.stride_w ? d.stride_w : matrix;
   if (a.stride_w < 0) return fail("%s: negative stride between matrices", what);
+  const hipStream_t s = core::pick_stream(d.stream);
+  if (const AnyTile* t = stream_tile(d.trans_w, a)) return launch_any(d, *t, false, a, s);
   if (d.dtype == XTC_HIP_BF16 && d.K % 8 == 0 && (d.trans_w || d.N % 8 == 0) && vectors(x, a.ldx) && vectors(w, a.ldw) &&
       a.stride_w % 8 == 0) {
-    const DmaTile& t = *dma_tile(d.T, d.E, d.N, false, d.K);
+    const DmaTile& t = dma_tile(false, d.T, d.E, d.K, d.N);
     DmaArgs v{};
     v.a = (const uint8_t*)x, v.b = (const uint8_t*)w, v.sizes = sizes, v.c = y;
     v.stride_b = 2 * a.stride_w;
     v.E = d.E, v.M = d.T, v.N = d.N, v.K = d.K / 8;
     v.lda = 2 * a.ldx, v.ldb = 2 * a.ldw, v.ldc = a.ldy, v.out16 = d.out_dtype == XTC_HIP_BF16;
-    v.tiles_m = (int)most_tiles(d.T, d.E, t.bm);
-    return launch_dma(t, d.trans_w ? t.transposed : t.natural, v, 1, core::pick_stream(d.stream));
+    v.tiles_m = (int)most_tiles(d.T, d.E, t.cost.bm);
+    return launch_dma(t, d.trans_w ? t.transposed : t.natural, v, 1, s);
   }
-  return launch_any<false>(d, a, core::pick_stream(d.stream));
+  return launch_any(d, any_tile(false, a), false, a, s);
 }
 
 int xtc_hip_grouped_matmul_grad_w(const xtc_hip_grouped_matmul_desc* desc, const void* x, const void* dy,
@@ -161,16 +196,16 @@ int xtc_hip_grouped_matmul_grad_w(const xtc_hip_grouped_matmul_desc* desc, const
   a.stride_y = d.stride_w ? d.stride_w : matrix;
   if (a.stride_y < matrix) return fail("%s: a stride of %lld lets the gradients of two groups overlap", what, (long long)d.stride_w);
   if (d.dtype == XTC_HIP_BF16 && d.K % 8 == 0 && d.N % 8 == 0 && vectors(x, a.ldx) && vectors(dy, a.ldw)) {
-    const DmaTile& t = *dma_tile(d.T, d.E, d.N, true, d.K);
+    const DmaTile& t = dma_tile(true, d.T, d.E, d.K, d.N);
     DmaArgs v{};
     v.a = (const uint8_t*)x, v.b = (const uint8_t*)dy, v.sizes = sizes, v.c = dw;
     v.stride_c = a.stride_y;
     v.E = d.E, v.M = d.T, v.N = d.N, v.K = d.K;
     v.lda = 2 * a.ldx, v.ldb = 2 * a.ldw, v.ldc = a.ldy, v.out16 = d.out_dtype == XTC_HIP_BF16;
-    v.tiles_m = (d.K + t.bm - 1) / t.bm;
+    v.tiles_m = (d.K + t.cost.bm - 1) / t.cost.bm;
     return launch_dma(t, t.grad, v, d.E, core::pick_stream(d.stream));
   }
-  return launch_any<true>(d, a, core::pick_stream(d.stream));
+  return launch_any(d, any_tile(true, a), true, a, core::pick_stream(d.stream));
 }
 
 }  // extern "C"

@@ -15,8 +15,9 @@
 // lane's 8 k of a slab in any order as long as A and B agree).  Sums are fp32;
 // a bf16 result is rounded once, at the store.
 //
-// grouped_small takes the calls whose 64 x 64 tiles do not fill the card: a
-// workgroup computes a 32 x 32 tile with 8 waves that share out the depth in turn,
+// grouped_small takes the calls whose 64 x 64 tiles do not fill the card, and few
+// rows a group (then it streams the matrices): a workgroup computes a tile of 16
+// or 32 rows with 8 waves that share out the depth in turn,
 // load their fragments straight into registers, two steps ahead, and add their sums
 // up in LDS, in order.  No barrier but that one: the loads of a whole call are in
 // flight together (777 fp32 rows over 5 experts of 509 x 301: 22 us in slabs).
@@ -108,8 +109,8 @@ __device__ __forceinline__ void put(__bf16* p, f32x4 v, int n) {
     if (i < n) p[i] = (__bf16)v[i];
 }
 
-// grouped_small: what a lane feeds to the 16 x 16 x STEP products of one step
-constexpr int SM = 32, SN = 32, SWAVES = 8;
+// grouped_small: what a lane feeds to the 16 x 16 products of one step
+constexpr int SWAVES = 8;
 template <typename T> struct Small;
 template <> struct Small<float> {
   static constexpr int STEP = 16, PER = 4;  // k of a step, of a lane in it
@@ -128,30 +129,74 @@ template <> struct Small<__bf16> {
   }
 };
 
-// PER elements along k from q, of which the first n exist, zeros for the others;
-// `ld` from one to the next unless KC
-template <typename T, bool KC, int PER>
-__device__ __forceinline__ void small_load(T (&v)[PER], const T* q, int64_t ld, int n) {
-  if (n >= PER) {
+// An operand's part of a step: W fragments of 16 rows (or columns) each.
+// KC: k contiguous, a lane takes PER k of rows l16, 16 + l16, ...; otherwise its W
+// neighbouring rows W l16 .. W l16 + W - 1 at PER k, loaded together.
+template <typename T, bool KC, int W>
+struct SmallOperand {
+  static constexpr int PER = Small<T>::PER;
+  const T* at[KC ? W : 1];
+  int64_t ld, next;  // between k rows; to the wave's next step
+  int lines;         // !KC: rows from the lane's first to the tile's edge
+
+  static __device__ __forceinline__ int line(int w, int l16) { return KC ? 16 * w + l16 : W * l16 + w; }
+
+  // lines past the tile's `edge` repeat the last one (KC) or are zeros
+  __device__ __forceinline__ void set(const T* p, int64_t stride, int l16, int k, int edge, int step) {
+    ld = stride;
+    next = KC ? step : step * stride;
+    lines = edge - W * l16;
     if constexpr (KC) {
-      __builtin_memcpy(v, q, sizeof(v));
+#pragma unroll
+      for (int w = 0; w < W; ++w) at[w] = p + min(line(w, l16), edge - 1) * stride + k;
     } else {
-#pragma unroll
-      for (int i = 0; i < PER; ++i) v[i] = q[i * ld];
+      at[0] = p + k * stride + W * l16;
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < PER; ++i) v[i] = i < n ? q[KC ? i : i * ld] : (T)0.f;
   }
-}
+  // the step's fragments, `left` k from the lane's first one to the end; then on
+  // to the next step
+  __device__ __forceinline__ void load(T (&v)[W][PER], int left) {
+    if constexpr (KC) {
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        if (left >= PER) {
+          __builtin_memcpy(v[w], at[w], sizeof(v[w]));
+        } else {
+#pragma unroll
+          for (int i = 0; i < PER; ++i) v[w][i] = i < left ? at[w][i] : (T)0.f;
+        }
+        at[w] += next;
+      }
+    } else {
+      T raw[PER][W];
+      if (left >= PER && lines >= W) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) __builtin_memcpy(raw[i], at[0] + i * ld, sizeof(raw[i]));
+      } else {
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+#pragma unroll
+          for (int w = 0; w < W; ++w) raw[i][w] = i < left && w < lines ? at[0][i * ld + w] : (T)0.f;
+      }
+#pragma unroll
+      for (int w = 0; w < W; ++w)
+#pragma unroll
+        for (int i = 0; i < PER; ++i) v[w][i] = raw[i][w];
+      at[0] += next;
+    }
+  }
+};
 
 }  // namespace gany
 
-template <typename T, typename U, bool WT, bool GRAD>
+// 16 TM x 16 TN tiles.
+template <typename T, typename U, bool WT, bool GRAD, int TM, int TN>
 __global__ void __launch_bounds__(64 * gany::SWAVES) grouped_small(GroupedArgs p) {
   using namespace gany;
   typedef Small<T> S;
-  constexpr bool A_KC = !GRAD, B_KC = WT && !GRAD;
+  typedef SmallOperand<T, !GRAD, TM> OpA;
+  typedef SmallOperand<T, WT && !GRAD, TN> OpB;
+  constexpr int SM = 16 * TM, SN = 16 * TN;
   __shared__ float sums[SWAVES][SM][SN + 4];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -180,29 +225,19 @@ __global__ void __launch_bounds__(64 * gany::SWAVES) grouped_small(GroupedArgs p
     depth = gr.e < p.E ? p.K : 0;  // rows of no group: zeros
   }
   const int cols = min(p.N - n0, SN);
-  // the lane's elements of the wave's first step; rows and columns past the
-  // tile's edge repeat the last one and are not stored
+
   constexpr int STRIDE = SWAVES * S::STEP, RING = 3;
   const int k0 = wave * S::STEP, kl = k0 + g * S::PER;
-  const int64_t a_next = A_KC ? STRIDE : STRIDE * (int64_t)p.ldx, b_next = B_KC ? STRIDE : STRIDE * (int64_t)p.ldw;
-  const T *pa[2], *pb[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = min(l16 + 16 * i, rows - 1), n = min(l16 + 16 * i, cols - 1);
-    pa[i] = a + (A_KC ? (int64_t)r * p.ldx + kl : (int64_t)kl * p.ldx + r);
-    pb[i] = b + (B_KC ? (int64_t)n * p.ldw + kl : (int64_t)kl * p.ldw + n);
-  }
-  f32x4 acc[2][2] = {};
-  T av[RING][2][S::PER], bv[RING][2][S::PER];
+  OpA oa;
+  OpB ob;
+  oa.set(a, p.ldx, l16, kl, rows, STRIDE);
+  ob.set(b, p.ldw, l16, kl, cols, STRIDE);
+  f32x4 acc[TM][TN] = {};
+  T av[RING][TM][S::PER], bv[RING][TN][S::PER];
   int left = depth - kl;  // k from the lane's next element on
   auto load = [&](int buf) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      small_load<T, A_KC>(av[buf][i], pa[i], p.ldx, left);
-      small_load<T, B_KC>(bv[buf][i], pb[i], p.ldw, left);
-      pa[i] += a_next;
-      pb[i] += b_next;
-    }
+    ob.load(bv[buf], left);
+    oa.load(av[buf], left);
     left -= STRIDE;
   };
   const int steps = (depth - k0 + STRIDE - 1) / STRIDE;  // of this wave
@@ -215,15 +250,17 @@ __global__ void __launch_bounds__(64 * gany::SWAVES) grouped_small(GroupedArgs p
       if (s + q >= steps) break;
       if (s + q + RING - 1 < steps) load((q + RING - 1) % RING);
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) S::mma(acc[i][j], bv[q][j], av[q][i]);
+        for (int j = 0; j < TN; ++j) S::mma(acc[i][j], bv[q][j], av[q][i]);
     }
   }
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < TM; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j) *(f32x4*)&sums[wave][i * 16 + l16][j * 16 + 4 * g] = acc[i][j];
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sums[wave][OpA::line(i, l16)][OpB::line(j, 4 * g + r)] = acc[i][j][r];
   __syncthreads();
   for (int t = threadIdx.x; t < SM * SN; t += 64 * SWAVES) {
     const int m = t / SN, n = t % SN;

@@ -43,6 +43,7 @@
 // 32 CUs then share 8 panels of A and 4 of B in its L2.
 #pragma once
 #include <hip/hip_runtime.h>
+#include <math.h>
 #include <stdint.h>
 
 #include <type_traits>
@@ -485,6 +486,23 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_dma(DmaArgs p) {
     }
   }
 }
+
+// What a tile's slab costs, from which the calls choose their tiles: microseconds
+// where a CU has one workgroup and the others none, and where every CU is full.
+struct DmaCost {
+  int bm, bn, per_cu;
+  double light, full;
+};
+// `tiles` of `slabs` on 256 CUs, without what every tile has in common.  Small
+// tiles even out over the CUs; a 256 x 256 one takes a CU for itself, so a last
+// round of few tiles costs as much as a full one.
+inline double dma_cost(const DmaCost& c, double tiles, double slabs) {
+  const double load = tiles / (256.0 * c.per_cu);
+  if (load <= 1) return slabs * (c.light + (c.full - c.light) * load);
+  return slabs * c.full * (c.per_cu == 1 ? ceil(load) : load);
+}
+// Tiles of bm rows that a fair share of T rows to E groups makes.
+inline double likely_tiles(double T, double E, int bm) { return fmax(fmin(E, T), T / bm + 0.5 * fmin(E, T)); }
 
 // Workgroups of `a` (its tiles and band set): bands and runs filled up.
 inline int64_t dma_groups(const DmaArgs& a, int64_t matrices) {

@@ -4,6 +4,7 @@
 #include "core.hpp"
 #include "grouped_dma.hpp"
 #include "mx4_any.hpp"
+#include "mx4_rows.hpp"
 
 using namespace xtc_hip;
 using core::aligned16;
@@ -65,23 +66,50 @@ int quantize(const xtc_hip_mx4_desc& d, const Mx4QuantArgs& a, const char* what)
 // ---- products of whole slabs (4 blocks)
 
 struct DmaTile {
-  int bm, bn;
+  DmaCost cost;
   void (*launch)(const DmaArgs&, unsigned, hipStream_t);
 };
 template <int WGM, int WGN, int TM, int TN, int STAGES, bool PP>
 void dma_launch(const DmaArgs& a, unsigned groups, hipStream_t s) {
   hipLaunchKernelGGL((grouped_dma<true, false, true, WGM, WGN, TM, TN, STAGES, PP>), dim3(groups), dim3(WGM * WGN * 64), 0, s, a);
 }
+// Costs as measured: 1 x 8192 x 8192 (light), 4096 x 8192 x 8192 and 8192^3 (full).
 const DmaTile kDmaTiles[] = {
-    {256, 256, &dma_launch<2, 4, 8, 4, 4, true>},
-    {128, 128, &dma_launch<2, 2, 4, 4, 4, false>},
-    {64, 64, &dma_launch<2, 2, 2, 2, 4, false>},
+    {{256, 256, 1, 0.53, 1.20}, &dma_launch<2, 4, 8, 4, 4, true>},
+    {{128, 128, 2, 0.27, 0.87}, &dma_launch<2, 2, 4, 4, 4, false>},
+    {{64, 64, 4, 0.15, 0.81}, &dma_launch<2, 2, 2, 2, 4, false>},
 };
 
-const DmaTile& dma_tile(int64_t rows, int N) {
-  for (const DmaTile& t : kDmaTiles)
-    if ((rows / t.bm + 1) * ((N + t.bn - 1) / t.bn) >= 192) return t;
-  return kDmaTiles[2];
+const DmaTile& dma_tile(int64_t rows, int64_t groups, int N, int blocks) {
+  const DmaTile* best = nullptr;
+  double least = 0;
+  for (const DmaTile& t : kDmaTiles) {
+    const double cost = dma_cost(t.cost, likely_tiles(rows, groups, t.cost.bm) * ((N + t.cost.bn - 1) / t.cost.bn), blocks / 4);
+    if (!best || cost < least) best = &t, least = cost;
+  }
+  return *best;
+}
+
+// ---- few rows
+
+struct RowsTile {
+  int bm, bn;
+  void (*run[2])(const Mx4Args&, unsigned, hipStream_t);  // to fp32, to bf16
+};
+template <typename U, int TM, int TN>
+void rows_launch(const Mx4Args& a, unsigned groups, hipStream_t s) {
+  hipLaunchKernelGGL((mx4_rows<U, TM, TN>), dim3(groups), dim3(64 * mx4::RWAVES), 0, s, a);
+}
+const RowsTile kRows16 = {16, 32, {&rows_launch<float, 1, 2>, &rows_launch<__bf16, 1, 2>}};
+const RowsTile kRows32 = {32, 32, {&rows_launch<float, 2, 2>, &rows_launch<__bf16, 2, 2>}};
+
+// Whole slabs: up to 16 rows of one product (x 8192 x 8192: 9.9 us, DMA tiles
+// 13.8) and up to 32 (12.3, 14.0); by group DMA tiles are as fast (32 rows over 16
+// experts of 4096 x 2048: 16.4, 13.3).  Otherwise up to 32 rows a group: beyond,
+// tiles that read their operands once for 64 rows.
+const RowsTile* rows_tile(int64_t rows, int64_t groups, bool slabs) {
+  if (slabs && groups > 1) return nullptr;
+  return rows <= 16 * groups ? &kRows16 : rows <= 32 * groups ? &kRows32 : nullptr;
 }
 
 }  // namespace
@@ -146,15 +174,23 @@ int xtc_hip_mx4_matmul(const xtc_hip_mx4_matmul_desc* desc, const uint8_t* a_cod
   Mx4Args a{};
   a.a_codes = a_codes, a.a_scales = a_scales, a.b_codes = b_codes, a.b_scales = b_scales, a.sizes = sizes, a.c = c;
   a.E = d.E > 0 ? d.E : 1, a.M = d.M, a.N = d.N, a.blocks = d.blocks, a.ldc = d.ldc ? d.ldc : d.N;
-  if (d.blocks % 4 == 0 && d.blocks < (1 << 19) && ((uintptr_t)a_scales & 3) == 0 && ((uintptr_t)b_scales & 3) == 0) {
-    const DmaTile& t = dma_tile(d.M, d.N);
+  const bool slabs = d.blocks % 4 == 0 && d.blocks < (1 << 19) && ((uintptr_t)a_scales & 3) == 0 && ((uintptr_t)b_scales & 3) == 0;
+  if (const RowsTile* t = rows_tile(d.M, a.E, slabs)) {
+    a.tiles_n = (d.N + t->bn - 1) / t->bn;
+    const int64_t groups = a.tiles_n * (sizes ? most_tiles(d.M, d.E, t->bm) : ((int64_t)d.M + t->bm - 1) / t->bm);
+    if (groups >= (int64_t)1 << 31) return fail("%s: %lld workgroups are too many", what, (long long)groups);
+    t->run[d.out_dtype](a, (unsigned)groups, core::pick_stream(d.stream));
+    return done(what);
+  }
+  if (slabs) {
+    const DmaTile& t = dma_tile(d.M, a.E, d.N, d.blocks);
     DmaArgs v{};
     v.a = a_codes, v.b = b_codes, v.sa = a_scales, v.sb = b_scales, v.sizes = sizes, v.c = c;
     v.E = a.E, v.M = d.M, v.N = d.N, v.K = d.blocks;
     v.lda = v.ldb = 16 * d.blocks, v.ldc = a.ldc;
     v.stride_b = (int64_t)d.N * v.ldb, v.stride_sb = (int64_t)d.N * d.blocks;
-    v.tiles_m = (int)(sizes ? most_tiles(d.M, d.E, t.bm) : ((int64_t)d.M + t.bm - 1) / t.bm);
-    v.tiles_n = (d.N + t.bn - 1) / t.bn;
+    v.tiles_m = (int)(sizes ? most_tiles(d.M, d.E, t.cost.bm) : ((int64_t)d.M + t.cost.bm - 1) / t.cost.bm);
+    v.tiles_n = (d.N + t.cost.bn - 1) / t.cost.bn;
     v.band = v.tiles_m < 8 ? v.tiles_m : 8;
     v.out16 = d.out_dtype == XTC_HIP_BF16;
     const int64_t groups = dma_groups(v, 1);

@@ -1,0 +1,136 @@
+// SPDX-License-Identifier: BSD-3-Clause
+// Microscaled 4-bit products of few rows, where the cost is reading b once:
+//   c[m, n] = sum_k a[m, k] b[n, k], the rows of a by group as in mx4_any.hpp.
+//
+// A workgroup computes 16 TM rows x 16 TN columns with 8 waves that share out
+// the blocks of k in turn, load their fragments straight into registers, a step
+// ahead, and add their sums up in LDS, in order.  k may be summed in any order as
+// long as a and b agree, so a lane takes 4 neighbouring blocks of its row (64
+// bytes of codes, 4 scales in one load) and feeds them to four
+// v_mfma_scale_f32_16x16x128_f8f6f4 one after the other, each picking its byte of
+// the scales: a step reads 256 bytes of every row (a block a lane and step: 16 x
+// 8192 x 8192 17 us).
+// Bound by memory: 16 x 8192 x 8192 reads 36 MB in 9.9 us.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "mx4_any.hpp"
+
+namespace xtc_hip {
+
+namespace mx4 {
+
+constexpr int RWAVES = 8;
+
+// one step's part of a row: 4 blocks and their scales
+struct Run {
+  u32x4 codes[4];
+  unsigned scales;
+};
+
+// `left` of the 4 blocks at `codes` exist; the others are zeros of scale 1
+__device__ __forceinline__ void load_run(Run& r, const uint8_t* codes, const uint8_t* scales, int left) {
+  if (left >= 4) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r.codes[j] = *(const u32x4*)(codes + 16 * j);
+    __builtin_memcpy(&r.scales, scales, 4);
+  } else {
+    r.scales = 0x7f7f7f7fu;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      r.codes[j] = u32x4{0, 0, 0, 0};
+      if (j < left) {
+        r.codes[j] = *(const u32x4*)(codes + 16 * j);
+        r.scales ^= (0x7fu ^ scales[j]) << (8 * j);
+      }
+    }
+  }
+}
+
+template <int BYTE>
+__device__ __forceinline__ f32x4 mfma_byte(u32x4 a, unsigned sa, u32x4 b, unsigned sb, f32x4 c) {
+  const i32x8 av = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0};
+  const i32x8 bv = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 4, BYTE, (int)sa, BYTE, (int)sb);
+}
+
+}  // namespace mx4
+
+template <typename U, int TM, int TN>
+__global__ void __launch_bounds__(64 * mx4::RWAVES) mx4_rows(Mx4Args p) {
+  using namespace mx4;
+  constexpr int SM = 16 * TM, SN = 16 * TN, STEP = 16, RING = 2;  // blocks of a step, steps in registers
+  __shared__ float sums[RWAVES][SM][SN + 4];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int l16 = lane & 15, g = lane >> 4;
+  const int mt = blockIdx.x / p.tiles_n, n0 = blockIdx.x % p.tiles_n * SN;
+  RowGroup gr{0, mt * SM, p.M};
+  if (p.sizes) gr = find_tile<SM>(p.sizes, p.E, p.M, mt);
+  if (gr.e < 0) return;
+  const int blocks = gr.e < p.E ? p.blocks : 0;  // rows of no group: zeros
+  const int e = gr.e < p.E ? gr.e : 0;
+  const int rows = min(gr.end - gr.begin, SM), cols = min(p.N - n0, SN);
+
+  // the lane's first block of each of its rows; rows past the tile's edge repeat
+  // the last one and are not stored
+  const int first = wave * STEP + g * 4;
+  int64_t at_a[TM], at_b[TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i) at_a[i] = (int64_t)(gr.begin + min(16 * i + l16, rows - 1)) * p.blocks + first;
+#pragma unroll
+  for (int j = 0; j < TN; ++j) at_b[j] = ((int64_t)e * p.N + n0 + min(16 * j + l16, cols - 1)) * p.blocks + first;
+  Run a[RING][TM], b[RING][TN];
+  int left = blocks - first;
+  auto load = [&](int buf) {
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      load_run(b[buf][j], p.b_codes + at_b[j] * 16, p.b_scales + at_b[j], left);
+      at_b[j] += RWAVES * STEP;
+    }
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      load_run(a[buf][i], p.a_codes + at_a[i] * 16, p.a_scales + at_a[i], left);
+      at_a[i] += RWAVES * STEP;
+    }
+    left -= RWAVES * STEP;
+  };
+  f32x4 acc[TM][TN] = {};
+  const int steps = (blocks - wave * STEP + RWAVES * STEP - 1) / (RWAVES * STEP);  // of this wave
+#pragma unroll
+  for (int s = 0; s < RING - 1; ++s)
+    if (s < steps) load(s);
+  for (int s = 0; s < steps; s += RING) {
+#pragma unroll
+    for (int q = 0; q < RING; ++q) {
+      if (s + q >= steps) break;
+      if (s + q + RING - 1 < steps) load((q + RING - 1) % RING);
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          const Run &ra = a[q][i], &rb = b[q][j];
+          f32x4& c = acc[i][j];
+          c = mfma_byte<0>(rb.codes[0], rb.scales, ra.codes[0], ra.scales, c);
+          c = mfma_byte<1>(rb.codes[1], rb.scales, ra.codes[1], ra.scales, c);
+          c = mfma_byte<2>(rb.codes[2], rb.scales, ra.codes[2], ra.scales, c);
+          c = mfma_byte<3>(rb.codes[3], rb.scales, ra.codes[3], ra.scales, c);
+        }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) *(f32x4*)&sums[wave][16 * i + l16][16 * j + 4 * g] = acc[i][j];
+  __syncthreads();
+  for (int t = threadIdx.x; t < SM * SN; t += 64 * RWAVES) {
+    const int m = t / SN, n = t % SN;
+    if (m >= rows || n >= cols) continue;
+    float v = sums[0][m][n];
+#pragma unroll
+    for (int w = 1; w < RWAVES; ++w) v += sums[w][m][n];
+    ((U*)p.c)[(int64_t)(gr.begin + m) * p.ldc + n0 + n] = (U)v;
+  }
+}
+
+}  // namespace xtc_hip

@@ -97,3 +97,23 @@ out.append(mx4_matmul((None,) * 6, M=0))
 out.append(mx4("xtc_hip_mx4_quantize", (None,) * 4, rows=0))
 """)
     assert got == [[]] * 3
+
+
+def test_gradients_are_split_where_scratch_can_be_had(run):  # noqa: F811
+    """Few tiles over many rows: in parts with scratch of the stream; one part on a
+    stream that is being captured and where there is no memory."""
+    got = run(CALLS + """
+def grad():
+    return grouped("xtc_hip_grouped_matmul_grad_w", E=1, T=32768, K=256, N=256)
+fake.fake_memory(1 << 10)
+out.append(grad())
+fake.fake_memory((1 << 32) - 1)
+fake.fake_capturing(1)
+out.append(grad())
+fake.fake_capturing(0)
+out.append(grad())
+""")
+    (none,), (captured,), (split, total) = got  # a second kernel adds the parts up
+    assert none == captured and none[0] == split[0] and total[0] == "grouped_grad_sum"
+    # 16 tiles in 16 parts; grids are filled up to whole runs (128 workgroups)
+    assert (int(none[1].split()[0]), int(split[1].split()[0])) == (128, 256)

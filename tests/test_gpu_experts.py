@@ -271,3 +271,17 @@ def test_large_gradient_tiles(out, K, N, sizes):
     x, dy = ints(23, (T, K), 3), ints(24, (T, N), 3)
     print(f"[experts gradient tiles] {out} {T}x{K}x{N}", flush=True)
     np.testing.assert_array_equal(grad_w(x, dy, sizes, "bfloat16", out), rounded(plain_grad_w(x, dy, sizes), out))
+
+
+# gradients of few tiles over many rows, summed in parts: groups of many slabs, of
+# one, of none, of fewer slabs than parts; tiles of every size, cut by K and N
+@pytest.mark.parametrize("out", ["float32", "bfloat16"])
+@pytest.mark.parametrize("K,N,sizes", [(64, 72, [4000]), (264, 520, [3000, 0, 40, 2900]), (128, 136, [1500, 31, 33, 1, 0, 2500]),
+                                       (520, 264, [6000]), (1032, 776, [5000, 20])])
+def test_gradients_in_parts(out, K, N, sizes):
+    T = sum(sizes) + 3
+    x, dy = ints(25, (T, K), 3), ints(26, (T, N), 3)
+    print(f"[experts parts] {out} {T}x{K}x{N}", flush=True)
+    want = rounded(plain_grad_w(x, dy, sizes), out)
+    for _ in range(2):  # the counters are left as they were
+        np.testing.assert_array_equal(grad_w(x, dy, sizes, "bfloat16", out, pad=(8, 8, 8)), want)

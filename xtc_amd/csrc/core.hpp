@@ -16,6 +16,12 @@ bool ready();
 // `stream`, or the library stream where it is null.
 hipStream_t pick_stream(void* stream);
 
+// `bytes` of scratch of stream `s` for partial sums (xtc_hip_matmul's), or null where
+// there is none: the stream is being captured (a graph must not keep the address
+// of a buffer that a later call replaces) or the memory cannot be had; the call
+// then sums in one part.
+float* partial_sums(size_t bytes, hipStream_t s);
+
 inline bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
 }  // namespace core

@@ -12,6 +12,8 @@ namespace {
 
 // Largest extent: tiles and slabs past it stay within 32 bits.
 constexpr int kMost = 0x7fffffff - 1023;
+// Bytes of partial sums that a split gradient may write and read.
+constexpr double kMostPartial = 1 << 28;
 // Workgroups that fill the card, two a CU.
 constexpr int64_t kFill = 512;
 
@@ -58,15 +60,36 @@ const DmaTile kDmaTiles[] = {
 // Strides of whole vectors whose offsets within a tile stay within 2^31 bytes.
 bool vectors(const void* p, int ld) { return core::aligned16(p) && ld % 8 == 0 && ld < (1 << 22) - 8; }
 
-// The cheapest tile for `slabs` of k a tile; grad: E matrices of K x N.
-const DmaTile& dma_tile(bool grad, int64_t T, int64_t E, int K, int N) {
+const DmaTile& dma_tile(int64_t T, int64_t E, int K, int N) {
   const DmaTile* best = nullptr;
   double least = 0;
   for (const DmaTile& t : kDmaTiles) {
-    const double tn = (N + t.cost.bn - 1) / t.cost.bn, tk = (K + t.cost.bm - 1) / t.cost.bm;
-    const double cost = grad ? dma_cost(t.cost, E * tk * tn, T / (32.0 * E) + 1)
-                             : dma_cost(t.cost, likely_tiles(T, E, t.cost.bm) * tn, K / 32.0);
+    const double cost = dma_cost(t.cost, likely_tiles(T, E, t.cost.bm) * ((N + t.cost.bn - 1) / t.cost.bn), K / 32.0);
     if (!best || cost < least) best = &t, least = cost;
+  }
+  return *best;
+}
+
+// The tile of E gradients of K x N and into how many parts each group's rows go.
+// The largest group decides where tiles are few (of a skewed choice it has some 1.7
+// times the mean), the sum of all where they are many; writing out a tile and
+// starting on it take 4 us for each 64 of its rows.  A part pays for writing and
+// reading its partial sums (4 MB a microsecond), all together for one more launch,
+// 4 us.  32768 rows: 1 matrix of 128 x 128 163 us whole, 18 in 16 parts of 64 x 64
+// tiles; 8 of 512 x 512 55 and 49 (4 parts of 128 x 128); 4096 rows, 8 of 512 x
+// 512, 11 us whole, 25 in parts.
+const DmaTile& grad_tile(int64_t T, int64_t E, int K, int N, int* splits) {
+  const DmaTile* best = nullptr;
+  double least = 0;
+  const double all = T / (32.0 * E) + 1, skew = E > 1 ? 1.7 : 1, plane = 8.0 * E * K * N;
+  for (const DmaTile& t : kDmaTiles) {
+    const DmaCost& c = t.cost;
+    const double tiles = E * (double)((K + c.bm - 1) / c.bm) * ((N + c.bn - 1) / c.bn);
+    for (int s = 1; s <= 16 && (s == 1 || (all / s >= 4 && s * plane <= kMostPartial)); s *= 2) {
+      const double slabs = all / s, load = tiles * s / (256.0 * c.per_cu);
+      const double cost = slabs * fmax(c.light * skew, c.full * load) + c.bm / 16 + (s > 1 ? 4 + s * plane / 4e6 : 0);
+      if (!best || cost < least) best = &t, least = cost, *splits = s;
+    }
   }
   return *best;
 }
@@ -167,7 +190,7 @@ int xtc_hip_grouped_matmul(const xtc_hip_grouped_matmul_desc* desc, const void* 
   if (const AnyTile* t = stream_tile(d.trans_w, a)) return launch_any(d, *t, false, a, s);
   if (d.dtype == XTC_HIP_BF16 && d.K % 8 == 0 && (d.trans_w || d.N % 8 == 0) && vectors(x, a.ldx) && vectors(w, a.ldw) &&
       a.stride_w % 8 == 0) {
-    const DmaTile& t = dma_tile(false, d.T, d.E, d.K, d.N);
+    const DmaTile& t = dma_tile(d.T, d.E, d.K, d.N);
     DmaArgs v{};
     v.a = (const uint8_t*)x, v.b = (const uint8_t*)w, v.sizes = sizes, v.c = y;
     v.stride_b = 2 * a.stride_w;
@@ -196,14 +219,26 @@ int xtc_hip_grouped_matmul_grad_w(const xtc_hip_grouped_matmul_desc* desc, const
   a.stride_y = d.stride_w ? d.stride_w : matrix;
   if (a.stride_y < matrix) return fail("%s: a stride of %lld lets the gradients of two groups overlap", what, (long long)d.stride_w);
   if (d.dtype == XTC_HIP_BF16 && d.K % 8 == 0 && d.N % 8 == 0 && vectors(x, a.ldx) && vectors(dy, a.ldw)) {
-    const DmaTile& t = dma_tile(true, d.T, d.E, d.K, d.N);
+      const hipStream_t s = core::pick_stream(d.stream);
+    int splits = 1;
+    const DmaTile* t = &grad_tile(d.T, d.E, d.K, d.N, &splits);
     DmaArgs v{};
     v.a = (const uint8_t*)x, v.b = (const uint8_t*)dy, v.sizes = sizes, v.c = dw;
     v.stride_c = a.stride_y;
     v.E = d.E, v.M = d.T, v.N = d.N, v.K = d.K;
     v.lda = 2 * a.ldx, v.ldb = 2 * a.ldw, v.ldc = a.ldy, v.out16 = d.out_dtype == XTC_HIP_BF16;
-    v.tiles_m = (d.K + t.cost.bm - 1) / t.cost.bm;
-    return launch_dma(t, t.grad, v, d.E, core::pick_stream(d.stream));
+    v.tiles_m = (d.K + t->cost.bm - 1) / t->cost.bm;
+    v.splits = splits;
+    if (splits > 1) {
+      v.partial = core::partial_sums((size_t)splits * d.E * d.K * d.N * 4, s);
+      if (!v.partial) v.splits = 1;
+    }
+    if (launch_dma(*t, t->grad, v, (int64_t)d.E * v.splits, s)) return 1;
+    if (v.splits == 1) return 0;
+    const int chunks = (int)(((int64_t)d.K * (d.N / 4) + 255) / 256);  // partial sums are small: kMostPartial
+    hipLaunchKernelGGL(grouped_grad_sum, dim3((unsigned)(d.E * chunks)), dim3(256), 0, s, v, chunks);
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? 0 : fail("%s: launch failed: %s", what, hipGetErrorString(e));
   }
   return launch_any(d, any_tile(true, a), true, a, core::pick_stream(d.stream));
 }

@@ -5,15 +5,15 @@
 // Both are sums C[i, j] = sum_k A[i, k] B[k, j]: i the rows and k the depth of w,
 // or i the depth of w and k the rows.
 //
-// One workgroup of 2 x 2 waves computes a 64 x 64 tile of C, k in slabs of 32
-// through two LDS buffers, the next slab in registers meanwhile.  An operand is
-// loaded 8 elements a lane along its contiguous axis (unaligned vectors, which
-// global memory takes at element alignment; element by element where the
-// operand ends inside) and kept in LDS with k contiguous, so that a lane's
-// fragment is one (bf16) or two (fp32) 16-byte reads.  bf16 runs on
-// v_mfma_f32_16x16x32_bf16, fp32 on v_mfma_f32_16x16x4_f32 (exact products, the
-// lane's 8 k of a slab in any order as long as A and B agree).  Sums are fp32;
-// a bf16 result is rounded once, at the store.
+// grouped_any: a workgroup of 2 x 2 waves computes a 64 x 64 tile of C, k in slabs
+// of 32 through two LDS buffers, the next slab in registers meanwhile.  An operand
+// is loaded 8 elements a lane along its contiguous axis (unaligned vectors, which
+// global memory takes at element alignment; element by element where the operand
+// ends inside) and kept in LDS as it came: bf16 in the layouts of grouped_dma.hpp,
+// fp32 in padded rows.  bf16 runs on v_mfma_f32_16x16x32_bf16, fp32 on
+// v_mfma_f32_16x16x4_f32 (exact products, a lane's 8 k of a slab in any order as
+// long as A and B agree).  Sums are fp32; a bf16 result is rounded once, at the
+// store.
 //
 // grouped_small takes the calls whose 64 x 64 tiles do not fill the card, and few
 // rows a group (then it streams the matrices): a workgroup computes a tile of 16
@@ -25,6 +25,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "grouped_dma.hpp"
 #include "groups.hpp"
 
 namespace xtc_hip {
@@ -47,8 +48,6 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int BM = 64, BN = 64, BK = 32, NT = 256;
-
-template <typename T> struct Row { static constexpr int STRIDE = BK + 16 / (int)sizeof(T); };  // elements; 16-byte rows
 
 // the 8 elements at p, of which the first n exist
 template <typename T>
@@ -74,28 +73,53 @@ __device__ __forceinline__ void load(T (&v)[8], const T* p, int64_t ld, int rows
   }
 }
 
-template <typename T, bool KC>
-__device__ __forceinline__ void store(T* lds, const T (&v)[8]) {
-  constexpr int S = Row<T>::STRIDE;
-  const int tid = threadIdx.x;
-  if constexpr (KC) {
-    __builtin_memcpy(__builtin_assume_aligned(lds + (tid >> 2) * S + (tid & 3) * 8, 16), v, 8 * sizeof(T));
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) lds[((tid & 7) * 8 + i) * S + (tid >> 3)] = v[i];
+// An operand's slab in LDS and a lane's fragment of 16 of its rows from 16 f on.
+template <typename T, bool KC> struct Slab;
+template <bool KC> struct Slab<__bf16, KC> {
+  static constexpr int BYTES = 64 * BK * 2;
+  static __device__ __forceinline__ void store(unsigned char* st, const __bf16 (&v)[8]) {
+    const int tid = threadIdx.x;
+    int at;
+    if constexpr (KC) at = (tid >> 2) * 64 + 16 * ((tid & 3) ^ gdma::swz_row<false>(tid >> 2));
+    else at = (tid >> 3) * 128 + 32 * ((tid & 7) / 2 ^ gdma::swz_col<64>(tid >> 3)) + 16 * (tid & 1);
+    __builtin_memcpy(__builtin_assume_aligned(st + at, 16), v, 16);
   }
-}
+  typedef gdma::u32x4 Fragment;
+  static __device__ __forceinline__ Fragment read(const unsigned char* st, int f, int l16, int g) {
+    return gdma::fragment<KC, 64>(st, 0, f, l16, g);
+  }
+};
+template <bool KC> struct Slab<float, KC> {
+  static constexpr int STRIDE = KC ? BK + 4 : 64 + 4, BYTES = (KC ? 64 : BK) * STRIDE * 4;
+  static __device__ __forceinline__ void store(unsigned char* st, const float (&v)[8]) {
+    const int tid = threadIdx.x;
+    float* const p = (float*)st + (KC ? (tid >> 2) * STRIDE + (tid & 3) * 8 : (tid >> 3) * STRIDE + (tid & 7) * 8);
+    __builtin_memcpy(__builtin_assume_aligned(p, 16), v, 32);
+  }
+  struct Fragment { f32x4 v[2]; };
+  static __device__ __forceinline__ Fragment read(const unsigned char* st, int f, int l16, int g) {
+    const float* const p = (const float*)st;
+    Fragment r;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if constexpr (KC) {
+        r.v[h] = *(const f32x4*)(p + (16 * f + l16) * STRIDE + 16 * h + 4 * g);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) r.v[h][q] = p[(16 * h + 4 * g + q) * STRIDE + 16 * f + l16];
+      }
+    }
+    return r;
+  }
+};
 
-__device__ __forceinline__ void mma(f32x4& c, const __bf16* b, const __bf16* a, int g) {
-  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(const bf16x8*)(b + 8 * g), *(const bf16x8*)(a + 8 * g), c, 0, 0, 0);
-}
-__device__ __forceinline__ void mma(f32x4& c, const float* b, const float* a, int g) {
+__device__ __forceinline__ void mma(f32x4& c, gdma::u32x4 b, gdma::u32x4 a) { c = gdma::mfma(b, a, c); }
+template <typename B, typename A>
+__device__ __forceinline__ void mma(f32x4& c, const B& b, const A& a) {
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const f32x4 bv = *(const f32x4*)(b + 16 * h + 4 * g), av = *(const f32x4*)(a + 16 * h + 4 * g);
+  for (int h = 0; h < 2; ++h)
 #pragma unroll
-    for (int q = 0; q < 4; ++q) c = __builtin_amdgcn_mfma_f32_16x16x4f32(bv[q], av[q], c, 0, 0, 0);
-  }
+    for (int q = 0; q < 4; ++q) c = __builtin_amdgcn_mfma_f32_16x16x4f32(b.v[h][q], a.v[h][q], c, 0, 0, 0);
 }
 
 __device__ __forceinline__ void put(float* p, f32x4 v, int n) {
@@ -276,9 +300,10 @@ __global__ void __launch_bounds__(64 * gany::SWAVES) grouped_small(GroupedArgs p
 template <typename T, typename U, bool WT, bool GRAD>
 __global__ void __launch_bounds__(256) grouped_any(GroupedArgs p) {
   using namespace gany;
-  constexpr int S = Row<T>::STRIDE;
   constexpr bool A_KC = !GRAD, B_KC = WT && !GRAD;
-  __shared__ __attribute__((aligned(16))) T lds[2][2][64 * S];
+  typedef Slab<T, A_KC> SlabA;
+  typedef Slab<T, B_KC> SlabB;
+  __shared__ __attribute__((aligned(16))) unsigned char lds_a[2][SlabA::BYTES], lds_b[2][SlabB::BYTES];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int l16 = lane & 15, g = lane >> 4, wm = wave >> 1, wn = wave & 1;
@@ -324,8 +349,8 @@ __global__ void __launch_bounds__(256) grouped_any(GroupedArgs p) {
   if (steps > 0) {
     load<T, A_KC>(av, a, p.ldx, rows, depth);
     load<T, B_KC>(bv, b, p.ldw, cols, depth);
-    store<T, A_KC>(lds[0][0], av);
-    store<T, B_KC>(lds[0][1], bv);
+    SlabA::store(lds_a[0], av);
+    SlabB::store(lds_b[0], bv);
   }
   for (int s = 0; s < steps; ++s) {
     __syncthreads();
@@ -336,15 +361,19 @@ __global__ void __launch_bounds__(256) grouped_any(GroupedArgs p) {
       load<T, A_KC>(av, a, p.ldx, rows, depth);
       load<T, B_KC>(bv, b, p.ldw, cols, depth);
     }
-    const T* la = lds[s & 1][0] + (wm * 32 + l16) * S;
-    const T* lb = lds[s & 1][1] + (wn * 32 + l16) * S;
+    typename SlabA::Fragment fa[2];
+    typename SlabB::Fragment fb[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) fa[i] = SlabA::read(lds_a[s & 1], wm * 2 + i, l16, g);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) fb[j] = SlabB::read(lds_b[s & 1], wn * 2 + j, l16, g);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) mma(acc[i][j], lb + j * 16 * S, la + i * 16 * S, g);
+      for (int j = 0; j < 2; ++j) mma(acc[i][j], fb[j], fa[i]);
     if (s + 1 < steps) {
-      store<T, A_KC>(lds[(s + 1) & 1][0], av);
-      store<T, B_KC>(lds[(s + 1) & 1][1], bv);
+      SlabA::store(lds_a[(s + 1) & 1], av);
+      SlabB::store(lds_b[(s + 1) & 1], bv);
     }
   }
   // a lane holds C[i][j .. j+3]: B is the first MFMA operand

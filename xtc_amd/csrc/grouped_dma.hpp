@@ -38,6 +38,11 @@
 // start the DMA of the slab STAGES - 1 ahead, read, compute; several workgroups
 // share a CU and fill each other's gaps.
 //
+// Few tiles of many rows (GRAD) are split over the rows, each group in as many
+// parts as it has slabs, at most `splits`: fp32 partial planes that a second kernel
+// adds up in order, all CUs at it (the last workgroup of each tile alone took 60 us
+// of 83 for 32768 rows over 2 matrices of 256 x 512).
+//
 // Raster.  Tiles run in bands of (at most 8) tile rows, down the band first;
 // 4 columns of a band go to one XCD (workgroups reach the XCDs in turn), whose
 // 32 CUs then share 8 panels of A and 4 of B in its L2.
@@ -68,6 +73,8 @@ struct DmaArgs {
   int ldc;            // elements
   int tiles_m, tiles_n;  // tiles_m: of all groups (at most), GRAD: of one C
   int band;           // tile rows of a band
+  int splits;         // GRAD: parts of a group's rows, at most
+  float* partial;     // GRAD, splits > 1: [splits][E][K][N]
   int out16;          // C is bf16
 };
 
@@ -209,6 +216,9 @@ __device__ __forceinline__ void store4(void* c, int out16, int64_t at, f32x4 v, 
   }
 }
 
+// Into how many parts the rows of a group of `slabs` slabs go.
+__device__ __forceinline__ int gradient_parts(int slabs, int splits) { return max(min(splits, slabs), 1); }
+
 // f(0) .. f(N - 1), the argument a compile-time constant
 template <int N, int I = 0, typename F>
 __device__ __forceinline__ void each_stage(F&& f) {
@@ -249,26 +259,35 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_dma(DmaArgs p) {
   const int slot = blockIdx.x >> 3, run = 4 * p.band;  // run: tiles that follow one another on an XCD
   const int t = (slot / run * 8 + (blockIdx.x & 7)) * run + slot % run;
   const int per_matrix = (p.tiles_m + p.band - 1) / p.band * p.band * p.tiles_n;
-  const int e_grad = GRAD ? t / per_matrix : 0;
-  const int tt = GRAD ? t - e_grad * per_matrix : t;
+  const int matrix = GRAD ? t / per_matrix : 0;  // part by part
+  const int e_grad = GRAD ? matrix % p.E : 0;
+  const int part = GRAD ? matrix / p.E : 0;
+  const int tt = GRAD ? t - matrix * per_matrix : t;
   const int in_band = tt % (p.band * p.tiles_n);
   const int mt = tt / (p.band * p.tiles_n) * p.band + in_band % p.band, n0 = in_band / p.band * BN;
-  if (mt >= p.tiles_m || (GRAD && e_grad >= p.E)) return;
+  if (mt >= p.tiles_m || (GRAD && part >= p.splits)) return;
 
   const uint8_t *a, *b;                        // tile corners
   const uint8_t *as = nullptr, *bs = nullptr;  // and those of the scales
   int64_t c_at;              // element of C at the tile's corner
   int rows, nk, chunks = 0;  // rows of C, slabs, 16-byte chunks of a ROW row
   int depth = 0;             // k rows of a COL operand
+  int parts = 1;             // of the group's rows
   const int cols = p.N - n0;
   if constexpr (GRAD) {
     const RowGroup gr = find_group(p.sizes, p.E, p.M, e_grad);
     const int m0 = mt * BM;
     rows = p.K - m0;
-    depth = gr.end - gr.begin;
-    nk = (depth + 31) / 32;
-    a = p.a + (int64_t)gr.begin * p.lda + 2 * m0;
-    b = p.b + (int64_t)gr.begin * p.ldb + 2 * n0;
+    // this part's slabs of the group's
+    const int slabs = (gr.end - gr.begin + 31) / 32;
+    parts = gradient_parts(slabs, p.splits);
+    if (part >= parts) return;
+    const int first = (int)((int64_t)slabs * part / parts);
+    nk = (int)((int64_t)slabs * (part + 1) / parts) - first;
+    const int64_t row0 = gr.begin + 32 * (int64_t)first;
+    depth = (int)min((int64_t)32 * nk, gr.end - row0);
+    a = p.a + row0 * p.lda + 2 * (int64_t)m0;
+    b = p.b + row0 * p.ldb + 2 * (int64_t)n0;
     c_at = (int64_t)e_grad * p.stride_c + (int64_t)m0 * p.ldc + n0;
   } else {
     RowGroup gr{0, mt * BM, p.M};
@@ -465,6 +484,23 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_dma(DmaArgs p) {
     __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
   }
 
+  if constexpr (GRAD) {
+    if (parts > 1) {
+      // whole quads of columns: N is one of whole vectors
+      float* const tile = p.partial + (((size_t)part * p.E + e_grad) * p.K + (p.K - rows)) * p.N + n0;
+#pragma unroll
+      for (int i = 0; i < IM; ++i) {
+        const int m = (wm * IM + i) * 16 + l16;
+#pragma unroll
+        for (int j = 0; j < JN; ++j) {
+          const int n = (wn * JN + j) * 16 + 4 * g;
+          if (m < rows && n < cols) *(f32x4*)(tile + (size_t)m * p.N + n) = acc[i][j];
+        }
+      }
+      return;
+    }
+  }
+
   // ---- a lane holds C[m][n .. n+3] of each 16 x 16, or n, n+8, n+16 and n+24 of
   // each 32 x 32
   const bool whole = (p.ldc & 3) == 0 && ((uintptr_t)p.c & (p.out16 ? 7 : 15)) == 0 && (!GRAD || (p.stride_c & 3) == 0);
@@ -485,6 +521,32 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_dma(DmaArgs p) {
       }
     }
   }
+}
+
+// Adds up the parts of the groups that have more than one, in order: a thread
+// four columns, `chunks` workgroups a matrix.
+static __global__ void __launch_bounds__(256) grouped_grad_sum(DmaArgs p, int chunks) {
+  using namespace gdma;
+  const int e = blockIdx.x / chunks;
+  const RowGroup gr = find_group(p.sizes, p.E, p.M, e);
+  const int parts = gradient_parts((gr.end - gr.begin + 31) / 32, p.splits);
+  if (parts == 1) return;
+  const int64_t q = (int64_t)(blockIdx.x % chunks) * 256 + threadIdx.x;
+  const int quads = p.N / 4, m = (int)(q / quads), n = (int)(q % quads) * 4;
+  if (m >= p.K) return;
+  const size_t plane = (size_t)p.E * p.K * p.N;
+  const float* const at = p.partial + ((size_t)e * p.K + m) * p.N + n;
+  f32x4 v = *(const f32x4*)at;
+  for (int s0 = 1; s0 < parts; s0 += 8) {
+    f32x4 t[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t[j] = *(const f32x4*)(at + min(s0 + j, parts - 1) * plane);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (s0 + j < parts) v += t[j];
+  }
+  const bool whole = (p.ldc & 3) == 0 && (p.stride_c & 3) == 0 && ((uintptr_t)p.c & (p.out16 ? 7 : 15)) == 0;
+  store4(p.c, p.out16, e * p.stride_c + (int64_t)m * p.ldc, v, n, p.N, whole);
 }
 
 // What a tile's slab costs, from which the calls choose their tiles: microseconds

@@ -2298,6 +2298,11 @@ int fail(const char* fmt, ...) {
 }
 bool ready() { return current_state() != nullptr; }
 hipStream_t pick_stream(void* stream) { return ::pick_stream(stream); }
+float* partial_sums(size_t bytes, hipStream_t s) {
+  void* p = capturing(s) ? nullptr : workspace(bytes, s);
+  if (!p) (void)hipGetLastError();  // an allocation that failed is no error of the launch
+  return (float*)p;
+}
 
 }  // namespace core
 }  // namespace xtc_hip

@@ -60,12 +60,11 @@ const DmaTile kDmaTiles[] = {
 // Strides of whole vectors whose offsets within a tile stay within 2^31 bytes.
 bool vectors(const void* p, int ld) { return core::aligned16(p) && ld % 8 == 0 && ld < (1 << 22) - 8; }
 
-const DmaTile& dma_tile(int64_t T, int64_t E, int K, int N) {
+const DmaTile& dma_tile(int64_t T, int64_t E, int K, int N, double* cost) {
   const DmaTile* best = nullptr;
-  double least = 0;
   for (const DmaTile& t : kDmaTiles) {
-    const double cost = dma_cost(t.cost, likely_tiles(T, E, t.cost.bm) * ((N + t.cost.bn - 1) / t.cost.bn), K / 32.0);
-    if (!best || cost < least) best = &t, least = cost;
+    const double c = dma_cost(t.cost, likely_tiles(T, E, t.cost.bm) * ((N + t.cost.bn - 1) / t.cost.bn), K / 32.0);
+    if (!best || c < *cost) best = &t, *cost = c;
   }
   return *best;
 }
@@ -190,7 +189,13 @@ int xtc_hip_grouped_matmul(const xtc_hip_grouped_matmul_desc* desc, const void* 
   if (const AnyTile* t = stream_tile(d.trans_w, a)) return launch_any(d, *t, false, a, s);
   if (d.dtype == XTC_HIP_BF16 && d.K % 8 == 0 && (d.trans_w || d.N % 8 == 0) && vectors(x, a.ldx) && vectors(w, a.ldw) &&
       a.stride_w % 8 == 0) {
-    const DmaTile& t = dma_tile(d.T, d.E, d.K, d.N);
+    double cost;
+    const DmaTile& t = dma_tile(d.T, d.E, d.K, d.N, &cost);
+    // few tiles of deep K: waves that share out the depth, 256 of it a step of at
+    // least .8 us, 3 where two workgroups a CU share it (512 rows over 2 experts of
+    // 3584 x 256: 25 us on DMA tiles, 15 so)
+    const double load = likely_tiles(d.T, d.E, 16) * ((d.N + 63) / 64) / 512;
+    if (d.K / 256.0 * fmax(0.8, 3 * load) < cost) return launch_any(d, kSmall64, false, a, s);
     DmaArgs v{};
     v.a = (const uint8_t*)x, v.b = (const uint8_t*)w, v.sizes = sizes, v.c = y;
     v.stride_b = 2 * a.stride_w;

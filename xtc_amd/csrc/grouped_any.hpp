@@ -6,7 +6,7 @@
 // or i the depth of w and k the rows.
 //
 // grouped_any: a workgroup of 2 x 2 waves computes a 64 x 64 tile of C, k in slabs
-// of 32 through two LDS buffers, the next slab in registers meanwhile.  An operand
+// of 32 through two LDS buffers, the next three in registers meanwhile.  An operand
 // is loaded 8 elements a lane along its contiguous axis (unaligned vectors, which
 // global memory takes at element alignment; element by element where the operand
 // ends inside) and kept in LDS as it came: bf16 in the layouts of grouped_dma.hpp,
@@ -18,7 +18,7 @@
 // grouped_small takes the calls whose 64 x 64 tiles do not fill the card, and few
 // rows a group (then it streams the matrices): a workgroup computes a tile of 16
 // or 32 rows with 8 waves that share out the depth in turn,
-// load their fragments straight into registers, two steps ahead, and add their sums
+// load their fragments straight into registers, two or three steps ahead, and add their sums
 // up in LDS, in order.  No barrier but that one: the loads of a whole call are in
 // flight together (777 fp32 rows over 5 experts of 509 x 301: 22 us in slabs).
 #pragma once
@@ -49,14 +49,14 @@ typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int BM = 64, BN = 64, BK = 32, NT = 256;
 
-// the 8 elements at p, of which the first n exist
-template <typename T>
-__device__ __forceinline__ void load8(T (&v)[8], const T* p, int n) {
-  if (n >= 8) {
-    __builtin_memcpy(v, p, 8 * sizeof(T));
+// the elements at p, of which the first n exist, zeros for the others
+template <typename T, int LEN>
+__device__ __forceinline__ void load_some(T (&v)[LEN], const T* p, int n) {
+  if (n >= LEN) {
+    __builtin_memcpy(v, p, LEN * sizeof(T));
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : (T)0.f;
+    for (int i = 0; i < LEN; ++i) v[i] = i < n ? p[i] : (T)0.f;
   }
 }
 
@@ -66,10 +66,10 @@ __device__ __forceinline__ void load(T (&v)[8], const T* p, int64_t ld, int rows
   const int tid = threadIdx.x;
   if constexpr (KC) {
     const int r = tid >> 2, k = (tid & 3) * 8;
-    load8(v, p + (int64_t)r * ld + k, r < rows ? depth - k : 0);
+    load_some(v, p + (int64_t)r * ld + k, r < rows ? depth - k : 0);
   } else {
     const int k = tid >> 3, r = (tid & 7) * 8;
-    load8(v, p + (int64_t)k * ld + r, k < depth ? rows - r : 0);
+    load_some(v, p + (int64_t)k * ld + r, k < depth ? rows - r : 0);
   }
 }
 
@@ -153,59 +153,57 @@ template <> struct Small<__bf16> {
   }
 };
 
-// An operand's part of a step: W fragments of 16 rows (or columns) each.
-// KC: k contiguous, a lane takes PER k of rows l16, 16 + l16, ...; otherwise its W
-// neighbouring rows W l16 .. W l16 + W - 1 at PER k, loaded together.
+// An operand's part of a step: W fragments of 16 lines (rows or columns) each.
+// KC: k contiguous, a lane takes PER k of lines l16, 16 + l16, ...; otherwise its W
+// neighbouring lines at PER k, loaded together: W l16 .. W l16 + W - 1, or the last
+// W of the tile where it ends among or before them.  What lanes hold twice comes
+// out the same twice; lines past a tile of less than W are zeros.
 template <typename T, bool KC, int W>
 struct SmallOperand {
   static constexpr int PER = Small<T>::PER;
   const T* at[KC ? W : 1];
   int64_t ld, next;  // between k rows; to the wave's next step
-  int lines;         // !KC: rows from the lane's first to the tile's edge
+  int edge;          // lines of the tile
 
-  static __device__ __forceinline__ int line(int w, int l16) { return KC ? 16 * w + l16 : W * l16 + w; }
-
-  // lines past the tile's `edge` repeat the last one (KC) or are zeros
-  __device__ __forceinline__ void set(const T* p, int64_t stride, int l16, int k, int edge, int step) {
+  __device__ __forceinline__ int line(int w, int l16) const {
+    return KC ? 16 * w + l16 : min(W * l16, max(edge - W, 0)) + w;
+  }
+  // lines past the edge repeat the last one (KC)
+  __device__ __forceinline__ void set(const T* p, int64_t stride, int l16, int k, int lines, int step) {
     ld = stride;
     next = KC ? step : step * stride;
-    lines = edge - W * l16;
+    edge = lines;
     if constexpr (KC) {
 #pragma unroll
       for (int w = 0; w < W; ++w) at[w] = p + min(line(w, l16), edge - 1) * stride + k;
     } else {
-      at[0] = p + k * stride + W * l16;
+      at[0] = p + k * stride + line(0, l16);
     }
   }
-  // the step's fragments, `left` k from the lane's first one to the end; then on
-  // to the next step
-  __device__ __forceinline__ void load(T (&v)[W][PER], int left) {
+  // a step as loaded: fragments, or W lines at each of PER k (turned over only when
+  // they are used, so that the loads stay in flight)
+  static constexpr int ROWS = KC ? W : PER, COLS = KC ? PER : W;
+  typedef T Raw[ROWS][COLS];
+  static __device__ __forceinline__ void fragment(T (&f)[PER], const Raw& v, int w) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) f[i] = KC ? v[w][i] : v[i][w];
+  }
+  // the step, `left` k from the lane's first one to the end; then on to the next
+  __device__ __forceinline__ void load(Raw& v, int left) {
     if constexpr (KC) {
 #pragma unroll
       for (int w = 0; w < W; ++w) {
-        if (left >= PER) {
-          __builtin_memcpy(v[w], at[w], sizeof(v[w]));
-        } else {
-#pragma unroll
-          for (int i = 0; i < PER; ++i) v[w][i] = i < left ? at[w][i] : (T)0.f;
-        }
+        load_some(v[w], at[w], left);
         at[w] += next;
       }
     } else {
-      T raw[PER][W];
-      if (left >= PER && lines >= W) {
+      if (left >= PER && edge >= W) {
 #pragma unroll
-        for (int i = 0; i < PER; ++i) __builtin_memcpy(raw[i], at[0] + i * ld, sizeof(raw[i]));
+        for (int i = 0; i < PER; ++i) __builtin_memcpy(v[i], at[0] + i * ld, sizeof(v[i]));
       } else {
 #pragma unroll
-        for (int i = 0; i < PER; ++i)
-#pragma unroll
-          for (int w = 0; w < W; ++w) raw[i][w] = i < left && w < lines ? at[0][i * ld + w] : (T)0.f;
+        for (int i = 0; i < PER; ++i) load_some(v[i], at[0] + i * ld, i < left ? edge : 0);
       }
-#pragma unroll
-      for (int w = 0; w < W; ++w)
-#pragma unroll
-        for (int i = 0; i < PER; ++i) v[w][i] = raw[i][w];
       at[0] += next;
     }
   }
@@ -250,14 +248,15 @@ __global__ void __launch_bounds__(64 * gany::SWAVES) grouped_small(GroupedArgs p
   }
   const int cols = min(p.N - n0, SN);
 
-  constexpr int STRIDE = SWAVES * S::STEP, RING = 3;
+  constexpr int STRIDE = SWAVES * S::STEP, RING = TM == 1 ? 4 : 3;
   const int k0 = wave * S::STEP, kl = k0 + g * S::PER;
   OpA oa;
   OpB ob;
   oa.set(a, p.ldx, l16, kl, rows, STRIDE);
   ob.set(b, p.ldw, l16, kl, cols, STRIDE);
   f32x4 acc[TM][TN] = {};
-  T av[RING][TM][S::PER], bv[RING][TN][S::PER];
+  typename OpA::Raw av[RING];
+  typename OpB::Raw bv[RING];
   int left = depth - kl;  // k from the lane's next element on
   auto load = [&](int buf) {
     ob.load(bv[buf], left);
@@ -273,10 +272,15 @@ __global__ void __launch_bounds__(64 * gany::SWAVES) grouped_small(GroupedArgs p
     for (int q = 0; q < RING; ++q) {
       if (s + q >= steps) break;
       if (s + q + RING - 1 < steps) load((q + RING - 1) % RING);
+      T fa[TM][S::PER], fb[TN][S::PER];
+#pragma unroll
+      for (int i = 0; i < TM; ++i) OpA::fragment(fa[i], av[q], i);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) OpB::fragment(fb[j], bv[q], j);
 #pragma unroll
       for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int j = 0; j < TN; ++j) S::mma(acc[i][j], bv[q][j], av[q][i]);
+        for (int j = 0; j < TN; ++j) S::mma(acc[i][j], fb[j], fa[i]);
     }
   }
 #pragma unroll
@@ -284,7 +288,7 @@ __global__ void __launch_bounds__(64 * gany::SWAVES) grouped_small(GroupedArgs p
 #pragma unroll
     for (int j = 0; j < TN; ++j)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) sums[wave][OpA::line(i, l16)][OpB::line(j, 4 * g + r)] = acc[i][j][r];
+      for (int r = 0; r < 4; ++r) sums[wave][oa.line(i, l16)][ob.line(j, 4 * g + r)] = acc[i][j][r];
   __syncthreads();
   for (int t = threadIdx.x; t < SM * SN; t += 64 * SWAVES) {
     const int m = t / SN, n = t % SN;
@@ -345,35 +349,47 @@ __global__ void __launch_bounds__(256) grouped_any(GroupedArgs p) {
 
   f32x4 acc[2][2] = {};
   const int steps = (depth + BK - 1) / BK;
-  T av[8], bv[8];
+  // slabs s + 1 .. s + RING in registers during step s
+  constexpr int RING = 3;
+  T av[RING][8], bv[RING][8];
+  auto load_next = [&](int buf) {
+    load<T, A_KC>(av[buf], a, p.ldx, rows, depth);
+    load<T, B_KC>(bv[buf], b, p.ldw, cols, depth);
+    a += a_step;
+    b += b_step;
+    depth -= BK;
+  };
+#pragma unroll
+  for (int q = 0; q < RING; ++q)
+    if (q < steps) load_next(q);
   if (steps > 0) {
-    load<T, A_KC>(av, a, p.ldx, rows, depth);
-    load<T, B_KC>(bv, b, p.ldw, cols, depth);
-    SlabA::store(lds_a[0], av);
-    SlabB::store(lds_b[0], bv);
+    SlabA::store(lds_a[0], av[0]);
+    SlabB::store(lds_b[0], bv[0]);
+    if (RING < steps) load_next(0);
   }
-  for (int s = 0; s < steps; ++s) {
-    __syncthreads();
-    if (s + 1 < steps) {
-      a += a_step;
-      b += b_step;
-      depth -= BK;
-      load<T, A_KC>(av, a, p.ldx, rows, depth);
-      load<T, B_KC>(bv, b, p.ldw, cols, depth);
-    }
-    typename SlabA::Fragment fa[2];
-    typename SlabB::Fragment fb[2];
+  for (int s0 = 0; s0 < steps; s0 += RING) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) fa[i] = SlabA::read(lds_a[s & 1], wm * 2 + i, l16, g);
+    for (int q = 0; q < RING; ++q) {
+      const int s = s0 + q;
+      if (s >= steps) break;
+      __syncthreads();
+      typename SlabA::Fragment fa[2];
+      typename SlabB::Fragment fb[2];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) fb[j] = SlabB::read(lds_b[s & 1], wn * 2 + j, l16, g);
+      for (int i = 0; i < 2; ++i) fa[i] = SlabA::read(lds_a[s & 1], wm * 2 + i, l16, g);
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+      for (int j = 0; j < 2; ++j) fb[j] = SlabB::read(lds_b[s & 1], wn * 2 + j, l16, g);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) mma(acc[i][j], fb[j], fa[i]);
-    if (s + 1 < steps) {
-      SlabA::store(lds_a[(s + 1) & 1], av);
-      SlabB::store(lds_b[(s + 1) & 1], bv);
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) mma(acc[i][j], fb[j], fa[i]);
+      if (s + 1 < steps) {
+        constexpr int NEXT_OF[RING] = {1, 2, 0};
+        const int next = NEXT_OF[q];
+        SlabA::store(lds_a[(s + 1) & 1], av[next]);
+        SlabB::store(lds_b[(s + 1) & 1], bv[next]);
+        if (s + 1 + RING < steps) load_next(next);
+      }
     }
   }
   // a lane holds C[i][j .. j+3]: B is the first MFMA operand

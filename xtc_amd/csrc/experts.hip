@@ -123,7 +123,8 @@ struct AnyTile {
   {16 * TM, 16 * TN, {XTC_TYPES(small_launch, false, false, TM, TN), XTC_TYPES(small_launch, true, false, TM, TN), {}}}
 const AnyTile kSlabs = {gany::BM, gany::BN, {XTC_TYPES(any_launch, false, false), XTC_TYPES(any_launch, true, false),
                                             XTC_TYPES(any_launch, false, true)}};
-const AnyTile kSmall16 = XTC_SMALL(1, 1), kSmall32 = XTC_SMALL(1, 2), kSmall64 = XTC_SMALL(1, 4);
+const AnyTile kSmall16 = {16, 16, {{}, XTC_TYPES(small_launch, true, false, 1, 1), {}}};  // streams transposed matrices
+const AnyTile kSmall32 = XTC_SMALL(1, 2), kSmall64 = XTC_SMALL(1, 4);
 const AnyTile kSmallGrad = {32, 32, {{}, {}, XTC_TYPES(small_launch, false, true, 2, 2)}};
 #undef XTC_SMALL
 #undef XTC_TYPES

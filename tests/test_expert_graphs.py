@@ -222,3 +222,26 @@ def test_equal_graphs_make_equal_payloads():
         return backend.get_compiler().compile(backend.get_scheduler().schedule()).source
 
     assert source() == source()
+
+
+def test_example_graphs_lower():
+    """The graphs of the example: their launches, and their numpy semantics chained."""
+    from xtc_amd.cli import experts
+
+    T, E, K, N = 20, 3, 64, 96
+    rng = np.random.default_rng(5)
+    kinds = {}
+    for graph in (experts.step_graph(T, E, K, N), experts.quantize_graph(E, N, K), experts.serve_graph(T, E, K, N)):
+        backend = Backend(graph)
+        backend.get_compiler(schedule_policy="strict").compile(backend.get_scheduler().schedule())
+        kinds[graph.name] = [launch.kind for launch in backend.plan.launches]
+    assert kinds == {"experts_step": ["grouped_matmul"] * 2 + ["grouped_matmul_grad_w"], "experts_quantize": ["mx4_quantize"],
+                     "experts_serve": ["mx4_quantize", "mx4_matmul", "relu", "mx4_quantize", "mx4_matmul"]}
+    up, down = (rng.normal(size=s).astype(np.float32) for s in ((E, N, K), (E, K, N)))
+    x, sizes = rng.normal(size=(T, K)).astype(np.float32), np.array([7, 0, 9], np.int32)
+    packed = [a for w in (up, down) for a in forward(experts.quantize_graph(*w.shape), w)]
+    y, = forward(experts.serve_graph(T, E, K, N), x, *packed, sizes)
+    full = np.concatenate([np.maximum(x[b:e] @ up[i].T, 0) @ down[i].T for i, (b, e) in enumerate(((0, 7), (7, 7), (7, 16)))])
+    assert y.shape == (T, K) and not y[16:].any()
+    # each of the four 4-bit operands is off by about a tenth of its norm
+    assert np.linalg.norm(y[:16] - full) < 0.5 * np.linalg.norm(full)

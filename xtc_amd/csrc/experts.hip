@@ -71,8 +71,9 @@ const DmaTile& dma_tile(int64_t T, int64_t E, int K, int N, double* cost) {
 
 // The tile of E gradients of K x N and into how many parts each group's rows go.
 // The largest group decides where tiles are few (of a skewed choice it has some 1.7
-// times the mean), the sum of all where they are many; writing out a tile and
-// starting on it take 4 us for each 64 of its rows.  A part pays for writing and
+// times the mean), the sum of all where they are many; starting on a
+// round of tiles and writing them out take 5 (64 rows) to 15 us (256): 512 rows, 32
+// of 640 x 512, 21 us in 64 x 64 tiles, 14 in 128 x 128.  A part pays for writing and
 // reading its partial sums (4 MB a microsecond), all together for one more launch,
 // 4 us.  32768 rows: 1 matrix of 128 x 128 163 us whole, 18 in 16 parts of 64 x 64
 // tiles; 8 of 512 x 512 55 and 49 (4 parts of 128 x 128); 4096 rows, 8 of 512 x
@@ -86,7 +87,8 @@ const DmaTile& grad_tile(int64_t T, int64_t E, int K, int N, int* splits) {
     const double tiles = E * (double)((K + c.bm - 1) / c.bm) * ((N + c.bn - 1) / c.bn);
     for (int s = 1; s <= 16 && (s == 1 || (all / s >= 4 && s * plane <= kMostPartial)); s *= 2) {
       const double slabs = all / s, load = tiles * s / (256.0 * c.per_cu);
-      const double cost = slabs * fmax(c.light * skew, c.full * load) + c.bm / 16 + (s > 1 ? 4 + s * plane / 4e6 : 0);
+      const double cost = slabs * fmax(c.light * skew, c.full * load) + (2 + 0.05 * c.bm) * fmax(load, 1) +
+                          (s > 1 ? 4 + s * plane / 4e6 : 0);
       if (!best || cost < least) best = &t, least = cost, *splits = s;
     }
   }
@@ -225,7 +227,7 @@ int xtc_hip_grouped_matmul_grad_w(const xtc_hip_grouped_matmul_desc* desc, const
   a.stride_y = d.stride_w ? d.stride_w : matrix;
   if (a.stride_y < matrix) return fail("%s: a stride of %lld lets the gradients of two groups overlap", what, (long long)d.stride_w);
   if (d.dtype == XTC_HIP_BF16 && d.K % 8 == 0 && d.N % 8 == 0 && vectors(x, a.ldx) && vectors(dy, a.ldw)) {
-      const hipStream_t s = core::pick_stream(d.stream);
+    const hipStream_t s = core::pick_stream(d.stream);
     int splits = 1;
     const DmaTile* t = &grad_tile(d.T, d.E, d.K, d.N, &splits);
     DmaArgs v{};

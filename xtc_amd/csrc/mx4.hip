@@ -103,12 +103,19 @@ void rows_launch(const Mx4Args& a, unsigned groups, hipStream_t s) {
 const RowsTile kRows16 = {16, 32, {&rows_launch<float, 1, 2>, &rows_launch<__bf16, 1, 2>}};
 const RowsTile kRows32 = {32, 32, {&rows_launch<float, 2, 2>, &rows_launch<__bf16, 2, 2>}};
 
-// Whole slabs: up to 16 rows of one product (x 8192 x 8192: 9.9 us, DMA tiles
-// 13.8) and up to 32 (12.3, 14.0); by group DMA tiles are as fast (32 rows over 16
-// experts of 4096 x 2048: 16.4, 13.3).  Otherwise up to 32 rows a group: beyond,
-// tiles that read their operands once for 64 rows.
-const RowsTile* rows_tile(int64_t rows, int64_t groups, bool slabs) {
-  if (slabs && groups > 1) return nullptr;
+// As many tiles as fit the CUs at once: eight waves a tile then read b as fast as it
+// comes (8192 x 8192 with 16 rows: 9.9 us, DMA tiles 13.8; with 32: 12.3, 14.4;
+// 64 x 4096 x 4096: 7.3, 8.3; 1000 x 8192 x 128: 8.9, 15.1), beyond that whole slabs
+// go to tiles that read their operands once for 64 rows (64 x 8192 x 8192: 22.6,
+// 15.0).  By group twice as many, some of which stay empty (8 rows over 8 experts of
+// 4096 x 2048: 7.3, 9.6; 32 over 16: 16.4, 13.2).  Blocks of no whole slabs stay
+// here up to 32 rows a group (32 rows over 16 experts of 4128 x 2048: 14.1, the
+// kernel of any blocks 20.5).
+const RowsTile* rows_tile(int64_t rows, int64_t groups, int N, bool slabs) {
+  const double most = groups > 1 ? 512 : 256;
+  for (const RowsTile* t : {&kRows16, &kRows32})
+    if (likely_tiles(rows, groups, t->bm) * ((N + t->bn - 1) / t->bn) <= most) return t;
+  if (slabs) return nullptr;
   return rows <= 16 * groups ? &kRows16 : rows <= 32 * groups ? &kRows32 : nullptr;
 }
 
@@ -175,7 +182,7 @@ int xtc_hip_mx4_matmul(const xtc_hip_mx4_matmul_desc* desc, const uint8_t* a_cod
   a.a_codes = a_codes, a.a_scales = a_scales, a.b_codes = b_codes, a.b_scales = b_scales, a.sizes = sizes, a.c = c;
   a.E = d.E > 0 ? d.E : 1, a.M = d.M, a.N = d.N, a.blocks = d.blocks, a.ldc = d.ldc ? d.ldc : d.N;
   const bool slabs = d.blocks % 4 == 0 && d.blocks < (1 << 19) && ((uintptr_t)a_scales & 3) == 0 && ((uintptr_t)b_scales & 3) == 0;
-  if (const RowsTile* t = rows_tile(d.M, a.E, slabs)) {
+  if (const RowsTile* t = rows_tile(d.M, a.E, d.N, slabs)) {
     a.tiles_n = (d.N + t->bn - 1) / t->bn;
     const int64_t groups = a.tiles_n * (sizes ? most_tiles(d.M, d.E, t->bm) : ((int64_t)d.M + t->bm - 1) / t->bm);
     if (groups >= (int64_t)1 << 31) return fail("%s: %lld workgroups are too many", what, (long long)groups);

@@ -23,44 +23,12 @@ namespace mx4 {
 
 constexpr int RWAVES = 8;
 
-// one step's part of a row: 4 blocks and their scales
-struct Run {
-  u32x4 codes[4];
-  unsigned scales;
-};
-
-// `left` of the 4 blocks at `codes` exist; the others are zeros of scale 1
-__device__ __forceinline__ void load_run(Run& r, const uint8_t* codes, const uint8_t* scales, int left) {
-  if (left >= 4) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) r.codes[j] = *(const u32x4*)(codes + 16 * j);
-    __builtin_memcpy(&r.scales, scales, 4);
-  } else {
-    r.scales = 0x7f7f7f7fu;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      r.codes[j] = u32x4{0, 0, 0, 0};
-      if (j < left) {
-        r.codes[j] = *(const u32x4*)(codes + 16 * j);
-        r.scales ^= (0x7fu ^ scales[j]) << (8 * j);
-      }
-    }
-  }
-}
-
-template <int BYTE>
-__device__ __forceinline__ f32x4 mfma_byte(u32x4 a, unsigned sa, u32x4 b, unsigned sb, f32x4 c) {
-  const i32x8 av = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0};
-  const i32x8 bv = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 4, BYTE, (int)sa, BYTE, (int)sb);
-}
-
 }  // namespace mx4
 
 template <typename U, int TM, int TN>
 __global__ void __launch_bounds__(64 * mx4::RWAVES) mx4_rows(Mx4Args p) {
   using namespace mx4;
-  constexpr int SM = 16 * TM, SN = 16 * TN, STEP = 16, RING = 2;  // blocks of a step, steps in registers
+  constexpr int SM = 16 * TM, SN = 16 * TN;
   __shared__ float sums[RWAVES][SM][SN + 4];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l16 = lane & 15, g = lane >> 4;
@@ -108,14 +76,7 @@ __global__ void __launch_bounds__(64 * mx4::RWAVES) mx4_rows(Mx4Args p) {
 #pragma unroll
       for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int j = 0; j < TN; ++j) {
-          const Run &ra = a[q][i], &rb = b[q][j];
-          f32x4& c = acc[i][j];
-          c = mfma_byte<0>(rb.codes[0], rb.scales, ra.codes[0], ra.scales, c);
-          c = mfma_byte<1>(rb.codes[1], rb.scales, ra.codes[1], ra.scales, c);
-          c = mfma_byte<2>(rb.codes[2], rb.scales, ra.codes[2], ra.scales, c);
-          c = mfma_byte<3>(rb.codes[3], rb.scales, ra.codes[3], ra.scales, c);
-        }
+        for (int j = 0; j < TN; ++j) acc[i][j] = mfma_run(b[q][j], a[q][i], acc[i][j]);
     }
   }
 #pragma unroll

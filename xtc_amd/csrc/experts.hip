@@ -52,7 +52,7 @@ struct DmaTile {
 // 4096 rows over 32 experts of 4096 x 2048 (full).
 const DmaTile kDmaTiles[] = {
     {{256, 256, 1, 0.57, 0.80}, XTC_DMA(2, 4, 8, 4, 4, true)},
-    {{128, 128, 2, 0.29, 0.60}, XTC_DMA(2, 2, 4, 4, 4, false)},
+    {{128, 128, 2, 0.29, 0.62}, XTC_DMA(2, 2, 4, 4, 4, false)},
     {{64, 64, 4, 0.13, 0.73}, XTC_DMA(2, 2, 2, 2, 4, false)},
 };
 #undef XTC_DMA
@@ -60,10 +60,11 @@ const DmaTile kDmaTiles[] = {
 // Strides of whole vectors whose offsets within a tile stay within 2^31 bytes.
 bool vectors(const void* p, int ld) { return core::aligned16(p) && ld % 8 == 0 && ld < (1 << 22) - 8; }
 
-const DmaTile& dma_tile(int64_t T, int64_t E, int K, int N, double* cost) {
+const DmaTile& dma_tile(int64_t T, int64_t E, int K, int N, int out_bytes, double* cost) {
   const DmaTile* best = nullptr;
   for (const DmaTile& t : kDmaTiles) {
-    const double c = dma_cost(t.cost, likely_tiles(T, E, t.cost.bm) * ((N + t.cost.bn - 1) / t.cost.bn), K / 32.0);
+    const double tiles = likely_tiles(T, E, t.cost.bm) * ((N + t.cost.bn - 1) / t.cost.bn);
+    const double c = dma_cost(t.cost, tiles, (K + 31) / 32, out_bytes);
     if (!best || c < *cost) best = &t, *cost = c;
   }
   return *best;
@@ -193,7 +194,7 @@ int xtc_hip_grouped_matmul(const xtc_hip_grouped_matmul_desc* desc, const void* 
   if (d.dtype == XTC_HIP_BF16 && d.K % 8 == 0 && (d.trans_w || d.N % 8 == 0) && vectors(x, a.ldx) && vectors(w, a.ldw) &&
       a.stride_w % 8 == 0) {
     double cost;
-    const DmaTile& t = dma_tile(d.T, d.E, d.K, d.N, &cost);
+    const DmaTile& t = dma_tile(d.T, d.E, d.K, d.N, d.out_dtype == XTC_HIP_BF16 ? 2 : 4, &cost);
     // few tiles of deep K: waves that share out the depth, 256 of it a step of at
     // least .8 us, 3 where two workgroups a CU share it (512 rows over 2 experts of
     // 3584 x 256: 25 us on DMA tiles, 15 so)

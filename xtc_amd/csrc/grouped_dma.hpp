@@ -7,29 +7,30 @@
 // not.
 //
 // Tile and slab.  A workgroup of WGM x WGN waves computes (16 WGM TM) x
-// (16 WGN TN) outputs, k in slabs of 64 bytes a row: 32 bf16, one
-// v_mfma_f32_16x16x32_bf16 deep, or 128 4-bit elements, two
+// (16 WGN TN) outputs, k in slabs of a row: 64 bytes or 32 bf16, one
+// v_mfma_f32_16x16x32_bf16 deep, or 128 bytes or 256 4-bit elements, four
 // v_mfma_scale_f32_32x32x64_f8f6f4 deep (registers only: 6.5 PFLOP/s, the
-// 16x16x128 form 5.6: the scales take issue slots).  A lane feeds either with 16
-// bytes of a row.  B is the first MFMA operand: a lane ends with four
-// neighbouring columns of one row.
+// 16x16x128 form 5.6: the scales take issue slots), read and multiplied in two
+// halves.  A lane feeds either with 16 bytes of a row.  B is the first MFMA operand:
+// a lane ends with four neighbouring columns of one row.  4-bit slabs are whole
+// cache lines, because half lines are what bounds the DMA from L2: 17 TB/s in 64
+// bytes a row, 26 in 128 (8192^3 349 us and 320, in 64 x 64 tiles 741 and 600).
 //
 // Operands come in two forms.
-//   ROW  k contiguous: staged [rows][64 B], its 16-byte chunk c of row r at
-//        c ^ ((r >> 1) & 3), 4-bit c ^ ((r >> 2) & 3), read by ds_read_b128.
+//   ROW  k contiguous: staged [rows][slab], its 16-byte chunk c of row r at
+//        c ^ ((r >> 1) & 3), 4-bit c ^ ((r >> 1) & 7), read by ds_read_b128.
 //   COL  k strided (bf16): staged [32 k][16-bit columns], its 32-byte chunk c of
 //        row k at c ^ swz(k), read transposed by ds_read_b64_tr_b16.
-// 4-bit operands bring 4 scale bytes a row and slab.  They are staged for four
-// slabs at a time, [rows][16], with every fourth slab and one group ahead (4 bytes
-// of each row a slab would touch as many cache lines as the codes), and a lane
-// reads its row's 16 at once and keeps the 8 of its k (byte reads for every slab
-// cost 8192^3 80 us).
+// 4-bit operands bring 8 scale bytes a row and slab.  They are staged for two
+// slabs at a time, [rows][16], with the pair's first (8 bytes of each row a slab
+// would touch as many cache lines as the codes), and a lane reads its row's 16 at
+// once and keeps the 8 of its k (byte reads for every step cost 8192^3 80 us).
 //
 // Edges cost nothing in the loop: every DMA goes through a buffer descriptor
 // that ends where the tile's rows end, and what lies past it arrives in LDS as
 // zeros.  Only a slab cut by K within ROW rows needs a lane to give up its chunk
-// (an offset past the descriptor's end).  Rows and columns past the tile's edge
-// hold zeros or neighbours and are not stored.
+// (an offset past the descriptor's end) and, 4-bit, scales of 1.  Rows and columns
+// past the tile's edge hold zeros or neighbours and are not stored.
 //
 // Schedules.  PP ("ping-pong", 2 x 4 waves, one workgroup a CU): two groups of
 // four waves, one of each on every SIMD, run half a step apart, so that one
@@ -61,7 +62,7 @@ namespace xtc_hip {
 struct DmaArgs {
   const uint8_t* a;   // ROW: [M] rows; GRAD: x, [M] rows of K columns
   const uint8_t* b;   // matrices of E groups, stride_b bytes apart; GRAD: dy
-  const uint8_t* sa;  // scales of 4-bit operands, `slabs` dwords a row
+  const uint8_t* sa;  // scales of 4-bit operands, a byte a chunk
   const uint8_t* sb;
   const int* sizes;   // null: one group of all rows
   void* c;
@@ -123,7 +124,7 @@ __device__ __forceinline__ unsigned lds_address(const void* p) {
 // from slab `slab`, then from the start; none once all `left` slabs are done, so
 // that the loops start a DMA with every step and wait for constant counts.  All
 // of it is wave-uniform.
-template <bool ROW>
+template <bool ROW, int SLAB>
 struct Walk {
   uint64_t start, at;  // tile's corner in slab 0, in the next slab
   uint64_t step;       // bytes from a slab to the next
@@ -134,7 +135,7 @@ struct Walk {
 
   __device__ __forceinline__ u32x4 next() {
     unsigned bytes;
-    if constexpr (ROW) bytes = width - 64u * (unsigned)slab;
+    if constexpr (ROW) bytes = width - (unsigned)(SLAB * slab);
     else bytes = (unsigned)((min(depth - 32 * slab, 32) - 1) * ld) + width;
     const u32x4 r = descriptor(at, left > 0 ? bytes : 0u);
     --left;
@@ -149,7 +150,7 @@ struct Walk {
 // chunk that 16-row (32-row) fragments find without bank conflicts
 template <bool MX>
 __device__ __forceinline__ int swz_row(int r) {
-  return MX ? (r >> 2) & 3 : (r >> 1) & 3;
+  return MX ? (r >> 1) & 7 : (r >> 1) & 3;
 }
 template <int COLS>
 __device__ __forceinline__ int swz_col(int k) {
@@ -161,8 +162,9 @@ __device__ __forceinline__ int swz_col(int k) {
 template <bool MX, bool ROW, int LEN>
 __device__ __forceinline__ unsigned source(int kb, int lane, int ld) {
   if constexpr (ROW) {
-    const int r = kb * 16 + (lane >> 2);
-    return (unsigned)r * (unsigned)ld + (unsigned)(((lane & 3) ^ swz_row<MX>(r)) * 16);
+    constexpr int CHUNKS = MX ? 8 : 4;
+    const int r = kb * (64 / CHUNKS) + lane / CHUNKS;
+    return (unsigned)r * (unsigned)ld + (unsigned)(((lane % CHUNKS) ^ swz_row<MX>(r)) * 16);
   } else {
     constexpr int SLOTS = LEN / 8, PER = 64 / SLOTS;  // 16-byte slots of a k row, k rows of a KB
     const int k = kb * PER + lane / SLOTS, slot = lane % SLOTS;
@@ -235,17 +237,18 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_dma(DmaArgs p) {
   using namespace gdma;
   constexpr bool A_ROW = !GRAD;
   constexpr int WAVES = WGM * WGN, BM = WGM * TM * 16, BN = WGN * TN * 16;
-  constexpr int A_KB = BM / 16, B_KB = BN / 16, PER = (A_KB + B_KB) / WAVES;  // DMA kilobytes
-  constexpr int S_ALL = MX ? (BM + BN) / 64 : 0;        // scale DMA of four slabs: 64 rows each
-  constexpr int S_PER = (S_ALL + WAVES - 1) / WAVES;    // a wave's with every fourth slab
-  constexpr int A_AT = 0, B_AT = BM * 64, STAGE = B_AT + BN * 64;
+  constexpr int SLAB = MX ? 128 : 64, CHUNKS = SLAB / 16, HALVES = SLAB / 64;  // bytes, 16-byte chunks, steps of a row
+  constexpr int A_KB = BM * SLAB / 1024, B_KB = BN * SLAB / 1024, PER = (A_KB + B_KB) / WAVES;  // DMA kilobytes
+  constexpr int S_ALL = MX ? (BM + BN) / 64 : 0;        // scale DMA of two slabs: 64 rows each
+  constexpr int S_PER = (S_ALL + WAVES - 1) / WAVES;    // a wave's with every second slab
+  constexpr int A_AT = 0, B_AT = BM * SLAB, STAGE = B_AT + BN * SLAB;
   constexpr int S_STAGE = S_ALL * 1024, S_STAGES = 2;
   constexpr int D = STAGES - 1;
   static_assert(PER * WAVES == A_KB + B_KB && A_KB % PER == 0, "a slab splits evenly over the waves, one operand each");
   static_assert(!MX || (B_ROW && !GRAD), "4-bit operands have k along their rows");
   static_assert(!PP || (WGM == 2 && WGN == 4), "two groups of four waves");
   static_assert(STAGES * STAGE + S_STAGES * S_STAGE <= 160 * 1024 && D * PER + S_PER < 64, "LDS and wait counts");
-  static_assert(!MX || STAGES == 4, "a slab's place in its group of four is its stage");
+  static_assert(STAGES % 2 == 0 && STAGES <= 4, "a slab's place in its pair follows from its stage; scales are read in time");
 
   __shared__ __attribute__((aligned(1024))) unsigned char lds[STAGES * STAGE + S_STAGES * S_STAGE];
   unsigned char* const lds_s = lds + STAGES * STAGE;
@@ -297,12 +300,12 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_dma(DmaArgs p) {
     rows = min(gr.end - gr.begin, BM);
     chunks = gr.e < p.E ? p.K : 0;  // rows of no group: zeros
     depth = 8 * chunks;
-    nk = (chunks + 3) / 4;
+    nk = (chunks + CHUNKS - 1) / CHUNKS;
     a = p.a + (int64_t)gr.begin * p.lda;
     b = p.b + e * p.stride_b + (B_ROW ? (int64_t)n0 * p.ldb : 2 * (int64_t)n0);
     if constexpr (MX) {
-      as = p.sa + (int64_t)gr.begin * 4 * nk;
-      bs = p.sb + e * p.stride_sb + (int64_t)n0 * 4 * nk;
+      as = p.sa + (int64_t)gr.begin * chunks;
+      bs = p.sb + e * p.stride_sb + (int64_t)n0 * chunks;
     }
     c_at = (int64_t)gr.begin * p.ldc + n0;
   }
@@ -312,25 +315,27 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_dma(DmaArgs p) {
   const int kb0 = is_a ? wave * PER : wave * PER - A_KB;  // in the operand's stage
   const int ld = is_a ? p.lda : p.ldb;
   const int lines = is_a ? min(rows, BM) : min(cols, BN);  // rows (ROW) or columns (COL) of the operand in the tile
-  unsigned off[PER];
-  int chunk[PER];  // ROW: chunk of the slab that the lane loads
+  // Where the lane finds its 16 bytes of each KB: the pattern of 4-bit rows repeats
+  // after two KB (16 rows)
+  constexpr int OFFS = MX ? 2 : PER;
+  unsigned off[OFFS];
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    off[i] = is_a ? source<MX, A_ROW, BM>(kb0 + i, lane, ld) : source<MX, B_ROW, BN>(kb0 + i, lane, ld);
-    chunk[i] = (lane & 3) ^ swz_row<MX>((kb0 + i) * 16 + (lane >> 2));
-  }
+  for (int i = 0; i < OFFS; ++i) off[i] = is_a ? source<MX, A_ROW, BM>(kb0 + i, lane, ld) : source<MX, B_ROW, BN>(kb0 + i, lane, ld);
+  auto offset = [&](int i, int step) { return off[i % OFFS] + (unsigned)(i / OFFS) * (unsigned)step; };
+  // the chunk of a ROW slab that it loads
+  auto chunk = [&](int i) { return (lane % CHUNKS) ^ swz_row<MX>((kb0 + i % OFFS) * (64 / CHUNKS) + lane / CHUNKS); };
   // K stagger: tiles that share a panel start their walk at different slabs
   // (bf16 8192^3 850 -> 830 us; 4-bit ones gain nothing from whole groups of four)
   const int kofs = !MX && nk > 0 ? ((mt + 2 * (n0 / BN)) & 15) % nk : 0;
   const bool row = is_a ? A_ROW : B_ROW;
-  Walk<true> by_row;
-  Walk<false> by_col;
+  Walk<true, SLAB> by_row;
+  Walk<false, SLAB> by_col;
   if (row) {
     by_row.start = (uint64_t)(is_a ? a : b);
-    by_row.step = 64;
+    by_row.step = SLAB;
     by_row.width = (unsigned)(lines - 1) * (unsigned)ld + 16u * (unsigned)chunks;
     by_row.slab = kofs, by_row.slabs = by_row.left = nk;
-    by_row.at = by_row.start + (uint64_t)kofs * 64;
+    by_row.at = by_row.start + (uint64_t)kofs * SLAB;
   } else {
     by_col.start = (uint64_t)(is_a ? a : b);
     by_col.step = (uint64_t)32 * (uint64_t)ld;
@@ -340,13 +345,14 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_dma(DmaArgs p) {
   }
   const unsigned lds0 = __builtin_amdgcn_readfirstlane(lds_address(lds)), share = (unsigned)((is_a ? 0 : B_AT) + kb0 * 1024);
 
-  // Scales of slabs 4 q .. 4 q + 3; past the last slab they are the next row's
-  // or zeros, and nobody reads them
+  // Scales of slabs 2 q and 2 q + 1, in the place of slabs 2 q - 4 and 2 q - 3, whose
+  // scales everyone has read with the first: slab 2 q - STAGES is read.  Past the
+  // last slab they are the next row's or zeros, and nobody reads them
   const int s_kb = min(wave * S_PER, S_ALL - S_PER);  // a wave without a share repeats the last one
   const bool s_is_a = s_kb < BM / 64;
   const uint64_t s_at = (uint64_t)(s_is_a ? as : bs);
-  const unsigned s_bytes = (unsigned)(s_is_a ? min(rows, BM) : min(cols, BN)) * 4u * (unsigned)nk;
-  const unsigned s_off = (unsigned)((s_is_a ? s_kb : s_kb - BM / 64) * 64 + lane) * 4u * (unsigned)nk;
+  const unsigned s_bytes = (unsigned)(s_is_a ? min(rows, BM) : min(cols, BN)) * (unsigned)chunks;
+  const unsigned s_off = (unsigned)((s_is_a ? s_kb : s_kb - BM / 64) * 64 + lane) * (unsigned)chunks;
   auto issue_scales = [&](int q) {
     static_assert(S_PER <= 1, "one DMA of scales a wave");
     dma16<true, 0>(descriptor(s_at + 16 * (uint64_t)q, (unsigned)max((int)s_bytes - 16 * q, 0)), s_off,
@@ -355,25 +361,27 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_dma(DmaArgs p) {
 
   auto issue = [&](int kt, const int stage) {
     const unsigned at = lds0 + share + stage * STAGE;
+    int step = 16 * ld;  // opaque: the sums of a lane's offsets would fill the registers
+    if constexpr (MX) asm volatile("" : "+s"(step));
     if (row) {
-      const int left = chunks - 4 * by_row.slab;
+      const int left = chunks - CHUNKS * by_row.slab;
       const u32x4 r = by_row.next();
-      if (!MX && left < 4) {
-        each_stage<PER>([&](auto i) { dma16<i == 0, i * 1024>(r, chunk[i] < left ? off[i] : PAST, at); });
+      if (left < CHUNKS) {
+        each_stage<PER>([&](auto i) { dma16<i == 0, i * 1024>(r, chunk(i) < left ? offset(i, step) : PAST, at); });
       } else {
-        each_stage<PER>([&](auto i) { dma16<i == 0, i * 1024>(r, off[i], at); });
+        each_stage<PER>([&](auto i) { dma16<i == 0, i * 1024>(r, offset(i, step), at); });
       }
     } else {
       const u32x4 r = by_col.next();
-      each_stage<PER>([&](auto i) { dma16<i == 0, i * 1024>(r, off[i], at); });
+      each_stage<PER>([&](auto i) { dma16<i == 0, i * 1024>(r, offset(i, step), at); });
     }
-    if (MX && kt % 4 == 0) issue_scales(kt / 4 + 1);
+    if (MX && kt % 2 == 0) issue_scales(kt / 2);
   };
 
-  // DMA instructions of this wave's slabs kt+first .. kt+last, kt % 4 == s
+  // DMA instructions of this wave's slabs kt+first .. kt+last, kt % STAGES == s
   auto dma_count = [](int s, int first, int last) constexpr {
     int n = 0;
-    for (int i = first; i <= last; ++i) n += PER + (MX && (s + i) % 4 == 0 ? S_PER : 0);
+    for (int i = first; i <= last; ++i) n += PER + (MX && (s + i) % 2 == 0 ? S_PER : 0);
     return n;
   };
 
@@ -387,21 +395,25 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_dma(DmaArgs p) {
     for (int j = 0; j < JN; ++j) acc[i][j] = Acc{};
 
   u32x4 fa[STEPS][IM], fb[STEPS][JN];
-  unsigned ha[IM][2], hb[JN][2];  // scales of this lane's row and half of k: slabs 0, 1 and 2, 3 of a group
+  unsigned ha[IM][2], hb[JN][2];  // scales of this lane's row and half of k, of a pair of slabs
   const int l32 = lane & 31, half = lane >> 5;
-  auto read = [&](int kt, const int s, const unsigned char* st) {
+  // half `hf` (64 bytes a row) of slab kt
+  auto read = [&](int kt, const int s, const int hf, const unsigned char* st) {
     if constexpr (MX) {
+      // chunk 4 hf + 2 h + half of the lane's rows; kept from being worked out for
+      // every stage ahead of the loop, which registers do not suffice for
+      unsigned at = (unsigned)(l32 * SLAB + 16 * (half ^ swz_row<MX>(l32)));
+      asm volatile("" : "+v"(at));
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
+        const unsigned char* const rows = st + (at ^ (unsigned)(16 * (4 * hf + 2 * h)));
 #pragma unroll
-        for (int i = 0; i < IM; ++i)
-          fa[h][i] = *(const lds_u32x4*)(st + A_AT + ((wm * IM + i) * 32 + l32) * 64 + 16 * ((2 * h + half) ^ swz_row<MX>(l32)));
+        for (int i = 0; i < IM; ++i) fa[h][i] = *(const lds_u32x4*)(rows + A_AT + (wm * IM + i) * 32 * SLAB);
 #pragma unroll
-        for (int j = 0; j < JN; ++j)
-          fb[h][j] = *(const lds_u32x4*)(st + B_AT + ((wn * JN + j) * 32 + l32) * 64 + 16 * ((2 * h + half) ^ swz_row<MX>(l32)));
+        for (int j = 0; j < JN; ++j) fb[h][j] = *(const lds_u32x4*)(rows + B_AT + (wn * JN + j) * 32 * SLAB);
       }
-      if (s == 0) {
-        const unsigned char* ss = lds_s + kt / 4 % S_STAGES * S_STAGE + l32 * 16;
+      if (s % 2 == 0 && hf == 0) {
+        const unsigned char* ss = lds_s + kt / 2 % S_STAGES * S_STAGE + l32 * 16;
         const unsigned pick = half ? 0x07050301u : 0x06040200u;
         auto keep = [&](unsigned (&h)[2], int row) {
           const u32x4 v = *(const lds_u32x4*)(ss + row * 16);
@@ -413,6 +425,13 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_dma(DmaArgs p) {
 #pragma unroll
         for (int j = 0; j < JN; ++j) keep(hb[j], BM + (wn * JN + j) * 32);
       }
+      // a last slab of four blocks: the others' codes are zeros, scaled by 1
+      if (hf == 1 && kt == nk - 1 && (chunks & 4)) {
+#pragma unroll
+        for (int i = 0; i < IM; ++i) ha[i][s % 2] = (ha[i][s % 2] & 0xffffu) | 0x7f7f0000u;
+#pragma unroll
+        for (int j = 0; j < JN; ++j) hb[j][s % 2] = (hb[j][s % 2] & 0xffffu) | 0x7f7f0000u;
+      }
     } else {
 #pragma unroll
       for (int i = 0; i < IM; ++i) fa[0][i] = fragment<A_ROW, BM>(st + A_AT, wm * TM, i, l16, g);
@@ -420,7 +439,7 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_dma(DmaArgs p) {
       for (int j = 0; j < JN; ++j) fb[0][j] = fragment<B_ROW, BN>(st + B_AT, wn * TN, j, l16, g);
     }
   };
-  auto mma = [&](const int s) {
+  auto mma = [&](const int s, const int hf) {
 #pragma unroll
     for (int h = 0; h < STEPS; ++h)
 #pragma unroll
@@ -428,8 +447,8 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_dma(DmaArgs p) {
 #pragma unroll
         for (int j = 0; j < JN; ++j) {
           if constexpr (MX) {
-            const unsigned sb = hb[j][s / 2], sa = ha[i][s / 2];
-            const int byte = s % 2 * 2 + h;
+            const unsigned sb = hb[j][s % 2], sa = ha[i][s % 2];
+            const int byte = 2 * hf + h;
             acc[i][j] = byte == 0 ? mfma<0>(fb[h][j], sb, fa[h][i], sa, acc[i][j])
                         : byte == 1 ? mfma<1>(fb[h][j], sb, fa[h][i], sa, acc[i][j])
                         : byte == 2 ? mfma<2>(fb[h][j], sb, fa[h][i], sa, acc[i][j])
@@ -440,8 +459,15 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_dma(DmaArgs p) {
         }
   };
 
+  // keeps the products of a compute phase within it
+  auto settle = [&] {
+#pragma unroll
+    for (int i = 0; i < IM; ++i)
+#pragma unroll
+      for (int j = 0; j < JN; ++j) asm volatile("" : "+v"(acc[i][j]));
+  };
+
   if (nk > 0) {
-    if constexpr (MX) issue_scales(0);
     each_stage<D>([&](auto s) { issue(s, s); });
     if constexpr (PP) {
       const int group = wm;
@@ -450,20 +476,24 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_dma(DmaArgs p) {
       if (group == 1) phase_barrier();
       auto step = [&](int kt, auto stage) {
         constexpr int s = decltype(stage)::value;
-        // ---- memory phase
-        issue(kt + D, (s + D) % STAGES);
-        read(kt, s, lds + s * STAGE);
-        __builtin_amdgcn_s_waitcnt(waitcnt_lgkm0());
-        // this wave's DMA of slab kt+1 has landed: group 0 waits after computing
-        if (group == 1) __builtin_amdgcn_s_waitcnt(waitcnt_vm(dma_count(s, 2, D)));
-        phase_barrier();
-        // ---- compute phase, ahead of the SIMD's other wave
-        __builtin_amdgcn_s_setprio(1);
-        mma(s);
-        __builtin_amdgcn_s_setprio(0);
-        __builtin_amdgcn_sched_barrier(0);
-        if (group == 0) __builtin_amdgcn_s_waitcnt(waitcnt_vm(dma_count(s, 2, D)));
-        phase_barrier();
+        each_stage<HALVES>([&](auto hf) {
+          constexpr bool last = hf == HALVES - 1;
+          // ---- memory phase
+          if (hf == 0) issue(kt + D, (s + D) % STAGES);
+          read(kt, s, hf, lds + s * STAGE);
+          __builtin_amdgcn_s_waitcnt(waitcnt_lgkm0());
+          // this wave's DMA of slab kt+1 has landed: group 0 waits after computing
+          if (last && group == 1) __builtin_amdgcn_s_waitcnt(waitcnt_vm(dma_count(s, 2, D)));
+          phase_barrier();
+          // ---- compute phase, ahead of the SIMD's other wave
+          __builtin_amdgcn_s_setprio(1);
+          mma(s, hf);
+          if constexpr (MX) settle();
+          __builtin_amdgcn_s_setprio(0);
+          __builtin_amdgcn_sched_barrier(0);
+          if (last && group == 0) __builtin_amdgcn_s_waitcnt(waitcnt_vm(dma_count(s, 2, D)));
+          phase_barrier();
+        });
       };
       for (int kt = 0; kt < nk; kt += STAGES) each_stage<STAGES>([&](auto s) { if (kt + s < nk) step(kt + s, s); });
       if (group == 0) phase_barrier();
@@ -473,10 +503,13 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_dma(DmaArgs p) {
         // slab kt has landed; the ones after it may be in flight
         __builtin_amdgcn_s_waitcnt(waitcnt_vm(dma_count(s, 1, D - 1)));
         // everyone has read slab kt-1, whose stage the DMA now fills
+        __builtin_amdgcn_s_waitcnt(waitcnt_lgkm0());
         phase_barrier();
         issue(kt + D, (s + D) % STAGES);
-        read(kt, s, lds + s * STAGE);
-        mma(s);
+        each_stage<HALVES>([&](auto hf) {
+          read(kt, s, hf, lds + s * STAGE);
+          mma(s, hf);
+        });
       };
       for (int kt = 0; kt < nk; kt += STAGES) each_stage<STAGES>([&](auto s) { if (kt + s < nk) step(kt + s, s); });
     }
@@ -555,16 +588,21 @@ struct DmaCost {
   int bm, bn, per_cu;
   double light, full;
 };
-// `tiles` of `slabs` on 256 CUs, without what every tile has in common.  Small
-// tiles even out over the CUs; a 256 x 256 one takes a CU for itself, so a last
-// round of few tiles costs as much as a full one.
-inline double dma_cost(const DmaCost& c, double tiles, double slabs) {
-  const double load = tiles / (256.0 * c.per_cu);
-  if (load <= 1) return slabs * (c.light + (c.full - c.light) * load);
-  return slabs * c.full * (c.per_cu == 1 ? ceil(load) : load);
+// `tiles` of `slabs` on 256 CUs, without what every tile has in common.  A round of
+// tiles ends with writing them out, a CU 24 bytes a nanosecond.  Small tiles even out
+// over the CUs (a last round of few 128 x 128 ones still costs half a full one: 4096
+// rows over 8 experts of 4096 x 2048, 1.1 rounds of them 128 us, one of 256 x 256
+// tiles 116); a 256 x 256 one takes a CU for itself, so nothing hides its first loads
+// (2 us) and a last round costs as much as a full one.
+inline double dma_cost(const DmaCost& c, double tiles, double slabs, int out_bytes) {
+  const double load = tiles / (256.0 * c.per_cu), out = c.per_cu * c.bm * c.bn * out_bytes / 24e3 + (c.per_cu == 1 ? 2 : 0);
+  if (load <= 1) return slabs * (c.light + (c.full - c.light) * load) + out;
+  return (slabs * c.full + out) * (load + (ceil(load) - load) / c.per_cu);
 }
 // Tiles of bm rows that a fair share of T rows to E groups makes.
-inline double likely_tiles(double T, double E, int bm) { return fmax(fmin(E, T), T / bm + 0.5 * fmin(E, T)); }
+inline double likely_tiles(double T, double E, int bm) {
+  return E == 1 ? ceil(T / bm) : fmax(fmin(E, T), T / bm + 0.5 * fmin(E, T));
+}
 
 // Workgroups of `a` (its tiles and band set): bands and runs filled up.
 inline int64_t dma_groups(const DmaArgs& a, int64_t matrices) {

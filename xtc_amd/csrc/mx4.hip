@@ -75,16 +75,17 @@ void dma_launch(const DmaArgs& a, unsigned groups, hipStream_t s) {
 }
 // Costs as measured: 1 x 8192 x 8192 (light), 4096 x 8192 x 8192 and 8192^3 (full).
 const DmaTile kDmaTiles[] = {
-    {{256, 256, 1, 0.53, 1.20}, &dma_launch<2, 4, 8, 4, 4, true>},
-    {{128, 128, 2, 0.27, 0.87}, &dma_launch<2, 2, 4, 4, 4, false>},
-    {{64, 64, 4, 0.15, 0.81}, &dma_launch<2, 2, 2, 2, 4, false>},
+    {{256, 256, 1, 1.25, 2.00}, &dma_launch<2, 4, 8, 4, 2, true>},
+    {{128, 128, 2, 0.73, 1.45}, &dma_launch<2, 2, 4, 4, 2, false>},
+    {{64, 64, 2, 0.24, 0.62}, &dma_launch<2, 2, 2, 2, 4, false>},
 };
 
-const DmaTile& dma_tile(int64_t rows, int64_t groups, int N, int blocks) {
+const DmaTile& dma_tile(int64_t rows, int64_t groups, int N, int blocks, int out_bytes) {
   const DmaTile* best = nullptr;
   double least = 0;
   for (const DmaTile& t : kDmaTiles) {
-    const double cost = dma_cost(t.cost, likely_tiles(rows, groups, t.cost.bm) * ((N + t.cost.bn - 1) / t.cost.bn), blocks / 4);
+const double tiles = likely_tiles(rows, groups, t.cost.bm) * ((N + t.cost.bn - 1) / t.cost.bn);
+    const double cost = dma_cost(t.cost, tiles, (blocks + 4) / 8, out_bytes);
     if (!best || cost < least) best = &t, least = cost;
   }
   return *best;
@@ -190,7 +191,7 @@ int xtc_hip_mx4_matmul(const xtc_hip_mx4_matmul_desc* desc, const uint8_t* a_cod
     return done(what);
   }
   if (slabs) {
-    const DmaTile& t = dma_tile(d.M, a.E, d.N, d.blocks);
+    const DmaTile& t = dma_tile(d.M, a.E, d.N, d.blocks, d.out_dtype == XTC_HIP_BF16 ? 2 : 4);
     DmaArgs v{};
     v.a = a_codes, v.b = b_codes, v.sa = a_scales, v.sb = b_scales, v.sizes = sizes, v.c = c;
     v.E = a.E, v.M = d.M, v.N = d.N, v.K = d.blocks;

@@ -285,7 +285,9 @@ int xtc_hip_grouped_matmul(const xtc_hip_grouped_matmul_desc *desc, const void *
  * it has none.  x [T][ldx >= K] and dy [T][ldy >= N] of type dtype, dw [K][ldw >=
  * N] matrices of type out_dtype, stride_w apart; trans_w must be 0 (the transposed
  * gradient is this one with x and dy exchanged).  The order of the sums depends
- * on the sizes alone. */
+ * on the extents and sizes[], but for bf16 calls of few matrices and many rows in
+ * whole 16-byte vectors: they are summed in parts in the stream's scratch, or in
+ * one part while the stream is captured or without memory for it. */
 int xtc_hip_grouped_matmul_grad_w(const xtc_hip_grouped_matmul_desc *desc, const void *x,
                                   const void *dy, const int32_t *sizes, void *dw);
 

@@ -131,15 +131,15 @@ template <> struct Quarter<__bf16> { typedef QuarterBf16 type; };
 // the first n of the 8 elements at p, zeros for the others
 template <typename T>
 __device__ __forceinline__ typename Quarter<T>::type load_quarter(const T* p, int n) {
-  typename Quarter<T>::type q;
   T raw[8];
   if (n >= 8) {
-    __builtin_memcpy(&q, p, sizeof(q));
+    __builtin_memcpy(raw, p, sizeof(raw));
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) raw[i] = i < n ? p[i] : (T)0.f;
-    __builtin_memcpy(&q, raw, sizeof(q));
   }
+  typename Quarter<T>::type q;
+  __builtin_memcpy(&q, raw, sizeof(q));
   return q;
 }
 

@@ -336,6 +336,16 @@ int xtc_hip_mx4_matmul(const xtc_hip_mx4_matmul_desc *desc, const uint8_t *a_cod
                        const uint8_t *a_scales, const uint8_t *b_codes,
                        const uint8_t *b_scales, const int32_t *sizes, void *c);
 
+/* The product of x brought to 4 bits: xtc_hip_mx4_quantize(rows, x) and
+ * xtc_hip_mx4_matmul(desc) with the same results, in one launch where x has few
+ * rows.  a_codes and a_scales are scratch of the operand's size that the call may
+ * or may not fill.  rows->rows is desc->M, ceil(rows->K / 32) desc->blocks, and
+ * both name one stream. */
+int xtc_hip_mx4_quantize_matmul(const xtc_hip_mx4_desc *rows,
+                                const xtc_hip_mx4_matmul_desc *desc, const void *x,
+                                uint8_t *a_codes, uint8_t *a_scales, const uint8_t *b_codes,
+                                const uint8_t *b_scales, const int32_t *sizes, void *c);
+
 /* sizeof(xtc_hip_matmul_desc) and sizeof(xtc_hip_conv2d_desc) as this library
  * was compiled (and of the other descriptors, below): a binding that declares the descriptors itself (ctypes, cgo)
  * checks its own struct sizes against these before the first call, so a

@@ -164,6 +164,25 @@ def mx4_matmul(ac, asc, bc, bsc, sizes=None, out_dtype="float32", pad=0, shift=0
     return got[:, :N]
 
 
+def mx4_quantize_matmul(x, dtype, bc, bsc, sizes=None, out_dtype="float32", pad=0, ldx=0, shift=0):
+    """The product with x quantised by the same call."""
+    (M, K), nb, N = x.shape, bsc.shape[-1], bsc.shape[-2]
+    r = capi.Mx4Desc(dtype=IDS[dtype], rows=M, K=K, ld=K + ldx)
+    d = capi.Mx4MatmulDesc(out_dtype=IDS[out_dtype], E=0 if sizes is None else len(sizes), M=M, N=N, blocks=nb, ldc=N + pad)
+    mx = Mem(padded(x, K + ldx), dtype, shift)
+    mems = [mx, Mem(np.zeros((M, 16 * nb)), "uint8"), Mem(np.zeros((M, nb)), "uint8"), Mem(bc, "uint8"), Mem(bsc, "uint8")]
+    sz = None if sizes is None else Mem(np.asarray(sizes), "int32")
+    out = Mem(padded(np.full((M, N), 7.0), N + pad), out_dtype)
+    capi.check(capi.lib().xtc_hip_mx4_quantize_matmul(ctypes.byref(r), ctypes.byref(d), *[m.ptr for m in mems],
+                                                      sz.ptr if sz else None, out.ptr))
+    capi.check(capi.lib().xtc_hip_synchronize())
+    got = out.numpy()
+    for m in (*mems, out, *([sz] if sz else [])):
+        m.free()
+    assert np.isnan(got[:, N:]).all(), "written past the columns"
+    return got[:, :N]
+
+
 def ints(seed, shape, top=4):
     """Whole numbers: sums below 2^24 are exact in fp32, in any order."""
     return np.random.default_rng(seed).integers(-top, top + 1, shape).astype(np.float32)

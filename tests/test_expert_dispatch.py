@@ -9,9 +9,9 @@ import pytest
 from test_dispatch import pytestmark, run  # noqa: F401
 
 CALLS = """
-def call(fn, desc, *args):
+def call(fn, *args):
     fake.fake_launches()
-    rc = getattr(L, fn)(ctypes.byref(desc) if desc is not None else None, *[ctypes.c_void_p(a) for a in args])
+    rc = getattr(L, fn)(*[ctypes.byref(a) if isinstance(a, ctypes.Structure) else a for a in args])
     got = fake.fake_launches().decode().splitlines()
     assert not (rc and got), got
     return capi.last_error() if rc else [[g.split("|")[0].replace("void ", "").replace("xtc_hip::", "").split("(")[0], g.split("|")[1]] for g in got]
@@ -88,6 +88,35 @@ for i in (0, 1, 2, 3, 5):
     want = [w for w, _ in wrong] + ["with sizes"] + ["16-byte aligned"] * 2 + ["null operand"] * 5
     for message, why in zip(got, want, strict=True):
         assert isinstance(message, str) and why in message, (why, message)
+
+
+def test_mx4_quantize_matmul_refusals(run):  # noqa: F811
+    wrong = [("unsupported dtype", dict(dtype=2), {}), ("row stride", dict(ld=31), {}), ("invalid sizes", {}, dict(N=0)),
+             ("without sizes", {}, dict(E=2)), ("to multiply", dict(rows=3), {}), ("to multiply", dict(K=33), {}),
+             ("to multiply", {}, dict(blocks=2)), ("two streams", dict(stream=512), {})]
+    got = run(CALLS + f"""
+def quantize_matmul(rows, desc, args=(256, 256, 256, 256, 256, None, 256)):
+    rows = capi.Mx4Desc(**{{**dict(dtype=1, rows=2, K=32), **rows}})
+    desc = capi.Mx4MatmulDesc(**{{**dict(out_dtype=0, M=2, N=8, blocks=1), **desc}})
+    return call("xtc_hip_mx4_quantize_matmul", rows, desc, *args)
+for rows, desc in {[w[1:] for w in wrong]!r}:
+    out.append(quantize_matmul(rows, desc))
+for i in (0, 1, 2, 3, 4, 6):
+    out.append(quantize_matmul({{}}, {{}}, [None if j in (i, 5) else 256 for j in range(7)]))
+for i in (1, 3):
+    out.append(quantize_matmul({{}}, {{}}, [260 if i == j else None if j == 5 else 256 for j in range(7)]))
+out.append(call("xtc_hip_mx4_quantize_matmul", None, capi.Mx4MatmulDesc(), *(256,) * 7))
+out.append(call("xtc_hip_mx4_quantize_matmul", capi.Mx4Desc(dtype=1, rows=2, K=32), *(None,) * 8))
+# few rows in one launch, others and fp32 ones in two
+out.append(quantize_matmul({{}}, {{}}))
+out.append(quantize_matmul(dict(dtype=0), {{}}))
+out.append(quantize_matmul(dict(rows=4096), dict(M=4096, N=4096)))
+out.append(quantize_matmul(dict(rows=0), dict(M=0)))
+""")
+    want = [w[0] for w in wrong] + ["null operand"] * 6 + ["16-byte aligned"] * 2 + ["null descriptor"] * 2
+    for message, why in zip(got, want):
+        assert isinstance(message, str) and why in message, (why, message)
+    assert [len(g) for g in got[len(want):]] == [1, 2, 2, 0], got[len(want):]
 
 
 def test_calls_without_rows_launch_nothing(run):  # noqa: F811

@@ -92,7 +92,12 @@ def test_mx4_graph_is_one_launch():
     # codes for the scales of another tensor, and the values of another type
     (["mx4_quantize", "mx4_encode"], lambda x: O.mx4_codes(O.relu(x), O.mx4_scales(x))),
     (["mx4_quantize", "mx4_dequantize"], lambda x: O.mx4_dequantize(*O.mx4_quantize(x), out_dtype="bfloat16")),
-    (["mx4_quantize", "mx4_matmul"], lambda x: O.mx4_matmul(*O.mx4_quantize(x), *O.mx4_quantize(x))),
+    (["mx4_quantize", "mx4_quantize_matmul"], lambda x: O.mx4_matmul(*O.mx4_quantize(x), *O.mx4_quantize(x))),
+    (["mx4_quantize", "mx4_matmul"], lambda x: (lambda q: O.mx4_matmul(*q, *q))(O.mx4_quantize(x))),
+    (["mx4_quantize", "mx4_matmul"], lambda x: (lambda q, w: O.outputs(*q, O.mx4_matmul(*q, *w)))(
+        O.mx4_quantize(x), O.mx4_quantize(x))),
+    (["mx4_quantize", "mx4_matmul"], lambda x: (lambda q, w: O.outputs(O.mx4_matmul(*q, *w), O.mx4_dequantize(*q, size=64)))(
+        O.mx4_quantize(x), O.mx4_quantize(x))),
 ])
 def test_mx4_plans(kinds, fn):
     graph = build(fn, ((64, 64), "float32"))
@@ -236,7 +241,7 @@ def test_example_graphs_lower():
         backend.get_compiler(schedule_policy="strict").compile(backend.get_scheduler().schedule())
         kinds[graph.name] = [launch.kind for launch in backend.plan.launches]
     assert kinds == {"experts_step": ["grouped_matmul"] * 2 + ["grouped_matmul_grad_w"], "experts_quantize": ["mx4_quantize"],
-                     "experts_serve": ["mx4_quantize", "mx4_matmul", "relu", "mx4_quantize", "mx4_matmul"]}
+                     "experts_serve": ["mx4_quantize_matmul", "relu", "mx4_quantize_matmul"]}
     up, down = (rng.normal(size=s).astype(np.float32) for s in ((E, N, K), (E, K, N)))
     x, sizes = rng.normal(size=(T, K)).astype(np.float32), np.array([7, 0, 9], np.int32)
     packed = [a for w in (up, down) for a in forward(experts.quantize_graph(*w.shape), w)]

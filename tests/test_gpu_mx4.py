@@ -16,7 +16,7 @@ import ctypes
 import numpy as np
 import pytest
 
-from expert_calls import bounds, dequantize, encode, mx4_matmul, quantize, rounded
+from expert_calls import bounds, dequantize, encode, mx4_matmul, mx4_quantize_matmul, quantize, rounded
 from xtc_amd.runtimes.hip import capi
 from xtc_amd.runtimes.hip.buffer import ensure_device
 from xtc_amd.runtimes.hip.device import HipDevice
@@ -237,3 +237,27 @@ def test_large_tiles(out, M, N, nb):
     b = operand(17, (6, N), nb)
     want, spread = plain(*a, *b, sizes)
     check_product(mx4_matmul(*a, *b, sizes=sizes, out_dtype=out), want, spread, 32 * nb, out)
+
+
+@pytest.mark.parametrize("out", ["float32", "bfloat16"])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("M,E,N,K", [(1, 0, 1, 8), (1, 0, 40, 4096), (3, 0, 200, 1000), (16, 0, 256, 96), (17, 0, 65, 31), (40, 0, 33, 5000),
+                                     (250, 0, 80, 640), (16, 0, 8192, 264), (700, 0, 500, 128), (1, 5, 64, 512), (20, 3, 100, 1032),
+                                     (300, 4, 256, 64)])
+def test_quantised_on_the_way(out, dtype, M, E, N, K):
+    """As by two calls, to the bit: blocks of NaN, infinities, zeros, the smallest and
+    the largest numbers among them."""
+    nb = -(-K // 32)
+    rng = np.random.default_rng(M + N)
+    x = rng.normal(size=(M, K)) * 2.0 ** rng.integers(-20, 21, (M, K))
+    for i, v in enumerate((np.nan, np.inf, 0.0, 2.0**-133, 3.3e38)):
+        x[i % M, 32 * i % K :: 97 * (i + 1)] = v
+    x = rounded(x, dtype)
+    bc, bsc = operand(K, ((E, N) if E else (N,)), nb)
+    sizes = rng.multinomial(M - M // 8, np.full(E, 1 / E)) if E else None
+    print(f"[mx4 quantise matmul] {M} {E} {N} {K} {dtype} {out}", flush=True)
+    codes, scales, _ = quantize(x, dtype)
+    want = mx4_matmul(codes, scales, bc, bsc, sizes, out)
+    for pad, ldx, shift in ((0, 0, 0), (3, 5, 1)):
+        got = mx4_quantize_matmul(x, dtype, bc, bsc, sizes, out, pad, ldx, shift)
+        np.testing.assert_array_equal(got, want)

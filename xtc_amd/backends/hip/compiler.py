@@ -317,13 +317,18 @@ def _emit_launch(plan: Plan, ln: Launch, cfg: GemmConfig | SplitConfig | None, i
             f"  {{ static const xtc_hip_mx4_desc d = {{{_DTYPE_ENUM[a['dtype']]}, {a['rows']}ll, {a['K']}, 0, 0}};"
         )
         lines.append(f"    if ((rc = xtc_hip_{ln.kind}(&d, {args}))) {{ record(rc, {where}); return; }} }}")
-    elif ln.kind == "mx4_matmul":
-        args = ", ".join([*(_ptr(plan, u) for u in ln.inputs), *(() if a["E"] else ("0",)), dst])
+    elif ln.kind in ("mx4_matmul", "mx4_quantize_matmul"):
+        args = ", ".join(["&d", *(_ptr(plan, u) for u in ln.inputs), *(() if a["E"] else ("0",)), dst])
         lines.append(
             f"  {{ static const xtc_hip_mx4_matmul_desc d = {{{_DTYPE_ENUM[a['out']]}, {a['E']}, {a['M']}, {a['N']}, "
             f"{a['blocks']}, 0, 0}};"
         )
-        lines.append(f"    if ((rc = xtc_hip_mx4_matmul(&d, {args}))) {{ record(rc, {where}); return; }} }}")
+        if ln.kind == "mx4_quantize_matmul":
+            lines.append(
+                f"    static const xtc_hip_mx4_desc r = {{{_DTYPE_ENUM[a['dtype']]}, {a['rows']}ll, {a['K']}, 0, 0}};"
+            )
+            args = f"&r, {args}"
+        lines.append(f"    if ((rc = xtc_hip_{ln.kind}({args}))) {{ record(rc, {where}); return; }} }}")
     else:
         raise ScheduleError(f"no code generator for launch kind {ln.kind}")
     return lines
@@ -492,7 +497,8 @@ class HipCompiler(Compiler):
             if ln.kind in ("matmul", "conv2d"):
                 configs[ln.node] = map_node(ln.attrs, ln.kind == "conv2d", schedule.node(ln.node), policy)
             elif ln.kind.startswith(("grouped_", "mx4_")):
-                check_unscheduled(ln.kind, schedule.node(ln.node))
+                for node in (ln.node, *ln.absorbed):
+                    check_unscheduled(ln.kind, schedule.node(node))
         return configs
 
     def check_fusions(self, schedule: HipSchedule) -> None:

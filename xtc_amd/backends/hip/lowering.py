@@ -64,7 +64,8 @@ class Launch:
 
     # "matmul" | "conv2d" | "relu" | "pad" | "unpad" | "copy" | "cast" |
     # "grouped_matmul" | "grouped_matmul_grad_w" |
-    # "mx4_quantize" | "mx4_encode" | "mx4_dequantize" | "mx4_matmul"
+    # "mx4_quantize" | "mx4_encode" | "mx4_dequantize" | "mx4_matmul" |
+    # "mx4_quantize_matmul" (inputs x, the scratch codes and scales, then mx4_matmul's)
     kind: str
     node: str
     inputs: list[str]
@@ -382,7 +383,17 @@ def lower_graph(graph: Any) -> Plan:
             bs = _shape(out_type(n.inputs[3]))
             attrs = {"out": _dtype(t_out), "E": bs[0] if name == "grouped_mx4_matmul" else 0,
                      "M": _shape(t_out)[0], "N": bs[-2], "blocks": bs[-1]}
-            launches.append(Launch("mx4_matmul", n.name, list(n.inputs), n.uid, attrs))
+            ln = Launch("mx4_matmul", n.name, list(n.inputs), n.uid, attrs)
+            # rows quantised for this product alone
+            q = next((q for q in launches if q.kind == "mx4_quantize"
+                      and [q.attrs["codes"], q.output] == ln.inputs[:2] and not q.attrs["values"]), None)
+            if (q and [u.uid for u in users[q.attrs["codes"]]] == [n.uid]
+                    and {u.uid for u in users[q.output]} == {q.attrs["codes"], n.uid}
+                    and not {q.attrs["codes"], q.output} & set(outputs)):
+                launches.remove(q)
+                ln = Launch("mx4_quantize_matmul", n.name, [*q.inputs, *ln.inputs], n.uid, {**attrs, **q.attrs},
+                            [q.node, *q.absorbed])
+            launches.append(ln)
             scheduled[n.name] = n
         elif name == "reshape":
             if n.uid in outputs:

@@ -97,12 +97,17 @@ struct RowsTile {
   int bm, bn;
   void (*run[2])(const Mx4Args&, unsigned, hipStream_t);  // to fp32, to bf16
 };
-template <typename U, int TM, int TN>
+template <typename U, int TM, int TN, bool QUANTIZE>
 void rows_launch(const Mx4Args& a, unsigned groups, hipStream_t s) {
-  hipLaunchKernelGGL((mx4_rows<U, TM, TN>), dim3(groups), dim3(64 * mx4::RWAVES), 0, s, a);
+  hipLaunchKernelGGL((mx4_rows<U, TM, TN, QUANTIZE>), dim3(groups), dim3(64 * mx4::RWAVES), 0, s, a);
 }
-const RowsTile kRows16 = {16, 32, {&rows_launch<float, 1, 2>, &rows_launch<__bf16, 1, 2>}};
-const RowsTile kRows32 = {32, 32, {&rows_launch<float, 2, 2>, &rows_launch<__bf16, 2, 2>}};
+const RowsTile kRows16 = {16, 32, {&rows_launch<float, 1, 2, false>, &rows_launch<__bf16, 1, 2, false>}};
+const RowsTile kRows32 = {32, 32, {&rows_launch<float, 2, 2, false>, &rows_launch<__bf16, 2, 2, false>}};
+const RowsTile kRowsX = {16, 32, {&rows_launch<float, 1, 2, true>, &rows_launch<__bf16, 1, 2, true>}};
+
+double rows_groups(const RowsTile& t, int64_t rows, int64_t groups, int N) {
+  return likely_tiles(rows, groups, t.bm) * ((N + t.bn - 1) / t.bn);
+}
 
 // As many tiles as fit the CUs at once: eight waves a tile then read b as fast as it
 // comes (8192 x 8192 with 16 rows: 9.9 us, DMA tiles 13.8; with 32: 12.3, 14.4;
@@ -115,9 +120,80 @@ const RowsTile kRows32 = {32, 32, {&rows_launch<float, 2, 2>, &rows_launch<__bf1
 const RowsTile* rows_tile(int64_t rows, int64_t groups, int N, bool slabs) {
   const double most = groups > 1 ? 512 : 256;
   for (const RowsTile* t : {&kRows16, &kRows32})
-    if (likely_tiles(rows, groups, t->bm) * ((N + t->bn - 1) / t->bn) <= most) return t;
+    if (rows_groups(*t, rows, groups, N) <= most) return t;
   if (slabs) return nullptr;
   return rows <= 16 * groups ? &kRows16 : rows <= 32 * groups ? &kRows32 : nullptr;
+}
+
+// Whole quarters of blocks, no more workgroups than the CUs take at once, since each
+// quantises its rows, and rows short enough: lanes read 64 bytes of different ones,
+// which costs more than a launch (4 us) from some 32768 elements on.  16 rows x 1024
+// x 2048 7.7 us in two launches, 4.9 in one; x 2048 x 8192 7.9, 7.0; x 4096 x 4096
+// 8.4, 10.2; 1 x 8192 x 8192 11.1 both.
+bool quantizes_on_the_way(int64_t rows, int64_t groups, int N, int K) {
+  const int64_t each = (rows + groups - 1) / groups;
+  return K % 8 == 0 && K < 8192 && (each < 16 ? each : 16) * K <= 32768 && rows_groups(kRowsX, rows, groups, N) <= 256;
+}
+
+int launch_rows(const xtc_hip_mx4_matmul_desc& d, const RowsTile& t, Mx4Args& a, const char* what) {
+  a.tiles_n = (d.N + t.bn - 1) / t.bn;
+  const int64_t groups = a.tiles_n * (a.sizes ? most_tiles(d.M, d.E, t.bm) : ((int64_t)d.M + t.bm - 1) / t.bm);
+  if (groups >= (int64_t)1 << 31) return fail("%s: %lld workgroups are too many", what, (long long)groups);
+  t.run[d.out_dtype](a, (unsigned)groups, core::pick_stream(d.stream));
+  return done(what);
+}
+
+// ---- products
+
+int check(const xtc_hip_mx4_matmul_desc* desc, const int32_t* sizes, const char* what) {
+  if (!core::ready()) return fail("xtc_hip_init not called");
+  if (!desc) return fail("%s: null descriptor", what);
+  const xtc_hip_mx4_matmul_desc& d = *desc;
+  if (d.out_dtype != XTC_HIP_F32 && d.out_dtype != XTC_HIP_BF16) return fail("%s: unsupported result dtype %d", what, d.out_dtype);
+  if (d.E < 0 || d.M < 0 || d.N < 1 || d.blocks < 1)
+    return fail("%s: invalid sizes E=%d M=%d N=%d blocks=%d", what, d.E, d.M, d.N, d.blocks);
+  if (d.E > kMost || d.M > kMost || d.N > kMost || d.blocks > kMost / 32)
+    return fail("%s: sizes E=%d M=%d N=%d blocks=%d are too many", what, d.E, d.M, d.N, d.blocks);
+  if ((d.E > 0) != (sizes != nullptr)) return fail("%s: E=%d groups %s sizes", what, d.E, sizes ? "with" : "without");
+  if (d.ldc && d.ldc < d.N) return fail("%s: row stride %d of c is below its %d columns", what, d.ldc, d.N);
+  return 0;
+}
+
+Mx4Args args_of(const xtc_hip_mx4_matmul_desc& d, const uint8_t* a_codes, const uint8_t* a_scales, const uint8_t* b_codes,
+                const uint8_t* b_scales, const int32_t* sizes, void* c) {
+  Mx4Args a{};
+  a.a_codes = a_codes, a.a_scales = a_scales, a.b_codes = b_codes, a.b_scales = b_scales, a.sizes = sizes, a.c = c;
+  a.E = d.E > 0 ? d.E : 1, a.M = d.M, a.N = d.N, a.blocks = d.blocks, a.ldc = d.ldc ? d.ldc : d.N;
+  return a;
+}
+
+int product(const xtc_hip_mx4_matmul_desc& d, Mx4Args& a, const char* what) {
+  const bool slabs = d.blocks % 4 == 0 && d.blocks < (1 << 19) && ((uintptr_t)a.a_scales & 3) == 0 && ((uintptr_t)a.b_scales & 3) == 0;
+  if (const RowsTile* t = rows_tile(d.M, a.E, d.N, slabs)) return launch_rows(d, *t, a, what);
+  if (slabs) {
+    const DmaTile& t = dma_tile(d.M, a.E, d.N, d.blocks, d.out_dtype == XTC_HIP_BF16 ? 2 : 4);
+    DmaArgs v{};
+    v.a = a.a_codes, v.b = a.b_codes, v.sa = a.a_scales, v.sb = a.b_scales, v.sizes = a.sizes, v.c = a.c;
+    v.E = a.E, v.M = d.M, v.N = d.N, v.K = d.blocks;
+    v.lda = v.ldb = 16 * d.blocks, v.ldc = a.ldc;
+    v.stride_b = (int64_t)d.N * v.ldb, v.stride_sb = (int64_t)d.N * d.blocks;
+    v.tiles_m = (int)(a.sizes ? most_tiles(d.M, d.E, t.cost.bm) : ((int64_t)d.M + t.cost.bm - 1) / t.cost.bm);
+    v.tiles_n = (d.N + t.cost.bn - 1) / t.cost.bn;
+    v.band = v.tiles_m < 8 ? v.tiles_m : 8;
+    v.out16 = d.out_dtype == XTC_HIP_BF16;
+    const int64_t groups = dma_groups(v, 1);
+    if (groups >= (int64_t)1 << 31) return fail("%s: %lld workgroups are too many", what, (long long)groups);
+    t.launch(v, (unsigned)groups, core::pick_stream(d.stream));
+    return done(what);
+  }
+  a.tiles_n = (d.N + mx4::BN - 1) / mx4::BN;
+  const int64_t rows = a.sizes ? most_tiles(d.M, d.E, mx4::BM) : ((int64_t)d.M + mx4::BM - 1) / mx4::BM;
+  if (rows * a.tiles_n < 1 || rows * a.tiles_n >= (int64_t)1 << 31)
+    return fail("%s: %lld workgroups are too many", what, (long long)(rows * a.tiles_n));
+  const dim3 grid((unsigned)(rows * a.tiles_n));
+  if (d.out_dtype == XTC_HIP_F32) hipLaunchKernelGGL(mx4_any<float>, grid, dim3(256), 0, core::pick_stream(d.stream), a);
+  else hipLaunchKernelGGL(mx4_any<__bf16>, grid, dim3(256), 0, core::pick_stream(d.stream), a);
+  return done(what);
 }
 
 }  // namespace
@@ -166,54 +242,33 @@ int xtc_hip_mx4_dequantize(const xtc_hip_mx4_desc* desc, const uint8_t* codes, c
 int xtc_hip_mx4_matmul(const xtc_hip_mx4_matmul_desc* desc, const uint8_t* a_codes, const uint8_t* a_scales,
                        const uint8_t* b_codes, const uint8_t* b_scales, const int32_t* sizes, void* c) {
   const char* const what = "mx4_matmul";
-  if (!core::ready()) return fail("xtc_hip_init not called");
-  if (!desc) return fail("%s: null descriptor", what);
-  const xtc_hip_mx4_matmul_desc& d = *desc;
-  if (d.out_dtype != XTC_HIP_F32 && d.out_dtype != XTC_HIP_BF16) return fail("%s: unsupported result dtype %d", what, d.out_dtype);
-  if (d.E < 0 || d.M < 0 || d.N < 1 || d.blocks < 1)
-    return fail("%s: invalid sizes E=%d M=%d N=%d blocks=%d", what, d.E, d.M, d.N, d.blocks);
-  if (d.E > kMost || d.M > kMost || d.N > kMost || d.blocks > kMost / 32)
-    return fail("%s: sizes E=%d M=%d N=%d blocks=%d are too many", what, d.E, d.M, d.N, d.blocks);
-  if ((d.E > 0) != (sizes != nullptr)) return fail("%s: E=%d groups %s sizes", what, d.E, sizes ? "with" : "without");
-  if (d.ldc && d.ldc < d.N) return fail("%s: row stride %d of c is below its %d columns", what, d.ldc, d.N);
-  if (d.M == 0) return 0;
+  if (check(desc, sizes, what)) return 1;
+  if (desc->M == 0) return 0;
   if (!a_codes || !a_scales || !b_codes || !b_scales || !c) return fail("%s: null operand", what);
   if (!aligned16(a_codes) || !aligned16(b_codes)) return fail("%s: codes must be 16-byte aligned", what);
-  Mx4Args a{};
-  a.a_codes = a_codes, a.a_scales = a_scales, a.b_codes = b_codes, a.b_scales = b_scales, a.sizes = sizes, a.c = c;
-  a.E = d.E > 0 ? d.E : 1, a.M = d.M, a.N = d.N, a.blocks = d.blocks, a.ldc = d.ldc ? d.ldc : d.N;
-  const bool slabs = d.blocks % 4 == 0 && d.blocks < (1 << 19) && ((uintptr_t)a_scales & 3) == 0 && ((uintptr_t)b_scales & 3) == 0;
-  if (const RowsTile* t = rows_tile(d.M, a.E, d.N, slabs)) {
-    a.tiles_n = (d.N + t->bn - 1) / t->bn;
-    const int64_t groups = a.tiles_n * (sizes ? most_tiles(d.M, d.E, t->bm) : ((int64_t)d.M + t->bm - 1) / t->bm);
-    if (groups >= (int64_t)1 << 31) return fail("%s: %lld workgroups are too many", what, (long long)groups);
-    t->run[d.out_dtype](a, (unsigned)groups, core::pick_stream(d.stream));
-    return done(what);
+  Mx4Args a = args_of(*desc, a_codes, a_scales, b_codes, b_scales, sizes, c);
+  return product(*desc, a, what);
+}
+
+int xtc_hip_mx4_quantize_matmul(const xtc_hip_mx4_desc* rows, const xtc_hip_mx4_matmul_desc* desc, const void* x,
+                                uint8_t* a_codes, uint8_t* a_scales, const uint8_t* b_codes, const uint8_t* b_scales,
+                                const int32_t* sizes, void* c) {
+  const char* const what = "mx4_quantize_matmul";
+  if (check(rows, what) || check(desc, sizes, what)) return 1;
+  if (rows->rows != desc->M || (rows->K + 31) / 32 != desc->blocks || rows->stream != desc->stream)
+    return fail("%s: %lld rows of %d elements to quantise, %d rows of %d blocks to multiply, or two streams", what,
+                (long long)rows->rows, rows->K, desc->M, desc->blocks);
+  if (desc->M == 0) return 0;
+  if (!x || !a_codes || !a_scales || !b_codes || !b_scales || !c) return fail("%s: null operand", what);
+  if (!aligned16(a_codes) || !aligned16(b_codes)) return fail("%s: codes must be 16-byte aligned", what);
+  Mx4Args a = args_of(*desc, a_codes, a_scales, b_codes, b_scales, sizes, c);
+  if (rows->dtype == XTC_HIP_BF16 && quantizes_on_the_way(desc->M, a.E, desc->N, rows->K)) {
+    a.x = (const __bf16*)x, a.K = rows->K, a.ldx = rows->ld ? rows->ld : rows->K;
+    return launch_rows(*desc, kRowsX, a, what);
   }
-  if (slabs) {
-    const DmaTile& t = dma_tile(d.M, a.E, d.N, d.blocks, d.out_dtype == XTC_HIP_BF16 ? 2 : 4);
-    DmaArgs v{};
-    v.a = a_codes, v.b = b_codes, v.sa = a_scales, v.sb = b_scales, v.sizes = sizes, v.c = c;
-    v.E = a.E, v.M = d.M, v.N = d.N, v.K = d.blocks;
-    v.lda = v.ldb = 16 * d.blocks, v.ldc = a.ldc;
-    v.stride_b = (int64_t)d.N * v.ldb, v.stride_sb = (int64_t)d.N * d.blocks;
-    v.tiles_m = (int)(sizes ? most_tiles(d.M, d.E, t.cost.bm) : ((int64_t)d.M + t.cost.bm - 1) / t.cost.bm);
-    v.tiles_n = (d.N + t.cost.bn - 1) / t.cost.bn;
-    v.band = v.tiles_m < 8 ? v.tiles_m : 8;
-    v.out16 = d.out_dtype == XTC_HIP_BF16;
-    const int64_t groups = dma_groups(v, 1);
-    if (groups >= (int64_t)1 << 31) return fail("%s: %lld workgroups are too many", what, (long long)groups);
-    t.launch(v, (unsigned)groups, core::pick_stream(d.stream));
-    return done(what);
-  }
-  a.tiles_n = (d.N + mx4::BN - 1) / mx4::BN;
-  const int64_t rows = sizes ? most_tiles(d.M, d.E, mx4::BM) : ((int64_t)d.M + mx4::BM - 1) / mx4::BM;
-  if (rows * a.tiles_n < 1 || rows * a.tiles_n >= (int64_t)1 << 31)
-    return fail("%s: %lld workgroups are too many", what, (long long)(rows * a.tiles_n));
-  const dim3 grid((unsigned)(rows * a.tiles_n));
-  if (d.out_dtype == XTC_HIP_F32) hipLaunchKernelGGL(mx4_any<float>, grid, dim3(256), 0, core::pick_stream(d.stream), a);
-  else hipLaunchKernelGGL(mx4_any<__bf16>, grid, dim3(256), 0, core::pick_stream(d.stream), a);
-  return done(what);
+  Mx4QuantArgs q = args_of(*rows);
+  q.x = x, q.codes = a_codes, q.scales = a_scales;
+  return quantize(*rows, q, what) || product(*desc, a, what);
 }
 
 }  // extern "C"

@@ -34,6 +34,8 @@ struct Mx4Args {
   void* c;                  // [M][ldc]
   int E, M, N, blocks, ldc;
   int tiles_n;
+  const __bf16* x;          // mx4_rows with QUANTIZE: [M][ldx] of K elements, in place of a
+  int K, ldx;
 };
 
 namespace mx4 {

@@ -11,6 +11,10 @@
 // the scales: a step reads 256 bytes of every row (a block a lane and step: 16 x
 // 8192 x 8192 17 us).
 // Bound by memory: 16 x 8192 x 8192 reads 36 MB in 9.9 us.
+//
+// QUANTIZE takes a in bf16 and brings it to 4 bits on the way, every workgroup for
+// itself: what mx4_quantize would write, without its launch.
+// Bound by the launch and one walk of loads: 16 x 1024 x 2048 4.9 us.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -23,12 +27,40 @@ namespace mx4 {
 
 constexpr int RWAVES = 8;
 
+// A run of a row of bf16 numbers before its quantisation
+struct RawRun {
+  QuarterBf16 quarters[16];
+};
+
+// `left` of the elements at x exist, whole quarters of blocks; zeros for the others
+__device__ __forceinline__ void load_raw(RawRun& r, const __bf16* x, int left) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    if (8 * i < left) __builtin_memcpy(&r.quarters[i], x + 8 * i, 16);
+    else r.quarters[i].v = u32x4{0, 0, 0, 0};
+  }
+}
+
+__device__ __forceinline__ void quantize_run(Run& r, const RawRun& x) {
+  r.scales = 0;
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {
+    const QuarterBf16* const q = x.quarters + 4 * b;
+    const int s = scale_of(max(max(q[0].top(), q[1].top()), max(q[2].top(), q[3].top())));
+    const float scale = scale_value(s);
+    r.scales |= (unsigned)s << (8 * b);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.codes[b][i] = s == 255 ? 0u : q[i].codes(scale);
+  }
+}
+
 }  // namespace mx4
 
-template <typename U, int TM, int TN>
+template <typename U, int TM, int TN, bool QUANTIZE>
 __global__ void __launch_bounds__(64 * mx4::RWAVES) mx4_rows(Mx4Args p) {
   using namespace mx4;
   constexpr int SM = 16 * TM, SN = 16 * TN;
+  static_assert(RING == 2, "a run is quantised a step ahead");
   __shared__ float sums[RWAVES][SM][SN + 4];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l16 = lane & 15, g = lane >> 4;
@@ -48,9 +80,23 @@ __global__ void __launch_bounds__(64 * mx4::RWAVES) mx4_rows(Mx4Args p) {
   for (int i = 0; i < TM; ++i) at_a[i] = (int64_t)(gr.begin + min(16 * i + l16, rows - 1)) * p.blocks + first;
 #pragma unroll
   for (int j = 0; j < TN; ++j) at_b[j] = ((int64_t)e * p.N + n0 + min(16 * j + l16, cols - 1)) * p.blocks + first;
-  Run a[RING][TM], b[RING][TN];
-  int left = blocks - first;
+  constexpr int A_RING = QUANTIZE ? 1 : RING;
+  Run a[A_RING][TM], b[RING][TN];
+  RawRun raw[TM];
+  const __bf16* at_x[TM];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+    if constexpr (QUANTIZE) at_x[i] = p.x + (int64_t)(gr.begin + min(16 * i + l16, rows - 1)) * p.ldx + 32 * first;
+  int left = blocks - first, left_x = blocks > 0 ? p.K - 32 * first : 0;
   auto load = [&](int buf) {
+    if constexpr (QUANTIZE) {
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        load_raw(raw[i], at_x[i], left_x);
+        at_x[i] += 32 * RWAVES * STEP;
+      }
+      left_x -= 32 * RWAVES * STEP;
+    }
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
       load_run(b[buf][j], p.b_codes + at_b[j] * 16, p.b_scales + at_b[j], left);
@@ -58,16 +104,21 @@ __global__ void __launch_bounds__(64 * mx4::RWAVES) mx4_rows(Mx4Args p) {
     }
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
-      load_run(a[buf][i], p.a_codes + at_a[i] * 16, p.a_scales + at_a[i], left);
+      if constexpr (!QUANTIZE) load_run(a[buf][i], p.a_codes + at_a[i] * 16, p.a_scales + at_a[i], left);
       at_a[i] += RWAVES * STEP;
     }
     left -= RWAVES * STEP;
+  };
+  auto quantize = [&] {
+#pragma unroll
+    for (int i = 0; i < TM; ++i) quantize_run(a[0][i], raw[i]);
   };
   f32x4 acc[TM][TN] = {};
   const int steps = (blocks - wave * STEP + RWAVES * STEP - 1) / (RWAVES * STEP);  // of this wave
 #pragma unroll
   for (int s = 0; s < RING - 1; ++s)
     if (s < steps) load(s);
+  if (QUANTIZE && steps > 0) quantize();
   for (int s = 0; s < steps; s += RING) {
 #pragma unroll
     for (int q = 0; q < RING; ++q) {
@@ -76,7 +127,8 @@ __global__ void __launch_bounds__(64 * mx4::RWAVES) mx4_rows(Mx4Args p) {
 #pragma unroll
       for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int j = 0; j < TN; ++j) acc[i][j] = mfma_run(b[q][j], a[q][i], acc[i][j]);
+        for (int j = 0; j < TN; ++j) acc[i][j] = mfma_run(b[q][j], a[q % A_RING][i], acc[i][j]);
+      if (QUANTIZE && s + q + 1 < steps) quantize();  // the step just loaded: one step ahead
     }
   }
 #pragma unroll

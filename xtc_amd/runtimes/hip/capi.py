@@ -238,6 +238,7 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "xtc_hip_mx4_encode": (_i, [ctypes.POINTER(Mx4Desc), _vp, _vp, _vp]),
     "xtc_hip_mx4_dequantize": (_i, [ctypes.POINTER(Mx4Desc), _vp, _vp, _vp]),
     "xtc_hip_mx4_matmul": (_i, [ctypes.POINTER(Mx4MatmulDesc), _vp, _vp, _vp, _vp, _vp, _vp]),
+    "xtc_hip_mx4_quantize_matmul": (_i, [ctypes.POINTER(Mx4Desc), ctypes.POINTER(Mx4MatmulDesc), *[_vp] * 7]),
     "xtc_hip_matmul_desc_size": (_i, []),
     "xtc_hip_conv2d_desc_size": (_i, []),
     "xtc_hip_grouped_matmul_desc_size": (_i, []),

@@ -13,14 +13,17 @@
 // fp32 in padded rows.  bf16 runs on v_mfma_f32_16x16x32_bf16, fp32 on
 // v_mfma_f32_16x16x4_f32 (exact products, a lane's 8 k of a slab in any order as
 // long as A and B agree).  Sums are fp32; a bf16 result is rounded once, at the
-// store.
+// store.  Bound by the unaligned loads and a barrier every slab: 4096 rows over 8
+// experts of 1001 x 999 bf16 68 us, the gradient of w 50; fp32 112 (half the MFMAs'
+// rate).
 //
 // grouped_small takes the calls whose 64 x 64 tiles do not fill the card, and few
 // rows a group (then it streams the matrices): a workgroup computes a tile of 16
 // or 32 rows with 8 waves that share out the depth in turn,
 // load their fragments straight into registers, two or three steps ahead, and add their sums
 // up in LDS, in order.  No barrier but that one: the loads of a whole call are in
-// flight together (777 fp32 rows over 5 experts of 509 x 301: 22 us in slabs).
+// flight together.  Bound by the latency of one walk: 777 fp32 rows over 5 experts of
+// 509 x 301 9.3 us (22 in slabs), 2 bf16 rows at 8 of 1024 x 1024 3.8, a launch.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>

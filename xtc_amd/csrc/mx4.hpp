@@ -157,8 +157,8 @@ __device__ __forceinline__ void values8(float (&v)[8], unsigned word, int s) {
 
 // Quantisation of dense rows of whole blocks (`quarters` of 8 elements in all):
 // a lane takes QUARTERS of them, a workgroup's width apart, all loads first.  Four
-// lanes share a block.  Bound by memory: 8192x8192 bf16 reads 134 MB and writes
-// 36 (codes, scales) or 170 MB (and values).
+// lanes share a block.  Bound by memory: 8192 x 8192 bf16 reads 134 MB and writes
+// 36 (codes, scales) in 29 us or 170 MB (and values) in 51-55, 5.5-6 TB/s.
 template <typename T, int QUARTERS>
 __global__ void __launch_bounds__(256) mx4_quantize_dense(Mx4QuantArgs p, int64_t quarters) {
   using namespace mx4;
@@ -187,7 +187,8 @@ __global__ void __launch_bounds__(256) mx4_quantize_dense(Mx4QuantArgs p, int64_
 }
 
 // The same for rows of any length, stride and alignment, and codes for given
-// scales.  A lane takes a quarter of a block of each of its rows.
+// scales.  A lane takes a quarter of a block of each of its rows.  Bound by memory
+// and unaligned rows: 8192 x 8100 bf16 41 us, with values 67; 8192 x 8100 fp32 55.
 template <typename T>
 __global__ void __launch_bounds__(256) mx4_quantize(Mx4QuantArgs p) {
   using namespace mx4;
@@ -215,6 +216,8 @@ __global__ void __launch_bounds__(256) mx4_quantize(Mx4QuantArgs p) {
   }
 }
 
+// The values of codes and scales.  Bound by memory: 8192 x 8192 to bf16 41 us (4.2
+// TB/s), to fp32 87.
 template <typename T>
 __global__ void __launch_bounds__(256) mx4_dequantize(Mx4QuantArgs p) {
   using namespace mx4;

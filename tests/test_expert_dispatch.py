@@ -146,3 +146,15 @@ out.append(grad())
     assert none == captured and none[0] == split[0] and total[0] == "grouped_grad_sum"
     # 16 tiles in 16 parts; grids are filled up to whole runs (128 workgroups)
     assert (int(none[1].split()[0]), int(split[1].split()[0])) == (128, 256)
+
+
+def test_mx4_tiles_by_size(run):  # noqa: F811
+    """Few tiles go to waves that share their depth, more to the DMA tiles that cost
+    least, blocks of no whole slabs to the kernel of any."""
+    got = run(CALLS + """
+for M, N, blocks in ((16, 8192, 256), (32, 8192, 256), (700, 1000, 12), (2100, 2056, 68), (4100, 3336, 36), (2100, 2056, 69)):
+    out.append(mx4_matmul(M=M, N=N, blocks=blocks))
+""")
+    want = ["mx4_rows<float, 1,", "mx4_rows<float, 2,", "2, 2, 2, 2, 4, false>", "2, 2, 4, 4, 2, false>", "2, 4, 8, 4, 2, true>", "mx4_any"]
+    for ((name, _),), part in zip(got, want, strict=True):
+        assert part in name, (name, part)

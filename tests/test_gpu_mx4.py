@@ -261,3 +261,46 @@ def test_quantised_on_the_way(out, dtype, M, E, N, K):
     for pad, ldx, shift in ((0, 0, 0), (3, 5, 1)):
         got = mx4_quantize_matmul(x, dtype, bc, bsc, sizes, out, pad, ldx, shift)
         np.testing.assert_array_equal(got, want)
+
+
+# calls of the 64 x 64, 128 x 128 and 256 x 256 tiles, whose last slab is cut
+TILES = [(700, 1000, 12), (2100, 2056, 68), (4100, 3336, 36)]
+
+
+@pytest.mark.parametrize("M,N,nb", TILES)
+def test_nan_beside_the_last_slab(M, N, nb):
+    """The scales after a row's last ones are the next row's: NaN there stays there."""
+    print(f"[mx4 nan tiles] {M}x{N} blocks {nb}", flush=True)
+    a, b = operand(41, (M,), nb), operand(42, (N,), nb)
+    want, spread = plain(*a, *b, None)
+    a[1][2::3, 0] = 255
+    b[1][4::5, :4] = 255
+    got = mx4_matmul(*a, *b)
+    assert np.isnan(got[2::3]).all() and np.isnan(got[:, 4::5]).all()
+    rest = np.ix_([i for i in range(M) if i % 3 != 2], [j for j in range(N) if j % 5 != 4])
+    check_product(got[rest], want[rest], spread[rest], 32 * nb, "float32")
+
+
+@pytest.mark.parametrize("M,N,nb", TILES)
+@pytest.mark.parametrize("sa,sb", [(254, 1), (0, 220)])
+def test_extreme_scales_of_tiles(M, N, nb, sa, sb):
+    print(f"[mx4 extreme tiles] {M}x{N} blocks {nb} {sa} {sb}", flush=True)
+    a, b = operand(43, (M,), nb, 0), operand(44, (N,), nb, 0)
+    a[1][:], b[1][:] = sa, sb
+    want, _ = plain(*a, *b, None)
+    np.testing.assert_array_equal(mx4_matmul(*a, *b), want.astype(np.float32))
+
+
+@pytest.mark.parametrize("M,N,nb", TILES)
+def test_groups_of_tiles_do_not_mix(M, N, nb):
+    print(f"[mx4 groups tiles] {M}x{N} blocks {nb}", flush=True)
+    sizes = [M // 3, M // 5, 0, M // 4]
+    b0, b1, end = sizes[0], sizes[0] + sizes[1], sum(sizes)
+    a, b = operand(45, (M,), nb), operand(46, (4, N), nb)
+    want, spread = plain(*a, *b, sizes)
+    a[1][b0:b1], a[1][end:], b[1][1:3] = 255, 255, 255
+    first = mx4_matmul(*a, *b, sizes=sizes)
+    rows = np.r_[0:b0, b1:M]
+    check_product(first[rows], want[rows], spread[rows], 32 * nb, "float32")
+    assert np.isnan(first[b0:b1]).all()
+    np.testing.assert_array_equal(mx4_matmul(*a, *b, sizes=sizes), first)

@@ -11,9 +11,11 @@ HBM):
   * relu on a matmul/conv2d(/bias_add) result -> GEMM epilogue.
 Such a fusion happens only when the intermediate is used once and is not a graph
 output.  mx4_scales, the mx4_codes of the same tensor for these scales and a
-mx4_dequantize of the pair are one launch that writes all of them.  A matmul operand with layout [1, 0] (stored transposed) becomes the
-launch's trans_a / trans_b flag; other operators require natural layouts.  reshape is a view; unpad
-is a crop kernel (16-byte row copies when the innermost dim is kept).  The reference lowers each node to its own
+mx4_dequantize of the pair are one launch that writes all of them; codes and scales
+made for the rows of one 4-bit product alone go into its call.  A matmul operand with
+layout [1, 0] (stored transposed) becomes the launch's trans_a / trans_b flag, a
+grouped_matmul's matrices with [0, 2, 1] its trans_w; other operators require natural
+layouts.  reshape is a view; unpad is a crop kernel (16-byte row copies when the innermost dim is kept).  The reference lowers each node to its own
 linalg op (src/xtc/backends/mlir/MlirOps.py:166-887) and fuses only through
 transform-dialect producer fusion (MlirCompilerPasses.py:378-412).
 

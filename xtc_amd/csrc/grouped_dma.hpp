@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_dma(DmaArgs p) {
   // the chunk of a ROW slab that it loads
   auto chunk = [&](int i) { return (lane % CHUNKS) ^ swz_row<MX>((kb0 + i % OFFS) * (64 / CHUNKS) + lane / CHUNKS); };
   // K stagger: tiles that share a panel start their walk at different slabs
-  // (bf16 8192^3 850 -> 830 us; 4-bit ones gain nothing from whole groups of four)
+  // (bf16 8192^3 850 -> 830 us; 4-bit slabs go in pairs, and gain nothing by it)
   const int kofs = !MX && nk > 0 ? ((mt + 2 * (n0 / BN)) & 15) % nk : 0;
   const bool row = is_a ? A_ROW : B_ROW;
   Walk<true, SLAB> by_row;

@@ -1,0 +1,60 @@
+# SPDX-License-Identifier: BSD-3-Clause
+"""Calls of the expert and 4-bit entry points by the kernel that each is meant to
+reach: the GPU compares their results with plain forms, the CPU checks that the
+call does launch that kernel."""
+
+from __future__ import annotations
+
+F, B = "float32", "bfloat16"
+TYPES = [(F, F), (B, F), (B, B)]
+_C = {F: "float", B: "__bf16"}
+
+
+def _bool(*flags):
+    return ", ".join("true" if f else "false" for f in flags)
+
+
+# ---- products by group: (kernel, operands, result, transposed, T, K, N, sizes)
+
+# 64 x 64 slabs of any operands: one slab, as many as a register ring holds, one more,
+# many; the last one cut; ragged groups, one of a row, an empty one, rows of nobody
+_SLABS = [(1500, k, 2057, [400, 0, 1, 700, 64, 300]) for k in (20, 95, 127, 201)]
+GROUPED_ANY = [(f"grouped_any<{_C[d]}, {_C[o]}, {_bool(t, False)}>", d, o, t, *size)
+               for d, o in TYPES for t in (False, True) for size in _SLABS]
+# whole vectors too in fp32, which has no other kernel of many tiles
+GROUPED_ANY += [(f"grouped_any<float, float, {_bool(t, False)}>", F, F, t, 1500, 264, 2056, [400, 0, 1, 700, 64, 300])
+                for t in (False, True)]
+
+# waves that share out the depth: 16 rows by 16, 32 or 64 columns, cut in both; depths of
+# one step of one wave, of every wave's, and of more than a register ring holds
+_SMALL = [(16, True, 9, 3, 2), (16, True, 9, 777, 50), (16, True, 5, 2500, 37), (32, False, 200, 45, 300),
+          (32, False, 200, 1300, 70), (32, True, 200, 45, 300), (32, True, 200, 1300, 70), (64, False, 20, 9, 3),
+          (64, False, 20, 2500, 130), (64, False, 700, 300, 723), (64, True, 700, 300, 723)]
+GROUPED_SMALL = [(f"grouped_small<{_C[d]}, {_C[o]}, {_bool(t, False)}, 1, {n // 16}>", d, o, t, T, k, N,
+                  [T // 2, 0, T // 3 + 1] if n != 64 or T > 20 else [T // 2, 0, T // 3])
+                 for d, o in TYPES for n, t, T, k, N in _SMALL]
+
+# ---- gradients: (kernel, in parts, operands, result, T, K, N, sizes)
+
+GRAD_ANY = [(f"grouped_any<{_C[d]}, {_C[o]}, false, true>", False, d, o, *size) for d, o in TYPES
+            for size in ((400, 905, 777, [200, 0, 33, 1, 96, 60]), (900, 1001, 721, [32, 700, 0, 160]))]
+GRAD_SMALL = [(f"grouped_small<{_C[d]}, {_C[o]}, false, true, 2, 2>", False, d, o, *size) for d, o in TYPES
+              for size in ((30, 19, 23, [1, 0, 29]), (2600, 77, 45, [300, 0, 2298, 1]), (900, 333, 250, [450, 33, 0, 417]))]
+
+# ---- 4-bit products: (kernel, result, M, N, blocks, sizes or None, bytes that the
+# scales of a and b lie past a 16-byte boundary)
+
+_GROUPS = [700, 1, 0, 420, 257, 700]
+MX4 = [(f"{kernel}{_C[o]}{rest}", o, *call) for o in (F, B) for kernel, rest, *call in (
+    # one step, two, more than the ring; the last run of blocks cut to 1, 2 and 3
+    ("mx4_any<", ">", 2100, 2056, 13, None, (0, 0)), ("mx4_any<", ">", 2100, 2056, 33, None, (0, 0)),
+    ("mx4_any<", ">", 700, 1000, 50, None, (0, 0)), ("mx4_any<", ">", 700, 1000, 103, None, (0, 0)),
+    ("mx4_any<", ">", 2100, 2056, 13, _GROUPS, (0, 0)), ("mx4_any<", ">", 700, 1500, 7, [300, 0, 399], (0, 0)),
+    # whole slabs whose scales cannot be staged in dwords
+    ("mx4_any<", ">", 2100, 2056, 12, None, (1, 0)), ("mx4_any<", ">", 2100, 2056, 36, _GROUPS, (0, 2)),
+    ("mx4_rows<", ", 1, 2, false>", 16, 1000, 12, None, (1, 3)), ("mx4_rows<", ", 1, 2, false>", 20, 200, 16, [9, 0, 10], (3, 1)),
+    ("mx4_rows<", ", 2, 2, false>", 32, 8192, 20, None, (2, 1)),
+)] + [(f"grouped_dma<true, false, true, {tile}>", o, *call, (0, 0)) for o in (F, B) for tile, *call in (
+    ("2, 2, 2, 2, 4, false", 700, 1000, 12, [300, 0, 1, 390]), ("2, 2, 4, 4, 2, false", 2100, 2056, 68, _GROUPS),
+    ("2, 4, 8, 4, 2, true", 2000, 4104, 68, [900, 1, 0, 600, 257]), ("2, 4, 8, 4, 2, true", 4100, 3336, 36, None),
+)]

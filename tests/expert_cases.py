@@ -34,6 +34,23 @@ GROUPED_SMALL = [(f"grouped_small<{_C[d]}, {_C[o]}, {_bool(t, False)}, 1, {n // 
                   [T // 2, 0, T // 3 + 1] if n != 64 or T > 20 else [T // 2, 0, T // 3])
                  for d, o in TYPES for n, t, T, k, N in _SMALL]
 
+
+def _dma(grad, t, tile):
+    return f"grouped_dma<false, {_bool(grad, t)}, {tile}>"
+
+
+TILE64, TILE128, TILE256 = "2, 2, 2, 2, 4, false", "2, 2, 4, 4, 4, false", "2, 4, 8, 4, 4, true"
+# LDS-DMA tiles cut in rows, columns and depth; K of fewer slabs than the three that
+# are in flight where the call takes the tile (256 x 256 ones start at deeper sums)
+_DMA = [(TILE64, B, 1500, 32, 2056, [500, 1, 0, 300, 257, 375]), (TILE64, B, 1500, 72, 2056, [500, 1, 0, 300, 257, 375]),
+        (TILE64, F, 1500, 200, 2056, [500, 1, 0, 300, 257, 375]),
+        (TILE128, B, 4100, 40, 3336, [1300, 1, 0, 800, 257, 1025]), (TILE128, F, 4100, 72, 3336, [1300, 1, 0, 800, 257, 1025]),
+        (TILE128, F, 4100, 264, 3336, [1300, 1, 0, 800, 257, 1025]),
+        (TILE256, B, 3300, 200, 4104, [1700, 0, 1, 1500]), (TILE256, F, 3300, 264, 4104, [1700, 0, 1, 1500]),
+        (TILE256, F, 3300, 520, 4104, [1, 257, 2900, 0]), (TILE256, B, 5000, 264, 2312, [2000, 1, 0, 1300, 257, 900]),
+        (TILE256, F, 2300, 1032, 3336, [100, 2100, 0])]
+GROUPED_DMA = [(_dma(False, t, tile), B, o, t, *size) for tile, o, *size in _DMA for t in (False, True)]
+
 # ---- gradients: (kernel, in parts, operands, result, T, K, N, sizes)
 
 GRAD_ANY = [(f"grouped_any<{_C[d]}, {_C[o]}, false, true>", False, d, o, *size) for d, o in TYPES

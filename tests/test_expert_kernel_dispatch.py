@@ -23,7 +23,7 @@ def names(run, script):  # noqa: F811
 
 @pytest.fixture(scope="module")
 def launched(run):  # noqa: F811
-    forward = cases.GROUPED_SMALL + cases.GROUPED_ANY
+    forward = cases.GROUPED_SMALL + cases.GROUPED_ANY + cases.GROUPED_DMA
     gradients = cases.GRAD_SMALL + cases.GRAD_ANY
     calls = [("", dict(dtype=IDS[d], out_dtype=IDS[o], trans_w=int(t), T=T, K=K, N=N, E=len(s)))
              for _, d, o, t, T, K, N, s in forward]

@@ -56,7 +56,7 @@ def gradient_data(T, K, N, sizes):
     return frozen(x, dy, want)
 
 
-FORWARD = cases.GROUPED_SMALL + cases.GROUPED_ANY
+FORWARD = cases.GROUPED_SMALL + cases.GROUPED_ANY + cases.GROUPED_DMA
 GRADIENTS = cases.GRAD_SMALL + cases.GRAD_ANY
 
 
@@ -83,7 +83,7 @@ def one_of(cs):
     return list({c[0]: c for c in cs if "float32" in c}.values())
 
 
-@pytest.mark.parametrize("kernel,dtype,out,trans,T,K,N,sizes", one_of(cases.GROUPED_ANY))
+@pytest.mark.parametrize("kernel,dtype,out,trans,T,K,N,sizes", one_of(cases.GROUPED_ANY + cases.GROUPED_DMA))
 def test_fractions(kernel, dtype, out, trans, T, K, N, sizes):
     rng = np.random.default_rng(55)
     x, w = (rounded(rng.uniform(-1, 1, s), dtype) for s in ((T, K), (len(sizes), K, N)))

@@ -57,6 +57,19 @@ GRAD_ANY = [(f"grouped_any<{_C[d]}, {_C[o]}, false, true>", False, d, o, *size) 
             for size in ((400, 905, 777, [200, 0, 33, 1, 96, 60]), (900, 1001, 721, [32, 700, 0, 160]))]
 GRAD_SMALL = [(f"grouped_small<{_C[d]}, {_C[o]}, false, true, 2, 2>", False, d, o, *size) for d, o in TYPES
               for size in ((30, 19, 23, [1, 0, 29]), (2600, 77, 45, [300, 0, 2298, 1]), (900, 333, 250, [450, 33, 0, 417]))]
+GRAD_DMA = [(_dma(True, False, tile), parts, B, o, *size) for o in (F, B) for tile, parts, *size in (
+    (TILE64, False, 420, 264, 520, [200, 0, 33, 1, 96, 60]),
+    (TILE128, False, 600, 648, 520, [16] * 20 + [33, 0, 1, 96] + [5] * 8),
+    (TILE256, False, 1500, 1544, 1800, [32, 300, 0, 5, 97, 1000]),
+    (TILE256, False, 900, 2056, 2312, [1, 96, 800, 0]),
+    # summed in parts: a group of fewer slabs than parts, one of a single slab, an empty
+    # one, next to groups that are split; tiles cut by K and N
+    (TILE64, True, 9000, 128, 136, [8600, 100, 20, 0]),
+    (TILE64, True, 16000, 72, 136, [0, 33, 6000, 9000, 900]),
+    (TILE64, True, 6000, 264, 520, [100, 5000, 32]),
+    (TILE128, True, 24000, 264, 520, [14000, 33, 0, 9000]),
+    (TILE128, True, 30000, 776, 520, [20, 20000, 9000]),
+)]
 
 # ---- 4-bit products: (kernel, result, M, N, blocks, sizes or None, bytes that the
 # scales of a and b lie past a 16-byte boundary)

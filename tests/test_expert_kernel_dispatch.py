@@ -1,9 +1,11 @@
 # SPDX-License-Identifier: BSD-3-Clause
 """That the GPU tests of the expert and 4-bit kernels reach the kernels that they
-name: on the CPU, libxtc_hip.so against
+name, and that together they reach all of them: on the CPU, libxtc_hip.so against
 the stand-in for the HIP runtime."""
 
 from __future__ import annotations
+
+from itertools import product
 
 import pytest
 
@@ -24,7 +26,7 @@ def names(run, script):  # noqa: F811
 @pytest.fixture(scope="module")
 def launched(run):  # noqa: F811
     forward = cases.GROUPED_SMALL + cases.GROUPED_ANY + cases.GROUPED_DMA
-    gradients = cases.GRAD_SMALL + cases.GRAD_ANY
+    gradients = cases.GRAD_SMALL + cases.GRAD_ANY + cases.GRAD_DMA
     calls = [("", dict(dtype=IDS[d], out_dtype=IDS[o], trans_w=int(t), T=T, K=K, N=N, E=len(s)))
              for _, d, o, t, T, K, N, s in forward]
     calls += [("_grad_w", dict(dtype=IDS[d], out_dtype=IDS[o], T=T, K=K, N=N, E=len(s))) for _, _, d, o, T, K, N, s in gradients]
@@ -44,3 +46,16 @@ for args, kw in {mx4!r}:
 def test_cases_reach_their_kernels(launched):
     for case, got, want in launched:
         assert got == want, case
+
+
+def test_all_kernels_are_reached(launched):
+    types = [("float", "float"), ("__bf16", "float"), ("__bf16", "__bf16")]
+    want = {f"grouped_any<{t}, {u}, {w}>" for (t, u), w in product(types, ("false, false", "true, false", "false, true"))}
+    want |= {f"grouped_small<{t}, {u}, {w}>" for (t, u), w in product(types, (
+        "true, false, 1, 1", "false, false, 1, 2", "true, false, 1, 2", "false, false, 1, 4", "true, false, 1, 4", "false, true, 2, 2"))}
+    want |= {f"grouped_dma<false, {w}, {tile}>" for w, tile in product(
+        ("false, false", "false, true", "true, false"), (cases.TILE64, cases.TILE128, cases.TILE256))}
+    want |= {f"grouped_dma<true, false, true, {tile}>" for tile in ("2, 2, 2, 2, 4, false", "2, 2, 4, 4, 2, false", "2, 4, 8, 4, 2, true")}
+    want |= {f"mx4_any<{u}>" for u in ("float", "__bf16")} | {"grouped_grad_sum"}
+    want |= {f"mx4_rows<{u}, {m}, 2, false>" for u, m in product(("float", "__bf16"), (1, 2))}
+    assert {name for _, got, _ in launched for name in got} == want

@@ -57,7 +57,7 @@ def gradient_data(T, K, N, sizes):
 
 
 FORWARD = cases.GROUPED_SMALL + cases.GROUPED_ANY + cases.GROUPED_DMA
-GRADIENTS = cases.GRAD_SMALL + cases.GRAD_ANY
+GRADIENTS = cases.GRAD_SMALL + cases.GRAD_ANY + cases.GRAD_DMA
 
 
 # by size, so that calls of one size share their data
@@ -93,7 +93,7 @@ def test_fractions(kernel, dtype, out, trans, T, K, N, sizes):
     np.testing.assert_array_equal(grouped(x, w, sizes, dtype, out, trans), got)
 
 
-@pytest.mark.parametrize("kernel,parts,dtype,out,T,K,N,sizes", one_of(cases.GRAD_ANY))
+@pytest.mark.parametrize("kernel,parts,dtype,out,T,K,N,sizes", one_of(cases.GRAD_ANY + cases.GRAD_DMA))
 def test_gradients_of_fractions(kernel, parts, dtype, out, T, K, N, sizes):
     rng = np.random.default_rng(56)
     x, dy = (rounded(rng.uniform(-1, 1, s), dtype) for s in ((T, K), (T, N)))

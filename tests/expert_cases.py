@@ -88,3 +88,23 @@ MX4 = [(f"{kernel}{_C[o]}{rest}", o, *call) for o in (F, B) for kernel, rest, *c
     ("2, 2, 2, 2, 4, false", 700, 1000, 12, [300, 0, 1, 390]), ("2, 2, 4, 4, 2, false", 2100, 2056, 68, _GROUPS),
     ("2, 4, 8, 4, 2, true", 2000, 4104, 68, [900, 1, 0, 600, 257]), ("2, 4, 8, 4, 2, true", 4100, 3336, 36, None),
 )]
+
+# ---- operands whose rows or matrices lie more than 2^32 bytes apart:
+# (kernel, T, K, N, sizes, row strides of x, y and (gradients) dy, between matrices)
+
+FAR = [(_dma(False, False, TILE64), 700, 264, 2056, [300, 0, 390], 2**22 - 16, 2**21 + 8, 2**30 + 16),
+       (_dma(False, True, TILE64), 700, 264, 2056, [300, 0, 390], 2**22 - 16, 2**21 + 8, 2**30 + 16),
+       (f"grouped_any<__bf16, float, {_bool(False, False)}>", 1100, 201, 2057, [500, 0, 590], 2**21 + 5, 2**20 + 3, 2**30 + 15),
+       (f"grouped_any<__bf16, float, {_bool(True, False)}>", 1100, 201, 2057, [500, 0, 590], 2**21 + 5, 2**20 + 3, 2**30 + 15)]
+FAR_GRAD = [(_dma(True, False, TILE64), 700, 264, 520, [300, 0, 390], 2**22 - 16, 2**22 - 24, 2**30 + 16),
+            ("grouped_any<__bf16, float, false, true>", 1100, 1001, 721, [500, 0, 590], 2**21 + 5, 2**21 + 7, 2**30 + 15)]
+# (kernel, M, N, blocks, sizes or None, row stride of c or 0)
+FAR_MX4 = [("grouped_dma<true, false, true, 2, 2, 2, 2, 4, false>", 40, 400000, 256, [15, 0, 25], 2**25 + 4),
+           ("grouped_dma<true, false, true, 2, 2, 2, 2, 4, false>", 2**20 + 40, 64, 256, None, 0),
+           ("mx4_any<float>", 40, 2**20 + 72, 257, None, 2**25 + 1), ("mx4_any<float>", 2**20 + 40, 64, 257, None, 0),
+           ("mx4_rows<float, 1, 2, false>", 16, 2**20 + 72, 257, None, 0)]
+
+
+def transposed(kernel):
+    """Whether a kernel of FAR takes transposed matrices."""
+    return kernel.startswith(("grouped_dma<false, false, true", "grouped_any<__bf16, float, true"))

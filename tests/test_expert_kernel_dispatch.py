@@ -59,3 +59,18 @@ def test_all_kernels_are_reached(launched):
     want |= {f"mx4_any<{u}>" for u in ("float", "__bf16")} | {"grouped_grad_sum"}
     want |= {f"mx4_rows<{u}, {m}, 2, false>" for u, m in product(("float", "__bf16"), (1, 2))}
     assert {name for _, got, _ in launched for name in got} == want
+
+
+def test_far_operands_reach_their_kernels(run):  # noqa: F811
+    calls = [("", dict(trans_w=int(cases.transposed(k)), T=T, K=K, N=N, E=len(s), ldx=ldx, ldy=ldy, stride_w=sw))
+             for k, T, K, N, s, ldx, ldy, sw in cases.FAR]
+    calls += [("_grad_w", dict(T=T, K=K, N=N, E=len(s), ldx=ldx, ldy=ldy, stride_w=sw)) for _, T, K, N, s, ldx, ldy, sw in cases.FAR_GRAD]
+    mx4 = [((256,) * 4 + (256 if s else None, 256), dict(M=M, N=N, blocks=nb, E=len(s or []), ldc=ldc))
+           for _, M, N, nb, s, ldc in cases.FAR_MX4]
+    got = names(run, f"""
+for fn, kw in {calls!r}:
+    out.append(grouped("xtc_hip_grouped_matmul" + fn, **kw))
+for args, kw in {mx4!r}:
+    out.append(mx4_matmul(args, **kw))
+""")
+    assert got == [[c[0]] for c in cases.FAR + cases.FAR_GRAD + cases.FAR_MX4]

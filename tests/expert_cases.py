@@ -49,6 +49,10 @@ _DMA = [(TILE64, B, 1500, 32, 2056, [500, 1, 0, 300, 257, 375]), (TILE64, B, 150
         (TILE256, B, 3300, 200, 4104, [1700, 0, 1, 1500]), (TILE256, F, 3300, 264, 4104, [1700, 0, 1, 1500]),
         (TILE256, F, 3300, 520, 4104, [1, 257, 2900, 0]), (TILE256, B, 5000, 264, 2312, [2000, 1, 0, 1300, 257, 900]),
         (TILE256, F, 2300, 1032, 3336, [100, 2100, 0])]
+# one slab and less of it, with results of either type
+_DMA += [(tile, o, T, K, N, sizes) for o in (F, B) for K in (8, 32) for tile, T, N, sizes in (
+    (TILE64, 1500, 2056, [500, 1, 0, 300, 257, 375]), (TILE128, 4100, 3336, [1300, 1, 0, 800, 257, 1025]))
+    if (tile, o, T, K) != (TILE64, B, 1500, 32)]
 GROUPED_DMA = [(_dma(False, t, tile), B, o, t, *size) for tile, o, *size in _DMA for t in (False, True)]
 
 # ---- gradients: (kernel, in parts, operands, result, T, K, N, sizes)

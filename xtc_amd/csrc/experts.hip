@@ -197,9 +197,11 @@ int xtc_hip_grouped_matmul(const xtc_hip_grouped_matmul_desc* desc, const void* 
     const DmaTile& t = dma_tile(d.T, d.E, d.K, d.N, d.out_dtype == XTC_HIP_BF16 ? 2 : 4, &cost);
     // few tiles of deep K: waves that share out the depth, 256 of it a step of at
     // least .8 us, 3 where two workgroups a CU share it (512 rows over 2 experts of
-    // 3584 x 256: 25 us on DMA tiles, 15 so)
+    // 3584 x 256: 25 us on DMA tiles, 15 so), and a round of tiles has 4 us of its own:
+    // finding the rows, the first loads, adding up and storing the sums (fp32 results:
+    // 4100 rows over 6 of 32 x 3336 113 us so, 19 on DMA tiles; 9000 of 8 x 4104 456, 40)
     const double load = likely_tiles(d.T, d.E, 16) * ((d.N + 63) / 64) / 512;
-    if (d.K / 256.0 * fmax(0.8, 3 * load) < cost) return launch_any(d, kSmall64, false, a, s);
+    if (d.K / 256.0 * fmax(0.8, 3 * load) + 4 * load < cost) return launch_any(d, kSmall64, false, a, s);
     DmaArgs v{};
     v.a = (const uint8_t*)x, v.b = (const uint8_t*)w, v.sizes = sizes, v.c = y;
     v.stride_b = 2 * a.stride_w;

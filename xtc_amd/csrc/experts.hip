@@ -96,14 +96,14 @@ const DmaTile& grad_tile(int64_t T, int64_t E, int K, int N, int* splits) {
   return *best;
 }
 
-int launch_dma(const DmaTile& t, DmaLaunch run, DmaArgs& a, int64_t matrices, hipStream_t s) {
+int launch_dma(const DmaTile& t, DmaLaunch run, DmaArgs& a, int64_t matrices, hipStream_t s, const char* what) {
   a.tiles_n = (a.N + t.cost.bn - 1) / t.cost.bn;
   a.band = a.tiles_m < 8 ? a.tiles_m : 8;
   const int64_t groups = dma_groups(a, matrices);
-  if (groups < 1 || groups >= (int64_t)1 << 31) return fail("grouped_matmul: %lld workgroups are too many", (long long)groups);
+  if (groups < 1 || groups >= (int64_t)1 << 31) return fail("%s: %lld workgroups are too many", what, (long long)groups);
   run(a, (unsigned)groups, s);
   const hipError_t e = hipGetLastError();
-  return e == hipSuccess ? 0 : fail("grouped_matmul: launch failed: %s", hipGetErrorString(e));
+  return e == hipSuccess ? 0 : fail("%s: launch failed: %s", what, hipGetErrorString(e));
 }
 
 // ---- any operands
@@ -132,14 +132,14 @@ const AnyTile kSmallGrad = {32, 32, {{}, {}, XTC_TYPES(small_launch, false, true
 #undef XTC_SMALL
 #undef XTC_TYPES
 
-int launch_any(const xtc_hip_grouped_matmul_desc& d, const AnyTile& t, bool grad, GroupedArgs& a, hipStream_t s) {
+int launch_any(const xtc_hip_grouped_matmul_desc& d, const AnyTile& t, bool grad, GroupedArgs& a, hipStream_t s, const char* what) {
   a.tiles_n = (a.N + t.bn - 1) / t.bn;
   a.tiles_k = (a.K + t.bm - 1) / t.bm;
   const int64_t groups = a.tiles_n * (grad ? (int64_t)a.E * a.tiles_k : most_tiles(a.T, a.E, t.bm));
-  if (groups < 1 || groups >= (int64_t)1 << 31) return fail("grouped_matmul: %lld workgroups are too many", (long long)groups);
+  if (groups < 1 || groups >= (int64_t)1 << 31) return fail("%s: %lld workgroups are too many", what, (long long)groups);
   t.run[grad ? 2 : d.trans_w ? 1 : 0][d.dtype == XTC_HIP_F32 ? 0 : 1 + d.out_dtype](a, (unsigned)groups, s);
   const hipError_t e = hipGetLastError();
-  return e == hipSuccess ? 0 : fail("grouped_matmul: launch failed: %s", hipGetErrorString(e));
+  return e == hipSuccess ? 0 : fail("%s: launch failed: %s", what, hipGetErrorString(e));
 }
 
 // Tiles that a call has at most.
@@ -190,7 +190,7 @@ int xtc_hip_grouped_matmul(const xtc_hip_grouped_matmul_desc* desc, const void* 
   a.stride_w = d.stride_w ? d.stride_w : matrix;
   if (a.stride_w < 0) return fail("%s: negative stride between matrices", what);
   const hipStream_t s = core::pick_stream(d.stream);
-  if (const AnyTile* t = stream_tile(d.trans_w, a)) return launch_any(d, *t, false, a, s);
+  if (const AnyTile* t = stream_tile(d.trans_w, a)) return launch_any(d, *t, false, a, s, what);
   if (d.dtype == XTC_HIP_BF16 && d.K % 8 == 0 && (d.trans_w || d.N % 8 == 0) && vectors(x, a.ldx) && vectors(w, a.ldw) &&
       a.stride_w % 8 == 0) {
     double cost;
@@ -201,16 +201,16 @@ int xtc_hip_grouped_matmul(const xtc_hip_grouped_matmul_desc* desc, const void* 
     // finding the rows, the first loads, adding up and storing the sums (fp32 results:
     // 4100 rows over 6 of 32 x 3336 113 us so, 19 on DMA tiles; 9000 of 8 x 4104 456, 40)
     const double load = likely_tiles(d.T, d.E, 16) * ((d.N + 63) / 64) / 512;
-    if (d.K / 256.0 * fmax(0.8, 3 * load) + 4 * load < cost) return launch_any(d, kSmall64, false, a, s);
+    if (d.K / 256.0 * fmax(0.8, 3 * load) + 4 * load < cost) return launch_any(d, kSmall64, false, a, s, what);
     DmaArgs v{};
     v.a = (const uint8_t*)x, v.b = (const uint8_t*)w, v.sizes = sizes, v.c = y;
     v.stride_b = 2 * a.stride_w;
     v.E = d.E, v.M = d.T, v.N = d.N, v.K = d.K / 8;
     v.lda = 2 * a.ldx, v.ldb = 2 * a.ldw, v.ldc = a.ldy, v.out16 = d.out_dtype == XTC_HIP_BF16;
     v.tiles_m = (int)most_tiles(d.T, d.E, t.cost.bm);
-    return launch_dma(t, d.trans_w ? t.transposed : t.natural, v, 1, s);
+    return launch_dma(t, d.trans_w ? t.transposed : t.natural, v, 1, s, what);
   }
-  return launch_any(d, any_tile(false, a), false, a, s);
+  return launch_any(d, any_tile(false, a), false, a, s, what);
 }
 
 int xtc_hip_grouped_matmul_grad_w(const xtc_hip_grouped_matmul_desc* desc, const void* x, const void* dy,
@@ -244,14 +244,14 @@ int xtc_hip_grouped_matmul_grad_w(const xtc_hip_grouped_matmul_desc* desc, const
       v.partial = core::partial_sums((size_t)splits * d.E * d.K * d.N * 4, s);
       if (!v.partial) v.splits = 1;
     }
-    if (launch_dma(*t, t->grad, v, (int64_t)d.E * v.splits, s)) return 1;
+    if (launch_dma(*t, t->grad, v, (int64_t)d.E * v.splits, s, what)) return 1;
     if (v.splits == 1) return 0;
     const int chunks = (int)(((int64_t)d.K * (d.N / 4) + 255) / 256);  // partial sums are small: kMostPartial
     hipLaunchKernelGGL(grouped_grad_sum, dim3((unsigned)(d.E * chunks)), dim3(256), 0, s, v, chunks);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? 0 : fail("%s: launch failed: %s", what, hipGetErrorString(e));
   }
-  return launch_any(d, any_tile(true, a), true, a, core::pick_stream(d.stream));
+  return launch_any(d, any_tile(true, a), true, a, core::pick_stream(d.stream), what);
 }
 
 }  // extern "C"

@@ -27,6 +27,9 @@ int check(const xtc_hip_mx4_desc* d, const char* what) {
   if (d->rows < 0 || d->K < 1 || d->K > kMost)
     return fail("%s: invalid sizes rows=%lld K=%d", what, (long long)d->rows, d->K);
   if (d->ld && d->ld < d->K) return fail("%s: row stride %d is below the %d elements of a row", what, d->ld, d->K);
+  // no operand has more bytes a row than 4 of each element and 16 of each block
+  const int64_t row = 4 * (int64_t)(d->ld ? d->ld : d->K) + 16 * (((int64_t)d->K + 31) / 32);
+  if (d->rows > INT64_MAX / row) return fail("%s: sizes rows=%lld K=%d are too many", what, (long long)d->rows, d->K);
   return 0;
 }
 
@@ -84,7 +87,7 @@ const DmaTile& dma_tile(int64_t rows, int64_t groups, int N, int blocks, int out
   const DmaTile* best = nullptr;
   double least = 0;
   for (const DmaTile& t : kDmaTiles) {
-const double tiles = likely_tiles(rows, groups, t.cost.bm) * ((N + t.cost.bn - 1) / t.cost.bn);
+    const double tiles = likely_tiles(rows, groups, t.cost.bm) * ((N + t.cost.bn - 1) / t.cost.bn);
     const double cost = dma_cost(t.cost, tiles, (blocks + 4) / 8, out_bytes);
     if (!best || cost < least) best = &t, least = cost;
   }

@@ -313,7 +313,8 @@ typedef struct {
 int xtc_hip_mx4_quantize(const xtc_hip_mx4_desc *desc, const void *x, uint8_t *codes,
                          uint8_t *scales, void *values);
 
-/* Codes for given scales (0 in blocks whose scale is 255, and for NaN). */
+/* Codes for given scales: 0 in blocks whose scale is 255; elsewhere a NaN gives a
+ * zero of its sign (0 or 8), an infinity the largest code of its sign. */
 int xtc_hip_mx4_encode(const xtc_hip_mx4_desc *desc, const void *x, const uint8_t *scales,
                        uint8_t *codes);
 
@@ -347,10 +348,10 @@ int xtc_hip_mx4_quantize_matmul(const xtc_hip_mx4_desc *rows,
                                 const uint8_t *b_scales, const int32_t *sizes, void *c);
 
 /* sizeof(xtc_hip_matmul_desc) and sizeof(xtc_hip_conv2d_desc) as this library
- * was compiled (and of the other descriptors, below): a binding that declares the descriptors itself (ctypes, cgo)
- * checks its own struct sizes against these before the first call, so a
- * field it lacks fails loudly instead of being read past the end of its
- * struct.  No counterpart in the reference, whose mgpu* calls
+ * was compiled (and of the other descriptors, below): a binding that declares
+ * the descriptors itself (ctypes, cgo) checks its own struct sizes against
+ * these before the first call, so a field it lacks fails loudly instead of
+ * being read past the end of its struct.  No counterpart in the reference, whose mgpu* calls
  * (GPUDevice.py:131-207) take no structs. */
 int xtc_hip_matmul_desc_size(void);
 int xtc_hip_conv2d_desc_size(void);

@@ -167,7 +167,8 @@ class XTCOperMx4Scales(_Blocks, XTCOperator):
 
 
 class XTCOperMx4Codes(_Blocks, XTCOperator):
-    """Codes of x for given scales: (..., K), (..., ceil(K / 32)) -> (..., 16 ceil(K / 32)) uint8."""
+    """Codes of x for given scales: (..., K), (..., ceil(K / 32)) -> (..., 16 ceil(K / 32)) uint8.
+    0 where the scale is 255; elsewhere a NaN gives a zero of its sign."""
 
     def __init__(self, **attrs: Any) -> None:
         super().__init__("mx4_codes", **attrs)

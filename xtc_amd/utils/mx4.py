@@ -41,7 +41,8 @@ def mx4_scales(x: np.ndarray) -> np.ndarray:
 
 
 def mx4_codes(x: np.ndarray, scales: np.ndarray) -> np.ndarray:
-    """(..., K) and its scales -> (..., 16 ceil(K / 32)) uint8."""
+    """(..., K) and its scales -> (..., 16 ceil(K / 32)) uint8.  Codes are 0 where
+    the scale is 255; elsewhere a NaN gives a zero of its sign."""
     v = _blocks(x)
     s = np.asarray(scales).astype(np.int32)[..., None]
     # exact in double precision: 24-bit elements times a power of two

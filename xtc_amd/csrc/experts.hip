@@ -71,8 +71,10 @@ const DmaTile& dma_tile(int64_t T, int64_t E, int K, int N, int out_bytes, doubl
 }
 
 // The tile of E gradients of K x N and into how many parts each group's rows go.
-// The largest group decides where tiles are few (of a skewed choice it has some 1.7
-// times the mean), the sum of all where they are many; starting on a
+// The largest group decides where tiles are few, the sum of all where they are many;
+// the host does not know the sizes and takes 1.7 times the mean for the largest (shares
+// drawn from a Dirichlet distribution of parameter 2: 1.4 times at 2 groups, 2.2 at 8, 3.4
+// at 64); starting on a
 // round of tiles and writing them out take 5 (64 rows) to 15 us (256): 512 rows, 32
 // of 640 x 512, 21 us in 64 x 64 tiles, 14 in 128 x 128.  A part pays for writing and
 // reading its partial sums (4 MB a microsecond), all together for one more launch,
@@ -152,7 +154,15 @@ int64_t tiles_of(const AnyTile& t, bool grad, const GroupedArgs& a) {
 // depth.  Matrices in rows of n are read 64 columns wide (8 rows over 8 experts of
 // 4096 x 2048: 19 us, 25 at 32 columns, DMA tiles 27), matrices in rows of k 16
 // columns a tile (16 us, 22; DMA 21).  From 8 and 4 rows a group on DMA tiles are
-// as fast (8: 31 and 35 us against 35 and 33).
+// as fast (8: 31 and 35 us against 35 and 33).  With more matrices the natural ones lose
+// from fewer rows on (bf16, 8 rows at each of 16 of 4096 x 2048: 75 us, DMA tiles 49; of
+// 64 of 1024 x 1024: 38, 29), the transposed ones do not (4 rows at each of 32 of 4096 x
+// 2048: 97, 96; one: 56, 73).
+// fp32 has slabs only to turn to: 64 rows over 8 of 4096 x 2048 51 us, 121 in slabs,
+// 56 at 32 columns, which are faster for a row or two (1 x 4096 x 4096 18 us, 27).
+// The rows of each group are not known here, only their mean: 512 rows that all fall to
+// one of 64 groups stream its matrix once per 16, 70 us (DMA tiles 29), where they spread
+// 243 (192).
 const AnyTile* stream_tile(bool trans_w, const GroupedArgs& a) {
   const int rows = trans_w ? 4 : 8;
   return a.T > rows * (int64_t)a.E ? nullptr : trans_w ? &kSmall16 : &kSmall64;
@@ -196,7 +206,8 @@ int xtc_hip_grouped_matmul(const xtc_hip_grouped_matmul_desc* desc, const void* 
     double cost;
     const DmaTile& t = dma_tile(d.T, d.E, d.K, d.N, d.out_dtype == XTC_HIP_BF16 ? 2 : 4, &cost);
     // few tiles of deep K: waves that share out the depth, 256 of it a step of at
-    // least .8 us, 3 where two workgroups a CU share it (512 rows over 2 experts of
+    // least .8 us, 3 in a round of 512 tiles (two a CU, one after the other in the natural
+    // bf16 kernel, whose registers leave room for one; 512 rows over 2 experts of
     // 3584 x 256: 25 us on DMA tiles, 15 so), and a round of tiles has 4 us of its own:
     // finding the rows, the first loads, adding up and storing the sums (fp32 results:
     // 4100 rows over 6 of 32 x 3336 113 us so, 19 on DMA tiles; 9000 of 8 x 4104 456, 40)

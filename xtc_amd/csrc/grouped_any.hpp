@@ -13,9 +13,11 @@
 // fp32 in padded rows.  bf16 runs on v_mfma_f32_16x16x32_bf16, fp32 on
 // v_mfma_f32_16x16x4_f32 (exact products, a lane's 8 k of a slab in any order as
 // long as A and B agree).  Sums are fp32; a bf16 result is rounded once, at the
-// store.  Bound by the unaligned loads and a barrier every slab: 4096 rows over 8
-// experts of 1001 x 999 bf16 68 us, the gradient of w 50; fp32 112 (half the MFMAs'
-// rate).
+// store.  4096 rows over 8 experts of 1001 x 999: bf16 68 us, the gradient of w 50, where
+// memory and MFMAs need 7 and 10; fp32 112, where the MFMAs need 53.  The time goes into
+// loads by way of registers, in pieces of 8 elements, into tiles so small that x is read N / 64
+// times and a group's matrix once for every 64 of its rows, with a barrier every slab;
+// LDS-DMA from copies in whole vectors has not been tried.
 //
 // grouped_small takes the calls whose 64 x 64 tiles do not fill the card, and few
 // rows a group (then it streams the matrices): a workgroup computes a tile of 16

@@ -27,10 +27,11 @@
 // once and keeps the 8 of its k (byte reads for every step cost 8192^3 80 us).
 //
 // What bounds it: bf16, the board's power (32768 rows over 16 experts of 4096 x 4096
-// 912-922 us, 1.2 PFLOP/s, as a large library product); gradients, writing fp32 tiles
-// of shallow sums (16384 rows over 16 of 2048 x 2048 172-209 us, 268 MB); 4-bit, LDS:
-// two slabs of 64 KB, so that the DMA is one slab ahead (8192^3 300-320 us, 3.4-3.7
-// PFLOP/s).
+// 912-957 us by card, 1.15-1.2 PFLOP/s, as a large library product); gradients, writing
+// fp32 tiles of shallow sums after their products (16384 rows over 16 of 2048 x 2048
+// 172-209 us by card, 268 MB); 4-bit, LDS: two slabs of 64 KB, so that the DMA is one slab
+// ahead (8192^3 300-320 us, 3.4-3.7 PFLOP/s).  Of 256 registers that two waves a SIMD leave
+// each, the 256 x 256 tiles take 190 (bf16, transposed) to 218 (gradients), 128 of them sums.
 //
 // Edges cost nothing in the loop: every DMA goes through a buffer descriptor
 // that ends where the tile's rows end, and what lies past it arrives in LDS as

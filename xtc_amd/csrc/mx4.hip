@@ -132,7 +132,9 @@ const RowsTile* rows_tile(int64_t rows, int64_t groups, int N, bool slabs) {
 // quantises its rows, and rows short enough: lanes read 64 bytes of different ones,
 // which costs more than a launch (4 us) from some 32768 elements on.  16 rows x 1024
 // x 2048 7.7 us in two launches, 4.9 in one; x 2048 x 8192 7.9, 7.0; x 4096 x 4096
-// 8.4, 10.2; 1 x 8192 x 8192 11.1 both.
+// 8.4, 10.2.  Rows of 8192 and more are no faster in one launch, however few: 1, 2 and
+// 4 x 8192 x 8192 11.2, 11.2 and 11.4 us in two, 11.1, 11.4 and 11.7 in one; 1 x 16384 x
+// 4096 15.7, 16.6; 1 x 32768 x 1024 23.8, 28.2.
 bool quantizes_on_the_way(int64_t rows, int64_t groups, int N, int K) {
   const int64_t each = (rows + groups - 1) / groups;
   return K % 8 == 0 && K < 8192 && (each < 16 ? each : 16) * K <= 32768 && rows_groups(kRowsX, rows, groups, N) <= 256;

@@ -70,7 +70,7 @@ def listed() -> list[dict[str, Any]]:
         # one decode step of 16 sequences through a square projection: streams the 8-bit weights
         _mm("fp8_decode", "fp8_mm", "bfloat16", 16, 8192, 8192),
         # the headline matmul size on 8-bit operands
-        _mm("fp8_8192", "fp8_mm", "float32", 8192, 8192, 8192),
+        _mm("fp8_8192", "fp8_mm", "bfloat16", 8192, 8192, 8192),
         # a training step of one projection, gradients among it
         _mm("fp8_step", "fp8_step", "bfloat16", 4096, 4096, 2048),
         # one token at two of eight bf16 experts: latency and six matrices

@@ -347,6 +347,128 @@ int xtc_hip_mx4_quantize_matmul(const xtc_hip_mx4_desc *rows,
                                 uint8_t *a_codes, uint8_t *a_scales, const uint8_t *b_codes,
                                 const uint8_t *b_scales, const int32_t *sizes, void *c);
 
+/* Layer norm over the K elements of a row; no counterpart in the reference.
+ *   m = sum x / K, r = 1 / sqrt(sum (x - m)^2 / K + eps), y = (x - m) r w + b
+ * w and b [K] may be NULL (1 and 0).  Sums are fp32, results are rounded once.
+ * An infinity or a NaN makes its own row NaN, no other. */
+typedef struct {
+  int dtype;             /* XTC_HIP_F32 or XTC_HIP_BF16: x, y, dy, dx */
+  int param_dtype;       /* of w and b: XTC_HIP_F32, or XTC_HIP_BF16 for bf16 rows */
+  int64_t rows;          /* below 2^31; 0: nothing to do (gradients: zeros) */
+  int K;
+  int ldx, ldy;          /* row strides in elements, of x and dx, and of y or dy; 0 = dense */
+  float eps;             /* >= 0 */
+  void *stream;          /* hipStream_t, NULL = library stream */
+} xtc_hip_layer_norm_desc;
+
+int xtc_hip_layer_norm(const xtc_hip_layer_norm_desc *desc, const void *x, const void *w,
+                       const void *b, void *y);
+
+/* Its gradients for dy: dx (type dtype), dw and db (fp32, [K]); each may be NULL.
+ *   xh = (x - m) r, g = dy w, dx = r (g - sum g / K - xh sum (g xh) / K)
+ *   dw = sum over rows of dy xh, db = sum over rows of dy, in an order that depends
+ *   on the sizes alone
+ * dw and db need a workspace of 2 min(rows, XTC_HIP_LAYER_NORM_PARTS) K + 2 rows
+ * floats, 16-byte aligned, that no other call uses meanwhile.  Results overlap no
+ * operand. */
+#define XTC_HIP_LAYER_NORM_PARTS 512
+int xtc_hip_layer_norm_grad(const xtc_hip_layer_norm_desc *desc, const void *x, const void *w,
+                            const void *dy, void *dx, float *dw, float *db, float *workspace);
+
+/* 8-bit floats (E4M3: sign, 4 exponent bits, 3 mantissa bits, no infinities) with an
+ * E8M0 scale for every 128 elements of a row (block_rows 1) or for every 128 x 128
+ * block (block_rows 128).  No counterpart in the reference.
+ *   scales  [ceil(rows / block_rows)][ceil(K / 128)] bytes s, the scale is 2^(s -
+ *           127): the smallest power of two (from 2^-127 on) with max|x| <= 448
+ *           scale; 255 (all of the block stands for NaN) where the block holds an
+ *           infinity or a NaN
+ *   codes   [rows][128 ceil(K / 128)] bytes: x / scale to the nearest, ties to even
+ * The last block of a row is filled up with zeros.  `matrices` of rows x K follow one
+ * another, each with its own blocks.  transpose: codes and scales are those of the
+ * transposed matrices: codes [K][128 ceil(rows / 128)], scales [ceil(K /
+ * block_rows)][ceil(rows / 128)].  Codes are 16-byte aligned. */
+typedef struct {
+  int dtype;             /* XTC_HIP_F32 or XTC_HIP_BF16: x and the values */
+  int matrices;          /* >= 0; 0: nothing to do */
+  int64_t rows;          /* of a matrix; 0: nothing to do */
+  int K;                 /* elements of a row */
+  int ld;                /* row stride in elements of x (dequantize: of the values), 0 = dense */
+  int block_rows;        /* 1 or 128 */
+  int transpose;         /* 0 or 1; not for dequantize */
+  void *stream;          /* hipStream_t, NULL = library stream */
+} xtc_hip_fp8_desc;
+
+/* Codes, scales and the (dense) values that they stand for; each may be NULL, and
+ * values must be where transpose is set. */
+int xtc_hip_fp8_quantize(const xtc_hip_fp8_desc *desc, const void *x, uint8_t *codes,
+                         uint8_t *scales, void *values);
+
+/* Those of x and of its transpose from one pass over x, with one block_rows (the
+ * descriptor's transpose is 0). */
+int xtc_hip_fp8_quantize_both(const xtc_hip_fp8_desc *desc, const void *x, uint8_t *codes,
+                              uint8_t *scales, uint8_t *codes_t, uint8_t *scales_t);
+
+/* Codes for given scales: 0 in blocks whose scale is 255; elsewhere what passes 448
+ * scale, infinities among it, gives 448 of its sign and a NaN the NaN code of its sign. */
+int xtc_hip_fp8_encode(const xtc_hip_fp8_desc *desc, const void *x, const uint8_t *scales,
+                       uint8_t *codes);
+
+int xtc_hip_fp8_dequantize(const xtc_hip_fp8_desc *desc, const uint8_t *codes,
+                           const uint8_t *scales, void *values);
+
+/* c[m, n] = sum_k a[m, k] b[n, k] of such operands, both with k along their rows;
+ * fp32 sums.  a has a scale for every 128 elements of a row, b that or (b_block_rows
+ * 128) one for every 128 x 128 block.  Calls of few tiles are summed in parts in the
+ * stream's scratch, or in one part while the stream is captured or without memory for
+ * it. */
+typedef struct {
+  int out_dtype;         /* XTC_HIP_F32 or XTC_HIP_BF16 */
+  int M, N, blocks;      /* rows of a (0: nothing to do), rows of b, blocks of 128 of k */
+  int b_block_rows;      /* 1 or 128 */
+  int ldc;               /* row stride of c in elements, 0 = dense */
+  void *stream;          /* hipStream_t, NULL = library stream */
+} xtc_hip_fp8_matmul_desc;
+
+int xtc_hip_fp8_matmul(const xtc_hip_fp8_matmul_desc *desc, const uint8_t *a_codes,
+                       const uint8_t *a_scales, const uint8_t *b_codes,
+                       const uint8_t *b_scales, void *c);
+
+/* A whole layer of experts for a few tokens; no counterpart in the reference.
+ *   l = x router^T (fp32 sums); of the top_k largest l of a token (ties: the lowest
+ *   expert) y = sum p_e down[e] act(up[e] x), p = softmax(l), with `normalize` divided
+ *   by the sum of the chosen ones
+ * act: relu of up's H rows, or silu of up's first H rows times its last H.  A NaN among
+ * a token's l makes its row of y NaN; rows of other tokens stay as they are.
+ * Matrices are dense, [E][H or 2 H][K] and [E][K][H]: of x's type, or for bf16 x codes with
+ * scales, of 8-bit floats in blocks of 128 x 128 (xtc_hip_fp8_quantize with
+ * `matrices` E and block_rows 128) or of microscaled 4-bit floats
+ * (xtc_hip_mx4_quantize, E rows together). */
+#define XTC_HIP_WEIGHTS_DENSE 0
+#define XTC_HIP_WEIGHTS_FP8 1
+#define XTC_HIP_WEIGHTS_MX4 2
+#define XTC_HIP_RELU 0
+#define XTC_HIP_SWIGLU 1
+typedef struct {
+  int dtype;             /* XTC_HIP_F32 or XTC_HIP_BF16: x, router, y */
+  int weights;           /* XTC_HIP_WEIGHTS_.. of up and down */
+  int activation;        /* XTC_HIP_RELU or XTC_HIP_SWIGLU */
+  int T, E, K, H;        /* tokens (<= 64; 0: nothing to do), experts (<= 256), width, hidden */
+  int top_k;             /* experts of a token, <= 16 and E */
+  int normalize;
+  int ldx, ldy;          /* row strides in elements, 0 = dense */
+  void *stream;          /* hipStream_t, NULL = library stream */
+} xtc_hip_expert_layer_desc;
+
+/* Bytes of the workspace, 0 on an error. */
+uint64_t xtc_hip_expert_layer_workspace(const xtc_hip_expert_layer_desc *desc);
+
+/* The scales are NULL for dense matrices.  The workspace (16-byte aligned, any
+ * contents) is no other call's meanwhile; y overlaps no operand. */
+int xtc_hip_expert_layer(const xtc_hip_expert_layer_desc *desc, const void *x,
+                         const void *router, const void *up, const uint8_t *up_scales,
+                         const void *down, const uint8_t *down_scales, void *workspace,
+                         uint64_t workspace_bytes, void *y);
+
 /* sizeof(xtc_hip_matmul_desc) and sizeof(xtc_hip_conv2d_desc) as this library
  * was compiled (and of the other descriptors, below): a binding that declares
  * the descriptors itself (ctypes, cgo) checks its own struct sizes against
@@ -358,6 +480,10 @@ int xtc_hip_conv2d_desc_size(void);
 int xtc_hip_grouped_matmul_desc_size(void);
 int xtc_hip_mx4_desc_size(void);
 int xtc_hip_mx4_matmul_desc_size(void);
+int xtc_hip_layer_norm_desc_size(void);
+int xtc_hip_fp8_desc_size(void);
+int xtc_hip_fp8_matmul_desc_size(void);
+int xtc_hip_expert_layer_desc_size(void);
 
 /* Compiled kernel instances.  A schedule maps onto one of these; the HIP
  * Scheduler rejects schedules that map to none. */

@@ -219,7 +219,7 @@ def _emit_launch(plan: Plan, ln: Launch, cfg: GemmConfig | SplitConfig | None, i
     a = ln.attrs
     dst = _ptr(plan, ln.output)
     names = [ln.node, *ln.absorbed]
-    if ln.kind.startswith(("grouped_", "mx4_")):
+    if ln.kind.startswith(("grouped_", "mx4_", "layer_norm", "fp8_", "expert_")):
         names = [_label(plan, n) for n in names]
     where = f'"{ln.kind} {names[0]}"'
     lines: list[str] = [f"  /* {ln.kind} {names[0]}{' + ' + ', '.join(names[1:]) if ln.absorbed else ''} */"]
@@ -329,6 +329,51 @@ def _emit_launch(plan: Plan, ln: Launch, cfg: GemmConfig | SplitConfig | None, i
             )
             args = f"&r, {args}"
         lines.append(f"    if ((rc = xtc_hip_{ln.kind}({args}))) {{ record(rc, {where}); return; }} }}")
+    elif ln.kind in ("layer_norm", "layer_norm_grad"):
+        lines.append(
+            f"  {{ static const xtc_hip_layer_norm_desc d = {{{_DTYPE_ENUM[a['dtype']]}, {_DTYPE_ENUM[a['params']]}, {a['rows']}ll, "
+            f"{a['K']}, 0, 0, {_c_float(a['eps'])}, 0}};"
+        )
+        if ln.kind == "layer_norm":
+            args = ", ".join(_ptr(plan, u) for u in (*ln.inputs, ln.output))
+        else:
+            x, dy = ln.inputs
+            args = ", ".join(_ptr(plan, u) if u else "0" for u in (x, a["weight"], dy, *a["results"], a["workspace"]))
+        lines.append(f"    if ((rc = xtc_hip_{ln.kind}(&d, {args}))) {{ record(rc, {where}); return; }} }}")
+    elif ln.kind in ("fp8_quantize", "fp8_encode", "fp8_dequantize"):
+        entry, turned = ln.kind, a["transpose"]
+        uids = [*ln.inputs, ln.output]
+        if ln.kind == "fp8_quantize":
+            uids = [*ln.inputs, a["codes"], ln.output, a["values"]]
+            if a["other"]:
+                mine, other = [a["codes"], ln.output], [a["other"][1], a["other"][0]]
+                entry, uids = "fp8_quantize_both", [*ln.inputs, *(other + mine if turned else mine + other)]
+                turned = False
+        args = ", ".join(_ptr(plan, u) if u else "0" for u in uids)
+        lines.append(
+            f"  {{ static const xtc_hip_fp8_desc d = {{{_DTYPE_ENUM[a['dtype']]}, {a['matrices']}, {a['rows']}ll, {a['K']}, 0, "
+            f"{a['block_rows']}, {1 if turned else 0}, 0}};"
+        )
+        lines.append(f"    if ((rc = xtc_hip_{entry}(&d, {args}))) {{ record(rc, {where}); return; }} }}")
+    elif ln.kind == "fp8_matmul":
+        args = ", ".join(_ptr(plan, u) for u in (*ln.inputs, ln.output))
+        lines.append(
+            f"  {{ static const xtc_hip_fp8_matmul_desc d = {{{_DTYPE_ENUM[a['out']]}, {a['M']}, {a['N']}, {a['blocks']}, "
+            f"{a['b_block_rows']}, 0, 0}};"
+        )
+        lines.append(f"    if ((rc = xtc_hip_fp8_matmul(&d, {args}))) {{ record(rc, {where}); return; }} }}")
+    elif ln.kind == "expert_layer":
+        x, router, *matrices = ln.inputs
+        if a["weights"] == "dense":
+            matrices = [matrices[0], None, matrices[1], None]
+        args = ", ".join(_ptr(plan, u) if u else "0" for u in (x, router, *matrices, a["workspace"]))
+        lines.append(
+            f"  {{ static const xtc_hip_expert_layer_desc d = {{{_DTYPE_ENUM[a['dtype']]}, XTC_HIP_WEIGHTS_{a['weights'].upper()}, "
+            f"XTC_HIP_{a['activation'].upper()}, {a['T']}, {a['E']}, {a['K']}, {a['H']}, {a['top_k']}, {1 if a['normalize'] else 0}, "
+            f"0, 0, 0}};"
+        )
+        lines.append(f"    if ((rc = xtc_hip_expert_layer(&d, {args}, {plan.buffer(a['workspace']).nbytes}ull, {dst}))) "
+                     f"{{ record(rc, {where}); return; }} }}")
     else:
         raise ScheduleError(f"no code generator for launch kind {ln.kind}")
     return lines

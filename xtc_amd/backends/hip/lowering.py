@@ -12,7 +12,9 @@ HBM):
 Such a fusion happens only when the intermediate is used once and is not a graph
 output.  mx4_scales, the mx4_codes of the same tensor for these scales and a
 mx4_dequantize of the pair are one launch that writes all of them; codes and scales
-made for the rows of one 4-bit product alone go into its call.  A matmul operand with
+made for the rows of one 4-bit product alone go into its call.  The fp8_scales and
+fp8_codes of a tensor are one launch too, with the values of the pair or with the scales
+and codes of the transposed tensor; the gradients of one layer_norm are one call.  A matmul operand with
 layout [1, 0] (stored transposed) becomes the launch's trans_a / trans_b flag, a
 grouped_matmul's matrices with [0, 2, 1] its trans_w; other operators require natural
 layouts.  reshape is a view; unpad is a crop kernel (16-byte row copies when the innermost dim is kept).  The reference lowers each node to its own
@@ -67,7 +69,9 @@ class Launch:
     # "matmul" | "conv2d" | "relu" | "pad" | "unpad" | "copy" | "cast" |
     # "grouped_matmul" | "grouped_matmul_grad_w" |
     # "mx4_quantize" | "mx4_encode" | "mx4_dequantize" | "mx4_matmul" |
-    # "mx4_quantize_matmul" (inputs x, the scratch codes and scales, then mx4_matmul's)
+    # "mx4_quantize_matmul" (inputs x, the scratch codes and scales, then mx4_matmul's) |
+    # "layer_norm" | "layer_norm_grad" | "fp8_quantize" | "fp8_encode" | "fp8_dequantize" |
+    # "fp8_matmul" | "expert_layer"
     kind: str
     node: str
     inputs: list[str]
@@ -113,6 +117,31 @@ def _pad_hw(node: Any, rank: int) -> tuple[int, int, int, int] | None:
     top, bottom = per.get(rank - 3, (0, 0))
     left, right = per.get(rank - 2, (0, 0))
     return int(top), int(bottom), int(left), int(right)
+
+
+_NORM_GRADS = ("layer_norm_grad_x", "layer_norm_grad_weight", "layer_norm_grad_bias")
+NORM_PARTS = 512  # XTC_HIP_LAYER_NORM_PARTS
+
+
+def fp8_key(op: Any) -> tuple[int, bool]:
+    return int(op.attrs.get("rows", 1)), bool(op.attrs.get("transpose", False))
+
+
+def expert_layer_attrs(op: Any, shapes: list[tuple[int, ...]], dtype: str) -> dict[str, Any]:
+    (t, k), e = shapes[0], shapes[1][0]
+    dense = len(shapes) == 4
+    up = shapes[2][1]
+    activation = str(op.attrs.get("activation", "swiglu"))
+    weights = "dense" if dense else "mx4" if shapes[2][2] == 16 * shapes[3][2] and shapes[3][1] == up else "fp8"
+    return {"dtype": dtype, "weights": weights, "T": t, "E": e, "K": k, "H": up // 2 if activation == "swiglu" else up,
+            "top_k": int(op.attrs.get("top_k", 2)), "activation": activation, "normalize": bool(op.attrs.get("normalize", True))}
+
+
+def expert_layer_workspace(a: dict[str, Any]) -> int:
+    """What xtc_hip_expert_layer asks for, in bytes."""
+    slots, hidden = a["T"] * a["top_k"], -(-a["H"] // 32) * 32
+    parts = (4 * slots * hidden, 4 * slots * a["K"], 32 * a["T"] * a["E"], 4 * slots, 4 * -(-a["K"] // 16))
+    return sum(-(-p // 256) * 256 for p in parts)
 
 
 def lower_graph(graph: Any) -> Plan:
@@ -215,6 +244,12 @@ def lower_graph(graph: Any) -> Plan:
                     "(only [1, 0] on a 2-D matmul operand and [0, 2, 1] on the matrices of grouped_matmul)"
                 )
         return tuple(flags)
+
+    def fp8_attrs(x: str, op: Any) -> dict[str, Any]:
+        xs = _shape(out_type(x))
+        block_rows, transpose = fp8_key(op)
+        return {"dtype": _dtype(out_type(x)), "matrices": prod(xs[:-2]), "rows": xs[-2], "K": xs[-1], "block_rows": block_rows,
+                "transpose": transpose, "codes": None, "values": None, "other": None}
 
     for n in order:
         trans = transposed_inputs(n)  # also checks the nodes a kernel absorbs
@@ -397,6 +432,101 @@ def lower_graph(graph: Any) -> Plan:
                             [q.node, *q.absorbed])
             launches.append(ln)
             scheduled[n.name] = n
+        elif name == "layer_norm":
+            xs = _shape(t_out)
+            attrs = {"dtype": _dtype(t_out), "params": _dtype(out_type(n.inputs[1])), "rows": prod(xs[:-1]), "K": xs[-1],
+                     "eps": float(op.attrs.get("eps", 1e-5))}
+            launches.append(Launch("layer_norm", n.name, list(n.inputs), n.uid, attrs))
+            scheduled[n.name] = n
+        elif name in _NORM_GRADS:
+            # the gradients that the graph asks for of one norm and dy: one call
+            x, dy = n.inputs[0], n.inputs[-1]  # the bias's alone has dy only
+            weight = n.inputs[1] if name == "layer_norm_grad_x" else None
+            xs = _shape(out_type(x))
+            eps = float(op.attrs.get("eps", 1e-5))
+            results: dict[str, str | None] = {g: None for g in _NORM_GRADS}
+            results[name] = n.uid
+            fused = []
+            for u in users.get(dy, []):
+                kind = u.operation.name
+                if u.uid in absorbed or u is n or kind not in _NORM_GRADS[1:] or results[kind]:
+                    continue
+                if kind == "layer_norm_grad_weight" and (list(u.inputs) != [x, dy] or float(u.operation.attrs.get("eps", 1e-5)) != eps):
+                    continue
+                if name == "layer_norm_grad_bias":
+                    continue
+                results[kind] = u.uid
+                fused.append(u)
+            for u in fused:
+                transposed_inputs(u)
+                absorbed.add(u.uid)
+                if u.uid not in buffers:
+                    buffers[u.uid] = Buffer(u.uid, _shape(u.outputs_types[0]), _dtype(u.outputs_types[0]), "temp")
+            rows = prod(xs[:-1])
+            ws = None
+            if results["layer_norm_grad_weight"] or results["layer_norm_grad_bias"]:
+                ws = n.uid + ".sums"
+                buffers[ws] = Buffer(ws, (2 * min(rows, NORM_PARTS) * xs[-1] + 2 * rows,), F32, "temp")
+            attrs = {"dtype": _dtype(out_type(x)), "params": _dtype(out_type(weight)) if weight else F32, "rows": rows, "K": xs[-1],
+                     "eps": eps, "weight": weight, "results": list(results.values()), "workspace": ws}
+            launches.append(Launch("layer_norm_grad", n.name, [x, dy], n.uid, attrs, [u.name for u in fused]))
+            scheduled[n.name] = n
+        elif name == "fp8_scales":
+            attrs = fp8_attrs(n.inputs[0], op)
+            key = (attrs["block_rows"], attrs["transpose"])
+
+            def codes_of(scales: Any, like: tuple[int, bool]) -> Any | None:
+                return next((u for u in users.get(scales.uid, []) if u.operation.name == "fp8_codes"
+                             and list(u.inputs) == [scales.inputs[0], scales.uid] and fp8_key(u.operation) == like), None)
+
+            fused = []
+            codes = codes_of(n, key)
+            if codes is not None:
+                attrs["codes"] = codes.uid
+                fused.append(codes)
+                # those of the transposed tensor from the same pass, or the values
+                turned = (key[0], not key[1])
+                other = next(((u, c) for u in users.get(n.inputs[0], []) if u.operation.name == "fp8_scales" and u.uid not in absorbed
+                              and fp8_key(u.operation) == turned and (c := codes_of(u, turned)) is not None), None)
+                if other is not None:
+                    attrs["other"] = [u.uid for u in other]
+                    fused += other
+                elif not key[1]:
+                    xs = _shape(out_type(n.inputs[0]))
+                    pair = [u for u in users.get(codes.uid, [])
+                            if u.operation.name == "fp8_dequantize" and list(u.inputs) == [codes.uid, n.uid]
+                            and _shape(u.outputs_types[0]) == xs and _dtype(u.outputs_types[0]) == attrs["dtype"]]
+                    if pair:
+                        attrs["values"] = pair[0].uid
+                        fused.append(pair[0])
+            for u in fused:
+                transposed_inputs(u)
+                absorbed.add(u.uid)
+                if u.uid not in buffers:
+                    buffers[u.uid] = Buffer(u.uid, _shape(u.outputs_types[0]), _dtype(u.outputs_types[0]), "temp")
+            launches.append(Launch("fp8_quantize", n.name, [n.inputs[0]], n.uid, attrs, [u.name for u in fused]))
+            scheduled[n.name] = n
+        elif name == "fp8_codes":
+            launches.append(Launch("fp8_encode", n.name, list(n.inputs), n.uid, fp8_attrs(n.inputs[0], op)))
+            scheduled[n.name] = n
+        elif name == "fp8_dequantize":
+            shape, ss = _shape(t_out), _shape(out_type(n.inputs[1]))
+            attrs = {"dtype": _dtype(t_out), "matrices": prod(shape[:-2]), "rows": shape[-2], "K": shape[-1], "transpose": False,
+                     "block_rows": 1 if ss[-2] == shape[-2] else 128}
+            launches.append(Launch("fp8_dequantize", n.name, list(n.inputs), n.uid, attrs))
+            scheduled[n.name] = n
+        elif name == "fp8_matmul":
+            bs, bss = _shape(out_type(n.inputs[2])), _shape(out_type(n.inputs[3]))
+            attrs = {"out": _dtype(t_out), "M": _shape(t_out)[0], "N": bs[0], "blocks": bss[1], "b_block_rows": 1 if bss[0] == bs[0] else 128}
+            launches.append(Launch("fp8_matmul", n.name, list(n.inputs), n.uid, attrs))
+            scheduled[n.name] = n
+        elif name == "expert_layer":
+            attrs = expert_layer_attrs(op, [_shape(out_type(u)) for u in n.inputs], _dtype(t_out))
+            ws = n.uid + ".layer"
+            buffers[ws] = Buffer(ws, (expert_layer_workspace(attrs),), "uint8", "temp")
+            attrs["workspace"] = ws
+            launches.append(Launch("expert_layer", n.name, list(n.inputs), n.uid, attrs))
+            scheduled[n.name] = n
         elif name == "reshape":
             if n.uid in outputs:
                 launches.append(Launch("copy", n.name, [n.inputs[0]], n.uid, {}))
@@ -408,7 +538,8 @@ def lower_graph(graph: Any) -> Plan:
                 f"operator {name} ({n.name}) is not supported by the HIP backend "
                 "(supported: matmul, conv2d, relu, pad, pad2d, unpad, bias_add after matmul/conv2d, reshape, "
                 "grouped_matmul, grouped_matmul_grad_w, mx4_scales, mx4_codes, mx4_dequantize, mx4_matmul, "
-                "grouped_mx4_matmul)"
+                "grouped_mx4_matmul, layer_norm and its gradients, fp8_scales, fp8_codes, fp8_dequantize, fp8_matmul, "
+                "expert_layer)"
             )
 
     # workspace layout: temps packed at 256-byte alignment

@@ -1,0 +1,355 @@
+// SPDX-License-Identifier: BSD-3-Clause
+// Products of 8-bit floats with a scale for every 128 elements (fp8.hpp), staged
+// through LDS by DMA:
+//   C[m, n] = sum_k A[m, k] B[n, k], both operands with k along their rows.
+//
+// Which instructions.  v_mfma_scale_f32_32x32x64_f8f6f4 takes the codes and scales as they
+// are, at twice the rate of bf16 ones (registers only, random codes: 3.3-3.8 PFLOP/s
+// against 1.9-2.0), but adds up eight products at a time with 16 bits below the
+// largest (2^16 + 1 gives 2^16 within eight neighbours, 2^16 + 2^-7 across): sums are
+// off by 1.5e-5 of themselves for normal data.  A result in bf16, whose own rounding is 250
+// times that, takes them (FAST); one in fp32 takes v_mfma_f32_32x32x16_bf16 on the
+// codes' values in bf16, scaled on the way, which are exact, with fp32 sums.  The
+// 8-bit instructions without scales (16x16x32) add up likewise and are no faster than
+// bf16 ones.
+//
+// Tile and slab.  A workgroup of WGM x WGN waves computes (32 WGM TM) x (32 WGN TN)
+// outputs, k in slabs of 64 bytes of a row, half a block.  k may be summed in any order
+// as long as A and B agree, and all of a row's slab has one scale: a lane takes 32
+// bytes of its row at once (FAST) or two times 16.  B is the first operand: a lane
+// ends with runs of four neighbouring columns of one row.
+//
+// Slabs are staged [rows][64 bytes], 16-byte chunk c of row r at c ^ ((r >> 3) & 3): a
+// ds_read_b128 of 32-row fragments serves lanes 0-3, 12-15, 20-27 at once, which then
+// find all banks.  DMA, walk and descriptors are those of grouped_dma.hpp: what lies
+// past the tile's rows arrives as zeros, rows are whole blocks, so that no slab is cut.
+//
+// Scales.  SCALES blocks of k of the tile's rows are copied to LDS by ordinary loads
+// (any alignment) before the slabs of those blocks are walked; a lane reads four
+// blocks' bytes of its rows at once.  A walk ends after SCALES blocks (8192 elements)
+// and the next begins.
+//
+// Schedules: PP and the plain one as in grouped_dma.hpp.
+//
+// Few tiles: the blocks are shared out over `splits` workgroups a tile, whose fp32
+// sums a second kernel adds up in order.
+#pragma once
+#include "grouped_dma.hpp"
+
+namespace xtc_hip {
+
+struct Fp8Args {
+  const uint8_t *a, *b;    // codes [M], [N] rows of 128 blocks bytes
+  const uint8_t *sa, *sb;  // scales [M][blocks]; [N][blocks] or [ceil(N / 128)][blocks]
+  void* c;
+  float* partial;          // splits > 1: [splits][M][N]
+  int M, N, blocks, ldc;
+  int b_shift;             // log2 of the rows of b that share a scale
+  int tiles_m, tiles_n, band, splits;
+  int out16;               // C is bf16
+};
+
+namespace fp8 {
+
+constexpr int SCALES = 64;  // blocks of a walk
+
+__device__ __forceinline__ int swz(int r) { return (r >> 3) & 3; }
+
+__device__ __forceinline__ gdma::f32x16 mfma(const gdma::u32x4 (&b)[2], unsigned sb, const gdma::u32x4 (&a)[2], unsigned sa, gdma::f32x16 c) {
+  using gdma::i32x8;
+  const i32x8 bv = {(int)b[0][0], (int)b[0][1], (int)b[0][2], (int)b[0][3], (int)b[1][0], (int)b[1][1], (int)b[1][2], (int)b[1][3]};
+  const i32x8 av = {(int)a[0][0], (int)a[0][1], (int)a[0][2], (int)a[0][3], (int)a[1][0], (int)a[1][1], (int)a[1][2], (int)a[1][3]};
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(bv, av, c, 0, 0, 0, (int)sb, 0, (int)sa);
+}
+
+// the blocks of part `part` of `splits`
+__device__ __forceinline__ int part_begin(int blocks, int splits, int part) { return (int)((int64_t)blocks * part / splits); }
+
+}  // namespace fp8
+
+template <bool FAST, int WGM, int WGN, int TM, int TN, int STAGES, bool PP>
+__global__ void __launch_bounds__(WGM* WGN * 64) fp8_dma(Fp8Args p) {
+  using namespace gdma;
+  constexpr int WAVES = WGM * WGN, BM = WGM * TM * 32, BN = WGN * TN * 32;
+  constexpr int SLAB = 64, HALVES = FAST ? 1 : 2;  // steps of a slab
+  constexpr int A_KB = BM * SLAB / 1024, B_KB = BN * SLAB / 1024, PER = (A_KB + B_KB) / WAVES;  // DMA kilobytes
+  constexpr int B_AT = BM * SLAB, STAGE = B_AT + BN * SLAB;
+  constexpr int D = STAGES - 1;
+  static_assert(PER * WAVES == A_KB + B_KB && A_KB % PER == 0 && PER % 2 == 0, "a slab splits evenly over the waves, one operand each");
+  static_assert(!PP || (WGM == 2 && WGN == 4), "two groups of four waves");
+  static_assert(STAGES == 4, "a slab's half of its block follows from its stage");
+  static_assert(STAGES * STAGE + (BM + BN) * fp8::SCALES <= 160 * 1024 && D * PER < 64, "LDS and wait counts");
+
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[STAGES * STAGE + (BM + BN) * fp8::SCALES];
+  unsigned char* const lds_s = lds + STAGES * STAGE;
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / WGN, wn = wave % WGN;
+  const int l32 = lane & 31, half = lane >> 5;
+
+  // ---- the workgroup's tile, bands and XCDs as in grouped_dma
+  const int slot = blockIdx.x >> 3, run = 4 * p.band;
+  const int t = (slot / run * 8 + (blockIdx.x & 7)) * run + slot % run;
+  const int per_part = (p.tiles_m + p.band - 1) / p.band * p.band * p.tiles_n;
+  const int part = t / per_part, tt = t - part * per_part;
+  const int in_band = tt % (p.band * p.tiles_n);
+  const int mt = tt / (p.band * p.tiles_n) * p.band + in_band % p.band, nt = in_band / p.band;
+  if (mt >= p.tiles_m || part >= p.splits) return;
+  const int m0 = mt * BM, n0 = nt * BN;
+  const int rows = min(p.M - m0, BM), cols = min(p.N - n0, BN);
+  const int block0 = fp8::part_begin(p.blocks, p.splits, part), block1 = fp8::part_begin(p.blocks, p.splits, part + 1);
+  const int ld = 128 * p.blocks;
+
+  // ---- this wave's share of a slab's DMA: PER kilobytes of one operand
+  const bool is_a = wave * PER < A_KB;
+  const int kb0 = is_a ? wave * PER : wave * PER - A_KB;
+  const int lines = is_a ? rows : cols;
+  const uint64_t corner = (uint64_t)(is_a ? p.a + (int64_t)m0 * ld : p.b + (int64_t)n0 * ld);
+  // a lane's 16 bytes of KB i: the pattern repeats after two KB (32 rows)
+  unsigned off[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = (kb0 + i) * 16 + lane / 4;
+    off[i] = (unsigned)r * (unsigned)ld + (unsigned)(((lane % 4) ^ fp8::swz(r)) * 16);
+  }
+  const unsigned lds0 = __builtin_amdgcn_readfirstlane(lds_address(lds)), share = (unsigned)((is_a ? 0 : B_AT) + kb0 * 1024);
+
+  f32x16 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = f32x16{};
+
+  for (int first = block0; first < block1; first += fp8::SCALES) {
+    const int blocks = min(block1 - first, fp8::SCALES), nk = 2 * blocks;
+    // K stagger, in whole reads of scales (8 slabs): tiles that share a panel start
+    // their walk at different slabs
+    const int kofs = ((mt + 2 * nt) & 15) * 8 % nk & ~7;
+    Walk<true, SLAB> walk;
+    walk.start = corner + (uint64_t)128 * first;
+    walk.step = SLAB;
+    walk.width = (unsigned)(lines - 1) * (unsigned)ld + 128u * (unsigned)blocks;
+    walk.slab = kofs, walk.slabs = walk.left = nk;
+    walk.at = walk.start + (uint64_t)kofs * SLAB;
+    auto issue = [&](const int stage) {
+      const unsigned at = lds0 + share + stage * STAGE;
+      int step = 32 * ld;  // opaque: the sums of a lane's offsets would fill the registers
+      asm volatile("" : "+s"(step));
+      const u32x4 r = walk.next();
+      each_stage<PER>([&](auto i) { dma16<i == 0, i * 1024>(r, off[i % 2] + (unsigned)(i / 2) * (unsigned)step, at); });
+    };
+
+    if (first != block0) __syncthreads();  // everyone is done with the last walk
+    each_stage<D>([&](auto s) { issue(s); });
+    // ---- the walk's scales: rows past the edge keep what was there, no one stores theirs
+    for (int r = threadIdx.x; r < BM + BN; r += 64 * WAVES) {
+      const bool of_a = r < BM;
+      const int row = of_a ? r : r - BM;
+      if (row >= (of_a ? rows : cols)) continue;
+      const uint8_t* const from = (of_a ? p.sa + (int64_t)(m0 + row) * p.blocks : p.sb + (int64_t)((n0 + row) >> p.b_shift) * p.blocks) + first;
+#pragma unroll
+      for (int q = 0; q < fp8::SCALES / 16; ++q) {
+        u32x4 v = {0, 0, 0, 0};
+        if (16 * q + 16 <= blocks) {
+          __builtin_memcpy(&v, from + 16 * q, 16);
+        } else if (16 * q < blocks) {
+          unsigned char* const at = lds_s + r * fp8::SCALES + 16 * (q ^ fp8::swz(r));
+          for (int i = 0; i < blocks - 16 * q; ++i) at[i] = from[16 * q + i];
+          continue;
+        }
+        *(u32x4*)(lds_s + r * fp8::SCALES + 16 * (q ^ fp8::swz(r))) = v;
+      }
+    }
+    __syncthreads();
+
+    u32x4 fa[TM][2], fb[TN][2];  // FAST: codes of 32 elements; otherwise 16 of them in bf16
+    unsigned ha[TM], hb[TN];     // scales of this lane's rows, four blocks
+    bool odd = false;            // a scale of 255 is among the wave's
+    int at = kofs;               // slab of the operand
+    auto read = [&](const int s, const int hf, const unsigned char* st) {
+      if (s % 2 == 0 && hf == 0) {
+        if ((at & 7) == 0) {
+          const unsigned char* const ss = lds_s + (at >> 1 & 12);
+          const int q = at >> 5;  // 16 blocks
+#pragma unroll
+          for (int i = 0; i < TM; ++i) {
+            const int r = (wm * TM + i) * 32 + l32;
+            ha[i] = *(const unsigned*)(ss + r * fp8::SCALES + 16 * (q ^ fp8::swz(r)));
+          }
+#pragma unroll
+          for (int j = 0; j < TN; ++j) {
+            const int r = BM + (wn * TN + j) * 32 + l32;
+            hb[j] = *(const unsigned*)(ss + r * fp8::SCALES + 16 * (q ^ fp8::swz(r)));
+          }
+        }
+        if constexpr (!FAST) {
+          bool any = false;
+#pragma unroll
+          for (int i = 0; i < TM; ++i) any = any || (ha[i] & 255) == 255;
+#pragma unroll
+          for (int j = 0; j < TN; ++j) any = any || (hb[j] & 255) == 255;
+          odd = __any(any);
+        }
+      }
+      if constexpr (FAST) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const unsigned char* const at_row = st + l32 * SLAB + 16 * ((2 * half + h) ^ fp8::swz(l32));
+#pragma unroll
+          for (int i = 0; i < TM; ++i) fa[i][h] = *(const lds_u32x4*)(at_row + (wm * TM + i) * 32 * SLAB);
+#pragma unroll
+          for (int j = 0; j < TN; ++j) fb[j][h] = *(const lds_u32x4*)(at_row + B_AT + (wn * TN + j) * 32 * SLAB);
+        }
+      } else {
+        const unsigned char* const at_row = st + l32 * SLAB + 16 * ((2 * hf + half) ^ fp8::swz(l32));
+        u32x4 ra[TM], rb[TN];
+#pragma unroll
+        for (int i = 0; i < TM; ++i) ra[i] = *(const lds_u32x4*)(at_row + (wm * TM + i) * 32 * SLAB);
+#pragma unroll
+        for (int j = 0; j < TN; ++j) rb[j] = *(const lds_u32x4*)(at_row + B_AT + (wn * TN + j) * 32 * SLAB);
+        if (odd) {  // blocks that stand for NaN: codes that do
+#pragma unroll
+          for (int i = 0; i < TM; ++i)
+            if ((ha[i] & 255) == 255) ra[i] = u32x4{0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu};
+#pragma unroll
+          for (int j = 0; j < TN; ++j)
+            if ((hb[j] & 255) == 255) rb[j] = u32x4{0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu};
+        }
+        auto convert = [](u32x4 (&to)[2], u32x4 v, unsigned h) {
+          const float scale = fp8::scale_value((int)(h & 255));
+#pragma unroll
+          for (int c = 0; c < 2; ++c) to[c] = __builtin_bit_cast(u32x4, fp8::values_bf16(v[2 * c], v[2 * c + 1], scale));
+        };
+#pragma unroll
+        for (int i = 0; i < TM; ++i) convert(fa[i], ra[i], ha[i]);
+#pragma unroll
+        for (int j = 0; j < TN; ++j) convert(fb[j], rb[j], hb[j]);
+      }
+    };
+    auto mma = [&](const int s, const int hf) {
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          if constexpr (FAST) {
+            acc[i][j] = fp8::mfma(fb[j], hb[j], fa[i], ha[i], acc[i][j]);
+          } else {
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+              acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, fb[j][c]), __builtin_bit_cast(bf16x8, fa[i][c]), acc[i][j], 0, 0, 0);
+          }
+        }
+      if (hf < HALVES - 1) return;
+      ++at;
+      if (s % 2 == 1) {  // the next block's bytes
+#pragma unroll
+        for (int i = 0; i < TM; ++i) ha[i] >>= 8;
+#pragma unroll
+        for (int j = 0; j < TN; ++j) hb[j] >>= 8;
+        if (at == nk) at = 0;
+      }
+    };
+
+    if constexpr (PP) {
+      const int group = wm;
+      __builtin_amdgcn_s_waitcnt(waitcnt_vm((D - 1) * PER));
+      phase_barrier();
+      if (group == 1) phase_barrier();
+      auto step = [&](auto stage) {
+        constexpr int s = decltype(stage)::value;
+        each_stage<HALVES>([&](auto hf) {
+          constexpr bool last = hf == HALVES - 1;
+          // ---- memory phase
+          if (hf == 0) issue((s + D) % STAGES);
+          read(s, hf, lds + s * STAGE);
+          __builtin_amdgcn_s_waitcnt(waitcnt_lgkm0());
+          // this wave's DMA of the next slab has landed: group 0 waits after computing
+          if (last && group == 1) __builtin_amdgcn_s_waitcnt(waitcnt_vm((D - 1) * PER));
+          phase_barrier();
+          // ---- compute phase, ahead of the SIMD's other wave
+          __builtin_amdgcn_s_setprio(1);
+          mma(s, hf);
+          __builtin_amdgcn_s_setprio(0);
+          __builtin_amdgcn_sched_barrier(0);
+          if (last && group == 0) __builtin_amdgcn_s_waitcnt(waitcnt_vm((D - 1) * PER));
+          phase_barrier();
+        });
+      };
+      for (int kt = 0; kt < nk; kt += STAGES) each_stage<STAGES>([&](auto s) { if (kt + s < nk) step(s); });
+      if (group == 0) phase_barrier();
+    } else {
+      auto step = [&](auto stage) {
+        constexpr int s = decltype(stage)::value;
+        // this slab has landed; the ones after it may be in flight
+        __builtin_amdgcn_s_waitcnt(waitcnt_vm((D - 1) * PER));
+        // everyone has read the last slab, whose stage the DMA now fills
+        __builtin_amdgcn_s_waitcnt(waitcnt_lgkm0());
+        phase_barrier();
+        issue((s + D) % STAGES);
+        each_stage<HALVES>([&](auto hf) {
+          read(s, hf, lds + s * STAGE);
+          mma(s, hf);
+        });
+      };
+      for (int kt = 0; kt < nk; kt += STAGES) each_stage<STAGES>([&](auto s) { if (kt + s < nk) step(s); });
+    }
+    // no DMA may write LDS after the workgroup has left it, or the walk
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+  }
+
+  // ---- a lane holds C[m][n .. n+3] for n, n+8, n+16 and n+24 of each 32 x 32
+  const bool to_part = p.splits > 1;
+  void* const c = to_part ? (void*)(p.partial + (size_t)part * p.M * p.N) : p.c;
+  const int ldc = to_part ? p.N : p.ldc, out16 = to_part ? 0 : p.out16;
+  const bool whole = (ldc & 3) == 0 && ((uintptr_t)c & (out16 ? 7 : 15)) == 0;
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+    const int m = (wm * TM + i) * 32 + l32;
+    if (m >= rows) continue;
+    const int64_t at = (int64_t)(m0 + m) * ldc + n0;
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        store4(c, out16, at, f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]},
+               (wn * TN + j) * 32 + 8 * q + 4 * half, cols, whole);
+  }
+}
+
+// Adds up the parts in order: a thread four elements.
+static __global__ void __launch_bounds__(256) fp8_sum(Fp8Args p) {
+  using namespace gdma;
+  const int64_t size = (int64_t)p.M * p.N, at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (at >= size) return;
+  f32x4 v = {0, 0, 0, 0};
+  const int n = (int)min((int64_t)4, size - at);
+  if (n == 4 && (size & 3) == 0) {
+    for (int s0 = 0; s0 < p.splits; s0 += 8) {
+      f32x4 t[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) t[j] = *(const f32x4*)(p.partial + (size_t)min(s0 + j, p.splits - 1) * size + at);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (s0 + j < p.splits) v += t[j];
+    }
+  } else {
+    for (int s = 0; s < p.splits; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i < n) v[i] += p.partial[(size_t)s * size + at + i];
+  }
+  if (p.ldc == p.N && n == 4) {
+    store4(p.c, p.out16, at, v, 0, 4, ((uintptr_t)p.c & (p.out16 ? 7 : 15)) == 0);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (i >= n) break;
+    const int64_t m = (at + i) / p.N, to = m * p.ldc + (at + i - m * p.N);
+    if (p.out16) ((__bf16*)p.c)[to] = (__bf16)v[i];
+    else ((float*)p.c)[to] = v[i];
+  }
+}
+
+}  // namespace xtc_hip

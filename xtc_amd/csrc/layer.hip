@@ -1,0 +1,116 @@
+// SPDX-License-Identifier: BSD-3-Clause
+// Entry points of the layer of experts for a few tokens.
+#include "xtc_hip.h"
+#include "core.hpp"
+#include "layer.hpp"
+
+using namespace xtc_hip;
+using core::aligned16;
+using core::fail;
+
+namespace {
+
+constexpr int kMost = 0x7fffffff - 1023;
+constexpr int kMostTokens = 64, kMostExperts = 256, kMostChosen = 16, kMostLogitParts = 8;
+
+int check(const xtc_hip_expert_layer_desc* d, const char* what) {
+  if (!d) return fail("%s: null descriptor", what);
+  if (d->dtype != XTC_HIP_F32 && d->dtype != XTC_HIP_BF16) return fail("%s: unsupported dtype %d", what, d->dtype);
+  if (d->weights != XTC_HIP_WEIGHTS_DENSE && d->weights != XTC_HIP_WEIGHTS_FP8 && d->weights != XTC_HIP_WEIGHTS_MX4)
+    return fail("%s: unsupported kind %d of matrices", what, d->weights);
+  if (d->weights != XTC_HIP_WEIGHTS_DENSE && d->dtype != XTC_HIP_BF16)
+    return fail("%s: 8-bit and 4-bit matrices take bf16 rows, not dtype %d", what, d->dtype);
+  if (d->activation != XTC_HIP_RELU && d->activation != XTC_HIP_SWIGLU) return fail("%s: unsupported activation %d", what, d->activation);
+  if (d->T < 0 || d->E < 1 || d->K < 1 || d->H < 1 || d->top_k < 1)
+    return fail("%s: invalid sizes T=%d E=%d K=%d H=%d top_k=%d", what, d->T, d->E, d->K, d->H, d->top_k);
+  if (d->T > kMostTokens || d->E > kMostExperts || d->top_k > kMostChosen || d->top_k > d->E)
+    return fail("%s: T=%d, E=%d or top_k=%d are too many: at most %d tokens, %d experts, and %d of them a token", what, d->T, d->E,
+                d->top_k, kMostTokens, kMostExperts, kMostChosen);
+  if (d->K > kMost || d->H > kMost / 2) return fail("%s: sizes K=%d H=%d are too many", what, d->K, d->H);
+  if ((d->ldx && d->ldx < d->K) || (d->ldy && d->ldy < d->K))
+    return fail("%s: row strides %d and %d are below the %d columns", what, d->ldx, d->ldy, d->K);
+  return 0;
+}
+
+uint64_t padded(uint64_t bytes) { return (bytes + 255) / 256 * 256; }
+
+struct Workspace {
+  uint64_t mid, parts, logits, choice, counters, total;
+};
+Workspace workspace_of(const xtc_hip_expert_layer_desc& d) {
+  const uint64_t slots = (uint64_t)d.T * d.top_k, hidden = ((uint64_t)d.H + 31) / 32 * 32;
+  Workspace w{};
+  w.parts = w.mid + padded(4 * slots * hidden);
+  w.logits = w.parts + padded(4 * slots * d.K);
+  w.choice = w.logits + padded(4ull * kMostLogitParts * d.T * d.E);
+  w.counters = w.choice + padded(4 * slots);
+  w.total = w.counters + padded(4 * (((uint64_t)d.K + 15) / 16));
+  return w;
+}
+
+}  // namespace
+
+extern "C" {
+
+int xtc_hip_expert_layer_desc_size(void) { return (int)sizeof(xtc_hip_expert_layer_desc); }
+
+uint64_t xtc_hip_expert_layer_workspace(const xtc_hip_expert_layer_desc* desc) {
+  return check(desc, "expert_layer_workspace") ? 0 : workspace_of(*desc).total;
+}
+
+int xtc_hip_expert_layer(const xtc_hip_expert_layer_desc* desc, const void* x, const void* router, const void* up,
+                         const uint8_t* up_scales, const void* down, const uint8_t* down_scales, void* workspace,
+                         uint64_t workspace_bytes, void* y) {
+  const char* const what = "expert_layer";
+  if (!core::ready()) return fail("xtc_hip_init not called");
+  if (check(desc, what)) return 1;
+  const xtc_hip_expert_layer_desc& d = *desc;
+  if (d.T == 0) return 0;
+  const bool packed = d.weights != XTC_HIP_WEIGHTS_DENSE;
+  if (!x || !router || !up || !down || !y || !workspace || (packed && (!up_scales || !down_scales))) return fail("%s: null operand", what);
+  if (!packed && (up_scales || down_scales)) return fail("%s: scales with matrices that have none", what);
+  if (packed && (!aligned16(up) || !aligned16(down))) return fail("%s: codes must be 16-byte aligned", what);
+  if (!aligned16(workspace)) return fail("%s: the workspace must be 16-byte aligned", what);
+  const Workspace w = workspace_of(d);
+  if (workspace_bytes < w.total)
+    return fail("%s: a workspace of %llu bytes, %llu are needed", what, (unsigned long long)workspace_bytes, (unsigned long long)w.total);
+  char* const ws = (char*)workspace;
+  LayerArgs a{};
+  a.x = x, a.router = router, a.up = up, a.down = down, a.up_scales = up_scales, a.down_scales = down_scales, a.y = y;
+  a.mid = ws + w.mid, a.parts = (float*)(ws + w.parts), a.choice = (int*)(ws + w.choice), a.counters = (unsigned*)(ws + w.counters);
+  a.T = d.T, a.E = d.E, a.K = d.K, a.H = d.H, a.Hp = (d.H + 31) / 32 * 32, a.top_k = d.top_k;
+  a.ldx = d.ldx ? d.ldx : d.K, a.ldy = d.ldy ? d.ldy : d.K;
+  a.normalize = d.normalize != 0, a.swiglu = d.activation == XTC_HIP_SWIGLU;
+  const hipStream_t s = core::pick_stream(d.stream);
+
+  // columns of workgroups: experts, or places of the choice where these are fewer
+  a.by_slot = d.T * d.top_k < d.E;
+  const int columns = a.by_slot ? d.T * d.top_k : d.E;
+  const bool two = d.T > 16 && d.T * d.top_k > 8 * d.E;
+  const int64_t wide_up = a.swiglu ? 32 : 64;
+  const bool wide = columns * (((int64_t)d.H + wide_up - 1) / wide_up) >= 512;
+  const int up_rows = (a.swiglu ? 8 : 16) * (wide ? 4 : 2), down_rows = 16 * (wide ? 4 : 2);
+  const int64_t up_slices = ((int64_t)a.Hp + up_rows - 1) / up_rows, down_slices = ((int64_t)d.K + down_rows - 1) / down_rows;
+  if (up_slices * columns >= 1 << 22 || down_slices * columns >= 1 << 22)
+    return fail("%s: %lld workgroups are too many", what, (long long)((up_slices > down_slices ? up_slices : down_slices) * columns));
+
+  // router and tokens that every workgroup of layer_up reads again
+  const int esz = d.dtype == XTC_HIP_F32 ? 4 : 2;
+  const int pairs = (d.E + 15) / 16 * ((d.T + 15) / 16);
+  if (d.T * d.E > layer::LOGITS || pairs > 8 || ((int64_t)d.T + d.E) * d.K * esz > 128 << 10) {
+    a.logits = (float*)(ws + w.logits);
+    a.logit_parts = pairs >= 16 ? 2 : pairs >= 4 ? 4 : 8;
+    const dim3 grid((unsigned)((d.T + 15) / 16), (unsigned)((d.E + 15) / 16), (unsigned)a.logit_parts);
+    if (d.dtype == XTC_HIP_F32) hipLaunchKernelGGL(layer_logits<float>, grid, dim3(512), 0, s, a);
+    else hipLaunchKernelGGL(layer_logits<__bf16>, grid, dim3(512), 0, s, a);
+  }
+  const LayerGrid grid{wide, two, (int)up_slices, (int)down_slices, columns};
+  if (d.dtype == XTC_HIP_F32) layer_launch<layer::F32>(a, grid, s);
+  else if (d.weights == XTC_HIP_WEIGHTS_FP8) layer_launch<layer::FP8>(a, grid, s);
+  else if (d.weights == XTC_HIP_WEIGHTS_MX4) layer_launch<layer::MX4>(a, grid, s);
+  else layer_launch<layer::BF16>(a, grid, s);
+  const hipError_t err = hipGetLastError();
+  return err == hipSuccess ? 0 : fail("%s: launch failed: %s", what, hipGetErrorString(err));
+}
+
+}  // extern "C"

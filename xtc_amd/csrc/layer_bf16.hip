@@ -1,0 +1,7 @@
+// SPDX-License-Identifier: BSD-3-Clause
+// The expert layer's kernels for matrices of one kind.
+#include "layer.hpp"
+
+namespace xtc_hip {
+XTC_HIP_LAYER_LAUNCH(layer::BF16)
+}  // namespace xtc_hip

@@ -22,6 +22,17 @@ from .expert_operators import (
     XTCOperMx4Matmul,
     XTCOperMx4Scales,
 )
+from .layer_operators import (
+    XTCOperExpertLayer,
+    XTCOperFp8Codes,
+    XTCOperFp8Dequantize,
+    XTCOperFp8Matmul,
+    XTCOperFp8Scales,
+    XTCOperLayerNorm,
+    XTCOperLayerNormGradBias,
+    XTCOperLayerNormGradWeight,
+    XTCOperLayerNormGradX,
+)
 from .operators import (
     XTCOperator,
     XTCOperBiasAdd,
@@ -187,10 +198,10 @@ class XTCOpExpr(XTCExpr):
         return f"{self.uid} = {self.op_name}({', '.join(params)})"
 
 
-def _op_expr(cls: type[XTCOperator], arity: int):  # type: ignore[no-untyped-def]
+def _op_expr(cls: type[XTCOperator], *arities: int):  # type: ignore[no-untyped-def]
     def make(*args: XTCExpr, **attrs: Any) -> XTCOpExpr:
-        if len(args) != arity:
-            raise TypeError(f"{cls.__name__} takes {arity} argument(s), got {len(args)}")
+        if len(args) not in arities:
+            raise TypeError(f"{cls.__name__} takes {' or '.join(map(str, arities))} argument(s), got {len(args)}")
         return XTCOpExpr(cls(**attrs), tuple(args))
 
     return make
@@ -214,4 +225,13 @@ OP_EXPRS = {
     "mx4_dequantize": _op_expr(XTCOperMx4Dequantize, 2),
     "mx4_matmul": _op_expr(XTCOperMx4Matmul, 4),
     "grouped_mx4_matmul": _op_expr(XTCOperGroupedMx4Matmul, 5),
+    "layer_norm": _op_expr(XTCOperLayerNorm, 3),
+    "layer_norm_grad_x": _op_expr(XTCOperLayerNormGradX, 3),
+    "layer_norm_grad_weight": _op_expr(XTCOperLayerNormGradWeight, 2),
+    "layer_norm_grad_bias": _op_expr(XTCOperLayerNormGradBias, 1),
+    "fp8_scales": _op_expr(XTCOperFp8Scales, 1),
+    "fp8_codes": _op_expr(XTCOperFp8Codes, 2),
+    "fp8_dequantize": _op_expr(XTCOperFp8Dequantize, 2),
+    "fp8_matmul": _op_expr(XTCOperFp8Matmul, 4),
+    "expert_layer": _op_expr(XTCOperExpertLayer, 4, 6),
 }

@@ -26,6 +26,10 @@ __all__ = [
     "GroupedMatmulDesc",
     "Mx4Desc",
     "Mx4MatmulDesc",
+    "LayerNormDesc",
+    "Fp8Desc",
+    "Fp8MatmulDesc",
+    "ExpertLayerDesc",
     "GemmInstance",
     "lib",
     "check",
@@ -148,6 +152,51 @@ class Mx4MatmulDesc(ctypes.Structure):
     ]
 
 
+class LayerNormDesc(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int),
+        ("param_dtype", ctypes.c_int),
+        ("rows", ctypes.c_int64),
+        ("K", ctypes.c_int),
+        ("ldx", ctypes.c_int),
+        ("ldy", ctypes.c_int),
+        ("eps", ctypes.c_float),
+        ("stream", ctypes.c_void_p),
+    ]
+
+
+class Fp8Desc(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int),
+        ("matrices", ctypes.c_int),
+        ("rows", ctypes.c_int64),
+        ("K", ctypes.c_int),
+        ("ld", ctypes.c_int),
+        ("block_rows", ctypes.c_int),
+        ("transpose", ctypes.c_int),
+        ("stream", ctypes.c_void_p),
+    ]
+
+
+class Fp8MatmulDesc(ctypes.Structure):
+    _fields_ = [
+        ("out_dtype", ctypes.c_int),
+        ("M", ctypes.c_int),
+        ("N", ctypes.c_int),
+        ("blocks", ctypes.c_int),
+        ("b_block_rows", ctypes.c_int),
+        ("ldc", ctypes.c_int),
+        ("stream", ctypes.c_void_p),
+    ]
+
+
+class ExpertLayerDesc(ctypes.Structure):
+    _fields_ = [
+        *[(n, ctypes.c_int) for n in ("dtype", "weights", "activation", "T", "E", "K", "H", "top_k", "normalize", "ldx", "ldy")],
+        ("stream", ctypes.c_void_p),
+    ]
+
+
 class GemmInstance(ctypes.Structure):
     _fields_ = [
         ("dtype", ctypes.c_int),
@@ -239,11 +288,24 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "xtc_hip_mx4_dequantize": (_i, [ctypes.POINTER(Mx4Desc), _vp, _vp, _vp]),
     "xtc_hip_mx4_matmul": (_i, [ctypes.POINTER(Mx4MatmulDesc), _vp, _vp, _vp, _vp, _vp, _vp]),
     "xtc_hip_mx4_quantize_matmul": (_i, [ctypes.POINTER(Mx4Desc), ctypes.POINTER(Mx4MatmulDesc), *[_vp] * 7]),
+    "xtc_hip_layer_norm": (_i, [ctypes.POINTER(LayerNormDesc), *[_vp] * 4]),
+    "xtc_hip_layer_norm_grad": (_i, [ctypes.POINTER(LayerNormDesc), *[_vp] * 7]),
+    "xtc_hip_fp8_quantize": (_i, [ctypes.POINTER(Fp8Desc), *[_vp] * 4]),
+    "xtc_hip_fp8_quantize_both": (_i, [ctypes.POINTER(Fp8Desc), *[_vp] * 5]),
+    "xtc_hip_fp8_encode": (_i, [ctypes.POINTER(Fp8Desc), *[_vp] * 3]),
+    "xtc_hip_fp8_dequantize": (_i, [ctypes.POINTER(Fp8Desc), *[_vp] * 3]),
+    "xtc_hip_fp8_matmul": (_i, [ctypes.POINTER(Fp8MatmulDesc), *[_vp] * 5]),
+    "xtc_hip_expert_layer_workspace": (ctypes.c_uint64, [ctypes.POINTER(ExpertLayerDesc)]),
+    "xtc_hip_expert_layer": (_i, [ctypes.POINTER(ExpertLayerDesc), *[_vp] * 7, ctypes.c_uint64, _vp]),
     "xtc_hip_matmul_desc_size": (_i, []),
     "xtc_hip_conv2d_desc_size": (_i, []),
     "xtc_hip_grouped_matmul_desc_size": (_i, []),
     "xtc_hip_mx4_desc_size": (_i, []),
     "xtc_hip_mx4_matmul_desc_size": (_i, []),
+    "xtc_hip_layer_norm_desc_size": (_i, []),
+    "xtc_hip_fp8_desc_size": (_i, []),
+    "xtc_hip_fp8_matmul_desc_size": (_i, []),
+    "xtc_hip_expert_layer_desc_size": (_i, []),
     "xtc_hip_gemm_instance_count": (_i, []),
     "xtc_hip_gemm_instance_get": (_i, [_i, ctypes.POINTER(GemmInstance)]),
     "xtc_hip_default_tile": (
@@ -310,7 +372,11 @@ def lib() -> ctypes.CDLL:
                                     (Conv2dDesc, handle.xtc_hip_conv2d_desc_size),
                                     (GroupedMatmulDesc, handle.xtc_hip_grouped_matmul_desc_size),
                                     (Mx4Desc, handle.xtc_hip_mx4_desc_size),
-                                    (Mx4MatmulDesc, handle.xtc_hip_mx4_matmul_desc_size)):
+                                    (Mx4MatmulDesc, handle.xtc_hip_mx4_matmul_desc_size),
+                                    (LayerNormDesc, handle.xtc_hip_layer_norm_desc_size),
+                                    (Fp8Desc, handle.xtc_hip_fp8_desc_size),
+                                    (Fp8MatmulDesc, handle.xtc_hip_fp8_matmul_desc_size),
+                                    (ExpertLayerDesc, handle.xtc_hip_expert_layer_desc_size)):
                 if ctypes.sizeof(struct) != size_fn():
                     raise HipError(f"{struct.__name__} is {ctypes.sizeof(struct)} bytes here but "
                                    f"{size_fn()} in {LIB_PATH.name}: the binding and include/xtc_hip.h differ")

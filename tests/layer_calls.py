@@ -225,10 +225,10 @@ def unclear(x, router, top_k):
     return (gap <= 2 * off.max(1)) & (gap != 0)
 
 
-def plain_layer(x, router, up, down, top_k, activation="swiglu", normalize=True):
+def plain_layer(x, router, up, down, top_k, activation="swiglu", normalize=True, mid=0.0):
     """y in float64 and what fp32 sums of K and H products may be off by: additions of
     the logits (which the weights follow), of up, of down, the activation's few
-    roundings and the 16 bits that the down product's operand keeps.  Inputs whose
+    roundings and `mid`, what the down product's operand is rounded by.  Inputs whose
     choice that could change are refused."""
     assert not unclear(x, router, top_k).any(), "a choice that rounding could change"
     logits, off_l = logits_of(x, router)
@@ -252,5 +252,5 @@ def plain_layer(x, router, up, down, top_k, activation="swiglu", normalize=True)
                 a, off_a = np.maximum(u, 0), off_u
             z, d = down[e] @ a, np.abs(down[e])
             y[t] += p[e] * z
-            off[t] += p[e] * (d @ (off_a + (2.0**-16 + (h + 16) * 2 * U) * np.abs(a)) + (off_p + 4 * U) * (d @ np.abs(a)))
+            off[t] += p[e] * (d @ (off_a + (mid + (h + 16) * 2 * U) * np.abs(a)) + (off_p + 4 * U) * (d @ np.abs(a)))
     return y, off + (top_k + 2) * U * np.abs(y)

@@ -34,7 +34,6 @@ struct Fp8QuantArgs {
 namespace fp8 {
 
 using mx4::f32x2;
-using mx4::scale_value;
 typedef short i16x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
@@ -43,6 +42,10 @@ __device__ __forceinline__ int scale_of(unsigned top) {
   const int e = (int)(top >> 23);
   return e == 255 ? 255 : max(e - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0), 0);
 }
+
+// A scale as the conversion instructions take it: they look at the exponent bits alone, 0
+// is 2^-127 and 255 makes everything NaN
+__device__ __forceinline__ float scale_of_byte(unsigned s) { return __uint_as_float(s << 23); }
 
 // Codes of two pairs for a scale, by the conversion instruction (which divides by the
 // scale's exponent and rounds to nearest even).
@@ -70,17 +73,16 @@ __device__ __forceinline__ float scaled(float x, int s) {
 __device__ __forceinline__ unsigned magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
 // the 4 values of a dword of codes
-__device__ __forceinline__ void values4(float* v, unsigned word, int s) {
-  const float scale = scale_value(s);
+__device__ __forceinline__ void values4(float* v, unsigned word, unsigned s) {
+  const float scale = scale_of_byte(s);
   const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(word, scale, false), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(word, scale, true);
-  v[0] = s == 255 ? scale : a[0], v[1] = s == 255 ? scale : a[1], v[2] = s == 255 ? scale : b[0], v[3] = s == 255 ? scale : b[1];
+  v[0] = a[0], v[1] = a[1], v[2] = b[0], v[3] = b[1];
 }
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
-// The values of 8 codes as bf16 numbers: exact, as scales are powers of two.  The
-// caller sees to scales of 255.
+// The values of 8 codes as bf16 numbers: exact, as scales are powers of two.
 __device__ __forceinline__ bf16x8 values_bf16(unsigned lo, unsigned hi, float scale) {
   const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true),
                c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
@@ -150,7 +152,7 @@ __global__ void __launch_bounds__(256) fp8_quantize_rows(Fp8QuantArgs p, int64_t
         for (int j = 0; j < 8; ++j) top = max(top, magnitude(x[i][j]));
         s = scale_of(max16(top));
       }
-      const float scale = p.scales_in ? 1.f : scale_value(s);
+      const float scale = p.scales_in ? 1.f : scale_of_byte(s);
       u32x2 w = {codes4(x[i][0], x[i][1], x[i][2], x[i][3], scale), codes4(x[i][4], x[i][5], x[i][6], x[i][7], scale)};
       if (p.scales_in) w = (w & 0x7f7f7f7fu) | signs;
       if (s == 255) w = u32x2{0, 0};
@@ -234,7 +236,7 @@ __global__ void __launch_bounds__(256) fp8_quantize_tiles(Fp8QuantArgs p) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) in[j] = scaled(in[j], si);
         }
-        const float scale = p.scales_in ? 1.f : scale_value(si);
+        const float scale = p.scales_in ? 1.f : scale_of_byte(si);
         u32x2 w = {codes4(in[0], in[1], in[2], in[3], scale), codes4(in[4], in[5], in[6], in[7], scale)};
         if (p.scales_in) w = (w & 0x7f7f7f7fu) | signs;
         if (si == 255) w = u32x2{0, 0};
@@ -264,7 +266,7 @@ __global__ void __launch_bounds__(256) fp8_quantize_tiles(Fp8QuantArgs p) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) in[i] = scaled(in[i], sj);
         }
-        const float scale = p.scales_in ? 1.f : scale_value(sj);
+        const float scale = p.scales_in ? 1.f : scale_of_byte(sj);
         u32x2 w = {codes4(in[0], in[1], in[2], in[3], scale), codes4(in[4], in[5], in[6], in[7], scale)};
         if (p.scales_in) w = (w & 0x7f7f7f7fu) | signs;
         if (sj == 255) w = u32x2{0, 0};

@@ -165,7 +165,6 @@ __global__ void __launch_bounds__(WGM* WGN * 64) fp8_dma(Fp8Args p) {
 
     u32x4 fa[TM][2], fb[TN][2];  // FAST: codes of 32 elements; otherwise 16 of them in bf16
     unsigned ha[TM], hb[TN];     // scales of this lane's rows, four blocks
-    bool odd = false;            // a scale of 255 is among the wave's
     int at = kofs;               // slab of the operand
     auto read = [&](const int s, const int hf, const unsigned char* st) {
       if (s % 2 == 0 && hf == 0) {
@@ -182,14 +181,6 @@ __global__ void __launch_bounds__(WGM* WGN * 64) fp8_dma(Fp8Args p) {
             const int r = BM + (wn * TN + j) * 32 + l32;
             hb[j] = *(const unsigned*)(ss + r * fp8::SCALES + 16 * (q ^ fp8::swz(r)));
           }
-        }
-        if constexpr (!FAST) {
-          bool any = false;
-#pragma unroll
-          for (int i = 0; i < TM; ++i) any = any || (ha[i] & 255) == 255;
-#pragma unroll
-          for (int j = 0; j < TN; ++j) any = any || (hb[j] & 255) == 255;
-          odd = __any(any);
         }
       }
       if constexpr (FAST) {
@@ -208,16 +199,8 @@ __global__ void __launch_bounds__(WGM* WGN * 64) fp8_dma(Fp8Args p) {
         for (int i = 0; i < TM; ++i) ra[i] = *(const lds_u32x4*)(at_row + (wm * TM + i) * 32 * SLAB);
 #pragma unroll
         for (int j = 0; j < TN; ++j) rb[j] = *(const lds_u32x4*)(at_row + B_AT + (wn * TN + j) * 32 * SLAB);
-        if (odd) {  // blocks that stand for NaN: codes that do
-#pragma unroll
-          for (int i = 0; i < TM; ++i)
-            if ((ha[i] & 255) == 255) ra[i] = u32x4{0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu};
-#pragma unroll
-          for (int j = 0; j < TN; ++j)
-            if ((hb[j] & 255) == 255) rb[j] = u32x4{0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu};
-        }
         auto convert = [](u32x4 (&to)[2], u32x4 v, unsigned h) {
-          const float scale = fp8::scale_value((int)(h & 255));
+          const float scale = fp8::scale_of_byte(h & 255);
 #pragma unroll
           for (int c = 0; c < 2; ++c) to[c] = __builtin_bit_cast(u32x4, fp8::values_bf16(v[2 * c], v[2 * c + 1], scale));
         };

@@ -40,8 +40,7 @@ __device__ __forceinline__ void load_run(Run& r, const uint8_t* codes, const uin
 // 8 of a lane's elements of block h
 __device__ __forceinline__ bf16x8 elements(const Run& r, int h, int i) {
   const gdma::u32x4 v = r.codes[2 * h + (i >> 1)];
-  const bf16x8 x = values_bf16(v[2 * (i & 1)], v[2 * (i & 1) + 1], scale_value((int)r.scale[h]));
-  return r.scale[h] == 255 ? __builtin_bit_cast(bf16x8, gdma::u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u}) : x;
+  return values_bf16(v[2 * (i & 1)], v[2 * (i & 1) + 1], scale_of_byte(r.scale[h]));
 }
 
 template <int TM, int TN>
@@ -115,6 +114,10 @@ __global__ void __launch_bounds__(64 * fp8::RWAVES) fp8_rows(Fp8Args p) {
       multiply(acc, fa[q], fb[q]);
     }
   }
+  // the sums are read behind branches: their wait states are spelled out
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_nop 15");
+  __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll

@@ -12,6 +12,8 @@ namespace {
 
 constexpr int kMost = 0x7fffffff - 1023;
 constexpr int kMostTokens = 64, kMostExperts = 256, kMostChosen = 16, kMostLogitParts = 8;
+// Workgroups of a launch, as many as the CUs hold at once: they walk over all pieces.
+int64_t groups_of(const xtc_hip_expert_layer_desc& d) { return d.weights == XTC_HIP_WEIGHTS_MX4 ? 512 : 768; }
 
 int check(const xtc_hip_expert_layer_desc* d, const char* what) {
   if (!d) return fail("%s: null descriptor", what);
@@ -83,28 +85,30 @@ int xtc_hip_expert_layer(const xtc_hip_expert_layer_desc* desc, const void* x, c
   a.normalize = d.normalize != 0, a.swiglu = d.activation == XTC_HIP_SWIGLU;
   const hipStream_t s = core::pick_stream(d.stream);
 
-  // columns of workgroups: experts, or places of the choice where these are fewer
-  a.by_slot = d.T * d.top_k < d.E;
-  const int columns = a.by_slot ? d.T * d.top_k : d.E;
-  const bool two = d.T > 16 && d.T * d.top_k > 8 * d.E;
-  const int64_t wide_up = a.swiglu ? 32 : 64;
-  const bool wide = columns * (((int64_t)d.H + wide_up - 1) / wide_up) >= 512;
-  const int up_rows = (a.swiglu ? 8 : 16) * (wide ? 4 : 2), down_rows = 16 * (wide ? 4 : 2);
+  LayerGrid grid{};
+  // experts that tokens may choose, and the tiles of 16 rows of all of them
+  const int most = d.T * d.top_k < d.E ? d.T * d.top_k : d.E;
+  const int64_t tiles = most * (((int64_t)d.H * (a.swiglu ? 2 : 1) + 15) / 16);
+  grid.shared = tiles < 1024;
+  const int up_rows = (a.swiglu ? 16 : 32) * (grid.shared ? 1 : 2), down_rows = 32 * (grid.shared ? 1 : 2);
   const int64_t up_slices = ((int64_t)a.Hp + up_rows - 1) / up_rows, down_slices = ((int64_t)d.K + down_rows - 1) / down_rows;
-  if (up_slices * columns >= 1 << 22 || down_slices * columns >= 1 << 22)
-    return fail("%s: %lld workgroups are too many", what, (long long)((up_slices > down_slices ? up_slices : down_slices) * columns));
+  if (up_slices * most >= 1 << 30 || down_slices * most >= 1 << 30)
+    return fail("%s: %lld pieces of work are too many", what, (long long)((up_slices > down_slices ? up_slices : down_slices) * most));
+  const int64_t groups = groups_of(d);
+  grid.up_slices = (int)up_slices, grid.down_slices = (int)down_slices;
+  grid.up = (unsigned)(up_slices * most < groups ? up_slices * most : groups);
+  grid.down = (unsigned)(down_slices * most < groups ? down_slices * most : groups);
 
   // router and tokens that every workgroup of layer_up reads again
   const int esz = d.dtype == XTC_HIP_F32 ? 4 : 2;
   const int pairs = (d.E + 15) / 16 * ((d.T + 15) / 16);
-  if (d.T * d.E > layer::LOGITS || pairs > 8 || ((int64_t)d.T + d.E) * d.K * esz > 128 << 10) {
+  if (d.T > layer::ROUND || d.T * d.E > layer::LOGITS || pairs > 4 || ((int64_t)d.T + d.E) * d.K * esz > 128 << 10) {
     a.logits = (float*)(ws + w.logits);
     a.logit_parts = pairs >= 16 ? 2 : pairs >= 4 ? 4 : 8;
-    const dim3 grid((unsigned)((d.T + 15) / 16), (unsigned)((d.E + 15) / 16), (unsigned)a.logit_parts);
-    if (d.dtype == XTC_HIP_F32) hipLaunchKernelGGL(layer_logits<float>, grid, dim3(512), 0, s, a);
-    else hipLaunchKernelGGL(layer_logits<__bf16>, grid, dim3(512), 0, s, a);
+    const dim3 logits((unsigned)((d.T + 15) / 16), (unsigned)((d.E + 15) / 16), (unsigned)a.logit_parts);
+    if (d.dtype == XTC_HIP_F32) hipLaunchKernelGGL(layer_logits<float>, logits, dim3(layer::THREADS), 0, s, a);
+    else hipLaunchKernelGGL(layer_logits<__bf16>, logits, dim3(layer::THREADS), 0, s, a);
   }
-  const LayerGrid grid{wide, two, (int)up_slices, (int)down_slices, columns};
   if (d.dtype == XTC_HIP_F32) layer_launch<layer::F32>(a, grid, s);
   else if (d.weights == XTC_HIP_WEIGHTS_FP8) layer_launch<layer::FP8>(a, grid, s);
   else if (d.weights == XTC_HIP_WEIGHTS_MX4) layer_launch<layer::MX4>(a, grid, s);

@@ -8,25 +8,30 @@
 // (mx4.hpp), whose values are bf16 numbers: activations keep their precision.
 //
 // The cost is reading the chosen experts' matrices once.  Two launches:
-//   layer_up    a workgroup takes one expert and a slice of its rows; it works out the
-//               choice for all tokens by itself (so no launch has to pass it on),
-//               gathers the tokens that chose its expert, and writes p_e act(U_e x) to
-//               the place (token, rank of e in its choice) of the workspace
-//   layer_down  the same for D_e; the last workgroup of a slice to arrive adds up the
-//               experts of every token in the order of their ranks (splitk.hpp's
+//   layer_up    every workgroup works out the choice for all tokens by itself (so no
+//               launch has to pass it on), then walks over pieces of work, each some
+//               rows of one chosen expert: it gathers the tokens that chose it and
+//               writes p_e act(U_e x) to the place (token, rank of e in its choice) of
+//               the workspace
+//   layer_down  the same for D_e; the last workgroup that brings a slice of rows adds up
+//               the experts of every token in the order of their ranks (splitk.hpp's
 //               protocol: results do not depend on who is last)
-// Where router and tokens are long (more than layer_up's workgroups should each read
+// Where router and tokens are long (more than every workgroup of layer_up should read
 // again from L2), layer_logits works the logits out first, in parts of k.
 //
-// A workgroup is eight waves that share out k in turn.  k may be summed in any order as
-// long as matrix and token agree, so a lane takes 32 neighbouring elements of its row
-// (16 of fp32): 64, 32 or 16 bytes, four v_mfma_f32_16x16x32_bf16 (or sixteen
-// v_mfma_f32_16x16x4_f32).  The matrix is the first MFMA operand: a lane ends with four
-// neighbouring rows of one token.  The waves' sums are added up in LDS, in order.
+// A workgroup is eight waves.  Where there are few rows in all, eight share out k in
+// turn and add their sums up in LDS, in order (DEPTH 8); where there are many, two do
+// (DEPTH 2).  k may be summed in any order as long as matrix and token
+// agree, so a lane takes 32 neighbouring elements of its row (16 of fp32): 64, 32 or 16
+// bytes, four v_mfma_f32_16x16x32_bf16 (or sixteen v_mfma_f32_16x16x4_f32).  The matrix
+// is the first MFMA operand: a lane ends with four neighbouring rows of one token.  A
+// tile of 16 rows of U holds 8 of its first half and the 8 of the second that these
+// are multiplied with, 32 lanes away.
 //
-// The down product's operand is kept in two bf16 numbers (value and rest, 16 bits in
-// all), multiplied one after the other: rounding it to one would cost as much
-// precision as rounding the result does, where the MFMAs wait for memory anyway.
+// The activations p_e act(U_e x) between the two products are rounded to bf16 where x is
+// bf16, as those between two bf16 products are: it is what the second one's instructions
+// take (in two bf16 numbers, value and rest, the down product reads twice the tokens
+// and issues twice the MFMAs).
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -43,7 +48,7 @@ struct LayerArgs {
   const void *up, *down;
   const uint8_t *up_scales, *down_scales;
   // workspace
-  void* mid;           // [T top_k] rows: 2 planes of Hp bf16, or Hp fp32
+  void* mid;           // [T top_k][Hp] of x's type
   float* parts;        // [T top_k][K]
   float* logits;       // [logit_parts][T][E], or null: layer_up works them out
   int* choice;         // [T][top_k]
@@ -52,7 +57,6 @@ struct LayerArgs {
   int T, E, K, H, Hp, top_k, ldx, ldy;
   int normalize, swiglu;
   int logit_parts;
-  int by_slot;         // workgroups per (token, rank) rather than per expert
   int slices;          // of the launch's rows
 };
 
@@ -65,120 +69,152 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
 enum Format { F32 = 0, BF16 = 1, FP8 = 2, MX4 = 3 };
 
-constexpr int WAVES = 8;
-constexpr int LOGITS = 4096;  // of a round of the choice, in LDS
+constexpr int WAVES = 4, THREADS = 64 * WAVES;
+
+// This thread's wave, known to be the same for all of its lanes
+__device__ __forceinline__ int wave_of() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
+constexpr int LOGITS = 4096;         // of a round of the choice, in LDS
+constexpr int ROUND = THREADS / 8;   // tokens of a round, at most
 
 // ---- runs of a row: UNIT elements a lane
 
-// Elements [k, k + 8) of a row of n elements, zeros past it
+// 16 bytes from element k of a row of n elements, zeros past it
 template <typename T>
 __device__ __forceinline__ u32x4 load16(const T* row, int k, int n) {
   constexpr int V = 16 / sizeof(T);
   u32x4 v = {0, 0, 0, 0};
-  if (k + V <= n) {
-    __builtin_memcpy(&v, row + k, 16);
-  } else if (k < n) {
-    T raw[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) raw[i] = k + i < n ? row[k + i] : (T)0.f;
-    __builtin_memcpy(&v, raw, 16);
+  if (k + V <= n) __builtin_memcpy(&v, row + k, 16);
+  if (n % V != 0 && k < n && k + V > n) {
+    unsigned __int128 w = 0;
+    if (n >= V) {
+      // the row's last 16 bytes, without those before k
+      __builtin_memcpy(&w, row + (n - V), 16);
+      w >>= 8 * (int)sizeof(T) * (k + V - n);
+    } else {
+#pragma unroll 1
+      for (int i = n - 1; i >= k; --i) {
+        uint32_t x = 0;
+        __builtin_memcpy(&x, row + i, sizeof(T));
+        w = w << (8 * sizeof(T)) | x;
+      }
+    }
+    __builtin_memcpy(&v, &w, 16);
   }
   return v;
 }
 
-// A run of a matrix row as stored
-template <int F> struct Raw;
-template <> struct Raw<F32> { u32x4 v[4]; };
-template <> struct Raw<BF16> { u32x4 v[4]; };
-template <> struct Raw<FP8> { u32x4 v[2]; int s; };
-template <> struct Raw<MX4> { u32x4 v[1]; int s; };
+// Lane g's 16 bytes of the four places of the step at element k
+template <typename T>
+__device__ __forceinline__ void load_step(u32x4 (&v)[4], const T* row, int k, int g, int n) {
+  constexpr int V = 16 / sizeof(T);
+  k = __builtin_amdgcn_readfirstlane(k);  // a step is a whole wave's
+  if (k + 16 * V <= n) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) __builtin_memcpy(&v[i], row + k + V * (4 * i + g), 16);
+  } else {
+    asm volatile("" : "+s"(k));  // a pointer for every place would take the loop's registers
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = load16(row, k + V * (4 * i + g), n);
+  }
+}
 
-// One matrix row: its runs, `unit` elements each
+// A step of a matrix row is 256 bytes, of which lane g of the row's four holds bytes 64 i +
+// 16 g: an instruction reads 64 neighbouring bytes of every row
+template <int F>
+struct Raw {
+  u32x4 v[4];
+  u32x4 s;  // scales: of 8-bit elements s[0] for i < 2 and s[1], of 4-bit ones byte g of s[i]
+};
+
+// One matrix row: its steps, STEP elements each.  Elements at step s, place i: s STEP + i
+// STEP / 4 + g STEP / 16 ..
 template <int F> struct Row;
-template <> struct Row<F32> {
-  static constexpr int UNIT = 16;
-  const float* p;
+template <typename T>
+struct DenseRow {
+  static constexpr int STEP = 256 / sizeof(T);
+  const T* p;
   int n;
-  __device__ __forceinline__ Row(const void* w, const uint8_t*, int64_t e, int rows, int r, int depth) : p((const float*)w + (e * rows + r) * depth), n(depth) {}
-  __device__ __forceinline__ void load(Raw<F32>& q, int u) const {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) q.v[i] = load16(p, u * 16 + 4 * i, n);
-  }
+  __device__ __forceinline__ DenseRow(const void* w, const uint8_t*, int64_t e, int rows, int r, int depth) : p((const T*)w + (e * rows + r) * depth), n(depth) {}
+  template <int F>
+  __device__ __forceinline__ void load(Raw<F>& q, int s, int g) const { load_step(q.v, p, s * STEP, g, n); }
 };
-template <> struct Row<BF16> {
-  static constexpr int UNIT = 32;
-  const __bf16* p;
-  int n;
-  __device__ __forceinline__ Row(const void* w, const uint8_t*, int64_t e, int rows, int r, int depth) : p((const __bf16*)w + (e * rows + r) * depth), n(depth) {}
-  __device__ __forceinline__ void load(Raw<BF16>& q, int u) const {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) q.v[i] = load16(p, u * 32 + 8 * i, n);
-  }
-};
+template <> struct Row<F32> : DenseRow<float> { using DenseRow::DenseRow; };
+template <> struct Row<BF16> : DenseRow<__bf16> { using DenseRow::DenseRow; };
 template <> struct Row<FP8> {
-  static constexpr int UNIT = 32;
+  static constexpr int STEP = 256;
   const uint8_t *p, *s;
-  int units;
+  int blocks;
   __device__ __forceinline__ Row(const void* w, const uint8_t* scales, int64_t e, int rows, int r, int depth) {
-    const int blocks = (depth + 127) / 128;
+    blocks = (depth + 127) / 128;
     p = (const uint8_t*)w + (e * rows + r) * blocks * 128;
     s = scales + (e * ((rows + 127) / 128) + r / 128) * blocks;
-    units = 4 * blocks;
   }
-  __device__ __forceinline__ void load(Raw<FP8>& q, int u) const {
-    if (u < units) {
-      q.v[0] = *(const u32x4*)(p + 32 * (int64_t)u), q.v[1] = *(const u32x4*)(p + 32 * (int64_t)u + 16);
-      q.s = s[u >> 2];
-    } else {
-      q.v[0] = q.v[1] = u32x4{0, 0, 0, 0}, q.s = 127;
-    }
+  __device__ __forceinline__ void load(Raw<FP8>& q, int st, int g) const {
+    st = __builtin_amdgcn_readfirstlane(st);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (2 * st + h < blocks) {
+        q.v[2 * h] = *(const u32x4*)(p + 256 * st + 128 * h + 16 * g), q.v[2 * h + 1] = *(const u32x4*)(p + 256 * st + 128 * h + 64 + 16 * g);
+        q.s[h] = s[2 * st + h];
+      } else {
+        q.v[2 * h] = q.v[2 * h + 1] = u32x4{0, 0, 0, 0}, q.s[h] = 127;
+      }
   }
 };
 template <> struct Row<MX4> {
-  static constexpr int UNIT = 32;
+  static constexpr int STEP = 512;
   const uint8_t *p, *s;
-  int units;
+  int blocks;
   __device__ __forceinline__ Row(const void* w, const uint8_t* scales, int64_t e, int rows, int r, int depth) {
-    units = (depth + 31) / 32;
-    p = (const uint8_t*)w + (e * rows + r) * units * 16;
-    s = scales + (e * rows + r) * units;
+    blocks = (depth + 31) / 32;
+    p = (const uint8_t*)w + (e * rows + r) * blocks * 16;
+    s = scales + (e * rows + r) * blocks;
   }
-  __device__ __forceinline__ void load(Raw<MX4>& q, int u) const {
-    if (u < units) q.v[0] = *(const u32x4*)(p + 16 * (int64_t)u), q.s = s[u];
-    else q.v[0] = u32x4{0, 0, 0, 0}, q.s = 127;
+  __device__ __forceinline__ void load(Raw<MX4>& q, int st, int g) const {
+    st = __builtin_amdgcn_readfirstlane(st);
+    if (16 * st + 16 <= blocks) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) q.v[i] = *(const u32x4*)(p + 256 * st + 64 * i + 16 * g);
+      __builtin_memcpy(&q.s, s + 16 * st, 16);
+    } else {
+      asm volatile("" : "+s"(st));  // a pointer for every place would take the loop's registers
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int block = 16 * st + 4 * i + g;
+        q.v[i] = block < blocks ? *(const u32x4*)(p + 16 * block) : u32x4{0, 0, 0, 0};
+        q.s[i] = (block < blocks ? (unsigned)s[block] : 127u) << (8 * g);
+      }
+    }
   }
 };
 
 __device__ __forceinline__ unsigned bits(bf16x2 v) { return __builtin_bit_cast(unsigned, v); }
 
-// Elements 8 i .. 8 i + 7 of a run as bf16 numbers: exact, as scales are powers of two
-__device__ __forceinline__ bf16x8 fragment(const Raw<BF16>& q, int i) { return __builtin_bit_cast(bf16x8, q.v[i]); }
-__device__ __forceinline__ bf16x8 fragment(const Raw<FP8>& q, int i) {
-  const bf16x8 v = fp8::values_bf16(q.v[i >> 1][2 * (i & 1)], q.v[i >> 1][2 * (i & 1) + 1], mx4::scale_value(q.s));
-  return q.s == 255 ? __builtin_bit_cast(bf16x8, u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u}) : v;
+// 8 elements, the c-th of place i, as bf16 numbers: exact, as scales are powers of two
+__device__ __forceinline__ bf16x8 fragment(const Raw<BF16>& q, int i, int) { return __builtin_bit_cast(bf16x8, q.v[i]); }
+__device__ __forceinline__ bf16x8 fragment(const Raw<FP8>& q, int i, int c) {
+  return fp8::values_bf16(q.v[i][2 * c], q.v[i][2 * c + 1], fp8::scale_of_byte(q.s[i >> 1]));
 }
-__device__ __forceinline__ bf16x8 fragment(const Raw<MX4>& q, int i) {
-  const float scale = mx4::scale_value(q.s);
-  const unsigned w = q.v[0][i];
-  u32x4 v = {bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0)), bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1)),
-             bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2)), bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3))};
-  if (q.s == 255) v = u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
-  return __builtin_bit_cast(bf16x8, v);
+__device__ __forceinline__ bf16x8 fragment(const Raw<MX4>& q, int i, int c) {
+  const float scale = fp8::scale_of_byte(q.s[i] >> (threadIdx.x >> 1 & 24));  // the bits above the byte fall on the sign, or out
+  const unsigned w = q.v[i][c];
+  return __builtin_bit_cast(bf16x8, u32x4{bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0)),
+                                          bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1)),
+                                          bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2)),
+                                          bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3))});
 }
 
-// acc += run of matrix rows times run of tokens
+// acc += 16 bytes of tokens times the same elements (the c-th of place i) of matrix rows
 template <int F>
-__device__ __forceinline__ f32x4 multiply(const Raw<F>& w, const u32x4 (&x)[4], f32x4 c) {
+__device__ __forceinline__ f32x4 multiply(const Raw<F>& w, int i, int c, u32x4 x, f32x4 acc) {
   if constexpr (F == F32) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(w.v[i][j]), __uint_as_float(x[i][j]), c, 0, 0, 0);
+    for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(w.v[i][j]), __uint_as_float(x[j]), acc, 0, 0, 0);
+    return acc;
   } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fragment(w, i), __builtin_bit_cast(bf16x8, x[i]), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(fragment(w, i, c), __builtin_bit_cast(bf16x8, x), acc, 0, 0, 0);
   }
-  return c;
 }
 
 // ---- the choice
@@ -194,335 +230,441 @@ struct Choice {
   float p[64 * 16];
 };
 
-// The experts of every token and their weights, from the logits; eight lanes a token.
-// `logits` is LDS of LOGITS floats.
+// The largest of the eight lanes of a token, to all of them, by moves within the vector unit
+template <typename T>
+__device__ __forceinline__ T among8(T v, int how) {
+  const int u = __builtin_bit_cast(int, v);
+  return __builtin_bit_cast(T, how == 0   ? __builtin_amdgcn_mov_dpp(u, 0xb1, 0xf, 0xf, true)     // lanes 1 0 3 2
+                               : how == 1 ? __builtin_amdgcn_mov_dpp(u, 0x4e, 0xf, 0xf, true)     // lanes 2 3 0 1
+                                          : __builtin_amdgcn_mov_dpp(u, 0x141, 0xf, 0xf, true));  // lanes 7 .. 0
+}
+
+// A token's choice by its eight lanes: lane sub looks after the experts sub, sub + 8, ..
+__device__ __forceinline__ void choose_token(const LayerArgs& p, const float* l, int* ids, float* shares) {
+  const int sub = threadIdx.x & 7;
+  uint32_t taken = 0;  // of this lane's experts
+  float top = 0.f, total = 0.f, picked = 0.f, mine[2] = {0.f, 0.f};  // of ranks sub and sub + 8
+  int id[2] = {0, 0};
+  for (int j = 0; j < p.top_k; ++j) {
+    unsigned best = 0;
+    int at = 0x7fffffff;
+    float value = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < (p.E + 7) / 8; ++i) {
+      const int e = min(sub + 8 * i, p.E - 1);
+      const float v = l[e];
+      const bool better = sub + 8 * i < p.E && !(taken >> i & 1) && (at == 0x7fffffff || key(v) > best);
+      best = better ? key(v) : best, at = better ? e : at, value = better ? v : value;
+    }
+#pragma unroll
+    for (int d = 0; d < 3; ++d) {
+      const unsigned ob = among8(best, d);
+      const int oa = among8(at, d);
+      const float ov = among8(value, d);
+      const bool better = oa != 0x7fffffff && (at == 0x7fffffff || ob > best || (ob == best && oa < at));
+      best = better ? ob : best, at = better ? oa : at, value = better ? ov : value;
+    }
+    if ((at & 7) == sub) taken |= 1u << (at >> 3);
+    if (j == 0) top = value;
+    const float share = expf(value - top);
+    picked += share;
+    if ((j & 7) == sub) mine[j >> 3] = share, id[j >> 3] = at;
+  }
+#pragma unroll 4
+  for (int i = sub; i < p.E; i += 8) total += expf(l[i] - top);  // NaN where one is
+#pragma unroll
+  for (int d = 0; d < 3; ++d) total += among8(total, d);
+  const float by = 1.f / (p.normalize && total == total ? picked : total);
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    if (sub + 8 * h < p.top_k) ids[sub + 8 * h] = id[h], shares[sub + 8 * h] = mine[h] * by;
+}
+
+// The experts of every token and their weights, from the logits.  `logits` is LDS of
+// LOGITS floats that fill(t0, tokens) writes.
 template <typename GetRound>
 __device__ __forceinline__ void choose(const LayerArgs& p, Choice& c, float* logits, GetRound&& fill) {
-  const int round = min(LOGITS / p.E, 64);  // tokens at once
-  const int sub = threadIdx.x & 7;
+  const int round = min(LOGITS / p.E, ROUND);  // tokens at once
   for (int t0 = 0; t0 < p.T; t0 += round) {
-    const int tokens = min(round, p.T - t0);
+    const int tokens = min(round, p.T - t0), t = threadIdx.x >> 3;
     __syncthreads();
     fill(t0, tokens);
     __syncthreads();
-    const int t = threadIdx.x >> 3;
     if (t >= tokens) continue;
     const float* const l = logits + t * p.E;
-    float top = 0.f, total = 0.f, picked = 0.f;
-    uint32_t taken = 0;  // of the experts sub, sub + 8, ..: at most 32
-    for (int j = 0; j < p.top_k; ++j) {
-      unsigned best = 0;
-      int at = 0x7fffffff;
-      for (int i = sub, b = 0; i < p.E; i += 8, ++b) {
-        const unsigned k = key(l[i]);
-        if (!(taken >> b & 1) && (k > best || at == 0x7fffffff)) best = k, at = i;
-      }
-#pragma unroll
-      for (int d = 1; d < 8; d *= 2) {
-        const unsigned ob = (unsigned)__shfl_xor((int)best, d);
-        const int oa = __shfl_xor(at, d);
-        if (oa != 0x7fffffff && (at == 0x7fffffff || ob > best || (ob == best && oa < at))) best = ob, at = oa;
-      }
-      if ((at & 7) == sub) taken |= 1u << (at >> 3);
-      const float v = l[at];
-      if (j == 0) top = v;
-      const float share = expf(v - top);
-      picked += share;
-      if (sub == 0) c.e[(t0 + t) * p.top_k + j] = at, c.p[(t0 + t) * p.top_k + j] = share;
-    }
-    for (int i = sub; i < p.E; i += 8) total += expf(l[i] - top);  // NaN where one is
-#pragma unroll
-    for (int d = 1; d < 8; d *= 2) total += __shfl_xor(total, d);
-    const float by = 1.f / (p.normalize && total == total ? picked : total);
-    if (sub == 0)
-      for (int j = 0; j < p.top_k; ++j) c.p[(t0 + t) * p.top_k + j] *= by;
+    int* const ids = c.e + (t0 + t) * p.top_k;
+    float* const shares = c.p + (t0 + t) * p.top_k;
+    choose_token(p, l, ids, shares);
   }
   __syncthreads();
 }
 
-// The expert of workgroup column `a` and the places (token top_k + rank) that chose it,
-// into `places`; how many, 0 where another workgroup has this expert.
-__device__ __forceinline__ int gather(const LayerArgs& p, const int* chosen, int a, int* places, int& e) {
+// The experts that any token chose, ascending, into `active`; how many.
+__device__ __forceinline__ int list_active(const LayerArgs& p, const int* chosen, int* active) {
+  __shared__ unsigned bits[256 / 32];
   const int slots = p.T * p.top_k, lane = threadIdx.x & 63;
-  e = p.by_slot ? chosen[a] : a;
+  if (threadIdx.x < 256 / 32) bits[threadIdx.x] = 0;
+  __syncthreads();
+  for (int s = threadIdx.x; s < slots; s += THREADS) atomicOr(&bits[chosen[s] >> 5], 1u << (chosen[s] & 31));
+  __syncthreads();
   int n = 0;
-  for (int s0 = 0; s0 < slots; s0 += 64) {
-    const int s = s0 + lane;
-    const bool hit = s < slots && chosen[s] == e;
+  for (int e0 = 0; e0 < p.E; e0 += 64) {
+    const int e = e0 + lane;
+    const bool hit = e < p.E && (bits[e >> 5] >> (e & 31) & 1);
     const uint64_t hits = __ballot(hit);
-    if (hit && threadIdx.x < 64) places[n + __popcll(hits & (((uint64_t)1 << lane) - 1))] = s;
-    if (p.by_slot && s0 <= a && hits) {
-      const int first = s0 + __builtin_ctzll(hits);
-      if (first < a && n == 0) return 0;  // an earlier place has it
-    }
+    if (hit && threadIdx.x < 64) active[n + __popcll(hits & (((uint64_t)1 << lane) - 1))] = e;
     n += __popcll(hits);
   }
   __syncthreads();
   return n;
 }
 
-// acc[j][i]: 16 matrix rows j times 16 tokens i, this wave's share of the depth.
-// `token(i, k)` gives the token run's 16 bytes at element k.
-template <int F, int TM, int TN, int PLANES, typename LoadX>
-__device__ __forceinline__ void product(f32x4 (&acc)[TN][TM], const Row<F> (&rows)[TN], int depth, int tiles, LoadX&& load_x) {
-  constexpr int UNIT = Row<F>::UNIT;
-  const int wave = threadIdx.x >> 6, g = (threadIdx.x & 63) >> 4;
-  const int units = (depth + UNIT - 1) / UNIT;
-  Raw<F> w[2][TN];
-  auto load_w = [&](int buf, int u) {
-#pragma unroll
-    for (int j = 0; j < TN; ++j) rows[j].load(w[buf][j], u);
-  };
-  const int u0 = 4 * wave + g, step = 4 * WAVES;
-  const int steps = (units - 4 * wave + step - 1) / step;  // of this wave
-  if (steps > 0) load_w(0, u0);
-  for (int s = 0; s < steps; s += 2) {
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      if (s + q >= steps) break;
-      const int u = u0 + (s + q) * step;
-      u32x4 x[PLANES][TM][4];
-#pragma unroll
-      for (int i = 0; i < TM; ++i)
-        if (i < tiles)
-#pragma unroll
-          for (int h = 0; h < PLANES; ++h) load_x(x[h][i], i, h, u * UNIT);
-      if (s + q + 1 < steps) load_w(1 - q, u + step);
-#pragma unroll
-      for (int i = 0; i < TM; ++i)
-        if (i < tiles)
-#pragma unroll
-          for (int j = 0; j < TN; ++j)
-#pragma unroll
-            for (int h = 0; h < PLANES; ++h) acc[j][i] = multiply<F>(w[q][j], x[h][i], acc[j][i]);
-    }
+// The places (token top_k + rank) that chose expert e, into the wave's own `places`; how
+// many.
+__device__ __forceinline__ int gather(const LayerArgs& p, const int* chosen, int e, int* places) {
+  const int slots = p.T * p.top_k, lane = threadIdx.x & 63;
+  int n = 0;
+  for (int s0 = 0; s0 < slots; s0 += 64) {
+    const int s = s0 + lane;
+    const bool hit = s < slots && chosen[s] == e;
+    const uint64_t hits = __ballot(hit);
+    if (hit) places[n + __popcll(hits & (((uint64_t)1 << lane) - 1))] = s;
+    n += __popcll(hits);
   }
-}
-
-template <int TM, int TN>
-struct Sums {
-  float v[WAVES][TN * 16][16 * TM + 1];
-};
-
-template <int TM, int TN>
-__device__ __forceinline__ void put(Sums<TM, TN>& sums, const f32x4 (&acc)[TN][TM]) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int j = 0; j < TN; ++j)
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) sums.v[wave][16 * j + 4 * (lane >> 4) + r][16 * i + (lane & 15)] = acc[j][i][r];
-}
-template <int TM, int TN>
-__device__ __forceinline__ float total(const Sums<TM, TN>& sums, int row, int token) {
-  float v = sums.v[0][row][token];
-#pragma unroll
-  for (int w = 1; w < WAVES; ++w) v += sums.v[w][row][token];
-  return v;
+  // a wave's LDS accesses keep their order; the compiler has to as well
+  __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+  return n;
 }
 
 template <int F> struct Type { typedef __bf16 type; };
 template <> struct Type<F32> { typedef float type; };
 
-}  // namespace layer
+// A piece's tokens in LDS: LEN elements of each, rows 16 bytes past a multiple of 256, so
+// that 16 tokens' 16 bytes fall on all banks
+template <int F>
+struct Tokens {
+  static constexpr int LEN = F == F32 ? 512 : F == MX4 ? 2048 : 1024;
+  typename Type<F>::type v[16][LEN + 16 / sizeof(typename Type<F>::type)];
+};
 
-// logits[part][t][e] of 16 tokens and 16 experts, part of k: blockIdx.x, .y, .z
-template <typename T>
-__global__ void __launch_bounds__(512) layer_logits(LayerArgs p) {
-  using namespace layer;
-  constexpr int F = sizeof(T) == 4 ? F32 : BF16, UNIT = Row<F>::UNIT;
-  __shared__ Sums<1, 1> sums;
-  const int l16 = threadIdx.x & 15;
-  const int t0 = blockIdx.x * 16, e0 = blockIdx.y * 16;
-  // whole runs of a part
-  const int units = (p.K + UNIT - 1) / UNIT;
-  const int from = (int)((int64_t)units * blockIdx.z / gridDim.z) * UNIT;
-  const int depth = min((int)((int64_t)units * (blockIdx.z + 1) / gridDim.z) * UNIT, p.K) - from;
-  const T* const x = (const T*)p.x + (int64_t)min(t0 + l16, p.T - 1) * p.ldx + from;
-  Row<F> rows[1] = {Row<F>(p.router, nullptr, 0, p.E, min(e0 + l16, p.E - 1), p.K)};
-  rows[0].p += from, rows[0].n = depth;
-  f32x4 acc[1][1] = {};
-  product<F, 1, 1, 1>(acc, rows, depth, 1, [&](u32x4 (&v)[4], int, int, int k) {
+// acc[j]: 16 matrix rows j times 16 tokens, part `part` of DEPTH of the depth, in
+// stretches of Tokens::LEN.  `token(t)` is row t < `count` of the tokens, `depth` elements.
+// Two tiles of tokens at once were tried: a branch round the MFMAs of the second leaves
+// out the wait states that the first one's sums need when it is taken.
+template <int F, int TN, int DEPTH, typename GetToken>
+__device__ __forceinline__ void product(f32x4 (&acc)[TN], Row<F> (&rows)[TN], Tokens<F>& x, int depth, int count, int part, GetToken&& token) {
+  typedef typename Type<F>::type T;
+  constexpr int STEP = Row<F>::STEP, V = 16 / sizeof(T), LEN = Tokens<F>::LEN, RING = 2;
+  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+  constexpr int EACH = LEN / STEP / DEPTH;  // steps of a wave on a stretch
+  static_assert(EACH * STEP * DEPTH == LEN, "every wave has as many steps on a stretch");
+  const int all = (depth + STEP - 1) / STEP;
+  const int steps = (all - part + DEPTH - 1) / DEPTH, most = (all + DEPTH - 1) / DEPTH;  // of this wave, of any
+  Raw<F> w[RING][TN];
+  auto load = [&](int buf, int s) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = load16(x, k + (UNIT / 4) * i, depth);
-  });
-  put(sums, acc);
-  __syncthreads();
-  const int e = threadIdx.x & 15, t = threadIdx.x >> 4;
-  if (t < 16 && t0 + t < p.T && e0 + e < p.E) p.logits[((int64_t)blockIdx.z * p.T + t0 + t) * p.E + e0 + e] = total(sums, e, t);
+    for (int j = 0; j < TN; ++j) rows[j].load(w[buf][j], part + s * DEPTH, g);
+  };
+#pragma unroll
+  for (int s = 0; s < RING - 1; ++s)
+    if (s < steps) load(s, s);
+  for (int s = 0; s < most; s += RING) {
+#pragma unroll
+    for (int q = 0; q < RING; ++q) {
+      if (s + q >= most) break;
+      if ((s + q) % EACH == 0) {
+        const int from = (s + q) * DEPTH * STEP, here = min(depth - from, LEN);
+        const int row = (here + STEP - 1) / STEP * (STEP / V), whole = here / V;  // 16-byte vectors, with zeros and without
+        __syncthreads();  // the last tokens, or sums, have been read
+        // a wave takes a token at a time
+        for (int t = wave_of(); t < count; t += WAVES) {
+          const T* const src = token(t) + from;
+          for (int k0 = lane; k0 < row; k0 += 64 * 4) {
+            u32x4 v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              v[i] = u32x4{0, 0, 0, 0};
+              if (k0 + 64 * i < whole) __builtin_memcpy(&v[i], src + (k0 + 64 * i) * V, 16);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (k0 + 64 * i < row) __builtin_memcpy(__builtin_assume_aligned(&x.v[t][(k0 + 64 * i) * V], 16), &v[i], 16);
+          }
+          // what is left of the row, after the zeros
+          if (lane < here % V) x.v[t][whole * V + lane] = src[whole * V + lane];
+        }
+        __syncthreads();
+      }
+      if (s + q >= steps) break;
+      if (s + q + RING - 1 < steps) load((q + RING - 1) % RING, s + q + RING - 1);
+      const int k = (part + (s + q) % EACH * DEPTH) * STEP + g * (STEP / 16);
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+#pragma unroll
+        for (int c = 0; c < STEP / 16 / V; ++c) {
+          const u32x4 v = *(const u32x4*)&x.v[l16][k + h * (STEP / 4) + V * c];
+#pragma unroll
+          for (int j = 0; j < TN; ++j) acc[j] = multiply<F>(w[q][j], h, c, v, acc[j]);
+        }
+        // a place's conversions follow those before it: all at once they fill the registers
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
+  // the sums are read behind branches: their wait states are spelled out
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_nop 15");
+  __builtin_amdgcn_sched_barrier(0);
 }
 
-// p act(U x) of one expert's tokens, rows [slice, slice + ROWS) of H
-template <int F, int TM, int TN, bool SWIGLU>
-__global__ void __launch_bounds__(512) layer_up(LayerArgs p) {
+// The sums of the DEPTH waves that share a piece's depth: f(v, q) with tile q of them, in
+// one wave each.
+template <int TN>
+struct Sums {
+  f32x4 v[WAVES][TN][64];
+};
+template <int DEPTH, int TN, typename Keep>
+__device__ __forceinline__ void summed(Sums<TN>& sums, const f32x4 (&acc)[TN], Keep&& f) {
+  const int lane = threadIdx.x & 63, wave = wave_of(), member = wave % DEPTH;
+  __syncthreads();  // the tokens, or the last sums, have been read
+#pragma unroll
+  for (int j = 0; j < TN; ++j) sums.v[wave][j][lane] = acc[j];
+  __syncthreads();
+#pragma unroll
+  for (int q0 = 0; q0 < TN; q0 += DEPTH) {
+    const int q = q0 + member;
+    if (q >= TN) break;
+    f32x4 v = {};
+#pragma unroll
+    for (int w = 0; w < DEPTH; ++w) v += sums.v[wave - member + w][q][lane];
+    f(v, q);
+  }
+}
+
+}  // namespace layer
+
+// Sixteen tokens' logits of sixteen experts: element r of lane (g, l16) is expert 4 g + r
+// of token l16.  `from` .. `from` + `depth` of K.
+template <typename T>
+__device__ __forceinline__ layer::f32x4 logit_tile(layer::Sums<1>& sums, const LayerArgs& p, int t0, int e0, int from, int depth) {
+  using namespace layer;
+  constexpr int F = sizeof(T) == 4 ? F32 : BF16;
+  const int l16 = threadIdx.x & 15;
+  const int wave = wave_of(), g = threadIdx.x >> 4 & 3;
+  const T* const x = (const T*)p.x + (int64_t)min(t0 + l16, p.T - 1) * p.ldx + from;
+  const T* const w = (const T*)p.router + (int64_t)min(e0 + l16, p.E - 1) * p.K + from;
+  constexpr int STEP = Row<F>::STEP;
+  f32x4 acc[1] = {};
+  for (int k = wave * STEP; k < depth; k += WAVES * STEP) {
+    Raw<F> a;
+    u32x4 b[4];
+    load_step(a.v, w, k, g, depth), load_step(b, x, k, g, depth);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[0] = multiply<F>(a, i, 0, b[i], acc[0]);
+  }
+  layer::f32x4 got = {};
+  summed<WAVES>(sums, acc, [&](layer::f32x4 v, int) { got = v; });
+  return got;
+}
+
+// logits[part][t][e]: blockIdx.x 16 tokens, .y 16 experts, .z a part of k
+template <typename T>
+__global__ void __launch_bounds__(layer::THREADS) layer_logits(LayerArgs p) {
+  using namespace layer;
+  constexpr int STEP = 256 / sizeof(T);
+  __shared__ Sums<1> sums;
+  const int t0 = blockIdx.x * 16, e0 = blockIdx.y * 16;
+  // whole steps of a part
+  const int steps = (p.K + STEP - 1) / STEP;
+  const int from = (int)((int64_t)steps * blockIdx.z / gridDim.z) * STEP;
+  const int depth = min((int)((int64_t)steps * (blockIdx.z + 1) / gridDim.z) * STEP, p.K) - from;
+  const f32x4 v = logit_tile<T>(sums, p, t0, e0, from, depth);
+  const int t = t0 + (threadIdx.x & 15), e = e0 + (threadIdx.x >> 4) * 4;
+  if (threadIdx.x < 64 && t < p.T)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (e + r < p.E) p.logits[((int64_t)blockIdx.z * p.T + t) * p.E + e + r] = v[r];
+}
+
+// p act(U x): pieces of TN tiles of rows for every DEPTH waves
+template <int F, int TN, bool SWIGLU, int DEPTH>
+__global__ void __launch_bounds__(layer::THREADS, F == layer::MX4 ? 2 : 3) layer_up(LayerArgs p) {
   using namespace layer;
   typedef typename Type<F>::type T;
-  constexpr int UNIT = Row<F>::UNIT, ROWS = SWIGLU ? 8 * TN : 16 * TN;
-  __shared__ union {
-    Sums<TM, TN> sums;
-    Sums<1, 1> logit_sums;
+  constexpr int TILE = SWIGLU ? 8 : 16, ROWS = TILE * TN * (WAVES / DEPTH);
+  __shared__ __attribute__((aligned(16))) union {
+    Tokens<F> tokens;
+    Sums<TN> sums;
+    Sums<1> logit_sums;
+    float logits[LOGITS];
   } lds;
-  __shared__ float logits[LOGITS];
   __shared__ Choice choice;
-  __shared__ int places[64];
-  const int lane = threadIdx.x & 63, l16 = lane & 15;
-  const int slice = blockIdx.x % p.slices, a = blockIdx.x / p.slices;
+  __shared__ int active[256], places_of[WAVES][64];
+  const int lane = threadIdx.x & 63, wave = wave_of(), l16 = lane & 15, g = lane >> 4;
   if (blockIdx.x == 0)
-    for (int i = threadIdx.x; i < (p.K + 15) / 16; i += 512) p.counters[i] = 0;
+    for (int i = threadIdx.x; i < (p.K + 15) / 16; i += THREADS) p.counters[i] = 0;
 
-  choose(p, choice, logits, [&](int t0, int tokens) {
+  choose(p, choice, lds.logits, [&](int t0, int tokens) {
     if (p.logits) {
-      for (int i = threadIdx.x; i < tokens * p.E; i += 512) {
+      for (int i = threadIdx.x; i < tokens * p.E; i += THREADS) {
         float v = 0.f;
         for (int s = 0; s < p.logit_parts; ++s) v += p.logits[((int64_t)s * p.T + t0) * p.E + i];
-        logits[i] = v;
+        lds.logits[i] = v;
       }
       return;
     }
-    // T E <= LOGITS: one round; 16 experts and 16 tokens after the other
-    constexpr int FR = sizeof(T) == 4 ? F32 : BF16, UR = Row<FR>::UNIT;
-    const int et = (p.E + 15) / 16, pairs = et * ((p.T + 15) / 16);
-    for (int q = 0; q < pairs; ++q) {
-      const int ce = q % et * 16, ct = q / et * 16;
-      const T* const x = (const T*)p.x + (int64_t)min(ct + l16, p.T - 1) * p.ldx;
-      const Row<FR> rows[1] = {Row<FR>(p.router, nullptr, 0, p.E, min(ce + l16, p.E - 1), p.K)};
-      f32x4 acc[1][1] = {};
-      product<FR, 1, 1, 1>(acc, rows, p.K, 1, [&](u32x4 (&v)[4], int, int, int k) {
+    // T <= ROUND and T E <= LOGITS: one round.  A tile's sums stay in registers until all are done
+    constexpr int MOST = 4;  // tiles that the caller allows
+    f32x4 mine[MOST];
+    const int et = (p.E + 15) / 16, tiles = et * ((p.T + 15) / 16);
+#pragma unroll 1
+    for (int q = 0; q < tiles; ++q) {
+      const f32x4 v = logit_tile<T>(lds.logit_sums, p, q / et * 16, q % et * 16, 0, p.K);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = load16(x, k + (UR / 4) * i, p.K);
-      });
-      __syncthreads();
-      put(lds.logit_sums, acc);
-      __syncthreads();
-      const int e = ce + (threadIdx.x & 15), t = ct + (threadIdx.x >> 4);
-      if (threadIdx.x < 256 && e < p.E && t < p.T) logits[t * p.E + e] = total(lds.logit_sums, threadIdx.x & 15, threadIdx.x >> 4);
+      for (int i = 0; i < MOST; ++i)
+        if (i == q) mine[i] = v;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < MOST; ++q) {
+      const int t = q / et * 16 + l16, e = q % et * 16 + 4 * g;
+      if (q < tiles && wave == 0 && t < p.T)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (e + r < p.E) lds.logits[t * p.E + e + r] = mine[q][r];
     }
   });
+  const int experts = list_active(p, choice.e, active);
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i < p.T * p.top_k; i += THREADS) p.choice[i] = choice.e[i];
 
-  int e;
-  const int n = gather(p, choice.e, a, places, e);
-  if (n == 0) return;
-  if (slice == 0 && (int)threadIdx.x < n) p.choice[places[threadIdx.x]] = e;
-
-  const int n0 = slice * ROWS;
-  for (int at = 0; at < n; at += 16 * TM) {
-    const int tokens = min(n - at, 16 * TM), tiles = (tokens + 15) / 16;
-    const T* x[TM];
+  int* const places = places_of[wave];
+  for (int piece = blockIdx.x; piece < experts * p.slices; piece += gridDim.x) {
+    const int e = active[piece / p.slices], slice = piece % p.slices;
+    const int n = gather(p, choice.e, e, places);
+    const int n0 = slice * ROWS + wave / DEPTH * (TILE * TN);  // first row of the wave's first tile
+    // h of four rows from `row` of the token at `place`
+    auto keep = [&](f32x4 v, int row, int place, bool there) {
+      f32x4 h;
+      if constexpr (SWIGLU) {
 #pragma unroll
-    for (int i = 0; i < TM; ++i) x[i] = (const T*)p.x + (int64_t)(places[min(at + 16 * i + l16, n - 1)] / p.top_k) * p.ldx;
-    f32x4 acc[TN][TM] = {};
-    // rows past the last one repeat it and are not kept
-    auto row = [&](int j) {
-      const int half = SWIGLU ? j / (TN / 2) : 0, r = n0 + 16 * (SWIGLU ? j % (TN / 2) : j) + l16;
-      return Row<F>(p.up, p.up_scales, e, SWIGLU ? 2 * p.H : p.H, half * p.H + min(r, p.H - 1), p.K);
-    };
-    auto run = [&](const Row<F> (&rows)[TN]) {
-      product<F, TM, TN, 1>(acc, rows, p.K, tiles, [&](u32x4 (&v)[4], int i, int, int k) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) v[c] = load16(x[i], k + (UNIT / 4) * c, p.K);
-      });
-    };
-    if constexpr (TN == 2) run({row(0), row(1)});
-    else run({row(0), row(1), row(2), row(3)});
-    __syncthreads();  // the last sums have been read
-    put(lds.sums, acc);
-    __syncthreads();
-    for (int i = threadIdx.x; i < tokens * ROWS; i += 512) {
-      const int r = i % ROWS, t = i / ROWS;
-      if (n0 + r >= p.Hp) continue;
-      float h = 0.f;
-      if (n0 + r < p.H) {
-        h = total(lds.sums, r, t);
-        if (SWIGLU) h = h / (1.f + expf(-h)) * total(lds.sums, r + 8 * TN, t);
-        else h = h < 0.f ? 0.f : h;
-        h *= choice.p[places[at + t]];
-      }
-      const int64_t to = (int64_t)places[at + t] * p.Hp;
-      if constexpr (F == F32) {
-        ((float*)p.mid)[to + n0 + r] = h;
+        for (int r = 0; r < 4; ++r) {
+          const float u = __shfl_xor(v[r], 32);
+          h[r] = v[r] / (1.f + expf(-v[r])) * u;
+        }
       } else {
-        const __bf16 hi = (__bf16)h;
-        ((__bf16*)p.mid)[2 * to + n0 + r] = hi;
-        ((__bf16*)p.mid)[2 * to + p.Hp + n0 + r] = (__bf16)(__builtin_isinf((float)hi) ? 0.f : h - (float)hi);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) h[r] = v[r] < 0.f ? 0.f : v[r];
       }
+      if (!there || row >= p.Hp || (SWIGLU && g >= 2)) return;
+      const float share = choice.p[place];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) h[r] = row + r < p.H ? h[r] * share : 0.f;
+      // Hp is a multiple of 32: four rows at once
+      if constexpr (F == F32) {
+        *(f32x4*)((float*)p.mid + (int64_t)place * p.Hp + row) = h;
+      } else {
+        typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+        const bf16x4 hi = __builtin_convertvector(h, bf16x4);
+        __bf16* const to = (__bf16*)p.mid + (int64_t)place * p.Hp + row;
+        *(bf16x4*)to = hi;
+      }
+    };
+    for (int at = 0; at < n; at += 16) {
+      f32x4 acc[TN] = {};
+      // rows past the last one repeat it and are not kept
+      auto row = [&](int j) {
+        const int r = n0 + TILE * j + (SWIGLU ? l16 & 7 : l16);
+        return Row<F>(p.up, p.up_scales, e, SWIGLU ? 2 * p.H : p.H, (SWIGLU && l16 >= 8 ? p.H : 0) + min(r, p.H - 1), p.K);
+      };
+      Row<F> rows[2] = {row(0), row(1)};
+      static_assert(TN == 2, "two tiles of rows a wave");
+      product<F, TN, DEPTH>(acc, rows, lds.tokens, p.K, min(n - at, 16), wave % DEPTH,
+                                [&](int t) { return (const T*)p.x + (int64_t)(places[at + t] / p.top_k) * p.ldx; });
+      summed<DEPTH>(lds.sums, acc, [&](f32x4 v, int q) {
+        const int t = at + l16;
+        keep(v, n0 + TILE * q + 4 * (SWIGLU ? g & 1 : g), places[min(t, n - 1)], t < n);
+      });
     }
   }
 }
 
-// D of one expert's tokens, rows [slice, slice + 16 TN) of K, and the sum over a token's
-// experts by the last workgroup of a slice
-template <int F, int TM, int TN>
-__global__ void __launch_bounds__(512) layer_down(LayerArgs p) {
+// D of the same, and the sum over a token's experts by the last workgroup of a slice
+template <int F, int TN, int DEPTH>
+__global__ void __launch_bounds__(layer::THREADS, F == layer::MX4 ? 2 : 3) layer_down(LayerArgs p) {
   using namespace layer;
   typedef typename Type<F>::type T;
-  constexpr int UNIT = Row<F>::UNIT, ROWS = 16 * TN, PLANES = F == F32 ? 1 : 2;
-  __shared__ Sums<TM, TN> sums;
-  __shared__ int chosen[64 * 16];
-  __shared__ int places[64];
-  const int lane = threadIdx.x & 63, l16 = lane & 15;
-  const int slice = blockIdx.x % p.slices, a = blockIdx.x / p.slices;
-  const int slots = p.T * p.top_k, n0 = slice * ROWS, rows_here = min(ROWS, p.K - n0);
-  for (int i = threadIdx.x; i < slots; i += 512) chosen[i] = p.choice[i];
+  constexpr int ROWS = 16 * TN * (WAVES / DEPTH);
+  __shared__ __attribute__((aligned(16))) union {
+    Tokens<F> tokens;
+    Sums<TN> sums;
+  } lds;
+  __shared__ int chosen[64 * 16], active[256], places_of[WAVES][64];
+  const int lane = threadIdx.x & 63, wave = wave_of(), l16 = lane & 15, g = lane >> 4;
+  for (int i = threadIdx.x; i < p.T * p.top_k; i += THREADS) chosen[i] = p.choice[i];
   __syncthreads();
-  int e;
-  const int n = gather(p, chosen, a, places, e);
-  for (int at = 0; at < n; at += 16 * TM) {
-    const int tokens = min(n - at, 16 * TM), tiles = (tokens + 15) / 16;
-    const T* x[TM];
+  const int experts = list_active(p, chosen, active);
+  int* const places = places_of[wave];
+  const bool whole = (p.K & 3) == 0;
+  for (int piece = blockIdx.x; piece < experts * p.slices; piece += gridDim.x) {
+    const int e = active[piece / p.slices], slice = piece % p.slices;
+    const int n = gather(p, chosen, e, places);
+    const int n0 = slice * ROWS + wave / DEPTH * (16 * TN);
+    auto keep = [&](f32x4 v, int row, int place, bool there) {
+      if (!there || row >= p.K) return;
+      float* const to = p.parts + (int64_t)place * p.K + row;
+      if (whole) {
+        splitk_store4(to, v);
+      } else {
 #pragma unroll
-    for (int i = 0; i < TM; ++i) x[i] = (const T*)p.mid + (int64_t)places[min(at + 16 * i + l16, n - 1)] * (PLANES * p.Hp);
-    f32x4 acc[TN][TM] = {};
-    auto row = [&](int j) { return Row<F>(p.down, p.down_scales, e, p.K, min(n0 + 16 * j + l16, p.K - 1), p.H); };
-    auto run = [&](const Row<F> (&rows)[TN]) {
-      product<F, TM, TN, PLANES>(acc, rows, p.H, tiles, [&](u32x4 (&v)[4], int i, int h, int k) {
-        // rows are Hp long, zeros past H
-#pragma unroll
-        for (int c = 0; c < 4; ++c) v[c] = k < p.Hp ? *(const u32x4*)(x[i] + h * p.Hp + k + (UNIT / 4) * c) : u32x4{0, 0, 0, 0};
-      });
+        for (int r = 0; r < 4; ++r)
+          if (row + r < p.K) splitk_store(to + r, v[r]);
+      }
     };
-    if constexpr (TN == 2) run({row(0), row(1)});
-    else run({row(0), row(1), row(2), row(3)});
-    __syncthreads();
-    put(sums, acc);
-    __syncthreads();
-    for (int i = threadIdx.x; i < tokens * ROWS; i += 512) {
-      const int r = i % ROWS, t = i / ROWS;
-      if (r < rows_here) splitk_store(p.parts + (int64_t)places[at + t] * p.K + n0 + r, total(sums, r, t));
+    for (int at = 0; at < n; at += 16) {
+      f32x4 acc[TN] = {};
+      auto row = [&](int j) { return Row<F>(p.down, p.down_scales, e, p.K, min(n0 + 16 * j + l16, p.K - 1), p.H); };
+      Row<F> rows[2] = {row(0), row(1)};
+      static_assert(TN == 2, "two tiles of rows a wave");
+      product<F, TN, DEPTH>(acc, rows, lds.tokens, p.H, min(n - at, 16), wave % DEPTH,
+                                [&](int t) { return (const T*)p.mid + (int64_t)places[at + t] * p.Hp; });
+      summed<DEPTH>(lds.sums, acc, [&](f32x4 v, int q) {
+        const int t = at + l16;
+        keep(v, n0 + 16 * q + 4 * g, places[min(t, n - 1)], t < n);
+      });
     }
-  }
-  if (!splitk_arrive(p.counters + slice, (int)gridDim.x / p.slices)) return;
-  for (int i = threadIdx.x; i < p.T * ROWS; i += 512) {
-    const int r = i % ROWS, t = i / ROWS;
-    if (r >= rows_here) continue;
-    ((T*)p.y)[(int64_t)t * p.ldy + n0 + r] = (T)splitk_sum1(p.parts + (int64_t)t * p.top_k * p.K + n0 + r, (size_t)p.K, p.top_k);
+    if (!splitk_arrive(p.counters + slice, experts)) continue;
+    const int first = slice * ROWS, rows_here = min(ROWS, p.K - first);
+    for (int i = threadIdx.x; i < p.T * ROWS; i += THREADS) {
+      const int r = i % ROWS, t = i / ROWS;
+      if (r >= rows_here) continue;
+      ((T*)p.y)[(int64_t)t * p.ldy + first + r] = (T)splitk_sum1(p.parts + (int64_t)t * p.top_k * p.K + first + r, (size_t)p.K, p.top_k);
+    }
   }
 }
 
 // The two launches.
 struct LayerGrid {
-  bool wide;  // slices of four tiles of rows, or of two
-  bool two;   // tiles of tokens at once, or one
-  int up_slices, down_slices, columns;
+  bool shared;  // eight waves share the depth, or two
+  int up_slices, down_slices;
+  unsigned up, down;  // workgroups
 };
 // Each of a translation unit of its own: layer_f32.hip, layer_bf16.hip, ..
 template <int F>
 void layer_launch(const LayerArgs& a, const LayerGrid& g, hipStream_t s);
 
-template <int F, int TM, int TN>
+template <int F, int DEPTH>
 void layer_launch_tiles(const LayerArgs& a, const LayerGrid& g, hipStream_t s) {
   LayerArgs u = a, d = a;
   u.slices = g.up_slices, d.slices = g.down_slices;
-  const dim3 up((unsigned)(g.up_slices * g.columns)), down((unsigned)(g.down_slices * g.columns));
-  if (a.swiglu) hipLaunchKernelGGL((layer_up<F, TM, TN, true>), up, dim3(512), 0, s, u);
-  else hipLaunchKernelGGL((layer_up<F, TM, TN, false>), up, dim3(512), 0, s, u);
-  hipLaunchKernelGGL((layer_down<F, TM, TN>), down, dim3(512), 0, s, d);
+  if (a.swiglu) hipLaunchKernelGGL((layer_up<F, 2, true, DEPTH>), dim3(g.up), dim3(layer::THREADS), 0, s, u);
+  else hipLaunchKernelGGL((layer_up<F, 2, false, DEPTH>), dim3(g.up), dim3(layer::THREADS), 0, s, u);
+  hipLaunchKernelGGL((layer_down<F, 2, DEPTH>), dim3(g.down), dim3(layer::THREADS), 0, s, d);
 }
-#define XTC_HIP_LAYER_LAUNCH(F)                                                              \
-  template <>                                                                                \
-  void layer_launch<F>(const LayerArgs& a, const LayerGrid& g, hipStream_t s) {              \
-    if (g.wide) g.two ? layer_launch_tiles<F, 2, 4>(a, g, s) : layer_launch_tiles<F, 1, 4>(a, g, s); \
-    else g.two ? layer_launch_tiles<F, 2, 2>(a, g, s) : layer_launch_tiles<F, 1, 2>(a, g, s);      \
+#define XTC_HIP_LAYER_LAUNCH(F)                                                  \
+  template <>                                                                    \
+  void layer_launch<F>(const LayerArgs& a, const LayerGrid& g, hipStream_t s) {  \
+    g.shared ? layer_launch_tiles<F, layer::WAVES>(a, g, s) : layer_launch_tiles<F, 2>(a, g, s); \
   }
 template <> void layer_launch<layer::F32>(const LayerArgs&, const LayerGrid&, hipStream_t);
 template <> void layer_launch<layer::BF16>(const LayerArgs&, const LayerGrid&, hipStream_t);

@@ -19,6 +19,7 @@ from typing import Any
 
 import numpy as np
 
+from ...utils.bf16 import is_bf16, round_to_bf16
 from ...utils.fp8 import BLOCK, blocks_of, fp8_codes, fp8_scales, fp8_values
 from ...utils.mx4 import blocks_of as mx4_blocks_of
 from ...utils.mx4 import mx4_values
@@ -317,7 +318,8 @@ class XTCOperExpertLayer(XTCOperator):
     x (T, K), T <= 64, router (E, K), E <= 256, up (E, H or 2 H, K), down (E, K, H) of
     x's type, or of bfloat16 x with up and down each as two uint8 tensors, codes and
     scales: 8-bit floats (scales (E, ceil(R / 128), B)) or microscaled 4-bit floats
-    (scales (E, R, B)) -> (T, K) of x's type.  A NaN among a token's l makes its row NaN.
+    (scales (E, R, B)) -> (T, K) of x's type, in which p[e] act(..) is kept between the
+    products.  A NaN among a token's l makes its row NaN.
     Attributes top_k (2), activation ("swiglu"), normalize (True).
     """
 
@@ -408,5 +410,6 @@ class XTCOperExpertLayer(XTCOperator):
                         u = u[: d["H"]] / (1 + np.exp(-u[: d["H"]])) * u[d["H"]:]
                     else:
                         u = np.where(u < 0, 0, u)
-                    y[t] += p[e] * np.dot(down[e], u)
+                    h = p[e] * u  # kept in x's type between the products
+                    y[t] += np.dot(down[e], round_to_bf16(h.astype(np.float32)) if is_bf16(inputs[0].type.dtype) else h)
         return [self._check(XTCTensor(y, dtype=inputs[0].type.dtype), inputs)]

@@ -59,13 +59,15 @@ int quantize(const xtc_hip_fp8_desc& d, const Fp8QuantArgs& a, const char* what)
     const int64_t runs = a.matrices * a.rows * a.blocks * 16;
     const dim3 grid(groups_of(runs, 256 * kRuns));
     const int dense = a.K % 128 == 0 && a.ldx == a.K;
-    if (d.dtype == XTC_HIP_F32) hipLaunchKernelGGL((fp8_quantize_rows<float, kRuns>), grid, dim3(256), 0, s, a, runs, dense);
-    else hipLaunchKernelGGL((fp8_quantize_rows<__bf16, kRuns>), grid, dim3(256), 0, s, a, runs, dense);
+    const auto kernel = d.dtype == XTC_HIP_F32 ? (a.scales_in ? fp8_quantize_rows<float, kRuns, true> : fp8_quantize_rows<float, kRuns, false>)
+                                               : (a.scales_in ? fp8_quantize_rows<__bf16, kRuns, true> : fp8_quantize_rows<__bf16, kRuns, false>);
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a, runs, dense);
     return done(what);
   }
   const dim3 grid(groups_of(a.matrices * ((a.rows + 127) / 128) * a.blocks, 1));
-  if (d.dtype == XTC_HIP_F32) hipLaunchKernelGGL(fp8_quantize_tiles<float>, grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL(fp8_quantize_tiles<__bf16>, grid, dim3(256), 0, s, a);
+  const auto kernel = d.dtype == XTC_HIP_F32 ? (a.scales_in ? fp8_quantize_tiles<float, true> : fp8_quantize_tiles<float, false>)
+                                             : (a.scales_in ? fp8_quantize_tiles<__bf16, true> : fp8_quantize_tiles<__bf16, false>);
+  hipLaunchKernelGGL(kernel, grid, dim3(512), 0, s, a);
   return done(what);
 }
 
@@ -75,14 +77,15 @@ struct DmaTile {
   DmaCost cost[2];  // to fp32, to bf16
   void (*launch[2])(const Fp8Args&, unsigned, hipStream_t);
 };
-template <bool FAST, int WGM, int WGN, int TM, int TN, bool PP>
+template <bool FAST, int WGM, int WGN, int TM, int TN, fp8::Schedule S>
 void dma_launch(const Fp8Args& a, unsigned groups, hipStream_t s) {
-  hipLaunchKernelGGL((fp8_dma<FAST, WGM, WGN, TM, TN, 4, PP>), dim3(groups), dim3(WGM * WGN * 64), 0, s, a);
+  hipLaunchKernelGGL((fp8_dma<FAST, WGM, WGN, TM, TN, 4, S>), dim3(groups), dim3(WGM * WGN * 64), 0, s, a);
 }
 const DmaTile kDmaTiles[] = {
-    {{{256, 256, 1, 2.5, 3.0}, {256, 256, 1, 1.25, 1.60}}, {&dma_launch<false, 2, 4, 4, 2, true>, &dma_launch<true, 2, 4, 4, 2, true>}},
-    {{{128, 128, 2, 1.4, 2.2}, {128, 128, 2, 0.73, 1.20}}, {&dma_launch<false, 2, 2, 2, 2, false>, &dma_launch<true, 2, 2, 2, 2, false>}},
-    {{{64, 64, 4, 0.80, 1.50}, {64, 64, 4, 0.40, 0.80}}, {&dma_launch<false, 2, 2, 1, 1, false>, &dma_launch<true, 2, 2, 1, 1, false>}},
+    {{{256, 256, 1, 2.5, 3.0}, {256, 256, 1, 1.25, 1.60}}, {&dma_launch<false, 2, 4, 4, 2, fp8::PINGPONG>, &dma_launch<true, 2, 2, 4, 4, fp8::AHEAD>}},
+    {{{256, 128, 1, 2.5, 3.0}, {256, 128, 1, 0.4, 1.40}}, {&dma_launch<false, 2, 2, 4, 2, fp8::PLAIN>, &dma_launch<true, 2, 2, 4, 2, fp8::AHEAD>}},
+    {{{128, 128, 2, 1.4, 2.2}, {128, 128, 2, 0.73, 1.20}}, {&dma_launch<false, 2, 2, 2, 2, fp8::PLAIN>, &dma_launch<true, 2, 2, 2, 2, fp8::PLAIN>}},
+    {{{64, 64, 4, 0.80, 1.50}, {64, 64, 4, 0.40, 0.80}}, {&dma_launch<false, 2, 2, 1, 1, fp8::PLAIN>, &dma_launch<true, 2, 2, 1, 1, fp8::PLAIN>}},
 };
 
 struct RowsTile {

@@ -35,6 +35,7 @@ namespace fp8 {
 
 using mx4::f32x2;
 typedef short i16x2 __attribute__((ext_vector_type(2)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
 // s of a block whose largest magnitude has the bits `top`: 448 is 1.75 x 2^8
@@ -61,7 +62,6 @@ __device__ __forceinline__ unsigned signs4(float a, float b, float c, float d) {
   return (__float_as_uint(a) >> 24 & 0x80u) | (__float_as_uint(b) >> 16 & 0x8000u) | (__float_as_uint(c) >> 8 & 0x800000u) |
          (__float_as_uint(d) & 0x80000000u);
 }
-__device__ __forceinline__ u32x2 signs8(const float (&v)[8]) { return u32x2{signs4(v[0], v[1], v[2], v[3]), signs4(v[4], v[5], v[6], v[7])}; }
 
 // x / 2^(s - 127) within 448; a NaN stays.  What the division rounds (below 2^-126) is
 // far below the smallest code.
@@ -89,18 +89,24 @@ __device__ __forceinline__ bf16x8 values_bf16(unsigned lo, unsigned hi, float sc
   return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+// 8 neighbours of a row as stored
 template <typename T>
-__device__ __forceinline__ void load8(float (&v)[8], const T* p, int n) {
-  T raw[8];
-  if (n >= 8) {
-    __builtin_memcpy(raw, p, sizeof(raw));
-  } else {
+struct Run8 {
+  T v[8];
+  // the first n of the 8 elements at p, zeros for the others
+  __device__ __forceinline__ void load(const T* p, int n) {
+    if (n >= 8) {
+      __builtin_memcpy(v, p, sizeof(v));
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) raw[i] = i < n ? p[i] : (T)0.f;
+      for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : (T)0.f;
+    }
   }
+  __device__ __forceinline__ void widen(float (&out)[8]) const {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = (float)raw[i];
-}
+    for (int i = 0; i < 8; ++i) out[i] = (float)v[i];
+  }
+};
 
 // The larger of the 16 lanes of a row of lanes
 __device__ __forceinline__ unsigned max16(unsigned v) {
@@ -109,18 +115,78 @@ __device__ __forceinline__ unsigned max16(unsigned v) {
   return max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x128, 0xf, 0xf, true));  // row_ror:8
 }
 
+// Largest magnitudes of pairs (bf16) or single elements (fp32) of 8 neighbours, kept as
+// words: bf16 numbers order by their bits, two a word.
+template <typename T>
+struct Tops {
+  static constexpr int WORDS = 8;
+  unsigned w[WORDS] = {};
+  __device__ __forceinline__ void add(const Run8<T>& x) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = max(w[j], magnitude(x.v[j]));
+  }
+  __device__ __forceinline__ unsigned all() const {
+    unsigned top = w[0];
+#pragma unroll
+    for (int j = 1; j < 8; ++j) top = max(top, w[j]);
+    return top;
+  }
+  static __device__ __forceinline__ unsigned larger(unsigned a, unsigned b) { return max(a, b); }
+  // of column j, from words of all the columns
+  static __device__ __forceinline__ unsigned column(const unsigned* words, int j) { return words[j]; }
+};
+template <>
+struct Tops<__bf16> {
+  static constexpr int WORDS = 4;
+  unsigned w[WORDS] = {};
+  static __device__ __forceinline__ unsigned larger(unsigned a, unsigned b) {
+    return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+  }
+  __device__ __forceinline__ void add(const Run8<__bf16>& x) {
+    unsigned raw[4];
+    __builtin_memcpy(raw, &x, sizeof(raw));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = larger(w[j], raw[j] & 0x7fff7fffu);
+  }
+  __device__ __forceinline__ unsigned all() const {
+    const unsigned top = larger(larger(w[0], w[1]), larger(w[2], w[3]));
+    return max(top & 0xffff0000u, top << 16);
+  }
+  static __device__ __forceinline__ unsigned column(const unsigned* words, int j) {
+    const unsigned top = words[j / 2];
+    return j % 2 ? top & 0xffff0000u : top << 16;
+  }
+};
+
+// 4 codes for a scale.  ENCODE: a scale that somebody chose, which elements may pass.
+template <bool ENCODE>
+__device__ __forceinline__ unsigned codes_for(float a, float b, float c, float d, int s) {
+  unsigned w;
+  if constexpr (ENCODE) {
+    w = codes4(scaled(a, s), scaled(b, s), scaled(c, s), scaled(d, s), 1.f);
+    w = (w & 0x7f7f7f7fu) | signs4(a, b, c, d);
+  } else {
+    w = codes4(a, b, c, d, scale_of_byte(s));
+  }
+  return s == 255 ? 0u : w;
+}
+template <bool ENCODE>
+__device__ __forceinline__ u32x2 codes8(const float (&x)[8], int s) {
+  return u32x2{codes_for<ENCODE>(x[0], x[1], x[2], x[3], s), codes_for<ENCODE>(x[4], x[5], x[6], x[7], s)};
+}
+
 }  // namespace fp8
 
 // Quantisation by rows: a lane takes RUNS runs of 8 elements, a workgroup's width
 // apart, all loads first; 16 lanes share a block.  `dense` says that run q of all
 // rows starts at element 8 q.
-template <typename T, int RUNS>
+template <typename T, int RUNS, bool ENCODE>
 __global__ void __launch_bounds__(256) fp8_quantize_rows(Fp8QuantArgs p, int64_t runs, int dense) {
   using namespace fp8;
   const unsigned per_row = 16u * (unsigned)p.blocks;
   const int64_t rows = p.rows * p.matrices;
   for (int64_t base = (int64_t)blockIdx.x * (256 * RUNS); base < runs; base += (int64_t)gridDim.x * (256 * RUNS)) {
-    float x[RUNS][8];
+    Run8<T> raw[RUNS];
     int64_t row[RUNS];
     int at[RUNS];  // the run's first element in its row
 #pragma unroll
@@ -133,29 +199,23 @@ __global__ void __launch_bounds__(256) fp8_quantize_rows(Fp8QuantArgs p, int64_t
         row[i] = q / per_row, at[i] = (int)(q - row[i] * per_row) * 8;
         from = row[i] * p.ldx + at[i], n = row[i] < rows ? min(p.K - at[i], 8) : 0;
       }
-      load8(x[i], (const T*)p.x + from, n);
+      raw[i].load((const T*)p.x + from, n);
     }
 #pragma unroll
     for (int i = 0; i < RUNS; ++i) {
       const int64_t q = base + i * 256 + threadIdx.x;
       if (q >= runs) break;  // whole blocks: never inside 16 lanes
+      float x[8];
+      raw[i].widen(x);
       int s;
-      u32x2 signs = {0, 0};
-      if (p.scales_in) {
-        signs = signs8(x[i]);
+      if constexpr (ENCODE) {
         s = p.scales_in[q >> 4];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[i][j] = scaled(x[i][j], s);
       } else {
-        unsigned top = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) top = max(top, magnitude(x[i][j]));
-        s = scale_of(max16(top));
+        Tops<T> tops;
+        tops.add(raw[i]);
+        s = scale_of(max16(tops.all()));
       }
-      const float scale = p.scales_in ? 1.f : scale_of_byte(s);
-      u32x2 w = {codes4(x[i][0], x[i][1], x[i][2], x[i][3], scale), codes4(x[i][4], x[i][5], x[i][6], x[i][7], scale)};
-      if (p.scales_in) w = (w & 0x7f7f7f7fu) | signs;
-      if (s == 255) w = u32x2{0, 0};
+      const u32x2 w = codes8<ENCODE>(x, s);
       if (p.codes) *(u32x2*)(p.codes + 8 * q) = w;
       if (p.scales && (threadIdx.x & 15) == 0) p.scales[q >> 4] = (uint8_t)s;
       if (p.values) {
@@ -168,16 +228,19 @@ __global__ void __launch_bounds__(256) fp8_quantize_rows(Fp8QuantArgs p, int64_t
   }
 }
 
-// Quantisation by 128 x 128 blocks, of the transposed matrix, or of both: a workgroup
-// takes a 128 x 128 piece, a thread 8 x 8 of it, so that the lanes next to one another
-// read 256 (bf16) bytes of a row, and the transposed codes leave through LDS as whole
-// lines of 128 bytes.
-template <typename T>
-__global__ void __launch_bounds__(256) fp8_quantize_tiles(Fp8QuantArgs p) {
+// Quantisation by 128 x 128 blocks, of the transposed matrix, or of both: a workgroup of
+// 512 threads takes a 128 x 128 piece, a thread 4 rows x 8 columns of it, so that 16 lanes
+// read 256 (bf16) neighbouring bytes of a row, and the transposed codes leave through LDS
+// as whole lines of 128 bytes.
+template <typename T, bool ENCODE>
+__global__ void __launch_bounds__(512) fp8_quantize_tiles(Fp8QuantArgs p) {
   using namespace fp8;
-  __shared__ unsigned col_top[4][128];
-  __shared__ unsigned all_top[4];
-  __shared__ __attribute__((aligned(16))) unsigned char turned[128][144];
+  constexpr int WORDS = Tops<T>::WORDS;
+  __shared__ unsigned col_top[8][16 * WORDS];
+  __shared__ unsigned all_top[8];
+  __shared__ uint8_t col_scale[128];
+  // rows of 33 words: the 16 lanes side by side write columns that lie 8 rows apart
+  __shared__ unsigned turned[128][33];
   const int tr = threadIdx.x >> 4, tc = threadIdx.x & 15, wave = threadIdx.x >> 6;
   const int64_t row_tiles = (p.rows + 127) / 128, tiles = row_tiles * p.blocks * p.matrices;
   const int64_t scale_rows = p.square ? row_tiles : p.rows;                    // of one matrix
@@ -185,61 +248,69 @@ __global__ void __launch_bounds__(256) fp8_quantize_tiles(Fp8QuantArgs p) {
   for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
     const int cb = (int)(tile % p.blocks);
     const int64_t rb = tile / p.blocks % row_tiles, e = tile / p.blocks / row_tiles;
-    const int64_t r0 = rb * 128 + tr * 8;
+    const int64_t r0 = rb * 128 + tr * 4;
     const int c0 = cb * 128 + tc * 8;
     const T* const x = (const T*)p.x + (e * p.rows + r0) * p.ldx + c0;
-    float v[8][8];  // row, column
+    Run8<T> raw[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) load8(v[i], x + (int64_t)i * p.ldx, r0 + i < p.rows ? p.K - c0 : 0);
-    unsigned row_top[8], ct[8] = {};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      row_top[i] = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) row_top[i] = max(row_top[i], magnitude(v[i][j])), ct[j] = max(ct[j], magnitude(v[i][j]));
-    }
+    for (int i = 0; i < 4; ++i) raw[i].load(x + (int64_t)i * p.ldx, r0 + i < p.rows ? p.K - c0 : 0);
     int s = 0;  // of the whole piece
-    if (p.square) {
-      unsigned top = 0;
+    if constexpr (!ENCODE) {
+      if (p.square) {
+        Tops<T> tops;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) top = max(top, row_top[i]);
+        for (int i = 0; i < 4; ++i) tops.add(raw[i]);
+        unsigned top = max16(tops.all());
+        top = max(top, (unsigned)__shfl_xor((int)top, 16));
+        top = max(top, (unsigned)__shfl_xor((int)top, 32));
+        __syncthreads();  // the last piece's readers are done
+        if ((threadIdx.x & 63) == 0) all_top[wave] = top;
+        __syncthreads();
+        top = all_top[0];
 #pragma unroll
-      for (int d = 1; d < 64; d *= 2) top = max(top, (unsigned)__shfl_xor((int)top, d));
-      __syncthreads();  // the last piece's readers are done
-      if ((threadIdx.x & 63) == 0) all_top[wave] = top;
-      __syncthreads();
-      s = scale_of(max(max(all_top[0], all_top[1]), max(all_top[2], all_top[3])));
-    } else if (p.codes_t || p.scales_t) {
+        for (int i = 1; i < 8; ++i) top = max(top, all_top[i]);
+        s = scale_of(top);
+      } else if (p.codes_t || p.scales_t) {
+        Tops<T> tops;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        ct[j] = max(ct[j], (unsigned)__shfl_xor((int)ct[j], 16));
-        ct[j] = max(ct[j], (unsigned)__shfl_xor((int)ct[j], 32));
+        for (int i = 0; i < 4; ++i) tops.add(raw[i]);
+#pragma unroll
+        for (int j = 0; j < WORDS; ++j) {
+          tops.w[j] = Tops<T>::larger(tops.w[j], (unsigned)__shfl_xor((int)tops.w[j], 16));
+          tops.w[j] = Tops<T>::larger(tops.w[j], (unsigned)__shfl_xor((int)tops.w[j], 32));
+        }
+        // the last piece's readers of col_top and col_scale have passed the barriers below
+        if ((threadIdx.x & 48) == 0)
+#pragma unroll
+          for (int j = 0; j < WORDS; ++j) col_top[wave][tc * WORDS + j] = tops.w[j];
+        __syncthreads();
+        if (threadIdx.x < 16 * WORDS) {
+          unsigned top = col_top[0][threadIdx.x];
+#pragma unroll
+          for (int i = 1; i < 8; ++i) top = Tops<T>::larger(top, col_top[i][threadIdx.x]);
+#pragma unroll
+          for (int j = 0; j < 8 / WORDS; ++j)
+            col_scale[threadIdx.x * (8 / WORDS) + j] = (uint8_t)scale_of(Tops<T>::column(&top, j));
+        }
+        __syncthreads();
       }
-      __syncthreads();
-      if ((threadIdx.x & 48) == 0)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) col_top[wave][tc * 8 + j] = ct[j];
-      __syncthreads();
     }
+    float v[4][8];  // row, column
+#pragma unroll
+    for (int i = 0; i < 4; ++i) raw[i].widen(v[i]);
     if (p.codes || p.scales || p.values) {
       const int64_t scales = (e * scale_rows + (p.square ? rb : r0)) * p.blocks + cb;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        int si = p.square ? s : scale_of(max16(row_top[i]));
-        float in[8];
-        u32x2 signs = {0, 0};
-#pragma unroll
-        for (int j = 0; j < 8; ++j) in[j] = v[i][j];
-        if (p.scales_in && r0 + i < p.rows) {
-          si = p.scales_in[p.square ? scales : scales + (int64_t)i * p.blocks];
-          signs = signs8(in);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) in[j] = scaled(in[j], si);
+      for (int i = 0; i < 4; ++i) {
+        int si = s;
+        if constexpr (ENCODE) {
+          if (r0 + i < p.rows) si = p.scales_in[p.square ? scales : scales + (int64_t)i * p.blocks];
+        } else if (!p.square) {
+          Tops<T> tops;
+          tops.add(raw[i]);
+          si = scale_of(max16(tops.all()));
         }
-        const float scale = p.scales_in ? 1.f : scale_of_byte(si);
-        u32x2 w = {codes4(in[0], in[1], in[2], in[3], scale), codes4(in[4], in[5], in[6], in[7], scale)};
-        if (p.scales_in) w = (w & 0x7f7f7f7fu) | signs;
-        if (si == 255) w = u32x2{0, 0};
+        const u32x2 w = codes8<ENCODE>(v[i], si);
         if (r0 + i >= p.rows) continue;
         if (p.codes) *(u32x2*)(p.codes + ((e * p.rows + r0 + i) * p.blocks + cb) * 128 + tc * 8) = w;
         if (p.scales && tc == 0 && (!p.square || (tr == 0 && i == 0))) p.scales[p.square ? scales : scales + (int64_t)i * p.blocks] = (uint8_t)si;
@@ -252,36 +323,26 @@ __global__ void __launch_bounds__(256) fp8_quantize_tiles(Fp8QuantArgs p) {
     }
     if (p.codes_t || p.scales_t) {
       const int64_t scales = (e * scale_rows_t + (p.square ? cb : c0)) * row_tiles + rb;
-      // the last piece's readers of `turned` have passed the barriers above
+      if constexpr (ENCODE) __syncthreads();  // the last piece's readers of `turned`; else they have passed the barriers above
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        int sj = p.square ? s : scale_of(max(max(col_top[0][tc * 8 + j], col_top[1][tc * 8 + j]), max(col_top[2][tc * 8 + j], col_top[3][tc * 8 + j])));
-        float in[8];
-        u32x2 signs = {0, 0};
-#pragma unroll
-        for (int i = 0; i < 8; ++i) in[i] = v[i][j];
-        if (p.scales_in && c0 + j < p.K) {
-          sj = p.scales_in[p.square ? scales : scales + j * row_tiles];
-          signs = signs8(in);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) in[i] = scaled(in[i], sj);
+        int sj = s;
+        if constexpr (ENCODE) {
+          if (c0 + j < p.K) sj = p.scales_in[p.square ? scales : scales + j * row_tiles];
+        } else if (!p.square) {
+          sj = col_scale[tc * 8 + j];
         }
-        const float scale = p.scales_in ? 1.f : scale_of_byte(sj);
-        u32x2 w = {codes4(in[0], in[1], in[2], in[3], scale), codes4(in[4], in[5], in[6], in[7], scale)};
-        if (p.scales_in) w = (w & 0x7f7f7f7fu) | signs;
-        if (sj == 255) w = u32x2{0, 0};
-        *(u32x2*)&turned[tc * 8 + j][tr * 8] = w;
+        turned[tc * 8 + j][tr] = codes_for<ENCODE>(v[0][j], v[1][j], v[2][j], v[3][j], sj);
         if (p.scales_t && tr == 0 && c0 + j < p.K && (!p.square || (tc == 0 && j == 0)))
           p.scales_t[p.square ? scales : scales + j * row_tiles] = (uint8_t)sj;
       }
       __syncthreads();
       if (p.codes_t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int c = i * 32 + (threadIdx.x >> 3);
-          if (cb * 128 + c < p.K)
-            *(mx4::u32x4*)(p.codes_t + ((e * p.K + cb * 128 + c) * row_tiles + rb) * 128 + (threadIdx.x & 7) * 16) =
-                *(const mx4::u32x4*)&turned[c][(threadIdx.x & 7) * 16];
+        for (int i = 0; i < 2; ++i) {
+          const int c = i * 64 + (threadIdx.x >> 3), at = (threadIdx.x & 7) * 4;
+          const mx4::u32x4 line = {turned[c][at], turned[c][at + 1], turned[c][at + 2], turned[c][at + 3]};
+          if (cb * 128 + c < p.K) *(mx4::u32x4*)(p.codes_t + ((e * p.K + cb * 128 + c) * row_tiles + rb) * 128 + at * 4) = line;
         }
     }
   }

@@ -53,6 +53,8 @@ namespace fp8 {
 
 constexpr int SCALES = 64;  // blocks of a walk
 
+enum Schedule { PLAIN, PINGPONG, AHEAD };
+
 __device__ __forceinline__ int swz(int r) { return (r >> 3) & 3; }
 
 __device__ __forceinline__ gdma::f32x16 mfma(const gdma::u32x4 (&b)[2], unsigned sb, const gdma::u32x4 (&a)[2], unsigned sa, gdma::f32x16 c) {
@@ -67,15 +69,17 @@ __device__ __forceinline__ int part_begin(int blocks, int splits, int part) { re
 
 }  // namespace fp8
 
-template <bool FAST, int WGM, int WGN, int TM, int TN, int STAGES, bool PP>
+template <bool FAST, int WGM, int WGN, int TM, int TN, int STAGES, fp8::Schedule SCHEDULE>
 __global__ void __launch_bounds__(WGM* WGN * 64) fp8_dma(Fp8Args p) {
   using namespace gdma;
   constexpr int WAVES = WGM * WGN, BM = WGM * TM * 32, BN = WGN * TN * 32;
   constexpr int SLAB = 64, HALVES = FAST ? 1 : 2;  // steps of a slab
-  constexpr int A_KB = BM * SLAB / 1024, B_KB = BN * SLAB / 1024, PER = (A_KB + B_KB) / WAVES;  // DMA kilobytes
+  constexpr int A_KB = BM * SLAB / 1024, B_KB = BN * SLAB / 1024;  // DMA kilobytes
+  constexpr int A_PER = A_KB / WAVES, B_PER = B_KB / WAVES, PER = A_PER + B_PER;
   constexpr int B_AT = BM * SLAB, STAGE = B_AT + BN * SLAB;
-  constexpr int D = STAGES - 1;
-  static_assert(PER * WAVES == A_KB + B_KB && A_KB % PER == 0 && PER % 2 == 0, "a slab splits evenly over the waves, one operand each");
+  constexpr bool PP = SCHEDULE == fp8::PINGPONG, RP = SCHEDULE == fp8::AHEAD;
+  constexpr int D = RP ? STAGES : STAGES - 1;  // slabs on their way before the first is waited for
+  static_assert(A_PER * WAVES == A_KB && B_PER * WAVES == B_KB, "a slab splits evenly over the waves");
   static_assert(!PP || (WGM == 2 && WGN == 4), "two groups of four waves");
   static_assert(STAGES == 4, "a slab's half of its block follows from its stage");
   static_assert(STAGES * STAGE + (BM + BN) * fp8::SCALES <= 160 * 1024 && D * PER < 64, "LDS and wait counts");
@@ -101,19 +105,17 @@ __global__ void __launch_bounds__(WGM* WGN * 64) fp8_dma(Fp8Args p) {
   const int block0 = fp8::part_begin(p.blocks, p.splits, part), block1 = fp8::part_begin(p.blocks, p.splits, part + 1);
   const int ld = 128 * p.blocks;
 
-  // ---- this wave's share of a slab's DMA: PER kilobytes of one operand
-  const bool is_a = wave * PER < A_KB;
-  const int kb0 = is_a ? wave * PER : wave * PER - A_KB;
-  const int lines = is_a ? rows : cols;
-  const uint64_t corner = (uint64_t)(is_a ? p.a + (int64_t)m0 * ld : p.b + (int64_t)n0 * ld);
+  // ---- this wave's share of a slab's DMA: A_PER kilobytes of A, B_PER of B
   // a lane's 16 bytes of KB i: the pattern repeats after two KB (32 rows)
-  unsigned off[2];
+  const int a_kb = wave * A_PER, b_kb = wave * B_PER;
+  unsigned a_off[2], b_off[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const int r = (kb0 + i) * 16 + lane / 4;
-    off[i] = (unsigned)r * (unsigned)ld + (unsigned)(((lane % 4) ^ fp8::swz(r)) * 16);
+    const int ra = (a_kb + i) * 16 + lane / 4, rb = (b_kb + i) * 16 + lane / 4;
+    a_off[i] = (unsigned)ra * (unsigned)ld + (unsigned)(((lane % 4) ^ fp8::swz(ra)) * 16);
+    b_off[i] = (unsigned)rb * (unsigned)ld + (unsigned)(((lane % 4) ^ fp8::swz(rb)) * 16);
   }
-  const unsigned lds0 = __builtin_amdgcn_readfirstlane(lds_address(lds)), share = (unsigned)((is_a ? 0 : B_AT) + kb0 * 1024);
+  const unsigned lds0 = __builtin_amdgcn_readfirstlane(lds_address(lds));
 
   f32x16 acc[TM][TN];
 #pragma unroll
@@ -126,18 +128,24 @@ __global__ void __launch_bounds__(WGM* WGN * 64) fp8_dma(Fp8Args p) {
     // K stagger, in whole reads of scales (8 slabs): tiles that share a panel start
     // their walk at different slabs
     const int kofs = ((mt + 2 * nt) & 15) * 8 % nk & ~7;
-    Walk<true, SLAB> walk;
-    walk.start = corner + (uint64_t)128 * first;
-    walk.step = SLAB;
-    walk.width = (unsigned)(lines - 1) * (unsigned)ld + 128u * (unsigned)blocks;
-    walk.slab = kofs, walk.slabs = walk.left = nk;
-    walk.at = walk.start + (uint64_t)kofs * SLAB;
+    auto walk_of = [&](const uint8_t* operand, int row, int lines) {
+      Walk<true, SLAB> w;
+      w.start = (uint64_t)(operand + (int64_t)row * ld) + (uint64_t)128 * first;
+      w.step = SLAB;
+      w.width = (unsigned)(lines - 1) * (unsigned)ld + 128u * (unsigned)blocks;
+      w.slab = kofs, w.slabs = w.left = nk;
+      w.at = w.start + (uint64_t)kofs * SLAB;
+      return w;
+    };
+    Walk<true, SLAB> walk_a = walk_of(p.a, m0, rows), walk_b = walk_of(p.b, n0, cols);
     auto issue = [&](const int stage) {
-      const unsigned at = lds0 + share + stage * STAGE;
+      const unsigned at = lds0 + stage * STAGE;
       int step = 32 * ld;  // opaque: the sums of a lane's offsets would fill the registers
       asm volatile("" : "+s"(step));
-      const u32x4 r = walk.next();
-      each_stage<PER>([&](auto i) { dma16<i == 0, i * 1024>(r, off[i % 2] + (unsigned)(i / 2) * (unsigned)step, at); });
+      const u32x4 ra = walk_a.next();
+      each_stage<A_PER>([&](auto i) { dma16<i == 0, i * 1024>(ra, a_off[i % 2] + (unsigned)(i / 2) * (unsigned)step, at + a_kb * 1024); });
+      const u32x4 rb = walk_b.next();
+      each_stage<B_PER>([&](auto i) { dma16<i == 0, i * 1024>(rb, b_off[i % 2] + (unsigned)(i / 2) * (unsigned)step, at + B_AT + b_kb * 1024); });
     };
 
     if (first != block0) __syncthreads();  // everyone is done with the last walk
@@ -261,6 +269,74 @@ __global__ void __launch_bounds__(WGM* WGN * 64) fp8_dma(Fp8Args p) {
       };
       for (int kt = 0; kt < nk; kt += STAGES) each_stage<STAGES>([&](auto s) { if (kt + s < nk) step(s); });
       if (group == 0) phase_barrier();
+    } else if constexpr (RP) {
+      static_assert(!RP || FAST, "the codes go into the matrix instructions as they are");
+      u32x4 na[2][TM][2], nb[2][TN][2];  // this slab's fragments and the next one's
+      auto scales = [&] {
+        const unsigned char* const ss = lds_s + (at >> 1 & 12);
+        const int q = at >> 5;
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+          const int r = (wm * TM + i) * 32 + l32;
+          ha[i] = *(const unsigned*)(ss + r * fp8::SCALES + 16 * (q ^ fp8::swz(r)));
+        }
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          const int r = BM + (wn * TN + j) * 32 + l32;
+          hb[j] = *(const unsigned*)(ss + r * fp8::SCALES + 16 * (q ^ fp8::swz(r)));
+        }
+      };
+      auto fetch = [&](u32x4 (&ta)[TM][2], u32x4 (&tb)[TN][2], const unsigned char* st) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const unsigned char* const at_row = st + l32 * SLAB + 16 * ((2 * half + h) ^ fp8::swz(l32));
+#pragma unroll
+          for (int i = 0; i < TM; ++i) ta[i][h] = *(const lds_u32x4*)(at_row + (wm * TM + i) * 32 * SLAB);
+#pragma unroll
+          for (int j = 0; j < TN; ++j) tb[j][h] = *(const lds_u32x4*)(at_row + B_AT + (wn * TN + j) * 32 * SLAB);
+        }
+      };
+      __builtin_amdgcn_s_waitcnt(waitcnt_vm((D - 1) * PER));
+      phase_barrier();
+      scales();
+      fetch(na[0], nb[0], lds);
+      auto step = [&](auto stage) {
+        constexpr int s = decltype(stage)::value, cur = s % 2;
+        // everyone has this slab in registers, its stage is free, and the next slab has landed
+        __builtin_amdgcn_s_waitcnt(waitcnt_lgkm0());
+        __builtin_amdgcn_s_waitcnt(waitcnt_vm((D - 2) * PER));
+        phase_barrier();
+        issue(s);
+        fetch(na[1 - cur], nb[1 - cur], lds + (s + 1) % STAGES * STAGE);
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int j = 0; j < TN; ++j) acc[i][j] = fp8::mfma(nb[cur][j], hb[j], na[cur][i], ha[i], acc[i][j]);
+#pragma unroll
+        for (int i = 0; i < TM * TN; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);  // a matrix instruction
+          if (i < 2 * (TM + TN)) __builtin_amdgcn_sched_group_barrier(0x100, (2 * (TM + TN) + TM * TN - 1) / (TM * TN), 0);  // reads of LDS
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        // the sums stay in this step: they would sink past the branch below and the next barrier
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int j = 0; j < TN; ++j) asm volatile("" : "+a"(acc[i][j]));
+        ++at;
+        if (s % 2 == 1) {
+#pragma unroll
+          for (int i = 0; i < TM; ++i) ha[i] >>= 8;
+#pragma unroll
+          for (int j = 0; j < TN; ++j) hb[j] >>= 8;
+          if (at == nk) at = 0;
+          if ((at & 7) == 0) scales();
+        }
+      };
+      // an even number of slabs.  No branch inside: matrix instructions would sink past it
+      int kt = 0;
+      for (; kt + STAGES <= nk; kt += STAGES) each_stage<STAGES>(step);
+      if (kt < nk) each_stage<2>(step);
     } else {
       auto step = [&](auto stage) {
         constexpr int s = decltype(stage)::value;

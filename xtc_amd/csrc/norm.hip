@@ -12,6 +12,7 @@ namespace {
 constexpr int kMost = 0x7fffffff - 16383;  // of K: a walk's step past it stays within 32 bits
 constexpr int kLong = 16384;               // elements of a row that registers hold
 constexpr int64_t kMostGroups = 1 << 20;   // of a launch: its threads stay within 32 bits
+constexpr int64_t kWalks = 1024;           // workgroups of 256 threads that walk over the rows: four a CU
 constexpr int kMostParts = XTC_HIP_LAYER_NORM_PARTS;
 
 int check(const xtc_hip_layer_norm_desc* d, const char* what) {
@@ -42,14 +43,24 @@ NormArgs args_of(const xtc_hip_layer_norm_desc& d, const void* x, const void* w)
   return a;
 }
 
-// Threads that share a row: as few as hold it in two runs of 8 elements each.
-int threads_of(int K) { return K <= 1024 ? 64 : K <= 4096 ? 256 : 1024; }
+// Threads that share a row: as few as hold it in two runs of 8 elements each; the backward
+// pass, whose registers then leave two workgroups a CU little to run, in one run from 2048
+// elements to 4096.
+int threads_of(int K, bool grad) { return K <= 1024 ? 64 : K <= (grad ? 2048 : 4096) ? 256 : grad && K <= 4096 ? 512 : 1024; }
 
 template <typename T, typename P, int THREADS, int VECS>
 void run_rows(const NormArgs& a, bool grad, unsigned groups, hipStream_t s) {
   const dim3 threads(THREADS < 256 ? 256 : THREADS);
   if (grad) hipLaunchKernelGGL((layer_norm_grad<T, P, THREADS, VECS>), dim3(groups), threads, 0, s, a);
   else hipLaunchKernelGGL((layer_norm<T, P, THREADS, VECS>), dim3(groups), threads, 0, s, a);
+}
+template <typename T, typename P, int THREADS, int VECS>
+void run_forward(const NormArgs& a, unsigned groups, hipStream_t s) {
+  hipLaunchKernelGGL((layer_norm<T, P, THREADS, VECS>), dim3(groups), dim3(THREADS), 0, s, a);
+}
+template <typename T, typename P, int THREADS, int VECS>
+void run_grad(const NormArgs& a, unsigned groups, hipStream_t s) {
+  hipLaunchKernelGGL((layer_norm_grad<T, P, THREADS, VECS>), dim3(groups), dim3(THREADS), 0, s, a);
 }
 
 template <typename T, typename P>
@@ -59,10 +70,11 @@ void run(const NormArgs& a, bool grad, unsigned groups, hipStream_t s) {
     else hipLaunchKernelGGL((layer_norm_long<T, P, false>), dim3(groups), dim3(1024), 0, s, a);
     return;
   }
-  const int threads = threads_of(a.K);
+  const int threads = threads_of(a.K, grad);
   const bool one = a.K <= 8 * threads;
   if (threads == 64) return one ? run_rows<T, P, 64, 1>(a, grad, groups, s) : run_rows<T, P, 64, 2>(a, grad, groups, s);
-  if (threads == 256) return one ? run_rows<T, P, 256, 1>(a, grad, groups, s) : run_rows<T, P, 256, 2>(a, grad, groups, s);
+  if (threads == 256) return one ? run_rows<T, P, 256, 1>(a, grad, groups, s) : run_forward<T, P, 256, 2>(a, groups, s);
+  if (threads == 512) return run_grad<T, P, 512, 1>(a, groups, s);
   return one ? run_rows<T, P, 1024, 1>(a, grad, groups, s) : run_rows<T, P, 1024, 2>(a, grad, groups, s);
 }
 
@@ -92,8 +104,8 @@ int xtc_hip_layer_norm(const xtc_hip_layer_norm_desc* desc, const void* x, const
   if (!x || !y) return fail("%s: null operand", what);
   NormArgs a = args_of(*desc, x, w);
   a.b = b, a.y = y;
-  const int64_t groups = a.K > 1024 ? a.rows : (a.rows + 3) / 4;
-  launch(*desc, a, false, (unsigned)(groups < kMostGroups ? groups : kMostGroups));
+  const int64_t groups = a.K > 1024 ? a.rows : (a.rows + 3) / 4, most = a.K > kLong ? kMostGroups : a.K > 4096 ? 512 : kWalks;
+  launch(*desc, a, false, (unsigned)(groups < most ? groups : most));
   return done(what);
 }
 

@@ -42,18 +42,27 @@ namespace norm {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
+// 8 elements as stored
+template <typename T>
+struct Raw8 {
+  T v[8];
+};
 // the first n of the 8 elements at p, zeros for the others
 template <typename T>
-__device__ __forceinline__ void load8(float (&v)[8], const T* p, int n) {
-  T raw[8];
+__device__ __forceinline__ void load8(Raw8<T>& r, const T* p, int n) {
   if (n >= 8) {
-    __builtin_memcpy(raw, p, sizeof(raw));
+    __builtin_memcpy(&r, p, sizeof(r));
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) raw[i] = i < n ? p[i] : (T)0.f;
+    for (int i = 0; i < 8; ++i) r.v[i] = i < n ? p[i] : (T)0.f;
   }
+}
+template <typename T>
+__device__ __forceinline__ void load8(float (&v)[8], const T* p, int n) {
+  Raw8<T> r;
+  load8(r, p, n);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = (float)raw[i];
+  for (int i = 0; i < 8; ++i) v[i] = (float)r.v[i];
 }
 
 template <typename T>
@@ -97,25 +106,35 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) layer_norm(Norm
   constexpr int ROWS = THREADS < 256 ? 256 / THREADS : 1;
   __shared__ float lds[2][2 * (THREADS / 64)];
   const int t = threadIdx.x % THREADS;
-  // uniform over the threads of a row: with THREADS > 64 over the workgroup
-  for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / THREADS; row < p.rows; row += (int64_t)gridDim.x * ROWS) {
-    float v[VECS][8], w[VECS][8], b[VECS][8];
-    float sum = 0.f, none = 0.f;
+  const int64_t step = (int64_t)gridDim.x * ROWS;
+  Raw8<T> raw[VECS];
+  auto load = [&](int64_t row) {
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
       const int k = (i * THREADS + t) * 8;
-      load8(v[i], (const T*)p.x + row * p.ldx + k, p.K - k);
+      load8(raw[i], (const T*)p.x + row * p.ldx + k, p.K - k);
     }
+  };
+  int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / THREADS;
+  if (row < p.rows) load(row);
+  float w[VECS][8], b[VECS][8];
 #pragma unroll
-    for (int i = 0; i < VECS; ++i) {  // ahead of the sums' latency
-      const int k = (i * THREADS + t) * 8;
-      if (p.w) load8(w[i], (const P*)p.w + k, p.K - k);
-      if (p.b) load8(b[i], (const P*)p.b + k, p.K - k);
-    }
+  for (int i = 0; i < VECS; ++i) {
+    const int k = (i * THREADS + t) * 8;
+    if (p.w) load8(w[i], (const P*)p.w + k, p.K - k);
+    if (p.b) load8(b[i], (const P*)p.b + k, p.K - k);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[i][j] = p.w ? w[i][j] : 1.f, b[i][j] = p.b ? b[i][j] : 0.f;
+  }
+  // uniform over the threads of a row: with THREADS > 64 over the workgroup
+  for (; row < p.rows; row += step) {
+    float v[VECS][8];
+    float sum = 0.f, none = 0.f;
 #pragma unroll
     for (int i = 0; i < VECS; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sum += v[i][j];
+      for (int j = 0; j < 8; ++j) v[i][j] = (float)raw[i].v[j], sum += v[i][j];
+    if (row + step < p.rows) load(row + step);
     row_sums<THREADS>(sum, none, lds[0]);
     const float mean = sum / (float)p.K;
     float var = 0.f;
@@ -133,7 +152,7 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) layer_norm(Norm
       const int k = (i * THREADS + t) * 8;
       float out[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) out[j] = v[i][j] * r * (p.w ? w[i][j] : 1.f) + (p.b ? b[i][j] : 0.f);
+      for (int j = 0; j < 8; ++j) out[j] = v[i][j] * r * w[i][j] + b[i][j];
       store8((T*)p.y + row * p.ldy + k, out, p.K - k);
     }
   }
@@ -159,20 +178,32 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) layer_norm_grad
     for (int j = 0; j < 8; ++j) dw[i][j] = db[i][j] = 0.f, w[i][j] = p.w ? w[i][j] : 1.f;
   }
   const float inv = 1.0f / (float)p.K;
-  // uniform over the threads of a row: with THREADS > 64 over the workgroup
-  for (int64_t row = (int64_t)blockIdx.x * ROWS + sub; row < p.rows; row += step) {
-    float x[VECS][8], dy[VECS][8];
-    float sum_x = 0.f, sum_g = 0.f;
+  Raw8<T> raw_x[VECS], raw_dy[VECS];
+  auto load = [&](int64_t row) {
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
       const int k = (i * THREADS + t) * 8;
-      load8(x[i], (const T*)p.x + row * p.ldx + k, p.K - k);
-      load8(dy[i], (const T*)p.dy + row * p.ldy + k, p.K - k);
+      load8(raw_x[i], (const T*)p.x + row * p.ldx + k, p.K - k);
+      load8(raw_dy[i], (const T*)p.dy + row * p.ldy + k, p.K - k);
     }
+  };
+  // the next row's loads are on their way during the sums of this one, where registers last
+  constexpr bool AHEAD = THREADS * VECS <= 1024;
+  int64_t row = (int64_t)blockIdx.x * ROWS + sub;
+  if (AHEAD && row < p.rows) load(row);
+  // uniform over the threads of a row: with THREADS > 64 over the workgroup
+  for (; row < p.rows; row += step) {
+    float x[VECS][8], dy[VECS][8];
+    float sum_x = 0.f, sum_g = 0.f;
+    if (!AHEAD) load(row);
 #pragma unroll
     for (int i = 0; i < VECS; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sum_x += x[i][j], sum_g += dy[i][j] * w[i][j];
+      for (int j = 0; j < 8; ++j) {
+        x[i][j] = (float)raw_x[i].v[j], dy[i][j] = (float)raw_dy[i].v[j];
+        sum_x += x[i][j], sum_g += dy[i][j] * w[i][j];
+      }
+    if (AHEAD && row + step < p.rows) load(row + step);
     row_sums<THREADS>(sum_x, sum_g, lds[0]);
     const float mean = sum_x / (float)p.K;
     float var = 0.f, cov = 0.f;

@@ -81,11 +81,18 @@ template <bool FAST, int WGM, int WGN, int TM, int TN, fp8::Schedule S>
 void dma_launch(const Fp8Args& a, unsigned groups, hipStream_t s) {
   hipLaunchKernelGGL((fp8_dma<FAST, WGM, WGN, TM, TN, 4, S>), dim3(groups), dim3(WGM * WGN * 64), 0, s, a);
 }
+// Microseconds a block, a CU with one workgroup and with all it takes, measured (us, the
+// three tiles in this order; M x N x k):
+//   to bf16:  4096 x 4096 x 2048  43, 48, 72    4096 x 2048 x 4096  68, 45, 76    2048 x 2048 x 2048  40, 17, 23
+//             512 x 4096 x 4096  54, 26, 23    1024 x 1024 x 8192  98, 52, 33    8192 x 8192 x 4096  250, 322, 502
+//   to fp32:  4096 x 4096 x 2048  80, 81, 100   4096 x 2048 x 4096  111, 73, 97   2048 x 2048 x 2048  56, 29, 30
+//             512 x 4096 x 4096  88, 40, 31    1024 x 1024 x 8192  167, 78, 44   8192 x 8192 x 4096  469, 497, 680
+// fp32 results are bound by the conversions, which take longer than the products: a
+// schedule of fragments read ahead and 256 x 128 tiles made 4096 x 2048 x 4096 no faster (79).
 const DmaTile kDmaTiles[] = {
-    {{{256, 256, 1, 2.5, 3.0}, {256, 256, 1, 1.25, 1.60}}, {&dma_launch<false, 2, 4, 4, 2, fp8::PINGPONG>, &dma_launch<true, 2, 2, 4, 4, fp8::AHEAD>}},
-    {{{256, 128, 1, 2.5, 3.0}, {256, 128, 1, 0.4, 1.40}}, {&dma_launch<false, 2, 2, 4, 2, fp8::PLAIN>, &dma_launch<true, 2, 2, 4, 2, fp8::AHEAD>}},
-    {{{128, 128, 2, 1.4, 2.2}, {128, 128, 2, 0.73, 1.20}}, {&dma_launch<false, 2, 2, 2, 2, fp8::PLAIN>, &dma_launch<true, 2, 2, 2, 2, fp8::PLAIN>}},
-    {{{64, 64, 4, 0.80, 1.50}, {64, 64, 4, 0.40, 0.80}}, {&dma_launch<false, 2, 2, 1, 1, fp8::PLAIN>, &dma_launch<true, 2, 2, 1, 1, fp8::PLAIN>}},
+    {{{256, 256, 1, 2.4, 3.3}, {256, 256, 1, 1.3, 1.8}}, {&dma_launch<false, 2, 4, 4, 2, fp8::PINGPONG>, &dma_launch<true, 2, 2, 4, 4, fp8::AHEAD>}},
+    {{{128, 128, 2, 1.0, 1.85}, {128, 128, 2, 0.6, 1.2}}, {&dma_launch<false, 2, 2, 2, 2, fp8::PLAIN>, &dma_launch<true, 2, 2, 2, 2, fp8::PLAIN>}},
+    {{{64, 64, 4, 0.55, 1.3}, {64, 64, 4, 0.4, 1.0}}, {&dma_launch<false, 2, 2, 1, 1, fp8::PLAIN>, &dma_launch<true, 2, 2, 1, 1, fp8::PLAIN>}},
 };
 
 struct RowsTile {
@@ -131,8 +138,8 @@ int product(const xtc_hip_fp8_matmul_desc& d, Fp8Args& a, const char* what) {
   }
   a.tiles_m = (int)tiles_of(d.M, best->cost[0].bm), a.tiles_n = (int)tiles_of(d.N, best->cost[0].bn);
   a.band = a.tiles_m < 8 ? a.tiles_m : 8;
-  const int64_t per_part = ((int64_t)a.tiles_m + a.band - 1) / a.band * a.band * a.tiles_n, whole = (int64_t)8 * 4 * a.band;
-  const int64_t groups = (a.splits * per_part + whole - 1) / whole * whole;
+  const int64_t tiles = ((int64_t)a.tiles_m + a.band - 1) / a.band * a.band * a.tiles_n, whole = (int64_t)8 * 4 * a.band;
+  const int64_t groups = (tiles + whole - 1) / whole * whole;
   if (groups >= (int64_t)1 << 22) return fail("%s: %lld workgroups are too many", what, (long long)groups);
   best->launch[a.out16](a, (unsigned)groups, s);
   return done(what);
@@ -208,7 +215,7 @@ int xtc_hip_fp8_matmul(const xtc_hip_fp8_matmul_desc* desc, const uint8_t* a_cod
   Fp8Args a{};
   a.a = a_codes, a.sa = a_scales, a.b = b_codes, a.sb = b_scales, a.c = c;
   a.M = desc->M, a.N = desc->N, a.blocks = desc->blocks, a.ldc = desc->ldc ? desc->ldc : desc->N;
-  a.b_shift = desc->b_block_rows == 128 ? 7 : 0, a.splits = 1, a.out16 = desc->out_dtype == XTC_HIP_BF16;
+  a.b_shift = desc->b_block_rows == 128 ? 7 : 0, a.out16 = desc->out_dtype == XTC_HIP_BF16;
   return product(*desc, a, what);
 }
 

@@ -29,10 +29,16 @@
 // blocks' bytes of its rows at once.  A walk ends after SCALES blocks (8192 elements)
 // and the next begins.
 //
-// Schedules: PP and the plain one as in grouped_dma.hpp.
+// Schedules.  PLAIN: a barrier a slab, two or more workgroups a CU cover each other's
+// waits.  AHEAD (256 x 256, FAST): four waves of 128 x 128, one a SIMD with all of its
+// registers, read the next slab's fragments between this one's matrix instructions: two
+// thirds of the LDS reads of eight waves of 128 x 64.  PINGPONG, as in grouped_dma.hpp:
+// eight waves, one of a SIMD's two computes while the other reads and converts.  At 8192 x
+// 8192 x 8192 to bf16 AHEAD takes 483 us (2.3 PFLOP/s), PINGPONG 511; to fp32 conversions
+// need the second wave.
 //
-// Few tiles: the blocks are shared out over `splits` workgroups a tile, whose fp32
-// sums a second kernel adds up in order.
+// The tiles walk k in step.  With the walks staggered, which spreads the first loads over
+// the memory channels, an XCD's L2 no longer holds what its tiles share: 600 us.
 #pragma once
 #include "grouped_dma.hpp"
 
@@ -42,10 +48,9 @@ struct Fp8Args {
   const uint8_t *a, *b;    // codes [M], [N] rows of 128 blocks bytes
   const uint8_t *sa, *sb;  // scales [M][blocks]; [N][blocks] or [ceil(N / 128)][blocks]
   void* c;
-  float* partial;          // splits > 1: [splits][M][N]
   int M, N, blocks, ldc;
   int b_shift;             // log2 of the rows of b that share a scale
-  int tiles_m, tiles_n, band, splits;
+  int tiles_m, tiles_n, band;
   int out16;               // C is bf16
 };
 
@@ -63,9 +68,6 @@ __device__ __forceinline__ gdma::f32x16 mfma(const gdma::u32x4 (&b)[2], unsigned
   const i32x8 av = {(int)a[0][0], (int)a[0][1], (int)a[0][2], (int)a[0][3], (int)a[1][0], (int)a[1][1], (int)a[1][2], (int)a[1][3]};
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(bv, av, c, 0, 0, 0, (int)sb, 0, (int)sa);
 }
-
-// the blocks of part `part` of `splits`
-__device__ __forceinline__ int part_begin(int blocks, int splits, int part) { return (int)((int64_t)blocks * part / splits); }
 
 }  // namespace fp8
 
@@ -95,14 +97,11 @@ __global__ void __launch_bounds__(WGM* WGN * 64) fp8_dma(Fp8Args p) {
   // ---- the workgroup's tile, bands and XCDs as in grouped_dma
   const int slot = blockIdx.x >> 3, run = 4 * p.band;
   const int t = (slot / run * 8 + (blockIdx.x & 7)) * run + slot % run;
-  const int per_part = (p.tiles_m + p.band - 1) / p.band * p.band * p.tiles_n;
-  const int part = t / per_part, tt = t - part * per_part;
-  const int in_band = tt % (p.band * p.tiles_n);
-  const int mt = tt / (p.band * p.tiles_n) * p.band + in_band % p.band, nt = in_band / p.band;
-  if (mt >= p.tiles_m || part >= p.splits) return;
+  const int in_band = t % (p.band * p.tiles_n);
+  const int mt = t / (p.band * p.tiles_n) * p.band + in_band % p.band, nt = in_band / p.band;
+  if (mt >= p.tiles_m) return;
   const int m0 = mt * BM, n0 = nt * BN;
   const int rows = min(p.M - m0, BM), cols = min(p.N - n0, BN);
-  const int block0 = fp8::part_begin(p.blocks, p.splits, part), block1 = fp8::part_begin(p.blocks, p.splits, part + 1);
   const int ld = 128 * p.blocks;
 
   // ---- this wave's share of a slab's DMA: A_PER kilobytes of A, B_PER of B
@@ -123,18 +122,15 @@ __global__ void __launch_bounds__(WGM* WGN * 64) fp8_dma(Fp8Args p) {
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = f32x16{};
 
-  for (int first = block0; first < block1; first += fp8::SCALES) {
-    const int blocks = min(block1 - first, fp8::SCALES), nk = 2 * blocks;
-    // K stagger, in whole reads of scales (8 slabs): tiles that share a panel start
-    // their walk at different slabs
-    const int kofs = ((mt + 2 * nt) & 15) * 8 % nk & ~7;
+  for (int first = 0; first < p.blocks; first += fp8::SCALES) {
+    const int blocks = min(p.blocks - first, fp8::SCALES), nk = 2 * blocks;
     auto walk_of = [&](const uint8_t* operand, int row, int lines) {
       Walk<true, SLAB> w;
       w.start = (uint64_t)(operand + (int64_t)row * ld) + (uint64_t)128 * first;
       w.step = SLAB;
       w.width = (unsigned)(lines - 1) * (unsigned)ld + 128u * (unsigned)blocks;
-      w.slab = kofs, w.slabs = w.left = nk;
-      w.at = w.start + (uint64_t)kofs * SLAB;
+      w.slab = 0, w.slabs = w.left = nk;
+      w.at = w.start;
       return w;
     };
     Walk<true, SLAB> walk_a = walk_of(p.a, m0, rows), walk_b = walk_of(p.b, n0, cols);
@@ -148,7 +144,7 @@ __global__ void __launch_bounds__(WGM* WGN * 64) fp8_dma(Fp8Args p) {
       each_stage<B_PER>([&](auto i) { dma16<i == 0, i * 1024>(rb, b_off[i % 2] + (unsigned)(i / 2) * (unsigned)step, at + B_AT + b_kb * 1024); });
     };
 
-    if (first != block0) __syncthreads();  // everyone is done with the last walk
+    if (first) __syncthreads();  // everyone is done with the last walk
     each_stage<D>([&](auto s) { issue(s); });
     // ---- the walk's scales: rows past the edge keep what was there, no one stores theirs
     for (int r = threadIdx.x; r < BM + BN; r += 64 * WAVES) {
@@ -173,7 +169,12 @@ __global__ void __launch_bounds__(WGM* WGN * 64) fp8_dma(Fp8Args p) {
 
     u32x4 fa[TM][2], fb[TN][2];  // FAST: codes of 32 elements; otherwise 16 of them in bf16
     unsigned ha[TM], hb[TN];     // scales of this lane's rows, four blocks
-    int at = kofs;               // slab of the operand
+    int at = 0;                  // slab of the walk
+    auto convert = [](u32x4 (&to)[2], u32x4 v, unsigned h) {
+      const float scale = fp8::scale_of_byte(h & 255);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) to[c] = __builtin_bit_cast(u32x4, fp8::values_bf16(v[2 * c], v[2 * c + 1], scale));
+    };
     auto read = [&](const int s, const int hf, const unsigned char* st) {
       if (s % 2 == 0 && hf == 0) {
         if ((at & 7) == 0) {
@@ -207,11 +208,6 @@ __global__ void __launch_bounds__(WGM* WGN * 64) fp8_dma(Fp8Args p) {
         for (int i = 0; i < TM; ++i) ra[i] = *(const lds_u32x4*)(at_row + (wm * TM + i) * 32 * SLAB);
 #pragma unroll
         for (int j = 0; j < TN; ++j) rb[j] = *(const lds_u32x4*)(at_row + B_AT + (wn * TN + j) * 32 * SLAB);
-        auto convert = [](u32x4 (&to)[2], u32x4 v, unsigned h) {
-          const float scale = fp8::scale_of_byte(h & 255);
-#pragma unroll
-          for (int c = 0; c < 2; ++c) to[c] = __builtin_bit_cast(u32x4, fp8::values_bf16(v[2 * c], v[2 * c + 1], scale));
-        };
 #pragma unroll
         for (int i = 0; i < TM; ++i) convert(fa[i], ra[i], ha[i]);
 #pragma unroll
@@ -238,7 +234,6 @@ __global__ void __launch_bounds__(WGM* WGN * 64) fp8_dma(Fp8Args p) {
         for (int i = 0; i < TM; ++i) ha[i] >>= 8;
 #pragma unroll
         for (int j = 0; j < TN; ++j) hb[j] >>= 8;
-        if (at == nk) at = 0;
       }
     };
 
@@ -270,7 +265,6 @@ __global__ void __launch_bounds__(WGM* WGN * 64) fp8_dma(Fp8Args p) {
       for (int kt = 0; kt < nk; kt += STAGES) each_stage<STAGES>([&](auto s) { if (kt + s < nk) step(s); });
       if (group == 0) phase_barrier();
     } else if constexpr (RP) {
-      static_assert(!RP || FAST, "the codes go into the matrix instructions as they are");
       u32x4 na[2][TM][2], nb[2][TN][2];  // this slab's fragments and the next one's
       auto scales = [&] {
         const unsigned char* const ss = lds_s + (at >> 1 & 12);
@@ -308,14 +302,40 @@ __global__ void __launch_bounds__(WGM* WGN * 64) fp8_dma(Fp8Args p) {
         phase_barrier();
         issue(s);
         fetch(na[1 - cur], nb[1 - cur], lds + (s + 1) % STAGES * STAGE);
+        constexpr int READS = 2 * (TM + TN);  // of LDS
+        if constexpr (FAST) {
 #pragma unroll
-        for (int i = 0; i < TM; ++i)
+          for (int i = 0; i < TM; ++i)
 #pragma unroll
-          for (int j = 0; j < TN; ++j) acc[i][j] = fp8::mfma(nb[cur][j], hb[j], na[cur][i], ha[i], acc[i][j]);
+            for (int j = 0; j < TN; ++j) acc[i][j] = fp8::mfma(nb[cur][j], hb[j], na[cur][i], ha[i], acc[i][j]);
 #pragma unroll
-        for (int i = 0; i < TM * TN; ++i) {
-          __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);  // a matrix instruction
-          if (i < 2 * (TM + TN)) __builtin_amdgcn_sched_group_barrier(0x100, (2 * (TM + TN) + TM * TN - 1) / (TM * TN), 0);  // reads of LDS
+          for (int i = 0; i < TM * TN; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);  // a matrix instruction
+            __builtin_amdgcn_sched_group_barrier(0x100, (READS + TM * TN - 1) / (TM * TN), 0);  // reads of LDS
+          }
+        } else {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int i = 0; i < TM; ++i) convert(fa[i], na[cur][i][h], ha[i]);
+#pragma unroll
+            for (int j = 0; j < TN; ++j) convert(fb[j], nb[cur][j][h], hb[j]);
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+              for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j)
+                  acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, fb[j][c]), __builtin_bit_cast(bf16x8, fa[i][c]), acc[i][j], 0, 0, 0);
+          }
+          // the second half's conversions run beside the first half's products
+          __builtin_amdgcn_sched_group_barrier(0x2, 8 * (TM + TN), 0);
+#pragma unroll
+          for (int i = 0; i < 4 * TM * TN; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x2, 4, 0);  // arithmetic
+            if (i < READS) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+          }
         }
         __builtin_amdgcn_sched_barrier(0);
         // the sums stay in this step: they would sink past the branch below and the next barrier
@@ -329,8 +349,7 @@ __global__ void __launch_bounds__(WGM* WGN * 64) fp8_dma(Fp8Args p) {
           for (int i = 0; i < TM; ++i) ha[i] >>= 8;
 #pragma unroll
           for (int j = 0; j < TN; ++j) hb[j] >>= 8;
-          if (at == nk) at = 0;
-          if ((at & 7) == 0) scales();
+            if ((at & 7) == 0) scales();
         }
       };
       // an even number of slabs.  No branch inside: matrix instructions would sink past it
@@ -357,57 +376,44 @@ __global__ void __launch_bounds__(WGM* WGN * 64) fp8_dma(Fp8Args p) {
     __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
   }
 
+  // the sums are read behind branches: their wait states are spelled out
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_nop 15\n\ts_nop 15");
+  __builtin_amdgcn_sched_barrier(0);
+
   // ---- a lane holds C[m][n .. n+3] for n, n+8, n+16 and n+24 of each 32 x 32
-  const bool to_part = p.splits > 1;
-  void* const c = to_part ? (void*)(p.partial + (size_t)part * p.M * p.N) : p.c;
-  const int ldc = to_part ? p.N : p.ldc, out16 = to_part ? 0 : p.out16;
+  void* const c = p.c;
+  const int ldc = p.ldc, out16 = p.out16;
   const bool whole = (ldc & 3) == 0 && ((uintptr_t)c & (out16 ? 7 : 15)) == 0;
+  const bool wide = out16 && (ldc & 7) == 0 && ((uintptr_t)c & 15) == 0;
+  auto pair16 = [](float lo, float hi) { return __builtin_bit_cast(unsigned, fp8::bf16x2{(__bf16)lo, (__bf16)hi}); };
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
     const int m = (wm * TM + i) * 32 + l32;
     if (m >= rows) continue;
     const int64_t at = (int64_t)(m0 + m) * ldc + n0;
 #pragma unroll
-    for (int j = 0; j < TN; ++j)
+    for (int j = 0; j < TN; ++j) {
+      if (wide && n0 + (wn * TN + j) * 32 + 32 <= p.N) {
+        // the two halves of the wave swap runs: eight neighbouring columns a lane
+#pragma unroll
+        for (int q = 0; q < 4; q += 2) {
+          u32x4 v;
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            const auto got = __builtin_amdgcn_permlane32_swap(pair16(acc[i][j][4 * q + 2 * w], acc[i][j][4 * q + 2 * w + 1]),
+                                                              pair16(acc[i][j][4 * q + 4 + 2 * w], acc[i][j][4 * q + 5 + 2 * w]), false, false);
+            v[w] = got[0], v[2 + w] = got[1];
+          }
+          *(u32x4*)((__bf16*)c + at + (wn * TN + j) * 32 + 8 * q + 8 * half) = v;
+        }
+        continue;
+      }
 #pragma unroll
       for (int q = 0; q < 4; ++q)
         store4(c, out16, at, f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]},
                (wn * TN + j) * 32 + 8 * q + 4 * half, cols, whole);
-  }
-}
-
-// Adds up the parts in order: a thread four elements.
-static __global__ void __launch_bounds__(256) fp8_sum(Fp8Args p) {
-  using namespace gdma;
-  const int64_t size = (int64_t)p.M * p.N, at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-  if (at >= size) return;
-  f32x4 v = {0, 0, 0, 0};
-  const int n = (int)min((int64_t)4, size - at);
-  if (n == 4 && (size & 3) == 0) {
-    for (int s0 = 0; s0 < p.splits; s0 += 8) {
-      f32x4 t[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) t[j] = *(const f32x4*)(p.partial + (size_t)min(s0 + j, p.splits - 1) * size + at);
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (s0 + j < p.splits) v += t[j];
     }
-  } else {
-    for (int s = 0; s < p.splits; ++s)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (i < n) v[i] += p.partial[(size_t)s * size + at + i];
-  }
-  if (p.ldc == p.N && n == 4) {
-    store4(p.c, p.out16, at, v, 0, 4, ((uintptr_t)p.c & (p.out16 ? 7 : 15)) == 0);
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (i >= n) break;
-    const int64_t m = (at + i) / p.N, to = m * p.ldc + (at + i - m * p.N);
-    if (p.out16) ((__bf16*)p.c)[to] = (__bf16)v[i];
-    else ((float*)p.c)[to] = v[i];
   }
 }
 

@@ -4,9 +4,10 @@
 //
 // A workgroup computes 16 TM rows x 16 TN columns with 8 waves that share out k in
 // steps of two blocks in turn, load their fragments straight into registers, a step
-// ahead, and add their sums up in LDS, in order.  A lane holds 32 neighbouring bytes of
-// its row's block, which it brings to bf16, scale and all, for four
-// v_mfma_f32_16x16x32_bf16: k may be summed in any order as long as a and b agree.
+// ahead, and add their sums up in LDS, in order.  A lane holds two times 16 bytes of its
+// row's block, so that the four lanes of a row read 64 neighbouring ones, and brings them
+// to bf16, scale and all, for four v_mfma_f32_16x16x32_bf16: k may be summed in any order as
+// long as a and b agree.
 // The sums are fp32 whatever the result's type (fp8_dma.hpp), as memory leaves the time.
 #pragma once
 #include "fp8_dma.hpp"
@@ -29,7 +30,7 @@ __device__ __forceinline__ void load_run(Run& r, const uint8_t* codes, const uin
   for (int h = 0; h < STEP; ++h)
     if (h < left) {
       r.codes[2 * h] = *(const gdma::u32x4*)(codes + 128 * h);
-      r.codes[2 * h + 1] = *(const gdma::u32x4*)(codes + 128 * h + 16);
+      r.codes[2 * h + 1] = *(const gdma::u32x4*)(codes + 128 * h + 64);
       r.scale[h] = scale[h];
     } else {
       r.codes[2 * h] = r.codes[2 * h + 1] = gdma::u32x4{0, 0, 0, 0};
@@ -79,12 +80,12 @@ __global__ void __launch_bounds__(64 * fp8::RWAVES) fp8_rows(Fp8Args p) {
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
     const int64_t at = (int64_t)(m0 + min(16 * i + l16, rows - 1)) * p.blocks + first;
-    a[i] = p.a + 128 * at + 32 * g, sa[i] = p.sa + at;
+    a[i] = p.a + 128 * at + 16 * g, sa[i] = p.sa + at;
   }
 #pragma unroll
   for (int j = 0; j < TN; ++j) {
     const int64_t n = n0 + min(16 * j + l16, cols - 1);
-    b[j] = p.b + 128 * (n * p.blocks + first) + 32 * g, sb[j] = p.sb + (n >> p.b_shift) * p.blocks + first;
+    b[j] = p.b + 128 * (n * p.blocks + first) + 16 * g, sb[j] = p.sb + (n >> p.b_shift) * p.blocks + first;
   }
   Run fa[RING][TM], fb[RING][TN];
   int left = p.blocks - first;

@@ -417,10 +417,9 @@ int xtc_hip_fp8_dequantize(const xtc_hip_fp8_desc *desc, const uint8_t *codes,
                            const uint8_t *scales, void *values);
 
 /* c[m, n] = sum_k a[m, k] b[n, k] of such operands, both with k along their rows;
- * fp32 sums.  a has a scale for every 128 elements of a row, b that or (b_block_rows
- * 128) one for every 128 x 128 block.  Calls of few tiles are summed in parts in the
- * stream's scratch, or in one part while the stream is captured or without memory for
- * it. */
+ * fp32 sums of exact products, or for a bf16 result those of the 8-bit matrix
+ * instructions, off by 1.5e-5 of themselves.  a has a scale for every 128 elements of a
+ * row, b that or (b_block_rows 128) one for every 128 x 128 block. */
 typedef struct {
   int out_dtype;         /* XTC_HIP_F32 or XTC_HIP_BF16 */
   int M, N, blocks;      /* rows of a (0: nothing to do), rows of b, blocks of 128 of k */

@@ -449,7 +449,7 @@ def lower_graph(graph: Any) -> Plan:
             fused = []
             for u in users.get(dy, []):
                 kind = u.operation.name
-                if u.uid in absorbed or u is n or kind not in _NORM_GRADS[1:] or results[kind]:
+                if u.uid in absorbed or u.name in scheduled or u is n or kind not in _NORM_GRADS[1:] or results[kind]:
                     continue
                 if kind == "layer_norm_grad_weight" and (list(u.inputs) != [x, dy] or float(u.operation.attrs.get("eps", 1e-5)) != eps):
                     continue

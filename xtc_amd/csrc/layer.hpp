@@ -19,14 +19,14 @@
 // Where router and tokens are long (more than every workgroup of layer_up should read
 // again from L2), layer_logits works the logits out first, in parts of k.
 //
-// A workgroup is eight waves.  Where there are few rows in all, eight share out k in
-// turn and add their sums up in LDS, in order (DEPTH 8); where there are many, two do
-// (DEPTH 2).  k may be summed in any order as long as matrix and token
-// agree, so a lane takes 32 neighbouring elements of its row (16 of fp32): 64, 32 or 16
-// bytes, four v_mfma_f32_16x16x32_bf16 (or sixteen v_mfma_f32_16x16x4_f32).  The matrix
-// is the first MFMA operand: a lane ends with four neighbouring rows of one token.  A
-// tile of 16 rows of U holds 8 of its first half and the 8 of the second that these
-// are multiplied with, 32 lanes away.
+// A workgroup is four waves, and as many workgroups as the CUs hold walk over the pieces.
+// Where there are few rows in all, the four share out k in turn and add their sums up in
+// LDS, in order (DEPTH 4); where there are many, two do (DEPTH 2), which halves the tokens'
+// trips through LDS.  k may be summed in any order as long as matrix and token agree, so
+// the four lanes of a row read 64 neighbouring bytes of it with an instruction, and a step
+// takes 256.  The matrix is the first MFMA operand: a lane ends with four neighbouring rows
+// of one token.  A tile of 16 rows of U holds 8 of its first half and the 8 of the second
+// that these are multiplied with, 32 lanes away.
 //
 // The activations p_e act(U_e x) between the two products are rounded to bf16 where x is
 // bf16, as those between two bf16 products are: it is what the second one's instructions

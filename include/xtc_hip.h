@@ -560,7 +560,7 @@ int xtc_hip_conv2d_pipeline_depths(const xtc_hip_conv2d_desc *desc, int *depths,
  *                host counters of the calling process through
  *                perf_event_open (perf_event_linux.c:37-54,72-81).
  * A name that cannot be opened yields -1, as in the reference.  At most 64
- * events; func is called with nargs (<= 8) pointer arguments. */
+ * events; func is called with nargs (<= 16) pointer arguments. */
 void xtc_hip_evaluate_perf(double *results, int events_num, const char *events_names[],
                            int repeat, int number, int min_repeat_ms,
                            void (*func)(void), void **args, int nargs);

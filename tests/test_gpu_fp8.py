@@ -217,3 +217,18 @@ def test_same_bits_on_a_stream_of_its_own():
         (ac, asc), (bc, bsc) = operand(M, M, nb, 1), operand(N, N, nb, 128)
         np.testing.assert_array_equal(fp8_matmul(ac, asc, bc, bsc), fp8_matmul(ac, asc, bc, bsc, stream=stream))
     capi.check(capi.lib().xtc_hip_stream_destroy(stream))
+
+
+@pytest.mark.parametrize("out", ["float32", "bfloat16"])
+@pytest.mark.parametrize("M,N,nb", [(4000, 3900, 65), (2500, 2000, 130), (520, 1030, 129)])
+def test_long_walks(M, N, nb, out):
+    """k past the blocks whose scales LDS holds at a time, in tiles of each size: whole
+    numbers whose sums stay below 2^15, exact in the 8-bit instructions too, and scales that
+    change from block to block by powers of two which a's and b's take from each other."""
+    a, b = ints(5, (M, 128 * nb), 1), ints(6, (N, 128 * nb), 1)
+    shift = np.random.default_rng(7).integers(-3, 4, nb)
+    codes = [fp8_codes(v, np.full((len(v), nb), 127, np.uint8)) for v in (a, b)]
+    scales = [np.broadcast_to(127 + s, (n, nb)).astype(np.uint8) for s, n in ((shift, M), (-shift, N))]
+    print(f"[fp8 long] {M}x{N}x{nb} {out}", flush=True)
+    got = fp8_matmul(codes[0], scales[0], codes[1], scales[1], out)
+    np.testing.assert_array_equal(got, rounded(a @ b.T, out))

@@ -229,3 +229,19 @@ out.append(layer(dtype=0) + layer(dtype=0, H=8192, activation=0))
     names = {g[0] for one in got[7:] for g in one}
     # up by activation and depth, down by depth; fp32 rows took one activation at each depth
     assert len(names) == 3 * 2 * 2 + 3 * 2 + 2 + 2, sorted(names)
+
+
+def test_payloads_of_sixteen_arguments(run):  # noqa: F811
+    """A norm, a router and matrices with scales are eight operands and a result."""
+    got = run("""
+seen = []
+P = ctypes.CFUNCTYPE(None, *[ctypes.c_void_p] * 16)
+fn = P(lambda *a: seen.append(a))
+res = (ctypes.c_double * 4)()
+for n in (9, 16, 17):
+    del seen[:]
+    args = (ctypes.c_void_p * 17)(*range(1, 18))
+    L.xtc_hip_evaluate_perf(res, 0, None, 1, 1, 0, ctypes.cast(fn, ctypes.c_void_p), args, n)
+    out.append([list(a) for a in seen[:1]] + [L.xtc_hip_evaluate_status()])
+""")
+    assert got[0] == [[*range(1, 10), *[None] * 7], 0] and got[1] == [list(range(1, 17)), 0] and got[2] == [1]

@@ -2975,13 +2975,14 @@ int xtc_hip_cast_bf16_to_f32(const uint16_t* x, float* y, uint64_t n, void* stre
 // ------------------------------------------------------------ timing harness
 
 typedef void (*fn0)(void);
-typedef void (*fn8)(void*, void*, void*, void*, void*, void*, void*, void*);
+typedef void (*fn16)(void*, void*, void*, void*, void*, void*, void*, void*, void*, void*, void*, void*, void*, void*, void*, void*);
+constexpr int kMostArgs = 16;
 
 static inline void call_payload(void (*func)(void), void** args, int nargs) {
-  void* a[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  for (int i = 0; i < nargs && i < 8; ++i) a[i] = args[i];
+  void* a[kMostArgs] = {};
+  for (int i = 0; i < nargs && i < kMostArgs; ++i) a[i] = args[i];
   // Extra trailing arguments are ignored by the callee under the SysV ABI.
-  ((fn8)func)(a[0], a[1], a[2], a[3], a[4], a[5], a[6], a[7]);
+  ((fn16)func)(a[0], a[1], a[2], a[3], a[4], a[5], a[6], a[7], a[8], a[9], a[10], a[11], a[12], a[13], a[14], a[15]);
 }
 
 }  // extern "C"
@@ -3066,7 +3067,7 @@ void xtc_hip_evaluate_perf(double* results, int events_num, const char* events_n
                            void** args, int nargs) {
   g_eval_status = 0;
   g_last_error.clear();
-  if (!results || repeat <= 0 || number < 0 || min_repeat_ms < 0 || !func || nargs < 0 || nargs > 8 ||
+  if (!results || repeat <= 0 || number < 0 || min_repeat_ms < 0 || !func || nargs < 0 || nargs > kMostArgs ||
       events_num < 0 || (events_num > 0 && !events_names)) {
     g_eval_status = 1;
     fail("evaluate_perf: invalid arguments");

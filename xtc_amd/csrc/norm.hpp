@@ -65,6 +65,17 @@ __device__ __forceinline__ void load8(float (&v)[8], const T* p, int n) {
   for (int i = 0; i < 8; ++i) v[i] = (float)r.v[i];
 }
 
+// v - mean, zeros past the first n
+__device__ __forceinline__ void centre(float (&v)[8], float mean, int n) {
+  if (n >= 8) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] -= mean;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? v[i] - mean : 0.f;
+  }
+}
+
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float (&v)[8], int n) {
   T out[8];
@@ -139,12 +150,11 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) layer_norm(Norm
     const float mean = sum / (float)p.K;
     float var = 0.f;
 #pragma unroll
-    for (int i = 0; i < VECS; ++i)
+    for (int i = 0; i < VECS; ++i) {
+      centre(v[i], mean, p.K - (i * THREADS + t) * 8);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        v[i][j] -= mean;
-        var += (i * THREADS + t) * 8 + j < p.K ? v[i][j] * v[i][j] : 0.f;
-      }
+      for (int j = 0; j < 8; ++j) var += v[i][j] * v[i][j];
+    }
     row_sums<THREADS>(var, none, lds[1]);
     const float r = 1.0f / sqrtf(var / (float)p.K + p.eps);
 #pragma unroll
@@ -193,7 +203,7 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) layer_norm_grad
   if (AHEAD && row < p.rows) load(row);
   // uniform over the threads of a row: with THREADS > 64 over the workgroup
   for (; row < p.rows; row += step) {
-    float x[VECS][8], dy[VECS][8];
+    float x[VECS][8], dy[VECS][8], gr[VECS][8];
     float sum_x = 0.f, sum_g = 0.f;
     if (!AHEAD) load(row);
 #pragma unroll
@@ -201,29 +211,29 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) layer_norm_grad
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         x[i][j] = (float)raw_x[i].v[j], dy[i][j] = (float)raw_dy[i].v[j];
-        sum_x += x[i][j], sum_g += dy[i][j] * w[i][j];
+        gr[i][j] = dy[i][j] * w[i][j];
+        sum_x += x[i][j], sum_g += gr[i][j];
       }
     if (AHEAD && row + step < p.rows) load(row + step);
     row_sums<THREADS>(sum_x, sum_g, lds[0]);
     const float mean = sum_x / (float)p.K;
     float var = 0.f, cov = 0.f;
 #pragma unroll
-    for (int i = 0; i < VECS; ++i)
+    for (int i = 0; i < VECS; ++i) {
+      centre(x[i], mean, p.K - (i * THREADS + t) * 8);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        x[i][j] = (i * THREADS + t) * 8 + j < p.K ? x[i][j] - mean : 0.f;
-        var += x[i][j] * x[i][j], cov += dy[i][j] * w[i][j] * x[i][j];
-      }
+      for (int j = 0; j < 8; ++j) var += x[i][j] * x[i][j], cov += gr[i][j] * x[i][j];
+    }
     row_sums<THREADS>(var, cov, lds[1]);
     const float r = 1.0f / sqrtf(var / (float)p.K + p.eps);
-    const float c1 = sum_g * inv, c2 = cov * r * inv;
+    const float c1 = r * (sum_g * inv), c2 = cov * r * inv;
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
       float out[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float xh = x[i][j] * r;
-        out[j] = r * (dy[i][j] * w[i][j] - c1 - xh * c2);
+        out[j] = r * (gr[i][j] - xh * c2) - c1;
         dw[i][j] += dy[i][j] * xh, db[i][j] += dy[i][j];
       }
       const int k = (i * THREADS + t) * 8;

@@ -147,3 +147,21 @@ def test_same_bits_on_a_stream_of_its_own():
         np.testing.assert_array_equal(a, c)
     np.testing.assert_array_equal(layer_norm(x, w, b, "bfloat16", "float32"), layer_norm(x, w, b, "bfloat16", "float32", stream=stream))
     capi.check(capi.lib().xtc_hip_stream_destroy(stream))
+
+
+@pytest.mark.parametrize("dtype,rows,K", [("bfloat16", 16448, 4104), ("bfloat16", 131200, 515), ("float32", 2112, 16384)])
+def test_results_past_the_caches(dtype, rows, K):
+    """A result of more than 128 MB is stored past the caches: the bits of a small call, whose
+    rows it repeats."""
+    rng = np.random.default_rng(K)
+    x, dy = (rounded(rng.normal(size=(64, K)), dtype) for _ in range(2))
+    w, b = (rng.normal(size=K).astype(np.float32) for _ in range(2))
+    assert rows * K * (2 if dtype == "bfloat16" else 4) > 128 << 20
+    big = np.tile(x, (-(-rows // 64), 1))[:rows]
+    y = layer_norm(big, w, b, dtype, "float32")
+    small = layer_norm(x, w, b, dtype, "float32")
+    assert np.array_equal(y, np.tile(small, (-(-rows // 64), 1))[:rows])
+    del y
+    dx = layer_norm_grad(big, w, np.tile(dy, (-(-rows // 64), 1))[:rows], dtype, "float32", want=(True, False, False))[0]
+    small = layer_norm_grad(x, w, dy, dtype, "float32", want=(True, False, False))[0]
+    assert np.array_equal(dx, np.tile(small, (-(-rows // 64), 1))[:rows])

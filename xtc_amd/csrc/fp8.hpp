@@ -15,6 +15,7 @@
 #include <stdint.h>
 
 #include "mx4.hpp"
+#include "stream.hpp"
 
 namespace xtc_hip {
 
@@ -96,7 +97,7 @@ struct Run8 {
   // the first n of the 8 elements at p, zeros for the others
   __device__ __forceinline__ void load(const T* p, int n) {
     if (n >= 8) {
-      __builtin_memcpy(v, p, sizeof(v));
+      stream::load(v, p);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : (T)0.f;

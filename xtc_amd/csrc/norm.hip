@@ -40,6 +40,7 @@ NormArgs args_of(const xtc_hip_layer_norm_desc& d, const void* x, const void* w)
   NormArgs a{};
   a.x = x, a.w = w, a.rows = d.rows, a.K = d.K, a.eps = d.eps;
   a.ldx = d.ldx ? d.ldx : d.K, a.ldy = d.ldy ? d.ldy : d.K;
+  a.once = d.rows * d.K * (d.dtype == XTC_HIP_F32 ? 4 : 2) >= stream::LARGE;
   return a;
 }
 

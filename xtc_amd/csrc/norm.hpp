@@ -23,6 +23,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "stream.hpp"
+
 namespace xtc_hip {
 
 struct NormArgs {
@@ -36,6 +38,7 @@ struct NormArgs {
   int64_t rows;
   int K, ldx, ldy;
   float eps;
+  bool once;       // y is larger than what the caches keep
 };
 
 namespace norm {
@@ -47,11 +50,12 @@ template <typename T>
 struct Raw8 {
   T v[8];
 };
-// the first n of the 8 elements at p, zeros for the others
-template <typename T>
+// the first n of the 8 elements at p, zeros for the others.  ONCE: nobody reads them again
+template <bool ONCE, typename T>
 __device__ __forceinline__ void load8(Raw8<T>& r, const T* p, int n) {
   if (n >= 8) {
-    __builtin_memcpy(&r, p, sizeof(r));
+    if constexpr (ONCE) stream::load(r, p);
+    else __builtin_memcpy(&r, p, sizeof(r));
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) r.v[i] = i < n ? p[i] : (T)0.f;
@@ -60,7 +64,7 @@ __device__ __forceinline__ void load8(Raw8<T>& r, const T* p, int n) {
 template <typename T>
 __device__ __forceinline__ void load8(float (&v)[8], const T* p, int n) {
   Raw8<T> r;
-  load8(r, p, n);
+  load8<false>(r, p, n);
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = (float)r.v[i];
 }
@@ -77,12 +81,13 @@ __device__ __forceinline__ void centre(float (&v)[8], float mean, int n) {
 }
 
 template <typename T>
-__device__ __forceinline__ void store8(T* p, const float (&v)[8], int n) {
+__device__ __forceinline__ void store8(T* p, const float (&v)[8], int n, bool once = false) {
   T out[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) out[i] = (T)v[i];
   if (n >= 8) {
-    __builtin_memcpy(p, out, sizeof(out));
+    if (once) stream::store(p, out);
+    else __builtin_memcpy(p, out, sizeof(out));
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -123,7 +128,7 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) layer_norm(Norm
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
       const int k = (i * THREADS + t) * 8;
-      load8(raw[i], (const T*)p.x + row * p.ldx + k, p.K - k);
+      load8<true>(raw[i], (const T*)p.x + row * p.ldx + k, p.K - k);
     }
   };
   int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / THREADS;
@@ -163,7 +168,7 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) layer_norm(Norm
       float out[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) out[j] = v[i][j] * r * w[i][j] + b[i][j];
-      store8((T*)p.y + row * p.ldy + k, out, p.K - k);
+      store8((T*)p.y + row * p.ldy + k, out, p.K - k, p.once);
     }
   }
 }
@@ -193,8 +198,8 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) layer_norm_grad
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
       const int k = (i * THREADS + t) * 8;
-      load8(raw_x[i], (const T*)p.x + row * p.ldx + k, p.K - k);
-      load8(raw_dy[i], (const T*)p.dy + row * p.ldy + k, p.K - k);
+      load8<true>(raw_x[i], (const T*)p.x + row * p.ldx + k, p.K - k);
+      load8<true>(raw_dy[i], (const T*)p.dy + row * p.ldy + k, p.K - k);
     }
   };
   // the next row's loads are on their way during the sums of this one, where registers last
@@ -237,7 +242,7 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) layer_norm_grad
         dw[i][j] += dy[i][j] * xh, db[i][j] += dy[i][j];
       }
       const int k = (i * THREADS + t) * 8;
-      if (p.y) store8((T*)p.y + row * p.ldx + k, out, p.K - k);
+      if (p.y) store8((T*)p.y + row * p.ldx + k, out, p.K - k, p.once);
     }
   }
   if (!p.parts) return;

@@ -138,7 +138,7 @@ int xtc_hip_layer_norm_grad(const xtc_hip_layer_norm_desc* desc, const void* x, 
     if (done(what)) return 1;
   }
   if (sums) {
-    hipLaunchKernelGGL(layer_norm_grad_sum, dim3((unsigned)(((int64_t)a.K + 63) / 64), 2), dim3(256), 0, s, workspace, dw, db, parts, a.K);
+    hipLaunchKernelGGL(layer_norm_grad_sum, dim3((unsigned)(((int64_t)a.K + 63) / 64), 2), dim3(1024), 0, s, workspace, dw, db, parts, a.K);
     return done(what);
   }
   return 0;

@@ -349,8 +349,8 @@ int xtc_hip_mx4_quantize_matmul(const xtc_hip_mx4_desc *rows,
 
 /* Layer norm over the K elements of a row; no counterpart in the reference.
  *   m = sum x / K, r = 1 / sqrt(sum (x - m)^2 / K + eps), y = (x - m) r w + b
- * w and b [K] may be NULL (1 and 0).  Sums are fp32, results are rounded once.
- * An infinity or a NaN makes its own row NaN, no other. */
+ * w and b [K] may be NULL (1 and 0).  Sums are fp32, results are rounded once; y
+ * overlaps no operand.  An infinity or a NaN makes its own row NaN, no other. */
 typedef struct {
   int dtype;             /* XTC_HIP_F32 or XTC_HIP_BF16: x, y, dy, dx */
   int param_dtype;       /* of w and b: XTC_HIP_F32, or XTC_HIP_BF16 for bf16 rows */
@@ -399,7 +399,7 @@ typedef struct {
 } xtc_hip_fp8_desc;
 
 /* Codes, scales and the (dense) values that they stand for; each may be NULL, and
- * values must be where transpose is set. */
+ * values must be where transpose is set.  Results overlap no operand, here and below. */
 int xtc_hip_fp8_quantize(const xtc_hip_fp8_desc *desc, const void *x, uint8_t *codes,
                          uint8_t *scales, void *values);
 

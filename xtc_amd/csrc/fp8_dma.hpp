@@ -265,6 +265,7 @@ __global__ void __launch_bounds__(WGM* WGN * 64) fp8_dma(Fp8Args p) {
       for (int kt = 0; kt < nk; kt += STAGES) each_stage<STAGES>([&](auto s) { if (kt + s < nk) step(s); });
       if (group == 0) phase_barrier();
     } else if constexpr (RP) {
+      static_assert(FAST, "the codes go into the matrix instructions as they are");
       u32x4 na[2][TM][2], nb[2][TN][2];  // this slab's fragments and the next one's
       auto scales = [&] {
         const unsigned char* const ss = lds_s + (at >> 1 & 12);
@@ -302,40 +303,15 @@ __global__ void __launch_bounds__(WGM* WGN * 64) fp8_dma(Fp8Args p) {
         phase_barrier();
         issue(s);
         fetch(na[1 - cur], nb[1 - cur], lds + (s + 1) % STAGES * STAGE);
-        constexpr int READS = 2 * (TM + TN);  // of LDS
-        if constexpr (FAST) {
+        constexpr int READS = 2 * (TM + TN), EACH = (READS + TM * TN - 1) / (TM * TN);  // of LDS
 #pragma unroll
-          for (int i = 0; i < TM; ++i)
+        for (int i = 0; i < TM; ++i)
 #pragma unroll
-            for (int j = 0; j < TN; ++j) acc[i][j] = fp8::mfma(nb[cur][j], hb[j], na[cur][i], ha[i], acc[i][j]);
+          for (int j = 0; j < TN; ++j) acc[i][j] = fp8::mfma(nb[cur][j], hb[j], na[cur][i], ha[i], acc[i][j]);
 #pragma unroll
-          for (int i = 0; i < TM * TN; ++i) {
-            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);  // a matrix instruction
-            __builtin_amdgcn_sched_group_barrier(0x100, (READS + TM * TN - 1) / (TM * TN), 0);  // reads of LDS
-          }
-        } else {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-#pragma unroll
-            for (int i = 0; i < TM; ++i) convert(fa[i], na[cur][i][h], ha[i]);
-#pragma unroll
-            for (int j = 0; j < TN; ++j) convert(fb[j], nb[cur][j][h], hb[j]);
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-              for (int i = 0; i < TM; ++i)
-#pragma unroll
-                for (int j = 0; j < TN; ++j)
-                  acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, fb[j][c]), __builtin_bit_cast(bf16x8, fa[i][c]), acc[i][j], 0, 0, 0);
-          }
-          // the second half's conversions run beside the first half's products
-          __builtin_amdgcn_sched_group_barrier(0x2, 8 * (TM + TN), 0);
-#pragma unroll
-          for (int i = 0; i < 4 * TM * TN; ++i) {
-            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x2, 4, 0);  // arithmetic
-            if (i < READS) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-          }
+        for (int i = 0; i < TM * TN; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);       // a matrix instruction
+          __builtin_amdgcn_sched_group_barrier(0x100, EACH, 0);  // reads of LDS
         }
         __builtin_amdgcn_sched_barrier(0);
         // the sums stay in this step: they would sink past the branch below and the next barrier

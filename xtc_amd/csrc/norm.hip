@@ -13,6 +13,7 @@ constexpr int kMost = 0x7fffffff - 16383;  // of K: a walk's step past it stays 
 constexpr int kLong = 16384;               // elements of a row that registers hold
 constexpr int64_t kMostGroups = 1 << 20;   // of a launch: its threads stay within 32 bits
 constexpr int64_t kWalks = 1024;           // workgroups of 256 threads that walk over the rows: four a CU
+                                           // (a row each and no walk: 149 us of 32768 x 4096, this 129)
 constexpr int kMostParts = XTC_HIP_LAYER_NORM_PARTS;
 
 int check(const xtc_hip_layer_norm_desc* d, const char* what) {

@@ -17,6 +17,14 @@
 // registers, column by column, and writes them as one part; a second kernel adds
 // the parts up in order, so that results do not depend on timing.
 //
+// Bound by memory: 32768 x 4096 bf16 97 us (5.5 TB/s, a copy reaches 5.2), the gradients of
+// 16384 x 4096 87 (4.6 TB/s, and 5 us of them the second kernel).  Rows are read past the
+// caches (stream.hpp), and a row's loads run during the sums of the one before: 149 us and
+// 145 without.  A row of the gradients from 2049 to 4096 elements has 512 threads, one run
+// each, as two runs leave registers for two workgroups of four waves a CU (152, 125); the
+// forward pass, which has them, two runs of 256 (129, 171 with 512).  Two rows ahead change
+// nothing (125).
+//
 // Rows past 16384 elements go through memory (L2) once for each sum: the kernels
 // named *_long.
 #pragma once

@@ -278,7 +278,8 @@ class XTCOperFp8Matmul(XTCOperator):
     """c[i, j] = sum_k a[i, k] b[j, k] of 8-bit operands.
 
     a codes (M, 128 B) and scales (M, B), b codes (N, 128 B) and scales (N, B) or
-    (ceil(N / 128), B) -> (M, N) of type out_dtype (float32).
+    (ceil(N / 128), B) -> (M, N) of type out_dtype (float32).  On the GPU float32
+    results are fp32 sums of exact products; those of bfloat16 results lose some 1.5e-5.
     """
 
     def __init__(self, **attrs: Any) -> None:

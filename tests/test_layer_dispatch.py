@@ -211,7 +211,7 @@ out.append(call("xtc_hip_expert_layer", None, 256, 256, 256, None, 256, None, 25
 
 def test_expert_layer_launches(run):  # noqa: F811
     """Logits by a launch of their own where router and tokens are long; waves that share
-    out k by fours where there are few rows and by twos where there are many."""
+    out k by fours, and by twos where there are many rows of packed matrices."""
     got = run(CALLS + """
 for kw in (dict(T=0), dict(T=1), dict(T=33), dict(T=32, E=144, top_k=1), dict(T=17, E=33), dict(T=4, E=8, K=8192), dict(T=64, E=256, top_k=16, K=4096, H=2048)):
     out.append(layer(**kw))
@@ -227,8 +227,8 @@ out.append(layer(dtype=0) + layer(dtype=0, H=8192, activation=0))
     groups = [int(g[1].split()[0]) for one in got for g in one if "logits" not in g[0]]
     assert max(groups) <= 768 and min(groups) >= 1
     names = {g[0] for one in got[7:] for g in one}
-    # up by activation and depth, down by depth; fp32 rows took one activation at each depth
-    assert len(names) == 3 * 2 * 2 + 3 * 2 + 2 + 2, sorted(names)
+    # up by activation and depth, down by depth; dense ones have one depth
+    assert len(names) == 2 * (2 * 2 + 2) + 2 * (2 + 1), sorted(names)
 
 
 def test_payloads_of_sixteen_arguments(run):  # noqa: F811

@@ -89,7 +89,11 @@ int xtc_hip_expert_layer(const xtc_hip_expert_layer_desc* desc, const void* x, c
   // experts that tokens may choose, and the tiles of 16 rows of all of them
   const int most = d.T * d.top_k < d.E ? d.T * d.top_k : d.E;
   const int64_t tiles = most * (((int64_t)d.H * (a.swiglu ? 2 : 1) + 15) / 16);
-  grid.shared = tiles < 1024;
+  // Waves that share k, four or two, us: dense matrices always take four (bf16, 512 tiles 19.8,
+  // 24.8, 2048 tiles 43.6, 47.7, 8192 tiles 109, 114); packed ones, whose tokens go through LDS
+  // twice as often a byte, two from 2048 tiles (4 bits, 256 tiles 23.2, 27.3, 1024 tiles 23.5,
+  // 25.0, 2048 tiles of 8 tokens 45.7, 43.9 and of 32 60.7, 54.8; 8 bits, 2048 tiles 41.6, 38.2)
+  grid.shared = !packed || tiles < 2048;
   const int up_rows = (a.swiglu ? 16 : 32) * (grid.shared ? 1 : 2), down_rows = 32 * (grid.shared ? 1 : 2);
   const int64_t up_slices = ((int64_t)a.Hp + up_rows - 1) / up_rows, down_slices = ((int64_t)d.K + down_rows - 1) / down_rows;
   if (up_slices * most >= 1 << 30 || down_slices * most >= 1 << 30)
@@ -99,10 +103,12 @@ int xtc_hip_expert_layer(const xtc_hip_expert_layer_desc* desc, const void* x, c
   grid.up = (unsigned)(up_slices * most < groups ? up_slices * most : groups);
   grid.down = (unsigned)(down_slices * most < groups ? down_slices * most : groups);
 
-  // router and tokens that every workgroup of layer_up reads again
+  // router and tokens that every workgroup of layer_up reads again: in a launch of their own
+  // from 64 KB (us, within layer_up and by themselves: 18 KB 19.8, 21.3, 34 KB 22.2, 24.7, 72 KB
+  // 37.2, 35.8, 96 KB 43.6, 42.3, 272 KB 56.9, 38.2)
   const int esz = d.dtype == XTC_HIP_F32 ? 4 : 2;
   const int pairs = (d.E + 15) / 16 * ((d.T + 15) / 16);
-  if (d.T > layer::ROUND || d.T * d.E > layer::LOGITS || pairs > 4 || ((int64_t)d.T + d.E) * d.K * esz > 128 << 10) {
+  if (d.T > layer::ROUND || d.T * d.E > layer::LOGITS || pairs > 4 || ((int64_t)d.T + d.E) * d.K * esz > 64 << 10) {
     a.logits = (float*)(ws + w.logits);
     a.logit_parts = pairs >= 16 ? 2 : pairs >= 4 ? 4 : 8;
     const dim3 logits((unsigned)((d.T + 15) / 16), (unsigned)((d.E + 15) / 16), (unsigned)a.logit_parts);

@@ -20,9 +20,8 @@
 // again from L2), layer_logits works the logits out first, in parts of k.
 //
 // A workgroup is four waves, and as many workgroups as the CUs hold walk over the pieces.
-// Where there are few rows in all, the four share out k in turn and add their sums up in
-// LDS, in order (DEPTH 4); where there are many, two do (DEPTH 2), which halves the tokens'
-// trips through LDS.  k may be summed in any order as long as matrix and token agree, so
+// The four share out k in turn and add their sums up in LDS, in order (DEPTH 4); for packed
+// matrices of many rows two do (DEPTH 2), which halves the tokens' trips through LDS.  k may be summed in any order as long as matrix and token agree, so
 // the four lanes of a row read 64 neighbouring bytes of it with an instruction, and a step
 // takes 256.  The matrix is the first MFMA operand: a lane ends with four neighbouring rows
 // of one token.  A tile of 16 rows of U holds 8 of its first half and the 8 of the second
@@ -650,7 +649,7 @@ __global__ void __launch_bounds__(layer::THREADS, F == layer::MX4 ? 2 : 3) layer
 
 // The two launches.
 struct LayerGrid {
-  bool shared;  // eight waves share the depth, or two
+  bool shared;  // four waves share the depth, or two
   int up_slices, down_slices;
   unsigned up, down;  // workgroups
 };
@@ -669,7 +668,9 @@ void layer_launch_tiles(const LayerArgs& a, const LayerGrid& g, hipStream_t s) {
 #define XTC_HIP_LAYER_LAUNCH(F)                                                  \
   template <>                                                                    \
   void layer_launch<F>(const LayerArgs& a, const LayerGrid& g, hipStream_t s) {  \
-    g.shared ? layer_launch_tiles<F, layer::WAVES>(a, g, s) : layer_launch_tiles<F, 2>(a, g, s); \
+    if constexpr (F == layer::FP8 || F == layer::MX4)                            \
+      if (!g.shared) return layer_launch_tiles<F, 2>(a, g, s);                   \
+    layer_launch_tiles<F, layer::WAVES>(a, g, s);                                \
   }
 template <> void layer_launch<layer::F32>(const LayerArgs&, const LayerGrid&, hipStream_t);
 template <> void layer_launch<layer::BF16>(const LayerArgs&, const LayerGrid&, hipStream_t);

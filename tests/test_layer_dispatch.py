@@ -227,6 +227,8 @@ out.append(layer(dtype=0) + layer(dtype=0, H=8192, activation=0))
     groups = [int(g[1].split()[0]) for one in got for g in one if "logits" not in g[0]]
     assert max(groups) <= 768 and min(groups) >= 1
     names = {g[0] for one in got[7:] for g in one}
+    # pieces of down have 32 rows where there are enough of them for the CUs
+    assert got[5][2][0].startswith("layer_down<1, 2, 4") and got[1][1][0].startswith("layer_down<1, 1, 4")
     # up by activation and depth, down by depth; dense ones have one depth
     assert len(names) == 2 * (2 * 2 + 2) + 2 * (2 + 1), sorted(names)
 

@@ -94,7 +94,10 @@ int xtc_hip_expert_layer(const xtc_hip_expert_layer_desc* desc, const void* x, c
   // twice as often a byte, two from 2048 tiles (4 bits, 256 tiles 23.2, 27.3, 1024 tiles 23.5,
   // 25.0, 2048 tiles of 8 tokens 45.7, 43.9 and of 32 60.7, 54.8; 8 bits, 2048 tiles 41.6, 38.2)
   grid.shared = !packed || tiles < 2048;
-  const int up_rows = (a.swiglu ? 16 : 32) * (grid.shared ? 1 : 2), down_rows = 32 * (grid.shared ? 1 : 2);
+  // pieces of 32 rows of `down` that leave CUs idle are halved (64 of them 9.1 us, 128 of 16 rows
+  // 7.0; from 256 on, a piece a CU, halves would only read the tokens twice)
+  grid.narrow = grid.shared && ((int64_t)d.K + 31) / 32 * most < 256;
+  const int up_rows = (a.swiglu ? 16 : 32) * (grid.shared ? 1 : 2), down_rows = (grid.narrow ? 16 : 32) * (grid.shared ? 1 : 2);
   const int64_t up_slices = ((int64_t)a.Hp + up_rows - 1) / up_rows, down_slices = ((int64_t)d.K + down_rows - 1) / down_rows;
   if (up_slices * most >= 1 << 30 || down_slices * most >= 1 << 30)
     return fail("%s: %lld pieces of work are too many", what, (long long)((up_slices > down_slices ? up_slices : down_slices) * most));

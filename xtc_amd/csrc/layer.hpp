@@ -29,7 +29,7 @@
 //
 // Bound by the matrices where there are many (16 tokens, 4 of 64 experts of 2048/1024 in
 // 8 bits: 40 us and 20, 4 TB/s), and by latency else: a token at 2 of 8 experts of
-// 1024/2048 in bf16 10 us and 9, of which starting, logits and choice are 6; 64 tokens at
+// 1024/2048 in bf16 10 us and 7, of which starting, logits and choice are 6; 64 tokens at
 // 2 of 16 of 4096/2048 in 4 bits 28 and 31.
 //
 // The activations p_e act(U_e x) between the two products are rounded to bf16 where x is
@@ -628,10 +628,15 @@ __global__ void __launch_bounds__(layer::THREADS, F == layer::MX4 ? 2 : 3) layer
     for (int at = 0; at < n; at += 16) {
       f32x4 acc[TN] = {};
       auto row = [&](int j) { return Row<F>(p.down, p.down_scales, e, p.K, min(n0 + 16 * j + l16, p.K - 1), p.H); };
-      Row<F> rows[2] = {row(0), row(1)};
-      static_assert(TN == 2, "two tiles of rows a wave");
-      product<F, TN, DEPTH>(acc, rows, lds.tokens, p.H, min(n - at, 16), wave % DEPTH,
-                                [&](int t) { return (const T*)p.mid + (int64_t)places[at + t] * p.Hp; });
+      auto token = [&](int t) { return (const T*)p.mid + (int64_t)places[at + t] * p.Hp; };
+      static_assert(TN == 1 || TN == 2, "one or two tiles of rows a wave");
+      if constexpr (TN == 1) {
+        Row<F> rows[1] = {row(0)};
+        product<F, TN, DEPTH>(acc, rows, lds.tokens, p.H, min(n - at, 16), wave % DEPTH, token);
+      } else {
+        Row<F> rows[2] = {row(0), row(1)};
+        product<F, TN, DEPTH>(acc, rows, lds.tokens, p.H, min(n - at, 16), wave % DEPTH, token);
+      }
       summed<DEPTH>(lds.sums, acc, [&](f32x4 v, int q) {
         const int t = at + l16;
         keep(v, n0 + 16 * q + 4 * g, places[min(t, n - 1)], t < n);
@@ -650,6 +655,7 @@ __global__ void __launch_bounds__(layer::THREADS, F == layer::MX4 ? 2 : 3) layer
 // The two launches.
 struct LayerGrid {
   bool shared;  // four waves share the depth, or two
+  bool narrow;  // pieces of layer_down have 16 rows, not 32
   int up_slices, down_slices;
   unsigned up, down;  // workgroups
 };
@@ -663,6 +669,11 @@ void layer_launch_tiles(const LayerArgs& a, const LayerGrid& g, hipStream_t s) {
   u.slices = g.up_slices, d.slices = g.down_slices;
   if (a.swiglu) hipLaunchKernelGGL((layer_up<F, 2, true, DEPTH>), dim3(g.up), dim3(layer::THREADS), 0, s, u);
   else hipLaunchKernelGGL((layer_up<F, 2, false, DEPTH>), dim3(g.up), dim3(layer::THREADS), 0, s, u);
+  if constexpr (DEPTH == layer::WAVES)
+    if (g.narrow) {
+      hipLaunchKernelGGL((layer_down<F, 1, DEPTH>), dim3(g.down), dim3(layer::THREADS), 0, s, d);
+      return;
+    }
   hipLaunchKernelGGL((layer_down<F, 2, DEPTH>), dim3(g.down), dim3(layer::THREADS), 0, s, d);
 }
 #define XTC_HIP_LAYER_LAUNCH(F)                                                  \

@@ -40,6 +40,7 @@
 // The tiles walk k in step.  With the walks staggered, which spreads the first loads over
 // the memory channels, an XCD's L2 no longer holds what its tiles share: 600 us.
 #pragma once
+#include "fp8_scales.hpp"
 #include "grouped_dma.hpp"
 
 namespace xtc_hip {
@@ -56,11 +57,7 @@ struct Fp8Args {
 
 namespace fp8 {
 
-constexpr int SCALES = 64;  // blocks of a walk
-
 enum Schedule { PLAIN, PINGPONG, AHEAD };
-
-__device__ __forceinline__ int swz(int r) { return (r >> 3) & 3; }
 
 __device__ __forceinline__ gdma::f32x16 mfma(const gdma::u32x4 (&b)[2], unsigned sb, const gdma::u32x4 (&a)[2], unsigned sa, gdma::f32x16 c) {
   using gdma::i32x8;
@@ -170,28 +167,20 @@ __global__ void __launch_bounds__(WGM* WGN * 64) fp8_dma(Fp8Args p) {
     u32x4 fa[TM][2], fb[TN][2];  // FAST: codes of 32 elements; otherwise 16 of them in bf16
     unsigned ha[TM], hb[TN];     // scales of this lane's rows, four blocks
     int at = 0;                  // slab of the walk
+    auto scales = [&] {
+#pragma unroll
+      for (int i = 0; i < TM; ++i) ha[i] = *(const unsigned*)(lds_s + fp8::scales_at((wm * TM + i) * 32 + l32, at));
+#pragma unroll
+      for (int j = 0; j < TN; ++j) hb[j] = *(const unsigned*)(lds_s + fp8::scales_at(BM + (wn * TN + j) * 32 + l32, at));
+    };
     auto convert = [](u32x4 (&to)[2], u32x4 v, unsigned h) {
       const float scale = fp8::scale_of_byte(h & 255);
 #pragma unroll
       for (int c = 0; c < 2; ++c) to[c] = __builtin_bit_cast(u32x4, fp8::values_bf16(v[2 * c], v[2 * c + 1], scale));
     };
     auto read = [&](const int s, const int hf, const unsigned char* st) {
-      if (s % 2 == 0 && hf == 0) {
-        if ((at & 7) == 0) {
-          const unsigned char* const ss = lds_s + (at >> 1 & 12);
-          const int q = at >> 5;  // 16 blocks
-#pragma unroll
-          for (int i = 0; i < TM; ++i) {
-            const int r = (wm * TM + i) * 32 + l32;
-            ha[i] = *(const unsigned*)(ss + r * fp8::SCALES + 16 * (q ^ fp8::swz(r)));
-          }
-#pragma unroll
-          for (int j = 0; j < TN; ++j) {
-            const int r = BM + (wn * TN + j) * 32 + l32;
-            hb[j] = *(const unsigned*)(ss + r * fp8::SCALES + 16 * (q ^ fp8::swz(r)));
-          }
-        }
-      }
+      if (s % 2 == 0 && hf == 0)
+        if ((at & 7) == 0) scales();
       if constexpr (FAST) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -267,20 +256,6 @@ __global__ void __launch_bounds__(WGM* WGN * 64) fp8_dma(Fp8Args p) {
     } else if constexpr (RP) {
       static_assert(FAST, "the codes go into the matrix instructions as they are");
       u32x4 na[2][TM][2], nb[2][TN][2];  // this slab's fragments and the next one's
-      auto scales = [&] {
-        const unsigned char* const ss = lds_s + (at >> 1 & 12);
-        const int q = at >> 5;
-#pragma unroll
-        for (int i = 0; i < TM; ++i) {
-          const int r = (wm * TM + i) * 32 + l32;
-          ha[i] = *(const unsigned*)(ss + r * fp8::SCALES + 16 * (q ^ fp8::swz(r)));
-        }
-#pragma unroll
-        for (int j = 0; j < TN; ++j) {
-          const int r = BM + (wn * TN + j) * 32 + l32;
-          hb[j] = *(const unsigned*)(ss + r * fp8::SCALES + 16 * (q ^ fp8::swz(r)));
-        }
-      };
       auto fetch = [&](u32x4 (&ta)[TM][2], u32x4 (&tb)[TN][2], const unsigned char* st) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -325,7 +300,7 @@ __global__ void __launch_bounds__(WGM* WGN * 64) fp8_dma(Fp8Args p) {
           for (int i = 0; i < TM; ++i) ha[i] >>= 8;
 #pragma unroll
           for (int j = 0; j < TN; ++j) hb[j] >>= 8;
-            if ((at & 7) == 0) scales();
+          if ((at & 7) == 0) scales();  // after the last slab too: scales_at stays in the row
         }
       };
       // an even number of slabs.  No branch inside: matrix instructions would sink past it

@@ -359,7 +359,7 @@ def _emit_launch(plan: Plan, ln: Launch, cfg: GemmConfig | SplitConfig | None, i
         args = ", ".join(_ptr(plan, u) for u in (*ln.inputs, ln.output))
         lines.append(
             f"  {{ static const xtc_hip_fp8_matmul_desc d = {{{_DTYPE_ENUM[a['out']]}, {a['M']}, {a['N']}, {a['blocks']}, "
-            f"{a['b_block_rows']}, 0, 0}};"
+            f"{a['b_block_rows']}, 0, XTC_HIP_SUMS_{a['sums'].upper()}, 0}};"
         )
         lines.append(f"    if ((rc = xtc_hip_fp8_matmul(&d, {args}))) {{ record(rc, {where}); return; }} }}")
     elif ln.kind == "expert_layer":

@@ -517,7 +517,8 @@ def lower_graph(graph: Any) -> Plan:
             scheduled[n.name] = n
         elif name == "fp8_matmul":
             bs, bss = _shape(out_type(n.inputs[2])), _shape(out_type(n.inputs[3]))
-            attrs = {"out": _dtype(t_out), "M": _shape(t_out)[0], "N": bs[0], "blocks": bss[1], "b_block_rows": 1 if bss[0] == bs[0] else 128}
+            attrs = {"out": _dtype(t_out), "M": _shape(t_out)[0], "N": bs[0], "blocks": bss[1], "b_block_rows": 1 if bss[0] == bs[0] else 128,
+                     "sums": str(op.attrs.get("sums", "fp32"))}
             launches.append(Launch("fp8_matmul", n.name, list(n.inputs), n.uid, attrs))
             scheduled[n.name] = n
         elif name == "expert_layer":

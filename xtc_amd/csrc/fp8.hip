@@ -74,7 +74,7 @@ int quantize(const xtc_hip_fp8_desc& d, const Fp8QuantArgs& a, const char* what)
 // ---- products
 
 struct DmaTile {
-  DmaCost cost[2];  // to fp32, to bf16
+  DmaCost cost[2];  // fp32 sums, those of the 8-bit instructions
   void (*launch[2])(const Fp8Args&, unsigned, hipStream_t);
 };
 template <bool FAST, int WGM, int WGN, int TM, int TN, fp8::Schedule S>
@@ -83,11 +83,13 @@ void dma_launch(const Fp8Args& a, unsigned groups, hipStream_t s) {
 }
 // Microseconds a block, a CU with one workgroup and with all it takes, measured (us, the
 // three tiles in this order; M x N x k):
-//   to bf16:  4096 x 4096 x 2048  43, 48, 72    4096 x 2048 x 4096  68, 45, 76    2048 x 2048 x 2048  40, 17, 23
+//   8-bit instructions, to bf16:
+//             4096 x 4096 x 2048  43, 48, 72    4096 x 2048 x 4096  68, 45, 76    2048 x 2048 x 2048  40, 17, 23
 //             512 x 4096 x 4096  54, 26, 23    1024 x 1024 x 8192  98, 52, 33    8192 x 8192 x 4096  250, 322, 502
-//   to fp32:  4096 x 4096 x 2048  80, 81, 100   4096 x 2048 x 4096  111, 73, 97   2048 x 2048 x 2048  56, 29, 30
+//   fp32 sums, to fp32:
+//             4096 x 4096 x 2048  80, 81, 100   4096 x 2048 x 4096  111, 73, 97   2048 x 2048 x 2048  56, 29, 30
 //             512 x 4096 x 4096  88, 40, 31    1024 x 1024 x 8192  167, 78, 44   8192 x 8192 x 4096  469, 497, 680
-// fp32 results are bound by the conversions, which take longer than the products: a
+// fp32 sums are bound by the conversions, which take longer than the products: a
 // schedule of fragments read ahead and 256 x 128 tiles made 4096 x 2048 x 4096 no faster (79).
 const DmaTile kDmaTiles[] = {
     {{{256, 256, 1, 2.4, 3.3}, {256, 256, 1, 1.3, 1.8}}, {&dma_launch<false, 2, 4, 4, 2, fp8::PINGPONG>, &dma_launch<true, 2, 2, 4, 4, fp8::AHEAD>}},
@@ -118,13 +120,17 @@ int check(const xtc_hip_fp8_matmul_desc* desc, const char* what) {
   if (d.M > kMost || d.N > kMost || d.blocks >= 1 << 16)
     return fail("%s: sizes M=%d N=%d blocks=%d are too many", what, d.M, d.N, d.blocks);
   if (d.ldc && d.ldc < d.N) return fail("%s: row stride %d of c is below its %d columns", what, d.ldc, d.N);
+  if (d.sums < XTC_HIP_SUMS_ANY || d.sums > XTC_HIP_SUMS_FP8) return fail("%s: unsupported sums %d", what, d.sums);
   return 0;
 }
 
 int product(const xtc_hip_fp8_matmul_desc& d, Fp8Args& a, const char* what) {
   const hipStream_t s = core::pick_stream(d.stream);
+  const bool fast = d.sums == XTC_HIP_SUMS_FP8 || (d.sums == XTC_HIP_SUMS_ANY && a.out16);
+  // few tiles: the kernel that sums in fp32, unless the caller has asked for one kind of sums
+  // whatever the rows
   for (const RowsTile* t : {&kRows16, &kRows32})
-    if (tiles_of(d.M, t->bm) * tiles_of(d.N, t->bn) <= 256) {
+    if (d.sums != XTC_HIP_SUMS_FP8 && tiles_of(d.M, t->bm) * tiles_of(d.N, t->bn) <= 256) {
       a.tiles_n = (int)tiles_of(d.N, t->bn);
       t->run[a.out16](a, (unsigned)(tiles_of(d.M, t->bm) * a.tiles_n), s);
       return done(what);
@@ -132,7 +138,7 @@ int product(const xtc_hip_fp8_matmul_desc& d, Fp8Args& a, const char* what) {
   const DmaTile* best = nullptr;
   double least = 0;
   for (const DmaTile& t : kDmaTiles) {
-    const DmaCost& c = t.cost[a.out16];
+    const DmaCost& c = t.cost[fast];
     const double cost = dma_cost(c, (double)tiles_of(d.M, c.bm) * tiles_of(d.N, c.bn), d.blocks, a.out16 ? 2 : 4);
     if (!best || cost < least) best = &t, least = cost;
   }
@@ -141,7 +147,7 @@ int product(const xtc_hip_fp8_matmul_desc& d, Fp8Args& a, const char* what) {
   const int64_t tiles = ((int64_t)a.tiles_m + a.band - 1) / a.band * a.band * a.tiles_n, whole = (int64_t)8 * 4 * a.band;
   const int64_t groups = (tiles + whole - 1) / whole * whole;
   if (groups >= (int64_t)1 << 22) return fail("%s: %lld workgroups are too many", what, (long long)groups);
-  best->launch[a.out16](a, (unsigned)groups, s);
+  best->launch[fast](a, (unsigned)groups, s);
   return done(what);
 }
 

@@ -41,10 +41,13 @@ __all__ = [
     "MOST_TOKENS",
     "MOST_EXPERTS",
     "MOST_CHOSEN",
+    "FP8_SUMS",
 ]
 
 # of expert_layer: tokens, experts, experts of a token
 MOST_TOKENS, MOST_EXPERTS, MOST_CHOSEN = 64, 256, 16
+# how fp8_matmul adds up: XTC_HIP_SUMS_..
+FP8_SUMS = ("fp32", "fp8", "any")
 
 
 def _eps(op: XTCOperator) -> float:
@@ -278,8 +281,11 @@ class XTCOperFp8Matmul(XTCOperator):
     """c[i, j] = sum_k a[i, k] b[j, k] of 8-bit operands.
 
     a codes (M, 128 B) and scales (M, B), b codes (N, 128 B) and scales (N, B) or
-    (ceil(N / 128), B) -> (M, N) of type out_dtype (float32).  On the GPU float32
-    results are fp32 sums of exact products; those of bfloat16 results lose some 1.5e-5.
+    (ceil(N / 128), B) -> (M, N) of type out_dtype (float32).  Attribute sums, on the
+    GPU: "fp32" (fp32 sums of exact products), "fp8" (those of the 8-bit matrix
+    instructions, at twice the rate: off by up to 2^-12 sum |a b|, by 1.5e-5 of themselves
+    for normal numbers) or "any" (the faster of the two for a bfloat16 result, whichever
+    its sizes make it).
     """
 
     def __init__(self, **attrs: Any) -> None:
@@ -292,6 +298,8 @@ class XTCOperFp8Matmul(XTCOperator):
             raise ValueError(f"{self.name} expects operands of one depth: codes {a} {b}")
         if a_rows != 1:
             raise ValueError(f"{self.name}: a has a scale for every {BLOCK} elements of a row, got {inputs_types[1]}")
+        if (sums := getattr(self.attrs, "sums", "fp32")) not in FP8_SUMS:
+            raise ValueError(f"{self.name}: sums {sums!r} are none of {FP8_SUMS}")
         out = _float_result(self.name, "uint8", getattr(self.attrs, "out_dtype", None) or "float32")
         return [XTCTensorType(shape=(a[0], b[0]), dtype=out, device=self.device)]
 

@@ -195,7 +195,8 @@ def fp8_matmul(a_codes: XTCExpr, a_scales: XTCExpr, b_codes: XTCExpr, b_scales: 
     """Extension: a (M, K) times b (N, K) transposed, both 8-bit floats, a with a scale
     for every 128 elements of a row, b that or one for every 128 x 128.  The
     gradients are products of the same kind: dx = dy w and dw = dy^T x, of operands
-    quantised along what is summed over (transpose).  Attribute out_dtype (float32)."""
+    quantised along what is summed over (transpose).  Attributes out_dtype (float32) and
+    sums ("fp32"; "fp8": those of the 8-bit matrix instructions, faster and less exact)."""
     return _append("fp8_matmul", a_codes, a_scales, b_codes, b_scales, name=name, **attrs)
 
 

@@ -186,6 +186,7 @@ class Fp8MatmulDesc(ctypes.Structure):
         ("blocks", ctypes.c_int),
         ("b_block_rows", ctypes.c_int),
         ("ldc", ctypes.c_int),
+        ("sums", ctypes.c_int),
         ("stream", ctypes.c_void_p),
     ]
 

@@ -447,9 +447,10 @@ int xtc_hip_fp8_matmul(const xtc_hip_fp8_matmul_desc *desc, const uint8_t *a_cod
  *   l = x router^T (fp32 sums); of the top_k largest l of a token (ties: the lowest
  *   expert) y = sum p_e down[e] act(up[e] x), p = softmax(l), with `normalize` divided
  *   by the sum of the chosen ones
- * act: relu of up's H rows, or silu of up's first H rows times its last H.  Between the
- * products p_e act(..) is kept in x's type, and sums are fp32.  A NaN among
- * a token's l makes its row of y NaN; rows of other tokens stay as they are.
+ * act: relu of up's H rows, or silu of up's first H rows times its last H.  Sums are fp32,
+ * and between the products p_e act(..) is kept in fp32 (hidden_f32: for bf16 x as the sum
+ * of three bf16 numbers, so that an infinity in down gives NaN) or rounded to x's type.  A
+ * NaN among a token's l makes its row of y NaN; rows of other tokens stay as they are.
  * Matrices are dense, [E][H or 2 H][K] and [E][K][H]: of x's type, or for bf16 x codes with
  * scales, of 8-bit floats in blocks of 128 x 128 (xtc_hip_fp8_quantize with
  * `matrices` E and block_rows 128) or of microscaled 4-bit floats
@@ -467,6 +468,7 @@ typedef struct {
   int top_k;             /* experts of a token, <= 16 and E */
   int normalize;
   int ldx, ldy;          /* row strides in elements, 0 = dense */
+  int hidden_f32;        /* 1: activations stay in fp32 between the products; 0: in x's type */
   void *stream;          /* hipStream_t, NULL = library stream */
 } xtc_hip_expert_layer_desc;
 

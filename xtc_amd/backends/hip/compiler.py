@@ -370,7 +370,7 @@ def _emit_launch(plan: Plan, ln: Launch, cfg: GemmConfig | SplitConfig | None, i
         lines.append(
             f"  {{ static const xtc_hip_expert_layer_desc d = {{{_DTYPE_ENUM[a['dtype']]}, XTC_HIP_WEIGHTS_{a['weights'].upper()}, "
             f"XTC_HIP_{a['activation'].upper()}, {a['T']}, {a['E']}, {a['K']}, {a['H']}, {a['top_k']}, {1 if a['normalize'] else 0}, "
-            f"0, 0, 0}};"
+            f"0, 0, {1 if a['hidden'] == 'float32' else 0}, 0}};"
         )
         lines.append(f"    if ((rc = xtc_hip_expert_layer(&d, {args}, {plan.buffer(a['workspace']).nbytes}ull, {dst}))) "
                      f"{{ record(rc, {where}); return; }} }}")

@@ -134,13 +134,14 @@ def expert_layer_attrs(op: Any, shapes: list[tuple[int, ...]], dtype: str) -> di
     activation = str(op.attrs.get("activation", "swiglu"))
     weights = "dense" if dense else "mx4" if shapes[2][2] == 16 * shapes[3][2] and shapes[3][1] == up else "fp8"
     return {"dtype": dtype, "weights": weights, "T": t, "E": e, "K": k, "H": up // 2 if activation == "swiglu" else up,
-            "top_k": int(op.attrs.get("top_k", 2)), "activation": activation, "normalize": bool(op.attrs.get("normalize", True))}
+            "top_k": int(op.attrs.get("top_k", 2)), "activation": activation, "normalize": bool(op.attrs.get("normalize", True)),
+            "hidden": str(op.attrs.get("hidden_dtype", "float32"))}
 
 
 def expert_layer_workspace(a: dict[str, Any]) -> int:
     """What xtc_hip_expert_layer asks for, in bytes."""
     slots, hidden = a["T"] * a["top_k"], -(-a["H"] // 32) * 32
-    parts = (4 * slots * hidden, 4 * slots * a["K"], 32 * a["T"] * a["E"], 4 * slots, 4 * -(-a["K"] // 16))
+    parts = ((4 if a["dtype"] == F32 else 6) * slots * hidden, 4 * slots * a["K"], 32 * a["T"] * a["E"], 4 * slots, 4 * -(-a["K"] // 16))
     return sum(-(-p // 256) * 256 for p in parts)
 
 

@@ -31,6 +31,7 @@ int check(const xtc_hip_expert_layer_desc* d, const char* what) {
   if (d->K > kMost || d->H > kMost / 2) return fail("%s: sizes K=%d H=%d are too many", what, d->K, d->H);
   if ((d->ldx && d->ldx < d->K) || (d->ldy && d->ldy < d->K))
     return fail("%s: row strides %d and %d are below the %d columns", what, d->ldx, d->ldy, d->K);
+  if (d->hidden_f32 != 0 && d->hidden_f32 != 1) return fail("%s: hidden_f32 %d is neither 0 nor 1", what, d->hidden_f32);
   return 0;
 }
 
@@ -42,7 +43,8 @@ struct Workspace {
 Workspace workspace_of(const xtc_hip_expert_layer_desc& d) {
   const uint64_t slots = (uint64_t)d.T * d.top_k, hidden = ((uint64_t)d.H + 31) / 32 * 32;
   Workspace w{};
-  w.parts = w.mid + padded(4 * slots * hidden);
+  // an activation is an fp32 number, or up to three bf16 ones
+  w.parts = w.mid + padded((d.dtype == XTC_HIP_F32 ? 4 : 6) * slots * hidden);
   w.logits = w.parts + padded(4 * slots * d.K);
   w.choice = w.logits + padded(4ull * kMostLogitParts * d.T * d.E);
   w.counters = w.choice + padded(4 * slots);
@@ -83,6 +85,7 @@ int xtc_hip_expert_layer(const xtc_hip_expert_layer_desc* desc, const void* x, c
   a.T = d.T, a.E = d.E, a.K = d.K, a.H = d.H, a.Hp = (d.H + 31) / 32 * 32, a.top_k = d.top_k;
   a.ldx = d.ldx ? d.ldx : d.K, a.ldy = d.ldy ? d.ldy : d.K;
   a.normalize = d.normalize != 0, a.swiglu = d.activation == XTC_HIP_SWIGLU;
+  a.planes = d.dtype == XTC_HIP_BF16 && d.hidden_f32 ? 3 : 1;
   const hipStream_t s = core::pick_stream(d.stream);
 
   LayerGrid grid{};

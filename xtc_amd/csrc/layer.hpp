@@ -32,13 +32,21 @@
 // 1024/2048 in bf16 10 us and 7, of which starting, logits and choice are 6; 64 tokens at
 // 2 of 16 of 4096/2048 in 4 bits 28 and 31.
 //
-// The activations p_e act(U_e x) between the two products are rounded to bf16 where x is
-// bf16, as those between two bf16 products are: it is what the second one's instructions
-// take (in two bf16 numbers, value and rest, the down product reads twice the tokens
-// and issues twice the MFMAs).
+// The activations p_e act(U_e x) between the two products: fp32, or as the caller has it
+// rounded to bf16 where x is bf16, which is what the second product's instructions take.
+// An fp32 number is the sum of three bf16 ones, its bits in turn, and layer_down
+// multiplies each matrix fragment by all three (PLANES 3).  The 16 rows of tokens in LDS
+// then hold five tokens, or 32 rows of half the length ten.  Whole calls, us, rounded and
+// in fp32: few tokens an expert 18.5, 19.6 (a token at 2 of 8 of 1024/2048 in bf16) and
+// 72.6, 74.9 (16 at 4 of 64 of 2048/1024 in 8 bits), eight 64, 82 (64 at 2 of 16 of
+// 4096/2048 in 4 bits: three times the MFMAs and LDS reads, stretches of half the length),
+// 32 61, 103 (64 at 2 of 4 of 2048/2048 in 8 bits: four passes over a matrix instead of
+// two).  With the planes read from L2 into registers instead of LDS: 19.8, 85.7, 86.9.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+
+#include <type_traits>
 
 #include "fp8.hpp"
 #include "gemm_bf16_lds.hpp"
@@ -52,7 +60,7 @@ struct LayerArgs {
   const void *up, *down;
   const uint8_t *up_scales, *down_scales;
   // workspace
-  void* mid;           // [T top_k][Hp] of x's type
+  void* mid;           // [T top_k][planes][Hp] of x's type
   float* parts;        // [T top_k][K]
   float* logits;       // [logit_parts][T][E], or null: layer_up works them out
   int* choice;         // [T][top_k]
@@ -60,6 +68,7 @@ struct LayerArgs {
   void* y;             // [T][ldy]
   int T, E, K, H, Hp, top_k, ldx, ldy;
   int normalize, swiglu;
+  int planes;          // bf16 numbers that add up to an activation: 1 or 3
   int logit_parts;
   int slices;          // of the launch's rows
 };
@@ -343,23 +352,25 @@ __device__ __forceinline__ int gather(const LayerArgs& p, const int* chosen, int
 template <int F> struct Type { typedef __bf16 type; };
 template <> struct Type<F32> { typedef float type; };
 
-// A piece's tokens in LDS: LEN elements of each, rows 16 bytes past a multiple of 256, so
-// that 16 tokens' 16 bytes fall on all banks
-template <int F>
+// A piece's tokens in LDS: a stretch of LEN elements of each, 16 rows or, in as much room,
+// 32 of half the length
+template <int F, int ROWS>
 struct Tokens {
-  static constexpr int LEN = F == F32 ? 512 : F == MX4 ? 2048 : 1024;
-  typename Type<F>::type v[16][LEN + 16 / sizeof(typename Type<F>::type)];
+  static constexpr int LEN = (F == F32 ? 512 : F == MX4 ? 2048 : 1024) * 16 / ROWS;
+  typename Type<F>::type v[ROWS][LEN + 16 / sizeof(typename Type<F>::type)];
 };
 
-// acc[j]: 16 matrix rows j times 16 tokens, part `part` of DEPTH of the depth, in
-// stretches of Tokens::LEN.  `token(t)` is row t < `count` of the tokens, `depth` elements.
+// acc[j]: 16 matrix rows j times `count` tokens, at most 16 and ROWS / PLANES, part `part` of
+// DEPTH of the depth, in stretches of Tokens::LEN.  `token(t)` is token t, the first of
+// PLANES rows of `depth` elements that add up to it, `wide` apart.  k is taken in the same
+// order whatever ROWS and `count`.
 // Two tiles of tokens at once were tried: a branch round the MFMAs of the second leaves
 // out the wait states that the first one's sums need when it is taken.
-template <int F, int TN, int DEPTH, typename GetToken>
-__device__ __forceinline__ void product(f32x4 (&acc)[TN], Row<F> (&rows)[TN], Tokens<F>& x, int depth, int count, int part, GetToken&& token) {
+template <int F, int TN, int DEPTH, int PLANES, int ROWS, typename GetToken>
+__device__ __forceinline__ void product(f32x4 (&acc)[TN], Row<F> (&rows)[TN], Tokens<F, ROWS>& x, int depth, int wide, int count, int part, GetToken&& token) {
   typedef typename Type<F>::type T;
-  constexpr int STEP = Row<F>::STEP, V = 16 / sizeof(T), LEN = Tokens<F>::LEN, RING = 2;
-  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+  constexpr int STEP = Row<F>::STEP, V = 16 / sizeof(T), LEN = Tokens<F, ROWS>::LEN, RING = 2;
+  const int lane = threadIdx.x & 63, l16 = PLANES == 1 ? lane & 15 : min(lane & 15, count - 1), g = lane >> 4;
   constexpr int EACH = LEN / STEP / DEPTH;  // steps of a wave on a stretch
   static_assert(EACH * STEP * DEPTH == LEN, "every wave has as many steps on a stretch");
   const int all = (depth + STEP - 1) / STEP;
@@ -378,24 +389,35 @@ __device__ __forceinline__ void product(f32x4 (&acc)[TN], Row<F> (&rows)[TN], To
       if (s + q >= most) break;
       if ((s + q) % EACH == 0) {
         const int from = (s + q) * DEPTH * STEP, here = min(depth - from, LEN);
-        const int row = (here + STEP - 1) / STEP * (STEP / V), whole = here / V;  // 16-byte vectors, with zeros and without
+        // 16-byte vectors, with zeros and without; rows of planes have zeros up to `wide`
+        const int row = (here + STEP - 1) / STEP * (STEP / V), whole = (PLANES == 1 ? here : here + V - 1) / V;
         __syncthreads();  // the last tokens, or sums, have been read
-        // a wave takes a token at a time
-        for (int t = wave_of(); t < count; t += WAVES) {
-          const T* const src = token(t) + from;
-          for (int k0 = lane; k0 < row; k0 += 64 * 4) {
-            u32x4 v[4];
+        // a wave takes AT_ONCE rows at a time, all of their loads first: as many as its registers
+        // leave room for (eight vectors for 4 bits 82 us of the call above, four 87; for 8 bits
+        // more than two spill)
+        constexpr int VECS = (LEN / V + 63) / 64, AT_ONCE = PLANES == 1 ? 1 : (F == MX4 ? 8 : F == FP8 ? 2 : 4) / VECS;
+        for (int t0 = wave_of(); t0 < count * PLANES; t0 += WAVES * AT_ONCE) {
+          u32x4 v[AT_ONCE][VECS];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              v[i] = u32x4{0, 0, 0, 0};
-              if (k0 + 64 * i < whole) __builtin_memcpy(&v[i], src + (k0 + 64 * i) * V, 16);
+          for (int r = 0; r < AT_ONCE; ++r) {
+            const int t = min(t0 + WAVES * r, count * PLANES - 1);
+            const T* const src = PLANES == 1 ? token(t) + from : token(t % count) + (int64_t)(t / count) * wide + from;
+#pragma unroll
+            for (int i = 0; i < VECS; ++i) {
+              v[r][i] = u32x4{0, 0, 0, 0};
+              if (lane + 64 * i < whole) __builtin_memcpy(&v[r][i], src + (lane + 64 * i) * V, 16);
             }
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (k0 + 64 * i < row) __builtin_memcpy(__builtin_assume_aligned(&x.v[t][(k0 + 64 * i) * V], 16), &v[i], 16);
           }
-          // what is left of the row, after the zeros
-          if (lane < here % V) x.v[t][whole * V + lane] = src[whole * V + lane];
+#pragma unroll
+          for (int r = 0; r < AT_ONCE; ++r) {
+            const int t = t0 + WAVES * r;
+            if (t >= count * PLANES) break;
+#pragma unroll
+            for (int i = 0; i < VECS; ++i)
+              if (lane + 64 * i < row) __builtin_memcpy(__builtin_assume_aligned(&x.v[t][(lane + 64 * i) * V], 16), &v[r][i], 16);
+            // what is left of the row, after the zeros
+            if (PLANES == 1 && lane < here % V) x.v[t][whole * V + lane] = token(t)[from + whole * V + lane];
+          }
         }
         __syncthreads();
       }
@@ -406,9 +428,12 @@ __device__ __forceinline__ void product(f32x4 (&acc)[TN], Row<F> (&rows)[TN], To
       for (int h = 0; h < 4; ++h) {
 #pragma unroll
         for (int c = 0; c < STEP / 16 / V; ++c) {
-          const u32x4 v = *(const u32x4*)&x.v[l16][k + h * (STEP / 4) + V * c];
 #pragma unroll
-          for (int j = 0; j < TN; ++j) acc[j] = multiply<F>(w[q][j], h, c, v, acc[j]);
+          for (int i = PLANES - 1; i >= 0; --i) {
+            const u32x4 v = *(const u32x4*)&x.v[i * count + l16][k + h * (STEP / 4) + V * c];
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[j] = multiply<F>(w[q][j], h, c, v, acc[j]);
+          }
         }
         // a place's conversions follow those before it: all at once they fill the registers
         __builtin_amdgcn_sched_barrier(0);
@@ -419,6 +444,16 @@ __device__ __forceinline__ void product(f32x4 (&acc)[TN], Row<F> (&rows)[TN], To
   __builtin_amdgcn_sched_barrier(0);
   asm volatile("s_nop 15");
   __builtin_amdgcn_sched_barrier(0);
+}
+
+// The three bf16 numbers, as their bits, that add up to v: its leading eight bits, the next
+// and the last.  Cut off, not rounded, so that the first is finite where v is.
+__device__ __forceinline__ void split3(float v, unsigned short (&out)[3]) {
+  const unsigned first = __float_as_uint(v) & 0xffff0000u;
+  const float rest = (first & 0x7f800000u) == 0x7f800000u ? 0.f : v - __uint_as_float(first);
+  const unsigned second = __float_as_uint(rest) & 0xffff0000u;
+  out[0] = (unsigned short)(first >> 16), out[1] = (unsigned short)(second >> 16);
+  out[2] = (unsigned short)(__float_as_uint(rest - __uint_as_float(second)) >> 16);
 }
 
 // The sums of the DEPTH waves that share a piece's depth: f(v, q) with tile q of them, in
@@ -497,7 +532,7 @@ __global__ void __launch_bounds__(layer::THREADS, F == layer::MX4 ? 2 : 3) layer
   typedef typename Type<F>::type T;
   constexpr int TILE = SWIGLU ? 8 : 16, ROWS = TILE * TN * (WAVES / DEPTH);
   __shared__ __attribute__((aligned(16))) union {
-    Tokens<F> tokens;
+    Tokens<F, 16> tokens;
     Sums<TN> sums;
     Sums<1> logit_sums;
     float logits[LOGITS];
@@ -569,9 +604,17 @@ __global__ void __launch_bounds__(layer::THREADS, F == layer::MX4 ? 2 : 3) layer
         *(f32x4*)((float*)p.mid + (int64_t)place * p.Hp + row) = h;
       } else {
         typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
-        const bf16x4 hi = __builtin_convertvector(h, bf16x4);
-        __bf16* const to = (__bf16*)p.mid + (int64_t)place * p.Hp + row;
-        *(bf16x4*)to = hi;
+        typedef unsigned short u16x4 __attribute__((ext_vector_type(4)));
+        __bf16* const to = (__bf16*)p.mid + (int64_t)place * p.planes * p.Hp + row;
+        if (p.planes == 1) {
+          *(bf16x4*)to = __builtin_convertvector(h, bf16x4);
+        } else {
+          unsigned short parts[4][3];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) split3(h[r], parts[r]);
+#pragma unroll
+          for (int i = 0; i < 3; ++i) *(u16x4*)(to + (int64_t)i * p.Hp) = u16x4{parts[0][i], parts[1][i], parts[2][i], parts[3][i]};
+        }
       }
     };
     for (int at = 0; at < n; at += 16) {
@@ -583,7 +626,7 @@ __global__ void __launch_bounds__(layer::THREADS, F == layer::MX4 ? 2 : 3) layer
       };
       Row<F> rows[2] = {row(0), row(1)};
       static_assert(TN == 2, "two tiles of rows a wave");
-      product<F, TN, DEPTH>(acc, rows, lds.tokens, p.K, min(n - at, 16), wave % DEPTH,
+      product<F, TN, DEPTH, 1, 16>(acc, rows, lds.tokens, p.K, p.K, min(n - at, 16), wave % DEPTH,
                                 [&](int t) { return (const T*)p.x + (int64_t)(places[at + t] / p.top_k) * p.ldx; });
       summed<DEPTH>(lds.sums, acc, [&](f32x4 v, int q) {
         const int t = at + l16;
@@ -594,13 +637,17 @@ __global__ void __launch_bounds__(layer::THREADS, F == layer::MX4 ? 2 : 3) layer
 }
 
 // D of the same, and the sum over a token's experts by the last workgroup of a slice
-template <int F, int TN, int DEPTH>
+template <int F, int TN, int DEPTH, int PLANES>
 __global__ void __launch_bounds__(layer::THREADS, F == layer::MX4 ? 2 : 3) layer_down(LayerArgs p) {
   using namespace layer;
   typedef typename Type<F>::type T;
   constexpr int ROWS = 16 * TN * (WAVES / DEPTH);
+  // with three planes 16 rows are five tokens; ten have 32 where a step of every wave is half a
+  // stretch
+  constexpr bool WIDE = PLANES > 1 && 2 * DEPTH * Row<F>::STEP <= Tokens<F, 16>::LEN;
   __shared__ __attribute__((aligned(16))) union {
-    Tokens<F> tokens;
+    Tokens<F, 16> tokens;
+    Tokens<F, WIDE ? 32 : 16> more;
     Sums<TN> sums;
   } lds;
   __shared__ int chosen[64 * 16], active[256], places_of[WAVES][64];
@@ -625,21 +672,27 @@ __global__ void __launch_bounds__(layer::THREADS, F == layer::MX4 ? 2 : 3) layer
           if (row + r < p.K) splitk_store(to + r, v[r]);
       }
     };
-    for (int at = 0; at < n; at += 16) {
+    for (int at = 0, here; at < n; at += here) {
+      here = min(n - at, WIDE ? 32 / PLANES : 16 / PLANES);
       f32x4 acc[TN] = {};
       auto row = [&](int j) { return Row<F>(p.down, p.down_scales, e, p.K, min(n0 + 16 * j + l16, p.K - 1), p.H); };
-      auto token = [&](int t) { return (const T*)p.mid + (int64_t)places[at + t] * p.Hp; };
+      auto token = [&](int t) { return (const T*)p.mid + (int64_t)places[at + t] * PLANES * p.Hp; };
+      auto sum = [&](Row<F>(&rows)[TN]) {
+        if constexpr (WIDE)
+          if (here > 16 / PLANES) return product<F, TN, DEPTH, PLANES, 32>(acc, rows, lds.more, p.H, p.Hp, here, wave % DEPTH, token);
+        product<F, TN, DEPTH, PLANES, 16>(acc, rows, lds.tokens, p.H, p.Hp, here, wave % DEPTH, token);
+      };
       static_assert(TN == 1 || TN == 2, "one or two tiles of rows a wave");
       if constexpr (TN == 1) {
         Row<F> rows[1] = {row(0)};
-        product<F, TN, DEPTH>(acc, rows, lds.tokens, p.H, min(n - at, 16), wave % DEPTH, token);
+        sum(rows);
       } else {
         Row<F> rows[2] = {row(0), row(1)};
-        product<F, TN, DEPTH>(acc, rows, lds.tokens, p.H, min(n - at, 16), wave % DEPTH, token);
+        sum(rows);
       }
       summed<DEPTH>(lds.sums, acc, [&](f32x4 v, int q) {
         const int t = at + l16;
-        keep(v, n0 + 16 * q + 4 * g, places[min(t, n - 1)], t < n);
+        keep(v, n0 + 16 * q + 4 * g, places[min(t, n - 1)], l16 < here);
       });
     }
     if (!splitk_arrive(p.counters + slice, experts)) continue;
@@ -663,18 +716,24 @@ struct LayerGrid {
 template <int F>
 void layer_launch(const LayerArgs& a, const LayerGrid& g, hipStream_t s);
 
+template <int F, int DEPTH, int PLANES>
+void layer_launch_down(const LayerArgs& a, const LayerGrid& g, hipStream_t s) {
+  if constexpr (DEPTH == layer::WAVES)
+    if (g.narrow) {
+      hipLaunchKernelGGL((layer_down<F, 1, DEPTH, PLANES>), dim3(g.down), dim3(layer::THREADS), 0, s, a);
+      return;
+    }
+  hipLaunchKernelGGL((layer_down<F, 2, DEPTH, PLANES>), dim3(g.down), dim3(layer::THREADS), 0, s, a);
+}
 template <int F, int DEPTH>
 void layer_launch_tiles(const LayerArgs& a, const LayerGrid& g, hipStream_t s) {
   LayerArgs u = a, d = a;
   u.slices = g.up_slices, d.slices = g.down_slices;
   if (a.swiglu) hipLaunchKernelGGL((layer_up<F, 2, true, DEPTH>), dim3(g.up), dim3(layer::THREADS), 0, s, u);
   else hipLaunchKernelGGL((layer_up<F, 2, false, DEPTH>), dim3(g.up), dim3(layer::THREADS), 0, s, u);
-  if constexpr (DEPTH == layer::WAVES)
-    if (g.narrow) {
-      hipLaunchKernelGGL((layer_down<F, 1, DEPTH>), dim3(g.down), dim3(layer::THREADS), 0, s, d);
-      return;
-    }
-  hipLaunchKernelGGL((layer_down<F, 2, DEPTH>), dim3(g.down), dim3(layer::THREADS), 0, s, d);
+  if constexpr (F != layer::F32)
+    if (a.planes == 3) return layer_launch_down<F, DEPTH, 3>(d, g, s);
+  layer_launch_down<F, DEPTH, 1>(d, g, s);
 }
 #define XTC_HIP_LAYER_LAUNCH(F)                                                  \
   template <>                                                                    \

@@ -327,9 +327,9 @@ class XTCOperExpertLayer(XTCOperator):
     x (T, K), T <= 64, router (E, K), E <= 256, up (E, H or 2 H, K), down (E, K, H) of
     x's type, or of bfloat16 x with up and down each as two uint8 tensors, codes and
     scales: 8-bit floats (scales (E, ceil(R / 128), B)) or microscaled 4-bit floats
-    (scales (E, R, B)) -> (T, K) of x's type, in which p[e] act(..) is kept between the
-    products.  A NaN among a token's l makes its row NaN.
-    Attributes top_k (2), activation ("swiglu"), normalize (True).
+    (scales (E, R, B)) -> (T, K) of x's type.  p[e] act(..) is kept in hidden_dtype between
+    the products, float32 or x's type.  A NaN among a token's l makes its row NaN.
+    Attributes top_k (2), activation ("swiglu"), normalize (True), hidden_dtype (float32).
     """
 
     def __init__(self, **attrs: Any) -> None:
@@ -345,6 +345,9 @@ class XTCOperExpertLayer(XTCOperator):
         xs = _rows_type(self.name, x)
         if len(xs) != 2 or len(router.constant_shape) != 2 or str(router.dtype) != str(x.dtype) or router.constant_shape[1] != xs[1]:
             raise ValueError(f"{self.name} expects x (T, K) and router (E, K) of one type: {x} {router}")
+        hidden = getattr(self.attrs, "hidden_dtype", "float32")
+        if hidden not in ("float32", str(x.dtype)):
+            raise ValueError(f"{self.name}: hidden_dtype {hidden!r} is neither float32 nor x's type {x.dtype}")
         (t, k), e = xs, router.constant_shape[0]
         if t > MOST_TOKENS or e > MOST_EXPERTS or not isinstance(top_k, int) or not 1 <= top_k <= min(e, MOST_CHOSEN):
             raise ValueError(f"{self.name}: {t} tokens (at most {MOST_TOKENS}), {e} experts (at most {MOST_EXPERTS}), top_k "
@@ -379,7 +382,7 @@ class XTCOperExpertLayer(XTCOperator):
         packed = {"dense": lambda n: n, "fp8": lambda n: BLOCK * blocks_of(n), "mx4": lambda n: 16 * mx4_blocks_of(n)}[weights]
         if h < 1 or shapes[0] != (e, shapes[0][1], packed(k)) or shapes[1] != (e, k, packed(h)):
             raise ValueError(f"{self.name}: up {shapes[0]} and down {shapes[1]} do not match {e} experts of width {k} and hidden {h}")
-        return {"T": t, "E": e, "K": k, "H": h, "top_k": top_k, "activation": activation, "weights": weights,
+        return {"T": t, "E": e, "K": k, "H": h, "top_k": top_k, "activation": activation, "weights": weights, "hidden": hidden,
                 "normalize": bool(getattr(self.attrs, "normalize", True))}
 
     def forward_types(self, inputs_types):  # type: ignore[override]
@@ -419,6 +422,6 @@ class XTCOperExpertLayer(XTCOperator):
                         u = u[: d["H"]] / (1 + np.exp(-u[: d["H"]])) * u[d["H"]:]
                     else:
                         u = np.where(u < 0, 0, u)
-                    h = p[e] * u  # kept in x's type between the products
-                    y[t] += np.dot(down[e], round_to_bf16(h.astype(np.float32)) if is_bf16(inputs[0].type.dtype) else h)
+                    h = p[e] * u
+                    y[t] += np.dot(down[e], round_to_bf16(h.astype(np.float32)) if is_bf16(d["hidden"]) else h)
         return [self._check(XTCTensor(y, dtype=inputs[0].type.dtype), inputs)]

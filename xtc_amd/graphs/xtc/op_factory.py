@@ -205,7 +205,8 @@ def expert_layer(x: XTCExpr, router: XTCExpr, up: Any, down: Any, name: str | No
     up (E, H or 2 H, K) and down (E, K, H) of x's type or each a pair (codes, scales) of
     8-bit floats in blocks of 128 x 128 or of microscaled 4-bit floats.  Attributes
     top_k (2), activation ("swiglu": up's first H rows are the gate; or "relu"),
-    normalize (True: the chosen experts' weights sum to 1)."""
+    normalize (True: the chosen experts' weights sum to 1), hidden_dtype (float32: the
+    activations between up and down keep it; bfloat16 for bfloat16 x: they are rounded)."""
     matrices = [m for w in (up, down) for m in (w if isinstance(w, (tuple, list)) else (w,))]
     return _append("expert_layer", x, router, *matrices, name=name, **attrs)
 

@@ -193,7 +193,8 @@ class Fp8MatmulDesc(ctypes.Structure):
 
 class ExpertLayerDesc(ctypes.Structure):
     _fields_ = [
-        *[(n, ctypes.c_int) for n in ("dtype", "weights", "activation", "T", "E", "K", "H", "top_k", "normalize", "ldx", "ldy")],
+        *[(n, ctypes.c_int) for n in ("dtype", "weights", "activation", "T", "E", "K", "H", "top_k", "normalize", "ldx", "ldy",
+                                          "hidden_f32")],
         ("stream", ctypes.c_void_p),
     ]
 

@@ -488,7 +488,7 @@ def lower_graph(graph: Any) -> Plan:
                 # those of the transposed tensor from the same pass, or the values
                 turned = (key[0], not key[1])
                 other = next(((u, c) for u in users.get(n.inputs[0], []) if u.operation.name == "fp8_scales" and u.uid not in absorbed
-                              and fp8_key(u.operation) == turned and (c := codes_of(u, turned)) is not None), None)
+                              and u.name not in scheduled and fp8_key(u.operation) == turned and (c := codes_of(u, turned)) is not None), None)
                 if other is not None:
                     attrs["other"] = [u.uid for u in other]
                     fused += other

@@ -368,9 +368,9 @@ int xtc_hip_layer_norm(const xtc_hip_layer_norm_desc *desc, const void *x, const
  *   xh = (x - m) r, g = dy w, dx = r (g - sum g / K - xh sum (g xh) / K)
  *   dw = sum over rows of dy xh, db = sum over rows of dy, in an order that depends
  *   on the sizes alone
- * dw and db need a workspace of 2 min(rows, XTC_HIP_LAYER_NORM_PARTS) K + 2 rows
- * floats, 16-byte aligned, that no other call uses meanwhile.  Results overlap no
- * operand. */
+ * dw and db need K <= 65535 2048 and a workspace of 2 min(rows,
+ * XTC_HIP_LAYER_NORM_PARTS) K + 2 rows floats, 16-byte aligned, that no other call uses
+ * meanwhile.  Results overlap no operand. */
 #define XTC_HIP_LAYER_NORM_PARTS 512
 int xtc_hip_layer_norm_grad(const xtc_hip_layer_norm_desc *desc, const void *x, const void *w,
                             const void *dy, void *dx, float *dw, float *db, float *workspace);

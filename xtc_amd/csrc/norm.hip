@@ -16,6 +16,8 @@ constexpr int64_t kWalks = 1024;           // workgroups of 256 threads that wal
                                            // (a row each and no walk: 149 us of 32768 x 4096, this 129)
 constexpr int kMostParts = XTC_HIP_LAYER_NORM_PARTS;
 
+constexpr int64_t kMostColumns = 65535ll * 2048;  // of the parameters' sums: a launch's second extent
+
 int check(const xtc_hip_layer_norm_desc* d, const char* what) {
   if (!core::ready()) return fail("xtc_hip_init not called");
   if (!d) return fail("%s: null descriptor", what);
@@ -119,6 +121,7 @@ int xtc_hip_layer_norm_grad(const xtc_hip_layer_norm_desc* desc, const void* x, 
   if (!dx && !sums) return fail("%s: no result is asked for", what);
   if (desc->rows && (!x || !dy)) return fail("%s: null operand", what);
   if (desc->rows && sums && !workspace) return fail("%s: sums over the rows need a workspace", what);
+  if (sums && desc->K > kMostColumns) return fail("%s: rows of %d elements are too many to sum over", what, desc->K);
   const hipStream_t s = core::pick_stream(desc->stream);
   NormArgs a = args_of(*desc, x, w);
   const int parts = (int)parts_of(*desc);
@@ -129,7 +132,6 @@ int xtc_hip_layer_norm_grad(const xtc_hip_layer_norm_desc* desc, const void* x, 
       launch(*desc, a, true, (unsigned)(a.rows < kMostGroups ? a.rows : kMostGroups));
       if (sums) {
         const dim3 grid((unsigned)parts, (unsigned)(((int64_t)a.K + 2047) / 2048));
-        if (grid.y > 65535) return fail("%s: rows of %d elements are too long", what, a.K);
         if (desc->dtype == XTC_HIP_F32) hipLaunchKernelGGL(layer_norm_grad_columns<float>, grid, dim3(256), 0, s, a);
         else hipLaunchKernelGGL(layer_norm_grad_columns<__bf16>, grid, dim3(256), 0, s, a);
       }

@@ -419,7 +419,10 @@ int xtc_hip_fp8_dequantize(const xtc_hip_fp8_desc *desc, const uint8_t *codes,
 /* c[m, n] = sum_k a[m, k] b[n, k] of such operands, both with k along their rows.  a has
  * a scale for every 128 elements of a row, b that or (b_block_rows 128) one for every 128 x
  * 128 block.  sums:
- *   XTC_HIP_SUMS_FP32  fp32 sums of exact products
+ *   XTC_HIP_SUMS_FP32  fp32 sums of exact products of bf16 numbers, which the values are
+ *                      for scale bytes from 3 to 246 (blocks whose largest element lies
+ *                      above 448 2^-125 and not above 448 2^119; other ones lose what lies
+ *                      under 2^-133, or pass bf16's range and make infinities)
  *   XTC_HIP_SUMS_FP8   those of the 8-bit matrix instructions, at twice the rate: of eight
  *                      products at a time they keep 16 bits below the largest, so that c is
  *                      off by up to 2^-12 sum_k |a b| (2^16 + 1 - 2^16 can give 0; sums of
@@ -454,7 +457,8 @@ int xtc_hip_fp8_matmul(const xtc_hip_fp8_matmul_desc *desc, const uint8_t *a_cod
  * Matrices are dense, [E][H or 2 H][K] and [E][K][H]: of x's type, or for bf16 x codes with
  * scales, of 8-bit floats in blocks of 128 x 128 (xtc_hip_fp8_quantize with
  * `matrices` E and block_rows 128) or of microscaled 4-bit floats
- * (xtc_hip_mx4_quantize, E rows together). */
+ * (xtc_hip_mx4_quantize, E rows together).  Their values are taken as bf16 numbers, which
+ * they are for 8-bit scale bytes from 3 to 246 and 4-bit ones up to 252. */
 #define XTC_HIP_WEIGHTS_DENSE 0
 #define XTC_HIP_WEIGHTS_FP8 1
 #define XTC_HIP_WEIGHTS_MX4 2

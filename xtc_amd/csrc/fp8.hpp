@@ -83,7 +83,9 @@ __device__ __forceinline__ void values4(float* v, unsigned word, unsigned s) {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
-// The values of 8 codes as bf16 numbers: exact, as scales are powers of two.
+// The values of 8 codes as bf16 numbers: exact for scale bytes from 3 to 246.  Below, a
+// code's last bits lie under bf16's smallest number, 2^-133; above, 448 scale lies past its
+// largest, below 2^128.
 __device__ __forceinline__ bf16x8 values_bf16(unsigned lo, unsigned hi, float scale) {
   const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true),
                c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);

@@ -5,7 +5,8 @@
 // with the p divided by their sum or not.  act is relu, or silu of U's first H rows
 // times its last H rows.  Matrices are stored [out][in], in the type of x, or of bf16 x
 // as 8-bit floats in blocks of 128 x 128 (fp8.hpp) or 4-bit ones in blocks of 32
-// (mx4.hpp), whose values are bf16 numbers: activations keep their precision.
+// (mx4.hpp), whose values are bf16 numbers (8-bit scale bytes from 3 to 246, 4-bit ones up
+// to 252): activations keep their precision.
 //
 // The cost is reading the chosen experts' matrices once.  Two launches:
 //   layer_up    every workgroup works out the choice for all tokens by itself (so no
@@ -204,7 +205,7 @@ template <> struct Row<MX4> {
 
 __device__ __forceinline__ unsigned bits(bf16x2 v) { return __builtin_bit_cast(unsigned, v); }
 
-// 8 elements, the c-th of place i, as bf16 numbers: exact, as scales are powers of two
+// 8 elements, the c-th of place i, as bf16 numbers
 __device__ __forceinline__ bf16x8 fragment(const Raw<BF16>& q, int i, int) { return __builtin_bit_cast(bf16x8, q.v[i]); }
 __device__ __forceinline__ bf16x8 fragment(const Raw<FP8>& q, int i, int c) {
   return fp8::values_bf16(q.v[i][2 * c], q.v[i][2 * c + 1], fp8::scale_of_byte(q.s[i >> 1]));

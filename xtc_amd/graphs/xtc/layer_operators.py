@@ -282,10 +282,10 @@ class XTCOperFp8Matmul(XTCOperator):
 
     a codes (M, 128 B) and scales (M, B), b codes (N, 128 B) and scales (N, B) or
     (ceil(N / 128), B) -> (M, N) of type out_dtype (float32).  Attribute sums, on the
-    GPU: "fp32" (fp32 sums of exact products), "fp8" (those of the 8-bit matrix
-    instructions, at twice the rate: off by up to 2^-12 sum |a b|, by 1.5e-5 of themselves
-    for normal numbers) or "any" (the faster of the two for a bfloat16 result, whichever
-    its sizes make it).
+    GPU: "fp32" (fp32 sums of exact products, for scale bytes from 3 to 246), "fp8" (those
+    of the 8-bit matrix instructions, at twice the rate: off by up to 2^-12 sum |a b|, by
+    1.5e-5 of themselves for normal numbers) or "any" (the faster of the two for a bfloat16
+    result, whichever its sizes make it).
     """
 
     def __init__(self, **attrs: Any) -> None:

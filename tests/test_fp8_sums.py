@@ -46,6 +46,19 @@ out.append([product(sums=s) for s in (-1, 3)])
     assert all(isinstance(m, str) and "unsupported sums" in m for m in got[4])
 
 
+def test_few_rows_of_wide_matrices(run):  # noqa: F811
+    """Two rounds of tiles take the kernels of few rows, three do not; tiles of 32 rows give
+    way to 8-bit sums, where those are wanted, past one."""
+    sizes = [(16, 8192), (16, 8224), (16, 11008), (16, 16384), (16, 16416), (17, 8192), (17, 8224), (32, 16384), (32, 16416), (512, 1024), (1, 28672)]
+    got = run(CALLS + f"""
+for sums in (1, 0):
+    out.append([product(out_dtype=1, sums=sums, M=M, N=N, blocks=64)[0][0] for M, N in {sizes!r}])
+""")
+    want = ["rows16"] * 4 + ["64", "rows32", "rows32", "rows32", "64", "rows32", "64"]
+    assert [kernel(n) for n in got[0]] == want, got[0]
+    assert [kernel(n) for n in got[1]] == [w if w != "rows32" or i == 5 else "64" for i, w in enumerate(want)], got[1]
+
+
 def test_the_operator_sums_in_fp32_unless_asked():
     types = [((200, 256), U8), ((200, 2), U8), ((300, 256), U8), ((3, 2), U8)]
     for out in (F, B):

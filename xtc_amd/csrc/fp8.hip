@@ -127,14 +127,21 @@ int check(const xtc_hip_fp8_matmul_desc* desc, const char* what) {
 int product(const xtc_hip_fp8_matmul_desc& d, Fp8Args& a, const char* what) {
   const hipStream_t s = core::pick_stream(d.stream);
   const bool fast = d.sums == XTC_HIP_SUMS_FP8 || (d.sums == XTC_HIP_SUMS_ANY && a.out16);
-  // few tiles: the kernel that sums in fp32, unless the caller has asked for one kind of sums
-  // whatever the rows
-  for (const RowsTile* t : {&kRows16, &kRows32})
-    if (d.sums != XTC_HIP_SUMS_FP8 && tiles_of(d.M, t->bm) * tiles_of(d.N, t->bn) <= 256) {
-      a.tiles_n = (int)tiles_of(d.N, t->bn);
-      t->run[a.out16](a, (unsigned)(tiles_of(d.M, t->bm) * a.tiles_n), s);
-      return done(what);
-    }
+  // Few tiles: the kernel that sums in fp32 (unless the caller has asked for the other sums),
+  // with as many rows a tile as take the fewer rounds of the 256 CUs, and up to two rounds.
+  // us, 16 rows a tile, 32, and the best tile of LDS-DMA with fp32 sums and 8-bit ones (M x N x k):
+  //   one round   16 x 8192 x 8192  18, 21, 50, 41   32 x 8192 x 8192  33, 23, 50, 42   16 x 4096 x 1024  5.1, 4.8, 8.1, 6.9
+  //   two         16 x 11008 x 8192  31, 35, 51, 42   16 x 14336 x 2048  11, 12, 15, 13   32 x 14336 x 8192  60, 43, 52, 45
+  //               128 x 4096 x 4096  31, 22, 22, 18   64 x 8192 x 1024  12, 8.4, 8.5, 7.3
+  //   four        16 x 28672 x 8192  63, 69, 64, 62   64 x 14336 x 8192  105, 81, 52, 46
+  // In two rounds tiles of 32 rows lose to 8-bit sums.
+  const auto rounds = [&](const RowsTile& t) { return (tiles_of(d.M, t.bm) * tiles_of(d.N, t.bn) + 255) / 256; };
+  const RowsTile& few = rounds(kRows16) <= rounds(kRows32) ? kRows16 : kRows32;
+  if (d.sums != XTC_HIP_SUMS_FP8 && rounds(few) <= (fast && few.bm == 32 ? 1 : 2)) {
+    a.tiles_n = (int)tiles_of(d.N, few.bn);
+    few.run[a.out16](a, (unsigned)(tiles_of(d.M, few.bm) * a.tiles_n), s);
+    return done(what);
+  }
   const DmaTile* best = nullptr;
   double least = 0;
   for (const DmaTile& t : kDmaTiles) {

@@ -12,8 +12,9 @@ namespace {
 constexpr int kMost = 0x7fffffff - 16383;  // of K: a walk's step past it stays within 32 bits
 constexpr int kLong = 16384;               // elements of a row that registers hold
 constexpr int64_t kMostGroups = 1 << 20;   // of a launch: its threads stay within 32 bits
-constexpr int64_t kWalks = 1024;           // workgroups of 256 threads that walk over the rows: four a CU
-                                           // (a row each and no walk: 149 us of 32768 x 4096, this 129)
+constexpr int64_t kWalks = 1024;           // workgroups of 256 threads that walk over the rows: four a CU (a
+                                           // row each and no walk: 149 us of 32768 x 4096, this 129, both
+                                           // with the rows read through the caches)
 constexpr int kMostParts = XTC_HIP_LAYER_NORM_PARTS;
 
 constexpr int64_t kMostColumns = 65535ll * 2048;  // of the parameters' sums: a launch's second extent
@@ -43,7 +44,6 @@ NormArgs args_of(const xtc_hip_layer_norm_desc& d, const void* x, const void* w)
   NormArgs a{};
   a.x = x, a.w = w, a.rows = d.rows, a.K = d.K, a.eps = d.eps;
   a.ldx = d.ldx ? d.ldx : d.K, a.ldy = d.ldy ? d.ldy : d.K;
-  a.once = d.rows * d.K * (d.dtype == XTC_HIP_F32 ? 4 : 2) >= stream::LARGE;
   return a;
 }
 
@@ -53,18 +53,24 @@ NormArgs args_of(const xtc_hip_layer_norm_desc& d, const void* x, const void* w)
 int threads_of(int K, bool grad) { return K <= 1024 ? 64 : K <= (grad ? 2048 : 4096) ? 256 : grad && K <= 4096 ? 512 : 1024; }
 
 template <typename T, typename P, int THREADS, int VECS>
-void run_rows(const NormArgs& a, bool grad, unsigned groups, hipStream_t s) {
-  const dim3 threads(THREADS < 256 ? 256 : THREADS);
-  if (grad) hipLaunchKernelGGL((layer_norm_grad<T, P, THREADS, VECS>), dim3(groups), threads, 0, s, a);
-  else hipLaunchKernelGGL((layer_norm<T, P, THREADS, VECS>), dim3(groups), threads, 0, s, a);
-}
-template <typename T, typename P, int THREADS, int VECS>
 void run_forward(const NormArgs& a, unsigned groups, hipStream_t s) {
-  hipLaunchKernelGGL((layer_norm<T, P, THREADS, VECS>), dim3(groups), dim3(THREADS), 0, s, a);
+  hipLaunchKernelGGL((layer_norm<T, P, THREADS, VECS>), dim3(groups), dim3(THREADS < 256 ? 256 : THREADS), 0, s, a);
 }
 template <typename T, typename P, int THREADS, int VECS>
 void run_grad(const NormArgs& a, unsigned groups, hipStream_t s) {
-  hipLaunchKernelGGL((layer_norm_grad<T, P, THREADS, VECS>), dim3(groups), dim3(THREADS), 0, s, a);
+  const dim3 threads(THREADS < 256 ? 256 : THREADS);
+  if constexpr (sizeof(T) == 4 && THREADS == 1024)
+    // a dx that the caches do not hold beside what was read (stream.hpp)
+    if (a.y && a.rows * a.K * 4 >= stream::LARGE) {
+      hipLaunchKernelGGL((layer_norm_grad<true, T, P, THREADS, VECS>), dim3(groups), threads, 0, s, a);
+      return;
+    }
+  hipLaunchKernelGGL((layer_norm_grad<false, T, P, THREADS, VECS>), dim3(groups), threads, 0, s, a);
+}
+template <typename T, typename P, int THREADS, int VECS>
+void run_rows(const NormArgs& a, bool grad, unsigned groups, hipStream_t s) {
+  if (grad) run_grad<T, P, THREADS, VECS>(a, groups, s);
+  else run_forward<T, P, THREADS, VECS>(a, groups, s);
 }
 
 template <typename T, typename P>

@@ -17,13 +17,18 @@
 // registers, column by column, and writes them as one part; a second kernel adds
 // the parts up in order, so that results do not depend on timing.
 //
-// Bound by memory: 32768 x 4096 bf16 97 us (5.5 TB/s, a copy reaches 5.2), the gradients of
-// 16384 x 4096 87 (4.6 TB/s, and 5 us of them the second kernel).  Rows are read past the
-// caches (stream.hpp), and a row's loads run during the sums of the one before: 149 us and
-// 145 without.  A row of the gradients from 2049 to 4096 elements has 512 threads, one run
-// each, as two runs leave registers for two workgroups of four waves a CU (152, 125); the
-// forward pass, which has them, two runs of 256 (129, 171 with 512).  Two rows ahead change
-// nothing (125).
+// Bound by memory: 32768 x 4096 bf16 97 us (5.5 TB/s, a copy reaches 5.2; fp32 204, 5.3),
+// the gradients of 16384 x 4096 87 (4.6 TB/s, and 5 us of them the second kernel; fp32 152,
+// 5.3).  Rows are read past the caches (stream.hpp).  A row's loads run during the sums of
+// the one before, a row of the gradients from 2049 to 4096 elements has 512 threads, one run
+// each, as two runs leave registers for two workgroups of four waves a CU, and of the
+// forward pass, which has them, two runs of 256 (an earlier form of both kernels, without
+// and with each: 149, 129 and 145, 125; 152, 125; 171, 129; two rows ahead 125).
+//
+// Slower: rows whose 1024 threads leave 128 registers a lane, of which the gradients spill
+// some inside the loop (fp32 16384 x 8192 415 us, 3.9 TB/s; 8192 x 16384 442, bf16 256);
+// and rows of fewer than 512 elements, whose 64 threads have eight each (2^20 x 64 bf16 346
+// us, 0.8 TB/s, gradients 956; 2^18 x 512 98, 5.5 TB/s).
 //
 // Rows past 16384 elements go through memory (L2) once for each sum: the kernels
 // named *_long.
@@ -46,7 +51,6 @@ struct NormArgs {
   int64_t rows;
   int K, ldx, ldy;
   float eps;
-  bool once;       // y is larger than what the caches keep
 };
 
 namespace norm {
@@ -88,14 +92,13 @@ __device__ __forceinline__ void centre(float (&v)[8], float mean, int n) {
   }
 }
 
-template <typename T>
-__device__ __forceinline__ void store8(T* p, const float (&v)[8], int n, bool once = false) {
+template <bool PAST = false, typename T>
+__device__ __forceinline__ void store8(T* p, const float (&v)[8], int n) {
   T out[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) out[i] = (T)v[i];
   if (n >= 8) {
-    if (once) stream::store(p, out);
-    else __builtin_memcpy(p, out, sizeof(out));
+    stream::store<PAST>(p, out);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -176,14 +179,15 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) layer_norm(Norm
       float out[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) out[j] = v[i][j] * r * w[i][j] + b[i][j];
-      store8((T*)p.y + row * p.ldy + k, out, p.K - k, p.once);
+      store8((T*)p.y + row * p.ldy + k, out, p.K - k);
     }
   }
 }
 
 // dx of the rows blockIdx.x, blockIdx.x + gridDim.x, .. (of ROWS at once), and this
-// workgroup's part of dw and db.
-template <typename T, typename P, int THREADS, int VECS>
+// workgroup's part of dw and db.  PAST: dx is stored past the caches (a choice at run time
+// between the two kinds of stores becomes one ordinary store).
+template <bool PAST, typename T, typename P, int THREADS, int VECS>
 __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) layer_norm_grad(NormArgs p) {
   using namespace norm;
   constexpr int ROWS = THREADS < 256 ? 256 / THREADS : 1;
@@ -250,7 +254,7 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) layer_norm_grad
         dw[i][j] += dy[i][j] * xh, db[i][j] += dy[i][j];
       }
       const int k = (i * THREADS + t) * 8;
-      if (p.y) store8((T*)p.y + row * p.ldx + k, out, p.K - k, p.once);
+      if (p.y) store8<PAST>((T*)p.y + row * p.ldx + k, out, p.K - k);
     }
   }
   if (!p.parts) return;

@@ -14,7 +14,8 @@ output.  mx4_scales, the mx4_codes of the same tensor for these scales and a
 mx4_dequantize of the pair are one launch that writes all of them; codes and scales
 made for the rows of one 4-bit product alone go into its call.  The fp8_scales and
 fp8_codes of a tensor are one launch too, with the values of the pair or with the scales
-and codes of the transposed tensor; the gradients of one layer_norm are one call.  A matmul operand with
+and codes of the transposed tensor; the gradients of one layer_norm are one call where x's
+comes first, or the sums alone are asked for.  A matmul operand with
 layout [1, 0] (stored transposed) becomes the launch's trans_a / trans_b flag, a
 grouped_matmul's matrices with [0, 2, 1] its trans_w; other operators require natural
 layouts.  reshape is a view; unpad is a crop kernel (16-byte row copies when the innermost dim is kept).  The reference lowers each node to its own

@@ -34,8 +34,8 @@
 // waits.  AHEAD (256 x 256, FAST): four waves of 128 x 128, one a SIMD with all of its
 // registers, read the next slab's fragments between this one's matrix instructions: two
 // thirds of the LDS reads of eight waves of 128 x 64.  Its loop spills nothing; before the
-// stores, unrolled over 16 tiles, 32 registers are put aside and read back (40 MB at 8192 x
-// 8192).  PINGPONG, as in grouped_dma.hpp:
+// stores, unrolled over 16 tiles, 32 registers are put aside and read back (8 KB a wave, 34
+// MB at 8192 x 8192).  PINGPONG, as in grouped_dma.hpp:
 // eight waves, one of a SIMD's two computes while the other reads and converts.  At 8192 x
 // 8192 x 8192 with 8-bit sums AHEAD takes 483 us (2.3 PFLOP/s), PINGPONG 511; for fp32
 // sums conversions need the second wave.

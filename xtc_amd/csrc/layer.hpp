@@ -29,9 +29,9 @@
 // that these are multiplied with, 32 lanes away.
 //
 // Bound by the matrices where there are many (16 tokens, 4 of 64 experts of 2048/1024 in
-// 8 bits: 40 us and 20, 4 TB/s), and by latency else: a token at 2 of 8 experts of
-// 1024/2048 in bf16 10 us and 7, of which starting, logits and choice are 6; 64 tokens at
-// 2 of 16 of 4096/2048 in 4 bits 28 and 31.
+// 8 bits: 40 us and 20, 4 TB/s, 24 with fp32 activations), and by latency else: a token at 2
+// of 8 experts of 1024/2048 in bf16 10 us and 7 (8), of which starting, logits and choice
+// are 6; 64 tokens at 2 of 16 of 4096/2048 in 4 bits 28 and 31 (53).
 //
 // The activations p_e act(U_e x) between the two products: fp32, or as the caller has it
 // rounded to bf16 where x is bf16, which is what the second product's instructions take.

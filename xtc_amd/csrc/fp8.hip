@@ -89,6 +89,13 @@ void dma_launch(const Fp8Args& a, unsigned groups, hipStream_t s) {
 //   fp32 sums, to fp32:
 //             4096 x 4096 x 2048  80, 81, 100   4096 x 2048 x 4096  111, 73, 97   2048 x 2048 x 2048  56, 29, 30
 //             512 x 4096 x 4096  88, 40, 31    1024 x 1024 x 8192  167, 78, 44   8192 x 8192 x 4096  469, 497, 680
+//   the other two kinds lose up to 5 % of a product by the choice, 13 % once (8-bit to fp32 at 2048^3):
+//   fp32 sums, to bf16
+//             4096 x 4096 x 2048  65, 73, 93    4096 x 2048 x 4096  106, 72, 94   2048 x 2048 x 2048  52, 25, 26
+//             512 x 4096 x 4096  84, 39, 30    1024 x 1024 x 8192  163, 76, 43   8192 x 8192 x 4096  432, 486, 676
+//   8-bit instructions, to fp32
+//             4096 x 4096 x 2048  57, 60, 85    4096 x 2048 x 4096  78, 55, 84    2048 x 2048 x 2048  41, 21, 24
+//             512 x 4096 x 4096  62, 33, 27    1024 x 1024 x 8192  102, 53, 33   8192 x 8192 x 4096  385, 374, 551
 // fp32 sums are bound by the conversions, which take longer than the products: a
 // schedule of fragments read ahead and 256 x 128 tiles made 4096 x 2048 x 4096 no faster (79).
 const DmaTile kDmaTiles[] = {

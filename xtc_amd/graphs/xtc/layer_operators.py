@@ -328,7 +328,9 @@ class XTCOperExpertLayer(XTCOperator):
     x's type, or of bfloat16 x with up and down each as two uint8 tensors, codes and
     scales: 8-bit floats (scales (E, ceil(R / 128), B)) or microscaled 4-bit floats
     (scales (E, R, B)) -> (T, K) of x's type.  p[e] act(..) is kept in hidden_dtype between
-    the products, float32 or x's type.  A NaN among a token's l makes its row NaN.
+    the products, float32 or x's type.  A NaN among a token's l makes its row NaN.  On the
+    GPU an infinity in down gives NaN where bfloat16 layers keep float32, and 8-bit scale
+    bytes below 3 or past 246 take values out of bfloat16's range.
     Attributes top_k (2), activation ("swiglu"), normalize (True), hidden_dtype (float32).
     """
 
